@@ -283,6 +283,146 @@ hipError_t launch_matvec_q4k_glu_ex(const unsigned char *w_gate, const unsigned 
                                     float *y, int out_dim, int blocks_per_row,
                                     hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions, and attention over a paged key/value cache held in 8 bits
+ * (inference; no counterpart in the reference's C ABI except as noted). The
+ * reference keeps f32 keys and values and launches launch_rope_neox, a copy
+ * and sdpa_decode per layer (rocm_gemma.rs:448-469).
+ * ------------------------------------------------------------------------ */
+
+/* Which dims of a head's first rot_dim turn together. */
+#define MGQ_ROPE_INTERLEAVED 0 /* (2i, 2i+1): GGUF files of the llama family */
+#define MGQ_ROPE_HALF 1        /* (i, i + rot_dim/2): "neox" */
+
+/* Frequencies of a rotary table (GGUF: rope.freq_base, rope.scaling.*,
+ * rope_freqs.weight). theta_i = base^(-2i/rot_dim) / factors[i];
+ * t_i = theta_i * freq_scale, and with ext_factor != 0 (YaRN)
+ *   t_i = theta_i * freq_scale * (1 - m_i) + theta_i * m_i,
+ *   m_i = ext_factor * (1 - clamp((i - lo) / max(hi - lo, 0.001), 0, 1)),
+ *   lo = max(0, floor(c(beta_fast))), hi = min(rot_dim - 1, ceil(c(beta_slow))),
+ *   c(n) = rot_dim * ln(orig_ctx / (2 pi n)) / (2 ln base).
+ * Both columns are multiplied by attn_factor, with ext_factor != 0 times
+ * (1 + 0.1 ln(1 / freq_scale)). */
+typedef struct mgq_rope_scaling {
+    double base;          /* > 0; with ext_factor > 1 */
+    double freq_scale;    /* > 0: 1 / (the factor that the context is stretched by) */
+    double ext_factor;    /* 0: no ramp */
+    double attn_factor;   /* 1 */
+    double beta_fast;     /* 32; > 0 */
+    double beta_slow;     /* 1; > 0 */
+    double orig_ctx;      /* the context trained on; > 0 with ext_factor */
+    const float *factors; /* device, rot_dim/2 divisors, or null */
+} mgq_rope_scaling;
+
+/* A table that launch_rope_table_ex wrote, for positions 0 .. n_pos-1. */
+typedef struct mgq_rope {
+    const float *table; /* device, [n_pos][rot_dim/2][2]: cos, sin */
+    int n_pos;
+    int rot_dim; /* dims of a head that turn: even, 2 .. 512 */
+    int style;   /* MGQ_ROPE_* */
+} mgq_rope;
+
+/* table[p][i] = mscale * (cos, sin)((first_pos + p) * t_i) for p < n_pos,
+ * i < rot_dim/2: angles in 64 bits, each entry rounded once. */
+hipError_t launch_rope_table_ex(float *table, int n_pos, int first_pos, int rot_dim,
+                                const mgq_rope_scaling *scaling, hipStream_t stream);
+
+/* y = x with the first rot_dim dims of every head turned to the token's
+ * position, (a, b) -> (a cos - b sin, a sin + b cos), each value rounded once
+ * (launch_rope_neox's function with MGQ_ROPE_HALF, rocm_gemma.rs:448-469).
+ * Token t's heads are at x + t*x_stride, head_dim floats each, one after
+ * another; strides are in floats, at least n_heads*head_dim. y may be x with
+ * the same stride, else they must not overlap. pos: n_tokens device ints; a
+ * position outside 0 .. n_pos-1 gives a row of NaN. head_dim is even. */
+hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_rope *rope,
+                          int n_tokens, int n_heads, int head_dim, int64_t x_stride,
+                          int64_t y_stride, hipStream_t stream);
+
+/* 8-bit formats of a cache. */
+#define MGQ_KV_I8 0   /* -127 .. 127 */
+#define MGQ_KV_E4M3 1 /* FP8 E4M3 (OCP), largest 448 */
+
+/* One layer's cache: pages of page_tokens tokens, and for each sequence the
+ * list of its pages. Page p, kv head h is the page_tokens*head_dim bytes from
+ * p*page_stride + h*page_tokens*head_dim, in k as [token][dim], in v as
+ * [dim][token]; its values are bytes times k_scale / v_scale [p*n_kv_heads + h].
+ * Position j of sequence b lies in page page_table[b*max_pages + j/page_tokens].
+ * An entry outside 0 .. n_pages-1 names no page: tokens there are not stored,
+ * and attention does not see them (pages behind a sliding window may be given
+ * back that way). A page that is appended to belongs to one sequence; pages
+ * that are only read may be shared.
+ * seq_len and cu_tokens describe a call: sequence b has seq_len[b] tokens,
+ * the call's new ones included, and rows cu_tokens[b] .. cu_tokens[b+1]-1 of
+ * the call's q, k and v are its last ones. cu_tokens null: row b is the one
+ * new token of sequence b. A sequence with seq_len 0 is an idle slot.
+ * These arrays are device memory, read when the kernels run, so a recorded
+ * call replays on the lengths of the day. */
+typedef struct mgq_kv_cache {
+    void *k, *v;             /* 16-byte aligned */
+    float *k_scale, *v_scale;
+    const int *page_table;   /* [n_seqs][max_pages] */
+    const int *seq_len;      /* [n_seqs] */
+    const int *cu_tokens;    /* [n_seqs + 1] or null */
+    int64_t page_stride;     /* bytes, a multiple of 16, >= n_kv_heads*page_tokens*head_dim */
+    int n_pages;
+    int page_tokens;         /* 16, 32, 64 or 128 */
+    int n_kv_heads;
+    int head_dim;            /* 64, 96, 128 or 256 */
+    int format;              /* MGQ_KV_* */
+    int n_seqs;
+    int max_pages;           /* max_pages*page_tokens, the most tokens of a sequence, < 2^30 */
+} mgq_kv_cache;
+
+/* Appends the rows of k and v (n_kv_heads heads of head_dim floats, rows
+ * kv_stride floats apart) as the last tokens of their sequences, and with
+ * `rope` turns k on the way, and q (n_q_heads heads; null: none) from q to
+ * q_out (which may be q with the same stride). rope null: k is stored and q
+ * copied as they are.
+ * n_tokens: rows of q, k, v. max_new: no sequence has more new tokens (further
+ * ones are left out).
+ * For each page, kv head and of K and V: s = max(s_old, f32(amax / M)), amax
+ * over the finite new values, M the format's largest, s_old the page's scale
+ * if it holds earlier tokens of the sequence, else 0 (as for a NaN). If s > s_old the held
+ * values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
+ * nearest even and saturates, NaN becomes 0; all of it in 64 bits. Bytes behind
+ * the sequence's last token are left as they are.
+ * Tokens past max_pages*page_tokens, or in no page, are not stored. The q_out
+ * row of a token at a position outside the table is NaN.
+ * hipErrorInvalidValue unless rope->rot_dim <= head_dim and rope->n_pos >=
+ * max_pages*page_tokens. */
+hipError_t launch_kv_append_ex(const mgq_kv_cache *cache, const mgq_rope *rope, const float *k,
+                               const float *v, int64_t kv_stride, const float *q,
+                               int64_t q_stride, float *q_out, int64_t q_out_stride,
+                               int n_q_heads, int n_tokens, int max_new, hipStream_t stream);
+
+/* n pages (device ints) as f32: k_out and v_out [n][n_kv_heads][page_tokens]
+ * [head_dim] get value * scale, zeros where the id names no page. */
+hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int n, float *k_out,
+                                float *v_out, hipStream_t stream);
+
+/* Result types of launch_kv_attention_ex. */
+#define MGQ_OUT_F32 0 /* for the matvecs */
+#define MGQ_OUT_F16 1 /* for launch_gemm_q4k_f16; IEEE half bits */
+
+/* out row t, head h = softmax(s) V over the positions j of t's sequence with
+ * j <= pos and, with window > 0, j > pos - window; pos is t's position,
+ * s_j = scale * q.k_j, or softcap*tanh(scale * q.k_j / softcap) with
+ * softcap > 0. Query head h reads kv head h / (n_q_heads / n_kv_heads). A row
+ * that sees nothing is zero. Rows of no sequence are left as they are.
+ * q and out: rows of n_q_heads*head_dim values, strides in values. Statistics
+ * and sums are f32. Where out is f32, the queries and the probabilities go
+ * into the products with 22 bits; with MGQ_OUT_F16 the probabilities may have
+ * 11. Scales of V below 2^-90 count as 2^-90.
+ * workspace: device memory, 16-byte aligned, of at least
+ * mgq_kv_attention_workspace_bytes bytes; its contents need not be set and do
+ * not matter afterwards. Calls that may overlap need distinct ones. */
+size_t mgq_kv_attention_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads, int max_new);
+hipError_t launch_kv_attention_ex(const mgq_kv_cache *cache, const float *q, int64_t q_stride,
+                                  int n_q_heads, void *out, int64_t out_stride, int out_type,
+                                  int n_tokens, int max_new, float scale, float softcap,
+                                  int window, void *workspace, size_t workspace_bytes,
+                                  hipStream_t stream);
+
 /* One matvec of a decode-step chain. */
 typedef struct mgq_gemv_desc {
     const unsigned char *w_q4; /* row-aligned Q4_K bytes */
@@ -367,6 +507,11 @@ hipError_t mgq_chain_destroy(void *chain);
  *   MGQ_OP_QUANTIZE_MATVEC_DP4A  the two above in one launch for Q4_K
  *                        (launch_quantize_matvec_q4k_dp4a_ex: y from x, same
  *                        bits; xq/xd/xsum unused).
+ * Attention (the arguments in a struct of their own, which w points to in host
+ * memory; read when the chain is created, not kept):
+ *   MGQ_OP_ROPE          launch_rope_ex of an mgq_rope_args.
+ *   MGQ_OP_KV_APPEND     launch_kv_append_ex of an mgq_kv_append_args.
+ *   MGQ_OP_KV_ATTENTION  launch_kv_attention_ex of an mgq_kv_attention_args.
  * No counterpart in the reference's C ABI: its chain is Rust code that
  * launches these kernels one by one; this records them into one graph. */
 #define MGQ_OP_MATVEC 0
@@ -378,6 +523,36 @@ hipError_t mgq_chain_destroy(void *chain);
 #define MGQ_OP_QUANTIZE_Q8_1 6
 #define MGQ_OP_MATVEC_DP4A 7
 #define MGQ_OP_QUANTIZE_MATVEC_DP4A 8
+#define MGQ_OP_ROPE 9
+#define MGQ_OP_KV_APPEND 10
+#define MGQ_OP_KV_ATTENTION 11
+/* The last three take their arguments from here: mgq_op_desc.w points to one
+ * in host memory. */
+typedef struct mgq_rope_args {
+    const float *x;
+    float *y;
+    const int *pos;
+    mgq_rope rope;
+    int n_tokens, n_heads, head_dim;
+    int64_t x_stride, y_stride;
+} mgq_rope_args;
+typedef struct mgq_kv_append_args {
+    mgq_kv_cache cache;
+    mgq_rope rope; /* table null: no rotation */
+    const float *k, *v, *q;
+    float *q_out;
+    int64_t kv_stride, q_stride, q_out_stride;
+    int n_q_heads, n_tokens, max_new;
+} mgq_kv_append_args;
+typedef struct mgq_kv_attention_args {
+    mgq_kv_cache cache;
+    const float *q;
+    void *out, *workspace;
+    size_t workspace_bytes;
+    int64_t q_stride, out_stride;
+    int n_q_heads, out_type, n_tokens, max_new, window;
+    float scale, softcap;
+} mgq_kv_attention_args;
 /* GGML tensor types (gguf.rs:9-40) of the quantized weights */
 #define MGQ_DTYPE_Q4_K 12
 #define MGQ_DTYPE_Q5_K 13
@@ -387,7 +562,8 @@ typedef struct mgq_op_desc {
     int dtype;                /* MGQ_DTYPE_* (matvec ops) */
     int layout;               /* MGQ_LAYOUT_* (MGQ_OP_MATVEC on Q4_K) */
     int act;                  /* MGQ_ACT_* (GLU ops) */
-    const unsigned char *w;   /* weights (the gate matrix for MGQ_OP_MATVEC_GLU) */
+    const unsigned char *w;   /* weights (the gate matrix for MGQ_OP_MATVEC_GLU), or
+                                 the host struct of ops 9 to 11 */
     const unsigned char *w2;  /* MGQ_OP_MATVEC_GLU: the up matrix */
     const float *x;           /* input */
     const float *x2;          /* MGQ_OP_GLU: the up vector */

@@ -1,0 +1,484 @@
+// Attention of the new tokens' queries over the paged 8-bit cache.
+//
+//   s_j = scale * q . k_j (or softcap * tanh(s_j / softcap)),
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j), j <= pos, j > pos - window
+//
+// k_j = ks[page] * K8_j, v_j = vs[page] * V8_j. The 8-bit values of either
+// format are exact in f16, so both products run on the f16 matrix cores with
+// f32 accumulation (v_mfma_f32_16x16x32_f16), and what has more than 11 bits,
+// the queries and the probabilities, goes in as two halves (hi + lo, 22 bits):
+// results stay within f32's own rounding of the sums.
+//
+// Operands. The product of a tile of 64 tokens is taken as S^T = K Q^T: 4
+// blocks of 16 tokens (matrix rows) against 16 query rows (columns), so that a
+// lane's 16 scores are all of ONE query row (column lane % 16) and of 16
+// NEIGHBOURING tokens (16 * (lane / 16) + 0..15; block t's row 4j + i is token
+// 16j + 4t + i). They are the B operand of O^T = V^T P^T as they stand: no
+// score ever moves between lanes. 16 neighbouring tokens lie in one page
+// (pages are 16 tokens or more), so a lane needs one K and one V scale a tile.
+// V^T's operand is 16 tokens of one dim, 16 contiguous bytes of the
+// [dim][token] block; K's is D/4 contiguous bytes of a token (the order of the
+// summed dims is free, so lane group j takes bytes j*D/4 ..). Every operand
+// byte goes from memory to its lane's registers by 8- and 16-byte loads,
+// without shared memory.
+//
+// Softmax in base 2 with V's scale in the exponent: t_j = s_j log2 e +
+// log2(vs), M the running maximum of t, w_j = 2^(t_j - M + 14) = p_j * vs *
+// const, O += w_j V8_j, l += w_j / vs. So w_j <= 2^14 whatever the scales are:
+// its f16 hi + lo pair keeps 22 bits down to 2^-24 of the largest. M, l and O
+// are f32.
+//
+// Split. All (sequence, kv head, 16 query rows) rows of tiles laid end to end
+// are cut into equal runs, one for each work-group, so ragged batches and one
+// long sequence balance alike. The 4 wavefronts of a work-group take tiles in
+// turn, each with its own softmax state, joined through LDS at the end of a
+// row; a row that a cut goes through leaves partial states in the workspace,
+// which kv_attn_join_kernel joins.
+#include "kv_device.hpp"
+#include "kv_launch.hpp"
+
+namespace mgq {
+
+constexpr int kTile = 64;       // tokens of a tile
+constexpr int kRows = 16;       // query rows of a work-group's row of tiles
+constexpr int kAttnGroups = 512;  // work-groups: two per CU
+constexpr int kMinTiles = 4;    // least tiles of a run: one for each wavefront
+constexpr float kTop = 14.0f;   // the largest w is 2^14
+constexpr float kLeastScale = 0x1p-90f;  // smaller scales of V count as this
+
+struct AttnArgs {
+    const float *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int group;  // query heads of a kv head
+    int out_f16;
+    float scale, softcap;  // scale without log2 e when softcap is on
+    int window;
+    float *ws;
+};
+
+// A row's tiles: rows of (sequence, kv head, row block), kv head and row block
+// within the sequence.
+struct AttnSeq {
+    SeqInfo s;
+    int tile0, tiles, blocks;  // first tile, tiles of a row, row blocks
+};
+__device__ __forceinline__ AttnSeq attn_seq(const KvView &c, const AttnArgs &a, int b) {
+    AttnSeq r;
+    r.s = kv_seq(c, b);
+    // tiles that some row sees: from the first one's window to the length
+    const int lo = a.window > 0 ? max(r.s.pos0 - a.window + 1, 0) : 0;
+    r.tile0 = lo / kTile;
+    const int hi = min(r.s.len, max(r.s.pos0 + r.s.n, 0));
+    // at least one: a row that sees nothing has its zeros written
+    r.tiles = max((hi + kTile - 1) / kTile - r.tile0, 1);
+    r.blocks = (r.s.n * a.group + kRows - 1) / kRows;
+    return r;
+}
+__device__ __forceinline__ int attn_units(const KvView &c, const AttnArgs &a, int b) {
+    const AttnSeq r = attn_seq(c, a, b);
+    return r.tiles * r.blocks * c.hkv;
+}
+
+// Sum of v over the work-group (256 threads) and the sum over lower threads.
+__device__ __forceinline__ int group_scan(int v, int *part, int &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(s, o, 64);
+        if (lane >= o) s += t;
+    }
+    if (lane == 63) part[w] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int k = 0; k < 4; ++k) {
+        if (k < w) before += part[k];
+        total += part[k];
+    }
+    __syncthreads();
+    return before + s - v;
+}
+
+// Units of all sequences.
+__device__ __forceinline__ int attn_total(const KvView &c, const AttnArgs &a, int *part) {
+    int total = 0;
+    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+        const int b = b0 + threadIdx.x;
+        int t;
+        group_scan(b < c.n_seqs ? attn_units(c, a, b) : 0, part, t);
+        total += t;
+    }
+    return total;
+}
+__device__ __forceinline__ int attn_run(int total, int groups) {
+    return max((total + groups - 1) / groups, kMinTiles);
+}
+// The sequence that unit `at` lies in, and its first unit.
+__device__ __forceinline__ void attn_find(const KvView &c, const AttnArgs &a, int at, int *part, int *found, int &b,
+                                          int &base) {
+    int before = 0;
+    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+        const int i = b0 + threadIdx.x;
+        const int u = i < c.n_seqs ? attn_units(c, a, i) : 0;
+        int t;
+        const int start = before + group_scan(u, part, t);
+        if (u > 0 && at >= start && at < start + u) {
+            found[0] = i;
+            found[1] = start;
+        }
+        __syncthreads();
+        before += t;
+        if (at < before) break;
+    }
+    b = found[0];
+    base = found[1];
+    __syncthreads();
+}
+
+template <int FMT>
+__device__ __forceinline__ half8 kv_half8(uint32_t lo, uint32_t hi) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    half2v r[4];
+    if constexpr (FMT == kFmtI8) {
+        // 0x6400 | u is 1024 + u in f16; u = b + 128 after the sign flip
+        const uint32_t x[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+        const half2v bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x[i / 2], i % 2 ? 0x04030402u : 0x04010400u)) + bias;
+    } else {
+        r[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+        r[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+        r[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+        r[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    }
+    return half8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+}
+
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+
+// Workspace of run w: slot 0 for a row begun by an earlier run, slot 1 for one
+// that this run begins; each [kRows] x {O[D], M, l}.
+template <int D>
+constexpr int slot_floats() {
+    return kRows * (D + 2);
+}
+
+template <int D, int FMT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a) {
+    constexpr int KB = D / 4;    // bytes of a token that a lane group has
+    constexpr int KS = D / 32;   // summed steps of S
+    constexpr int DB = D / 16;   // blocks of 16 dims of O
+    constexpr int OP = D + 4;    // LDS row of O
+    __shared__ float sO[4 * kRows * OP];
+    __shared__ float sM[4][kRows], sL[4][kRows];
+    __shared__ int part[4], found[2];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    const int page = 1 << c.page_shift;
+
+    const int total = attn_total(c, a, part);
+    const int run = attn_run(total, gridDim.x);
+    int at = blockIdx.x * run;
+    const int stop = min(at + run, total);
+    if (at >= stop) return;
+    int b, base;
+    attn_find(c, a, at, part, found, b, base);
+    AttnSeq q = attn_seq(c, a, b);
+
+    while (at < stop) {
+        while (at - base >= q.tiles * q.blocks * c.hkv) {  // the next sequence with rows
+            base += q.tiles * q.blocks * c.hkv;
+            q = attn_seq(c, a, ++b);
+        }
+        const int row = (at - base) / q.tiles, t0 = (at - base) % q.tiles;
+        const int t1 = min(q.tiles, t0 + stop - at);
+        at += t1 - t0;
+        const int h = row % c.hkv, r0 = (row / c.hkv) * kRows;  // kv head, first query row of the block
+        const int rows = q.s.n * a.group;
+
+        // ---- this lane's query row, as hi + lo halves of a normalized row
+        const int r = r0 + col;
+        const bool live = r < rows;
+        const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
+        const int pos = live ? q.s.pos0 + tq : -1;
+        const float *qp = a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB;
+        half8 qh[KS], ql[KS];
+        float kscale;
+        {
+            float v[KB], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KB; i += 4) {
+                const f32x4 x = ld_f32x4(qp + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[i + e] = live ? x[e] : 0.0f;
+                    top = fmaxf(top, fabsf(v[i + e]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // the largest of the row into [2^13, 2^14)
+            int ex = 0;
+            if (top > 0.0f && top < 3.4e38f) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+            kscale = a.scale;
+#pragma unroll
+            for (int i = 0; i < KB; ++i) {
+                const float x = ldexp2(v[i], ex);
+                const _Float16 hi = (_Float16)x;
+                qh[i / 8][i % 8] = hi;
+                ql[i / 8][i % 8] = (_Float16)(x - (float)hi);
+            }
+            kscale = ldexp2(kscale, -ex);
+        }
+
+        f32x4 O[DB] = {};
+        float M = -INFINITY, l = 0.0f;
+
+        const int tile_end = q.tile0 + t1;
+        const int kgrp = col >> 2;  // the 16 tokens that this lane's K rows are of
+        u32x4 vreg[DB];
+        uint32_t kreg[4][KB / 4];
+        float ksv, vsv;
+        int nv;  // of this lane group's 16 tokens, those that exist
+        const int *tab = c.table + (int64_t)b * c.max_pages;
+        const auto fetch = [&](int tile) {
+            // a page that the table does not name, or past the length, is read
+            // as page 0 and counts as no tokens
+            const int pk = tile * kTile + 16 * kgrp, pv = tile * kTile + 16 * grp;
+            int ik = pk < q.s.len ? tab[pk >> c.page_shift] : -1;
+            int iv = pv < q.s.len ? tab[pv >> c.page_shift] : -1;
+            const bool okv = iv >= 0 && iv < c.n_pages;
+            if (ik < 0 || ik >= c.n_pages) ik = 0;
+            if (!okv) iv = 0;
+            nv = okv ? min(q.s.len - pv, 16) : 0;
+            ksv = c.ks[(int64_t)iv * c.hkv + h];
+            vsv = c.vs[(int64_t)iv * c.hkv + h];
+            const uint8_t *kp = c.k + ik * c.page_stride + ((int64_t)h * page + (pk & (page - 1)) + (col & 3)) * D + grp * KB;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * t * D + 8 * i);
+                    kreg[t][2 * i] = x[0];
+                    kreg[t][2 * i + 1] = x[1];
+                }
+            const uint8_t *vp = c.v + iv * c.page_stride + ((int64_t)h * D + col) * page + (pv & (page - 1));
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vreg[d] = *reinterpret_cast<const u32x4 *>(vp + (int64_t)16 * d * page);
+        };
+
+        for (int tile = q.tile0 + t0 + wave; tile < tile_end; tile += 4) {
+            fetch(tile);
+            f32x4 S[4] = {};
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const half8 x = kv_half8<FMT>(kreg[t][2 * k], kreg[t][2 * k + 1]);
+                    S[t] = mfma16(x, qh[k], S[t]);
+                    S[t] = mfma16(x, ql[k], S[t]);
+                }
+            // a page of zeros has scale 0: its tokens still count in l
+            const float vs = fmaxf(vsv, kLeastScale);
+            const float lv = __log2f(vs), ks = kscale * ksv;
+            const int first = tile * kTile + 16 * grp;
+            const int see = min(pos + 1 - first, nv);  // tokens of the 16 up to the row's own
+            const int skip = a.window > 0 ? pos - a.window + 1 - first : 0;
+            float top = M;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float s = S[t][i] * ks;
+                    if (a.softcap > 0.0f) s = a.softcap * 1.4426950408889634f * tanhf(s / a.softcap);
+                    s += lv;
+                    const int e = 4 * t + i;
+                    s = (e < see && e >= skip) ? s : -INFINITY;
+                    S[t][i] = s;
+                    top = fmaxf(top, s);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float ref = top == -INFINITY ? 0.0f : top - kTop;
+            const float fac = M == -INFINITY ? 0.0f : exp2f(M - top);
+            M = top;
+            float sum = 0.0f;
+            half8 ph[2], pl[2];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = exp2f(S[t][i] - ref);
+                    sum += w;
+                    const _Float16 hi = (_Float16)w;
+                    ph[t / 2][4 * (t % 2) + i] = hi;
+                    pl[t / 2][4 * (t % 2) + i] = (_Float16)(w - (float)hi);
+                }
+            l = l * fac + sum / vs;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) O[d] *= fac;
+            if (nv < 16) {  // bytes behind the length may be NaN codes
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = nv - 4 * e;
+                        vreg[d][e] = k >= 4 ? vreg[d][e] : k <= 0 ? 0u : vreg[d][e] & (0xFFFFFFFFu >> (32 - 8 * k));
+                    }
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const half8 x = kv_half8<FMT>(vreg[d][2 * u], vreg[d][2 * u + 1]);
+                    O[d] = mfma16(x, ph[u], O[d]);
+                    O[d] = mfma16(x, pl[u], O[d]);
+                }
+        }
+
+        // ---- the 4 wavefronts' states into one
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        __syncthreads();
+        if (grp == 0) sM[wave][col] = M;
+        __syncthreads();
+        const float all = fmaxf(fmaxf(sM[0][col], sM[1][col]), fmaxf(sM[2][col], sM[3][col]));
+        const float fac = M == -INFINITY ? 0.0f : exp2f(M - all);
+        if (grp == 0) sL[wave][col] = l * fac;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == q.tiles;
+        float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * slot_floats<D>();
+        for (int i = tid; i < kRows * D; i += 256) {
+            const int rr = i / D, d = i % D;
+            if (r0 + rr >= rows) break;
+            float o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) o += sO[(w * kRows + rr) * OP + d];
+            if (whole) {
+                const float s = sL[0][rr] + sL[1][rr] + sL[2][rr] + sL[3][rr];
+                o = s == 0.0f ? 0.0f : o / s;
+                const int64_t to = (int64_t)(q.s.t0 + (r0 + rr) / a.group) * a.out_stride +
+                                   (h * a.group + (r0 + rr) % a.group) * D + d;
+                if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
+                else static_cast<float *>(a.out)[to] = o;
+            } else {
+                slot[rr * (D + 2) + d] = o;
+                if (d == 0) {
+                    slot[rr * (D + 2) + D] = fmaxf(fmaxf(sM[0][rr], sM[1][rr]), fmaxf(sM[2][rr], sM[3][rr]));
+                    slot[rr * (D + 2) + D + 1] = sL[0][rr] + sL[1][rr] + sL[2][rr] + sL[3][rr];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the partial states of query rows that a cut went through: one
+// work-group per (sequence, row block, kv head, query row).
+template <int D>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int groups, int max_blocks) {
+    constexpr int W = 256 / D;  // states read at once
+    __shared__ int part[4], found[2];
+    __shared__ float acc[W > 1 ? 256 : 1], sum[W];
+    int w = blockIdx.x;
+    const int rr = w % kRows;
+    w /= kRows;
+    const int h = w % c.hkv;
+    w /= c.hkv;
+    const int blk = w % max_blocks, b = w / max_blocks;
+    const AttnSeq q = attn_seq(c, a, b);
+    const int r = blk * kRows + rr;
+    if (blk >= q.blocks || r >= q.s.n * a.group) return;
+    // the units before this sequence, and all of them
+    int total = 0, base = 0;
+    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+        const int i = b0 + threadIdx.x;
+        int t;
+        const int before = total + group_scan(i < c.n_seqs ? attn_units(c, a, i) : 0, part, t);
+        if (i == b) found[0] = before;
+        total += t;
+    }
+    __syncthreads();
+    base = found[0] + (blk * c.hkv + h) * q.tiles;
+    const int run = attn_run(total, groups);
+    const int g0 = base / run, g1 = (base + q.tiles - 1) / run;
+    if (g0 == g1) return;  // one run had the whole row and has written it
+    const auto state = [&](int g) {
+        return a.ws + ((int64_t)g * 2 + (g == g0)) * slot_floats<D>() + rr * (D + 2);
+    };
+    float M = -INFINITY;
+    for (int g = g0; g <= g1; ++g) M = fmaxf(M, state(g)[D]);
+    const int d = threadIdx.x % D, k = threadIdx.x / D;
+    float o = 0.0f, l = 0.0f;
+    if (k < W)
+        for (int g = g0 + k; g <= g1; g += W) {
+            const float *s = state(g);
+            const float f = s[D] == -INFINITY ? 0.0f : exp2f(s[D] - M);
+            o += f * s[d];
+            l += f * s[D + 1];
+        }
+    if (W > 1) {
+        __syncthreads();
+        if (k < W) acc[threadIdx.x] = o;
+        if (k < W && d == 0) sum[k] = l;
+        __syncthreads();
+        o = l = 0.0f;
+        for (int i = 0; i < W; ++i) {
+            o += acc[i * D + d];
+            l += sum[i];
+        }
+    }
+    if (k > 0) return;
+    o = l == 0.0f ? 0.0f : o / l;
+    const int64_t to = (int64_t)(q.s.t0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D + d;
+    if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
+    else static_cast<float *>(a.out)[to] = o;
+}
+
+size_t kv_attn_workspace(int dim, int, int, int, int, int64_t) {
+    return (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float);
+}
+
+template <int D, int FMT>
+static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
+    const int max_blocks = (c.max_new * a.group + kRows - 1) / kRows;
+    const int64_t cap = (int64_t)c.max_pages << c.page_shift;
+    const int64_t most = (int64_t)c.n_seqs * c.hkv * max_blocks * ((cap + kTile - 1) / kTile);
+    const int groups = (int)std::min<int64_t>(kAttnGroups, (most + kMinTiles - 1) / kMinTiles);
+    kv_attn_kernel<D, FMT><<<(unsigned)groups, 256, 0, stream>>>(c, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || groups == 1) return e;
+    const unsigned rows = (unsigned)(c.n_seqs * max_blocks * c.hkv * kRows);
+    kv_attn_join_kernel<D><<<rows, 256, 0, stream>>>(c, a, groups, max_blocks);
+    return hipGetLastError();
+}
+
+hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hipStream_t stream) {
+    AttnArgs a;
+    a.q = x.q;
+    a.out = x.out;
+    a.q_stride = x.q_stride;
+    a.out_stride = x.out_stride;
+    a.group = x.hq / c.hkv;
+    a.out_f16 = x.out_f16;
+    a.scale = x.softcap > 0.0f ? x.scale : x.scale * 1.4426950408889634f;
+    a.softcap = x.softcap;
+    a.window = x.window;
+    a.ws = x.ws;
+    const bool i8 = fmt == MGQ_KV_I8;
+    switch (dim) {
+    case 64: return i8 ? attn_run_dim<64, kFmtI8>(c, a, stream) : attn_run_dim<64, kFmtE4M3>(c, a, stream);
+    case 96: return i8 ? attn_run_dim<96, kFmtI8>(c, a, stream) : attn_run_dim<96, kFmtE4M3>(c, a, stream);
+    case 128: return i8 ? attn_run_dim<128, kFmtI8>(c, a, stream) : attn_run_dim<128, kFmtE4M3>(c, a, stream);
+    default: return i8 ? attn_run_dim<256, kFmtI8>(c, a, stream) : attn_run_dim<256, kFmtE4M3>(c, a, stream);
+    }
+}
+
+}  // namespace mgq

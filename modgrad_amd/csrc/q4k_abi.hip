@@ -362,6 +362,10 @@ static hipError_t op_check(const mgq_op_desc &o) {
             o.in_dim <= 0 || o.in_dim % 256)
             return hipErrorInvalidValue;
         return hipSuccess;
+    case MGQ_OP_ROPE:
+    case MGQ_OP_KV_APPEND:
+    case MGQ_OP_KV_ATTENTION:
+        return mgq::kv_op_check(o.op, o.w);
     default:
         return hipErrorInvalidValue;
     }
@@ -396,6 +400,10 @@ static hipError_t op_launch(const mgq_op_desc &o, hipStream_t s) {
         return launch_matvec_q6k_dp4a_ex(o.w, o.xq, o.xd, o.xsum, o.y, o.out_dim, o.in_dim / 256, s);
     case MGQ_OP_QUANTIZE_MATVEC_DP4A:
         return launch_quantize_matvec_q4k_dp4a_ex(o.w, o.x, o.y, o.out_dim, o.in_dim / 256, s);
+    case MGQ_OP_ROPE:
+    case MGQ_OP_KV_APPEND:
+    case MGQ_OP_KV_ATTENTION:
+        return mgq::kv_op_launch(o.op, o.w, s);
     default:
         return launch_residual_add_ex(o.y, o.x, o.out_dim, s);
     }

@@ -266,6 +266,11 @@ hipError_t chain_persistent_launch(PersistentChain *p, hipStream_t stream);
 hipError_t chain_persistent_faults(PersistentChain *p, unsigned *faults);
 hipError_t chain_persistent_destroy(PersistentChain *p);
 
+// MGQ_OP_ROPE, _KV_APPEND and _KV_ATTENTION of an op chain: the host-side
+// checks of their argument struct, and the launch (kv_abi.hip).
+hipError_t kv_op_check(int op, const void *args);
+hipError_t kv_op_launch(int op, const void *args, hipStream_t stream);
+
 hipError_t gemm_f16_launch(const uint8_t *w, const uint16_t *a, float *c, int n, int bpr,
                            int m_tokens, hipStream_t stream);
 // LDS attribute of the GEMM kernel in every tile shape (safe to call often).

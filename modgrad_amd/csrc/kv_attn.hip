@@ -34,28 +34,13 @@
 // turn, each with its own softmax state, joined through LDS at the end of a
 // row; a row that a cut goes through leaves partial states in the workspace,
 // which kv_attn_join_kernel joins.
-#include "kv_device.hpp"
-#include "kv_launch.hpp"
+#include "kv_attn.hpp"
 
 namespace mgq {
 
-constexpr int kTile = 64;       // tokens of a tile
 constexpr int kRows = 16;       // query rows of a work-group's row of tiles
 constexpr int kAttnGroups = 512;  // work-groups: two per CU
 constexpr int kMinTiles = 4;    // least tiles of a run: one for each wavefront
-constexpr float kTop = 14.0f;   // the largest w is 2^14
-constexpr float kLeastScale = 0x1p-90f;  // smaller scales of V count as this
-
-struct AttnArgs {
-    const float *q;
-    void *out;
-    int64_t q_stride, out_stride;
-    int group;  // query heads of a kv head
-    int out_f16;
-    float scale, softcap;  // scale without log2 e when softcap is on
-    int window;
-    float *ws;
-};
 
 // A row's tiles: rows of (sequence, kv head, row block), kv head and row block
 // within the sequence.
@@ -101,74 +86,49 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
     return before + s - v;
 }
 
-// Units of all sequences.
-__device__ __forceinline__ int attn_total(const KvView &c, const AttnArgs &a, int *part) {
-    int total = 0;
-    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
-        const int b = b0 + threadIdx.x;
-        int t;
-        group_scan(b < c.n_seqs ? attn_units(c, a, b) : 0, part, t);
-        total += t;
+// All units, and where unit `at(total)` lies: its sequence and that one's first
+// unit. One pass over the sequences where they are no more than the threads.
+struct AttnPlace {
+    int total, b, base;
+};
+template <class At>
+__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int *part, int *found, At at) {
+    AttnPlace p = {0, 0, 0};
+    if (c.n_seqs == 1) {
+        p.total = attn_units(c, a, 0);
+        return p;
     }
-    return total;
-}
-__device__ __forceinline__ int attn_run(int total, int groups) {
-    return max((total + groups - 1) / groups, kMinTiles);
-}
-// The sequence that unit `at` lies in, and its first unit.
-__device__ __forceinline__ void attn_find(const KvView &c, const AttnArgs &a, int at, int *part, int *found, int &b,
-                                          int &base) {
+    if (c.n_seqs > 256)
+        for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+            int t;
+            group_scan(b0 + (int)threadIdx.x < c.n_seqs ? attn_units(c, a, b0 + threadIdx.x) : 0, part, t);
+            p.total += t;
+        }
     int before = 0;
     for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
         const int i = b0 + threadIdx.x;
         const int u = i < c.n_seqs ? attn_units(c, a, i) : 0;
         int t;
         const int start = before + group_scan(u, part, t);
-        if (u > 0 && at >= start && at < start + u) {
+        before += t;
+        if (c.n_seqs <= 256) p.total = t;
+        const int x = at(p.total);
+        if (x >= start && x < start + u) {
             found[0] = i;
             found[1] = start;
         }
-        __syncthreads();
-        before += t;
-        if (at < before) break;
     }
-    b = found[0];
-    base = found[1];
     __syncthreads();
+    p.b = found[0];
+    p.base = found[1];
+    return p;
 }
-
-template <int FMT>
-__device__ __forceinline__ half8 kv_half8(uint32_t lo, uint32_t hi) {
-    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-    half2v r[4];
-    if constexpr (FMT == kFmtI8) {
-        // 0x6400 | u is 1024 + u in f16; u = b + 128 after the sign flip
-        const uint32_t x[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
-        const half2v bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            r[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x[i / 2], i % 2 ? 0x04030402u : 0x04010400u)) + bias;
-    } else {
-        r[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
-        r[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-        r[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
-        r[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-    }
-    return half8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+__device__ __forceinline__ int attn_run(int total, int groups) {
+    return max((total + groups - 1) / groups, kMinTiles);
 }
-
-__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
 // Workspace of run w: slot 0 for a row begun by an earlier run, slot 1 for one
-// that this run begins; each [kRows] x {O[D], M, l}.
-template <int D>
-constexpr int slot_floats() {
-    return kRows * (D + 2);
-}
-
+// that this run begins.
 template <int D, int FMT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a) {
     constexpr int KB = D / 4;    // bytes of a token that a lane group has
@@ -181,13 +141,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
-    const int total = attn_total(c, a, part);
-    const int run = attn_run(total, gridDim.x);
+    const AttnPlace place = attn_place(
+        c, a, part, found, [&](int total) { return (int)blockIdx.x * attn_run(total, gridDim.x); });
+    const int run = attn_run(place.total, gridDim.x);
     int at = blockIdx.x * run;
-    const int stop = min(at + run, total);
+    const int stop = min(at + run, place.total);
     if (at >= stop) return;
-    int b, base;
-    attn_find(c, a, at, part, found, b, base);
+    int b = place.b, base = place.base;
     AttnSeq q = attn_seq(c, a, b);
 
     while (at < stop) {
@@ -206,35 +166,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
         const bool live = r < rows;
         const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
         const int pos = live ? q.s.pos0 + tq : -1;
-        const float *qp = a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB;
         half8 qh[KS], ql[KS];
-        float kscale;
-        {
-            float v[KB], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < KB; i += 4) {
-                const f32x4 x = ld_f32x4(qp + i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[i + e] = live ? x[e] : 0.0f;
-                    top = fmaxf(top, fabsf(v[i + e]));
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // the largest of the row into [2^13, 2^14)
-            int ex = 0;
-            if (top > 0.0f && top < 3.4e38f) ex = 14 - __builtin_amdgcn_frexp_expf(top);
-            kscale = a.scale;
-#pragma unroll
-            for (int i = 0; i < KB; ++i) {
-                const float x = ldexp2(v[i], ex);
-                const _Float16 hi = (_Float16)x;
-                qh[i / 8][i % 8] = hi;
-                ql[i / 8][i % 8] = (_Float16)(x - (float)hi);
-            }
-            kscale = ldexp2(kscale, -ex);
-        }
+        const float kscale = a.scale * load_query<D>(
+            a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qh, ql);
 
         f32x4 O[DB] = {};
         float M = -INFINITY, l = 0.0f;
@@ -322,13 +256,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
             l = l * fac + sum / vs;
 #pragma unroll
             for (int d = 0; d < DB; ++d) O[d] *= fac;
-            if (nv < 16) {  // bytes behind the length may be NaN codes
+            if (nv < 16) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int k = nv - 4 * e;
-                        vreg[d][e] = k >= 4 ? vreg[d][e] : k <= 0 ? 0u : vreg[d][e] & (0xFFFFFFFFu >> (32 - 8 * k));
+                    for (int u = 0; u < 2; ++u) {
+                        const u32x2 x = kv_keep(u32x2{vreg[d][2 * u], vreg[d][2 * u + 1]}, nv, u);
+                        vreg[d][2 * u] = x[0];
+                        vreg[d][2 * u + 1] = x[1];
                     }
             }
 #pragma unroll
@@ -354,25 +289,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
         for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;
         __syncthreads();
         const bool whole = t0 == 0 && t1 == q.tiles;
-        float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * slot_floats<D>();
+        float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * state_floats<D>(kRows);
         for (int i = tid; i < kRows * D; i += 256) {
             const int rr = i / D, d = i % D;
             if (r0 + rr >= rows) break;
             float o = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) o += sO[(w * kRows + rr) * OP + d];
+            const float s = (sL[0][rr] + sL[1][rr]) + (sL[2][rr] + sL[3][rr]);
             if (whole) {
-                const float s = sL[0][rr] + sL[1][rr] + sL[2][rr] + sL[3][rr];
-                o = s == 0.0f ? 0.0f : o / s;
-                const int64_t to = (int64_t)(q.s.t0 + (r0 + rr) / a.group) * a.out_stride +
-                                   (h * a.group + (r0 + rr) % a.group) * D + d;
-                if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
-                else static_cast<float *>(a.out)[to] = o;
+                put_out(a, q.s.t0 + (r0 + rr) / a.group, (h * a.group + (r0 + rr) % a.group) * D + d,
+                        s == 0.0f ? 0.0f : o / s);
             } else {
-                slot[rr * (D + 2) + d] = o;
+                slot[i] = o;
                 if (d == 0) {
-                    slot[rr * (D + 2) + D] = fmaxf(fmaxf(sM[0][rr], sM[1][rr]), fmaxf(sM[2][rr], sM[3][rr]));
-                    slot[rr * (D + 2) + D + 1] = sL[0][rr] + sL[1][rr] + sL[2][rr] + sL[3][rr];
+                    slot[kRows * D + 2 * rr] = fmaxf(fmaxf(sM[0][rr], sM[1][rr]), fmaxf(sM[2][rr], sM[3][rr]));
+                    slot[kRows * D + 2 * rr + 1] = s;
                 }
             }
         }
@@ -383,63 +315,43 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
 // Joins the partial states of query rows that a cut went through: one
 // work-group per (sequence, row block, kv head, query row).
 template <int D>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int groups, int max_blocks) {
-    constexpr int W = 256 / D;  // states read at once
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int groups, int max_blocks,
+                                                           int block_rows) {
     __shared__ int part[4], found[2];
-    __shared__ float acc[W > 1 ? 256 : 1], sum[W];
+    __shared__ float f[kMostStates], red[8 + 256];
     int w = blockIdx.x;
-    const int rr = w % kRows;
-    w /= kRows;
+    const int rr = w % block_rows;
+    w /= block_rows;
     const int h = w % c.hkv;
     w /= c.hkv;
     const int blk = w % max_blocks, b = w / max_blocks;
     const AttnSeq q = attn_seq(c, a, b);
     const int r = blk * kRows + rr;
     if (blk >= q.blocks || r >= q.s.n * a.group) return;
-    // the units before this sequence, and all of them
-    int total = 0, base = 0;
-    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
-        const int i = b0 + threadIdx.x;
-        int t;
-        const int before = total + group_scan(i < c.n_seqs ? attn_units(c, a, i) : 0, part, t);
-        if (i == b) found[0] = before;
-        total += t;
+    int total, base = (blk * c.hkv + h) * q.tiles;
+    if (c.n_seqs == 1) {
+        total = q.tiles * q.blocks * c.hkv;
+    } else {
+        total = 0;
+        for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+            const int i = b0 + threadIdx.x;
+            int t;
+            const int before = total + group_scan(i < c.n_seqs ? attn_units(c, a, i) : 0, part, t);
+            if (i == b) found[0] = before;
+            total += t;
+        }
+        __syncthreads();
+        base += found[0];
     }
-    __syncthreads();
-    base = found[0] + (blk * c.hkv + h) * q.tiles;
     const int run = attn_run(total, groups);
     const int g0 = base / run, g1 = (base + q.tiles - 1) / run;
     if (g0 == g1) return;  // one run had the whole row and has written it
-    const auto state = [&](int g) {
-        return a.ws + ((int64_t)g * 2 + (g == g0)) * slot_floats<D>() + rr * (D + 2);
+    const auto slot = [&](int i) {
+        return a.ws + ((int64_t)(g0 + i) * 2 + (i == 0)) * state_floats<D>(kRows);
     };
-    float M = -INFINITY;
-    for (int g = g0; g <= g1; ++g) M = fmaxf(M, state(g)[D]);
-    const int d = threadIdx.x % D, k = threadIdx.x / D;
-    float o = 0.0f, l = 0.0f;
-    if (k < W)
-        for (int g = g0 + k; g <= g1; g += W) {
-            const float *s = state(g);
-            const float f = s[D] == -INFINITY ? 0.0f : exp2f(s[D] - M);
-            o += f * s[d];
-            l += f * s[D + 1];
-        }
-    if (W > 1) {
-        __syncthreads();
-        if (k < W) acc[threadIdx.x] = o;
-        if (k < W && d == 0) sum[k] = l;
-        __syncthreads();
-        o = l = 0.0f;
-        for (int i = 0; i < W; ++i) {
-            o += acc[i * D + d];
-            l += sum[i];
-        }
-    }
-    if (k > 0) return;
-    o = l == 0.0f ? 0.0f : o / l;
-    const int64_t to = (int64_t)(q.s.t0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D + d;
-    if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
-    else static_cast<float *>(a.out)[to] = o;
+    const float o = join_row<D>(g1 - g0 + 1, kRows, rr, slot, f, red);
+    if ((int)threadIdx.x < D)
+        put_out(a, q.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
 }
 
 size_t kv_attn_workspace(int dim, int, int, int, int, int64_t) {
@@ -455,8 +367,9 @@ static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t s
     kv_attn_kernel<D, FMT><<<(unsigned)groups, 256, 0, stream>>>(c, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || groups == 1) return e;
-    const unsigned rows = (unsigned)(c.n_seqs * max_blocks * c.hkv * kRows);
-    kv_attn_join_kernel<D><<<rows, 256, 0, stream>>>(c, a, groups, max_blocks);
+    const int block_rows = std::min(kRows, c.max_new * a.group);
+    kv_attn_join_kernel<D><<<(unsigned)(c.n_seqs * max_blocks * c.hkv * block_rows), 256, 0, stream>>>(
+        c, a, groups, max_blocks, block_rows);
     return hipGetLastError();
 }
 

@@ -1,0 +1,159 @@
+// What the attention kernels share: operands, query rows, partial states.
+#pragma once
+#include "kv_device.hpp"
+#include "kv_launch.hpp"
+
+namespace mgq {
+
+constexpr int kTile = 64;    // tokens of a tile
+constexpr float kTop = 14.0f;  // the largest w is 2^14
+constexpr float kLeastScale = 0x1p-90f;  // smaller scales of V count as this
+
+struct AttnArgs {
+    const float *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int group;  // query heads of a kv head
+    int out_f16;
+    float scale, softcap;  // scale without log2 e when softcap is on
+    int window;
+    float *ws;
+};
+
+template <int FMT>
+__device__ __forceinline__ half8 kv_half8(uint32_t lo, uint32_t hi) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    half2v r[4];
+    if constexpr (FMT == kFmtI8) {
+        // 0x6400 | u is 1024 + u in f16; u = b + 128 after the sign flip
+        const uint32_t x[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+        const half2v bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x[i / 2], i % 2 ? 0x04030402u : 0x04010400u)) + bias;
+    } else {
+        r[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+        r[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+        r[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+        r[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    }
+    return half8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+}
+
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+
+
+// A query row's dims grp*KB .. +KB-1 (KB = D/4) as f16 hi + lo pairs of the row
+// times 2^ex, the largest of the row in [2^13, 2^14): 22 bits of every value
+// that is not 2^-24 of the largest. Lanes l, l^16, l^32, l^48 share a row.
+// Returns 2^-ex.
+template <int D>
+__device__ __forceinline__ float load_query(const float *qp, half8 (&qh)[D / 32], half8 (&ql)[D / 32]) {
+    constexpr int KB = D / 4;
+    float v[KB], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KB; i += 4) {
+        const f32x4 x = ld_f32x4(qp + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[i + e] = x[e];
+            top = fmaxf(top, fabsf(x[e]));
+        }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    int ex = 0;
+    if (top > 0.0f && top < 3.4e38f) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+        const float x = ldexp2(v[i], ex);
+        const _Float16 hi = (_Float16)x;
+        qh[i / 8][i % 8] = hi;
+        ql[i / 8][i % 8] = (_Float16)(x - (float)hi);
+    }
+    return ldexp2(1.0f, -ex);
+}
+
+// The first nv of a lane's 16 tokens of V kept, the bytes of the others (they
+// may be NaN codes) zero. u: which 8 of them x holds.
+__device__ __forceinline__ u32x2 kv_keep(u32x2 x, int nv, int u) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int k = nv - 8 * u - 4 * e;
+        x[e] = k >= 4 ? x[e] : k <= 0 ? 0u : x[e] & (0xFFFFFFFFu >> (32 - 8 * k));
+    }
+    return x;
+}
+
+// A partial state of R query rows: O[R][D] unnormalized, then (M, l)[R].
+template <int D>
+constexpr int state_floats(int rows) {
+    return rows * (D + 2);
+}
+
+// The states of one query row, read from `n` slots (slot(i) -> its first float),
+// joined by a work-group of 256 threads; the row's result on thread d < D.
+// f, red: LDS. n <= kMostStates.
+constexpr int kMostStates = 512;
+template <int D, class Slot>
+__device__ __forceinline__ float join_row(int n, int rows, int row, Slot slot, float *f, float *red) {
+    constexpr int W = 256 / D;  // states read at once
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float M = -INFINITY, m[2], l[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = tid + 256 * k;
+        m[k] = -INFINITY;
+        l[k] = 0.0f;
+        if (i < n) {
+            const float2 x = *reinterpret_cast<const float2 *>(slot(i) + rows * D + 2 * row);
+            m[k] = x.x;
+            l[k] = x.y;
+        }
+        M = fmaxf(M, m[k]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if (lane == 0) red[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = tid + 256 * k;
+        const float w = m[k] == -INFINITY ? 0.0f : exp2f(m[k] - M);
+        if (i < n) f[i] = w;
+        sum += w * l[k];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) red[4 + wave] = sum;
+    __syncthreads();
+    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    const int d = tid % D, k = tid / D;
+    float o = 0.0f;
+    if (k < W) {
+#pragma unroll 8
+        for (int i = k; i < n; i += W) o += f[i] * slot(i)[row * D + d];
+    }
+    if (W > 1) {
+        if (k < W) red[8 + tid] = o;
+        __syncthreads();
+        if (k == 0) {
+#pragma unroll
+            for (int i = 1; i < W; ++i) o += red[8 + i * D + d];
+        }
+    }
+    return sum == 0.0f ? 0.0f : o / sum;
+}
+
+__device__ __forceinline__ void put_out(const AttnArgs &a, int64_t token, int head_dim0, float o) {
+    const int64_t to = token * a.out_stride + head_dim0;
+    if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
+    else static_cast<float *>(a.out)[to] = o;
+}
+
+}  // namespace mgq

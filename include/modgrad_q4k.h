@@ -345,7 +345,8 @@ hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_ro
 /* One layer's cache: pages of page_tokens tokens, and for each sequence the
  * list of its pages. Page p, kv head h is the page_tokens*head_dim bytes from
  * p*page_stride + h*page_tokens*head_dim, in k as [token][dim], in v as
- * [dim][token]; its values are bytes times k_scale / v_scale [p*n_kv_heads + h].
+ * [dim][token]; its values are bytes times k_scale / v_scale [p*n_kv_heads + h],
+ * which are not negative.
  * Position j of sequence b lies in page page_table[b*max_pages + j/page_tokens].
  * An entry outside 0 .. n_pages-1 names no page: tokens there are not stored,
  * and attention does not see them (pages behind a sliding window may be given
@@ -409,7 +410,7 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * s_j = scale * q.k_j, or softcap*tanh(scale * q.k_j / softcap) with
  * softcap > 0. Query head h reads kv head h / (n_q_heads / n_kv_heads). A row
  * that sees nothing is zero. Rows of no sequence are left as they are.
- * q and out: rows of n_q_heads*head_dim values, strides in values. Statistics
+ * q and out: rows of n_q_heads*head_dim values, strides in values. scale >= 0. Statistics
  * and sums are f32. Where out is f32, the queries and the probabilities go
  * into the products with 22 bits; with MGQ_OUT_F16 the probabilities may have
  * 11. Scales of V below 2^-90 count as 2^-90.

@@ -114,7 +114,7 @@ hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq,
     const int64_t row = (int64_t)hq * c->head_dim;
     if (bad4(q) || !out || ((uintptr_t)out & (type == MGQ_OUT_F32 ? 3u : 1u)) || qs < row || os < row)
         return hipErrorInvalidValue;
-    if (!std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap) || window < 0)
+    if (!(scale >= 0.0f) || !std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap) || window < 0)
         return hipErrorInvalidValue;
     if (bad16(ws) || bytes < mgq_kv_attention_workspace_bytes(c, hq, max_new)) return hipErrorInvalidValue;
     return hipSuccess;

@@ -354,8 +354,13 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
         put_out(a, q.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
 }
 
-size_t kv_attn_workspace(int dim, int, int, int, int, int64_t) {
-    return (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float);
+// Rows of a kv head above which kv_attn_wide.hip takes the call.
+constexpr int kNarrowRows = 16;
+
+size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
+    const size_t narrow = (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float);
+    if (max_new * (hq / hkv) <= kNarrowRows) return narrow;
+    return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
 }
 
 template <int D, int FMT>
@@ -385,6 +390,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.softcap = x.softcap;
     a.window = x.window;
     a.ws = x.ws;
+    if (c.max_new * a.group > kNarrowRows) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;
     switch (dim) {
     case 64: return i8 ? attn_run_dim<64, kFmtI8>(c, a, stream) : attn_run_dim<64, kFmtE4M3>(c, a, stream);

@@ -20,6 +20,10 @@ struct AttnArgs {
     float *ws;
 };
 
+// kv_attn_wide.hip: many query rows of a sequence.
+hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap);
+
 template <int FMT>
 __device__ __forceinline__ half8 kv_half8(uint32_t lo, uint32_t hi) {
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));

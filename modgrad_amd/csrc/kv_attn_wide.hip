@@ -1,0 +1,363 @@
+// Attention over the paged 8-bit cache for many query rows of a sequence (a
+// prompt, a piece of one): the same operands and softmax as kv_attn.hip, with
+// a tile's K and V shared by a work-group through LDS.
+//
+// A work-group has 128 query rows of one (sequence, kv head): row r is new token
+// r / group, head r % group of the group, so the rows of a group's heads share
+// the tile. 4 wavefronts of 32 rows (two sets of 16 columns of S^T). Each tile
+// of 64 tokens is converted to f16 ONCE on its way into LDS (a 4-byte word
+// costs 5 operations; each wavefront converts a quarter), as the operands the
+// matrix cores take: 16 bytes of each of 64 lanes one after another, so every
+// LDS access is a contiguous 1 KiB. One operand read feeds four products of S
+// (two sets, q's hi and lo) and two (out f16) or four (out f32) of O.
+//
+// Tile i+2's bytes load into registers and tile i+1's go to the other LDS
+// buffer while tile i multiplies; one barrier a tile, which does not wait for
+// the loads. Bound by the matrix cores (6 products of a plain f16 attention's
+// 4 with out f16) and, nearly as much, by the softmax's exponentials and
+// conversions on the vector ALU, which the second wavefront of each SIMD
+// overlaps.
+//
+// Causal work is dealt longest first; work-groups of one kv head are neighbours
+// modulo the number of kv heads, so an XCD's L2 holds few heads' caches. With
+// too few rows to fill the chip, a row block's tiles are split and the partial
+// states joined by a second kernel.
+#include "kv_attn.hpp"
+
+namespace mgq {
+
+constexpr int kWideRows = 128;
+constexpr int kWideTarget = 512;  // work-groups worth having: two per CU
+
+struct WideBlock {
+    SeqInfo s;
+    int r0, rows;            // first query row, rows of the sequence
+    int tile0, tiles, chunk; // first tile, tiles, tiles of a split
+};
+__device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, int b, int rt, int splits, WideBlock &w) {
+    w.s = kv_seq(c, b);
+    w.rows = w.s.n * a.group;
+    w.r0 = rt * kWideRows;
+    if (w.r0 >= w.rows) return false;
+    const int first = w.s.pos0 + w.r0 / a.group, last = w.s.pos0 + (min(w.r0 + kWideRows, w.rows) - 1) / a.group;
+    const int lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+    const int hi = min(w.s.len, max(last + 1, 0));
+    w.tile0 = lo / kTile;
+    w.tiles = max((hi + kTile - 1) / kTile - w.tile0, 1);  // one, for the zeros of rows that see nothing
+    w.chunk = (w.tiles + splits - 1) / splits;
+    return true;
+}
+
+__device__ __forceinline__ void wide_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+}
+
+// The larger of each of the 4 lanes l, l^16, l^32, l^48.
+__device__ __forceinline__ float max_groups(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];  // a bit cast of an element would take the first
+    x = fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t q0 = q[0], q1 = q[1];
+    return fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+}
+
+// LO: the probabilities as hi + lo pairs.
+template <int D, int FMT, bool LO>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks,
+                                                                             int splits) {
+    constexpr int KB = D / 4, KS = D / 32, DB = D / 16;
+    constexpr int VP = DB / 2;               // 8-byte pieces of V that a wavefront stages
+    constexpr int kBuf = 2 * kTile * D / 8;  // 16-byte units of a buffer: K, then V
+    extern __shared__ half8 lds[];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    const int page = 1 << c.page_shift;
+
+    int id = blockIdx.x;
+    const int h = id % c.hkv;
+    id /= c.hkv;
+    const int sp = id % splits;
+    id /= splits;
+    const int b = id % c.n_seqs;
+    WideBlock w;
+    if (!wide_block(c, a, b, row_blocks - 1 - id / c.n_seqs, splits, w)) return;
+    const int t0 = sp * w.chunk, t1 = min(w.tiles, t0 + w.chunk);
+    if (t0 >= t1) return;
+
+    // ---- query rows; those past the last repeat it and are not written
+    half8 qh[2][KS], ql[2][KS];
+    float qs[2];
+    int pos[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int r = min(w.r0 + 32 * wave + 16 * s + col, w.rows - 1);
+        const int tq = r / a.group;
+        pos[s] = w.s.pos0 + tq;
+        qs[s] = a.scale * load_query<D>(a.q + (int64_t)(w.s.t0 + tq) * a.q_stride +
+                                            (h * a.group + r % a.group) * D + grp * KB,
+                                        qh[s], ql[s]);
+    }
+    const bool live = w.r0 + 32 * wave < w.rows;
+    // positions of the wavefront's first and last row
+    const int pos_lo = w.s.pos0 + min(w.r0 + 32 * wave, w.rows - 1) / a.group;
+    const int pos_hi = w.s.pos0 + min(w.r0 + 32 * wave + 31, w.rows - 1) / a.group;
+
+    // ---- staging: block `wave` of K's four, a quarter of V's pieces
+    const int kgrp = col >> 2;
+    const int *tab = c.table + (int64_t)b * c.max_pages;
+    uint32_t kst[KB / 4];
+    u32x2 vst[VP];
+    float ks_n, vs_n;  // scales and count of the tile in the staging registers
+    int nv_n;
+    const auto fetch = [&](int t) {
+        const int tile = w.tile0 + t;
+        const int pk = tile * kTile + 16 * kgrp, pv = tile * kTile + 16 * grp;
+        int ik = pk < w.s.len ? tab[pk >> c.page_shift] : -1;
+        int iv = pv < w.s.len ? tab[pv >> c.page_shift] : -1;
+        const bool okv = iv >= 0 && iv < c.n_pages;
+        if (ik < 0 || ik >= c.n_pages) ik = 0;
+        if (!okv) iv = 0;
+        nv_n = okv ? min(w.s.len - pv, 16) : 0;
+        // what lies in a page's place that is none of the sequence's may be anything
+        ks_n = okv ? c.ks[(int64_t)iv * c.hkv + h] : 0.0f;
+        vs_n = okv ? c.vs[(int64_t)iv * c.hkv + h] : 1.0f;
+        const uint8_t *kp = c.k + ik * c.page_stride +
+                            ((int64_t)h * page + (pk & (page - 1)) + 4 * wave + (col & 3)) * D + grp * KB;
+#pragma unroll
+        for (int i = 0; i < KB / 8; ++i) {
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 8 * i);
+            kst[2 * i] = x[0];
+            kst[2 * i + 1] = x[1];
+        }
+        const uint8_t *vp = c.v + iv * c.page_stride + ((int64_t)h * D + col) * page + (pv & (page - 1));
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int p = wave * VP + i, d = VP % 2 ? p >> 1 : wave * (VP / 2) + (i >> 1), u = VP % 2 ? p & 1 : i & 1;
+            vst[i] = *reinterpret_cast<const u32x2 *>(vp + 16 * d * page + 8 * u);
+        }
+    };
+    const auto stage = [&](half8 *buf) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) buf[(wave * KS + k) * 64 + lane] = kv_half8<FMT>(kst[2 * k], kst[2 * k + 1]);
+        half8 *vb = buf + kTile * D / 8;
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int p = wave * VP + i;  // piece: dims 16 (p/2) .., tokens 8 (p%2) ..
+            u32x2 x = vst[i];
+            if (nv_n < 16) x = kv_keep(x, nv_n, VP % 2 ? p & 1 : i & 1);
+            vb[p * 64 + lane] = kv_half8<FMT>(x[0], x[1]);
+        }
+    };
+
+    f32x4 O[2][DB] = {};
+    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    fetch(t0);
+    stage(lds);
+    float ks_c = ks_n, vs_c = vs_n;
+    int nv_c = nv_n;
+    if (t0 + 1 < t1) fetch(t0 + 1);
+    for (int t = t0; t < t1; ++t) {
+        wide_barrier();  // tile t is in its buffer, the other one is free
+        const half8 *buf = lds + ((t - t0) & 1) * kBuf;
+        const float ks = ks_c, vsv = vs_c;
+        const int nv = nv_c;
+        if (t + 1 < t1) {
+            stage(lds + ((t + 1 - t0) & 1) * kBuf);
+            ks_c = ks_n;
+            vs_c = vs_n;
+            nv_c = nv_n;
+            if (t + 2 < t1) fetch(t + 2);
+        }
+        const int first = (w.tile0 + t) * kTile;
+        if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
+
+        f32x4 S[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half8 x = buf[(i * KS + k) * 64 + lane];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    S[s][i] = mfma16(x, qh[s][k], S[s][i]);
+                    S[s][i] = mfma16(x, ql[s][k], S[s][i]);
+                }
+            }
+
+        const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = 1.0f / vs;
+        // all rows see all of the tile
+        const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
+                           __all(nv == 16);
+        half8 ph[2][2], pl[2][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float sc = qs[s] * ks;
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        S[s][i][e] = a.softcap * 1.4426950408889634f * tanhf(S[s][i][e] * sc / a.softcap);
+                sc = 1.0f;
+            }
+            if (!clear) {
+                const int at = first + 16 * grp;
+                const int see = min(pos[s] + 1 - at, nv), skip = a.window > 0 ? pos[s] - a.window + 1 - at : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? S[s][i][e] * sc : -INFINITY;
+                sc = 1.0f;
+            }
+            // the largest of t = S * sc + lv: sc, a lane's own, is not negative
+            float hi = S[s][0][0];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
+            const float top = max_groups(fmaf(hi, sc, lv));
+            if (__any(top > M[s])) {
+                const float m = fmaxf(M[s], top);
+                const float fac = M[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[s] - m);
+                M[s] = m;
+                l[s] *= fac;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) O[s][d] *= fac;
+            }
+            const float off = lv - (M[s] == -INFINITY ? 0.0f : M[s] - kTop);
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(S[s][i][e], sc, off));
+                    sum += x;
+                    const _Float16 xh = (_Float16)x;
+                    ph[s][i / 2][4 * (i % 2) + e] = xh;
+                    if (LO) pl[s][i / 2][4 * (i % 2) + e] = (_Float16)(x - (float)xh);
+                }
+            l[s] += sum * rvs;
+        }
+        const half8 *vb = buf + kTile * D / 8;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const half8 x = vb[(2 * d + u) * 64 + lane];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    O[s][d] = mfma16(x, ph[s][u], O[s][d]);
+                    if (LO) O[s][d] = mfma16(x, pl[s][u], O[s][d]);
+                }
+            }
+    }
+    if (!live) return;
+
+    const bool whole = w.chunk >= w.tiles;
+    float *st = a.ws + (int64_t)blockIdx.x * state_floats<D>(kWideRows);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        float sum = l[s];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int rr = 32 * wave + 16 * s + col, r = w.r0 + rr;
+        if (r >= w.rows) continue;
+        if (whole) {
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t to = (int64_t)(w.s.t0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D + 4 * grp;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float o = O[s][d][e] * f;
+                    if (a.out_f16) static_cast<_Float16 *>(a.out)[to + 16 * d + e] = (_Float16)o;
+                    else static_cast<float *>(a.out)[to + 16 * d + e] = o;
+                }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                *reinterpret_cast<f32x4_a4 *>(st + rr * D + 16 * d + 4 * grp) = O[s][d];
+            if (grp == 0) *reinterpret_cast<float2 *>(st + kWideRows * D + 2 * rr) = make_float2(M[s], sum);
+        }
+    }
+}
+
+// Joins a split row block: one work-group per (row block, sequence, kv head, row).
+template <int D>
+__global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
+    __shared__ float f[kMostStates], red[8 + 256];
+    int id = blockIdx.x;
+    const int rr = id % kWideRows;
+    id /= kWideRows;
+    const int h = id % c.hkv;
+    id /= c.hkv;
+    const int b = id % c.n_seqs, inv = id / c.n_seqs;
+    WideBlock w;
+    if (!wide_block(c, a, b, row_blocks - 1 - inv, splits, w)) return;
+    const int r = w.r0 + rr;
+    if (r >= w.rows || w.chunk >= w.tiles) return;
+    const int n = (w.tiles + w.chunk - 1) / w.chunk;
+    const auto slot = [&](int i) {
+        return a.ws + (int64_t)(((inv * c.n_seqs + b) * splits + i) * c.hkv + h) * state_floats<D>(kWideRows);
+    };
+    const float o = join_row<D>(n, kWideRows, rr, slot, f, red);
+    if ((int)threadIdx.x < D)
+        put_out(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
+}
+
+// Row blocks at most, and the splits of each that fill the chip.
+static void wide_plan(int group, int hkv, int n_seqs, int max_new, int64_t cap, int &row_blocks, int &splits) {
+    row_blocks = (max_new * group + kWideRows - 1) / kWideRows;
+    const int64_t items = (int64_t)row_blocks * hkv * n_seqs, tiles = (cap + kTile - 1) / kTile;
+    splits = 1;
+    if (items < kWideTarget)
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>((kWideTarget + items - 1) / items, (tiles + 1) / 2));
+}
+
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap) {
+    int row_blocks, splits;
+    wide_plan(group, hkv, n_seqs, max_new, cap, row_blocks, splits);
+    if (splits == 1) return 0;
+    return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
+}
+
+template <int D, int FMT, bool LO>
+static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
+    int row_blocks, splits;
+    wide_plan(a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
+    const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
+    constexpr size_t kLds = 2 * (2 * kTile * D / 8) * sizeof(half8);
+    static std::atomic<int> state[64];
+    if (kLds > 64 * 1024) {
+        const hipError_t e = allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
+        if (e != hipSuccess) return e;
+    }
+    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, 256, kLds, stream>>>(c, a, row_blocks, splits);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);
+    return hipGetLastError();
+}
+
+template <int D>
+static hipError_t wide_dim(const KvView &c, int fmt, const AttnArgs &a, hipStream_t stream) {
+    if (fmt == MGQ_KV_I8)
+        return a.out_f16 ? wide_run<D, kFmtI8, false>(c, a, stream) : wide_run<D, kFmtI8, true>(c, a, stream);
+    return a.out_f16 ? wide_run<D, kFmtE4M3, false>(c, a, stream) : wide_run<D, kFmtE4M3, true>(c, a, stream);
+}
+
+hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream) {
+    switch (dim) {
+    case 64: return wide_dim<64>(c, fmt, a, stream);
+    case 96: return wide_dim<96>(c, fmt, a, stream);
+    case 128: return wide_dim<128>(c, fmt, a, stream);
+    default: return wide_dim<256>(c, fmt, a, stream);
+    }
+}
+
+}  // namespace mgq

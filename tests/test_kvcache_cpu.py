@@ -124,7 +124,7 @@ def test_rope_table_refuses_sizes(L):
 @pytest.mark.parametrize("bad", [dict(q=None), dict(q=FAKE + 2), dict(qs=511), dict(out=None), dict(out=FAKE + 2),
                                  dict(out=FAKE + 1, kind=1), dict(os=511), dict(kind=2), dict(kind=-1), dict(hq=3),
                                  dict(hq=0), dict(n=0), dict(new=0), dict(new=8), dict(scale=float("nan")),
-                                 dict(scale=float("inf")), dict(cap=-1.0), dict(cap=float("nan")),
+                                 dict(scale=float("inf")), dict(scale=-0.5), dict(cap=-1.0), dict(cap=float("nan")),
                                  dict(cap=float("inf")), dict(win=-1), dict(ws=None), dict(ws=FAKE + 8),
                                  dict(nbytes=0), dict(new=1 << 28, n=1 << 28)])
 def test_attention_refuses(L, bad):

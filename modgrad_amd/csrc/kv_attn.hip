@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float s = S[t][i] * ks;
-                    if (a.softcap > 0.0f) s = a.softcap * 1.4426950408889634f * tanhf(s / a.softcap);
+                    if (a.softcap > 0.0f) s = softcap_log2(s, a.softcap);
                     s += lv;
                     const int e = 4 * t + i;
                     s = (e < see && e >= skip) ? s : -INFINITY;
@@ -386,8 +386,8 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.out_stride = x.out_stride;
     a.group = x.hq / c.hkv;
     a.out_f16 = x.out_f16;
-    a.scale = x.softcap > 0.0f ? x.scale : x.scale * 1.4426950408889634f;
-    a.softcap = x.softcap;
+    a.scale = x.softcap > 0.0f ? x.scale / x.softcap : x.scale * 1.4426950408889634f;
+    a.softcap = x.softcap * 1.4426950408889634f;
     a.window = x.window;
     a.ws = x.ws;
     if (c.max_new * a.group > kNarrowRows) return kv_attn_wide_launch(c, dim, fmt, a, stream);

@@ -15,7 +15,8 @@ struct AttnArgs {
     int64_t q_stride, out_stride;
     int group;  // query heads of a kv head
     int out_f16;
-    float scale, softcap;  // scale without log2 e when softcap is on
+    // softcap off: scale * log2 e; on: scale / softcap, and softcap * log2 e
+    float scale, softcap;
     int window;
     float *ws;
 };
@@ -49,6 +50,20 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
 }
 __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
+
+// cap * log2 e * tanh(x): a polynomial where the exponential's form would cancel
+// (|x| < 0.35, good to 2^-22 there).
+__device__ __forceinline__ float softcap_log2(float x, float cap_log2e) {
+    const float e = __builtin_amdgcn_exp2f(x * 2.8853900817779268f);  // exp(2x)
+    const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+    const float y = x * x;
+    float p = fmaf(y, -0.008863235529902197f, 0.021869488536155203f);
+    p = fmaf(y, p, -0.05396825396825397f);
+    p = fmaf(y, p, 0.13333333333333333f);
+    p = fmaf(y, p, -0.3333333333333333f);
+    const float small = fmaf(x * y, p, x);
+    return cap_log2e * (fabsf(x) < 0.35f ? small : big);
+}
 
 // A query row's dims grp*KB .. +KB-1 (KB = D/4) as f16 hi + lo pairs of the row
 // times 2^ex, the largest of the row in [2^13, 2^14): 22 bits of every value

@@ -112,15 +112,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
     u32x2 vst[VP];
     float ks_n, vs_n;  // scales and count of the tile in the staging registers
     int nv_n;
+    // page ids of the tile after it, a tile ahead of their use: -1 past the length
+    int ik_n, iv_n;
+    const int last = t1 - 1;
+    const auto look = [&](int t) {
+        const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
+        ik_n = pk < w.s.len ? tab[pk >> c.page_shift] : -1;
+        iv_n = pv < w.s.len ? tab[pv >> c.page_shift] : -1;
+    };
+    // bytes of tile t, whose ids `look` has brought; past the last tile, the last again
     const auto fetch = [&](int t) {
-        const int tile = w.tile0 + t;
-        const int pk = tile * kTile + 16 * kgrp, pv = tile * kTile + 16 * grp;
-        int ik = pk < w.s.len ? tab[pk >> c.page_shift] : -1;
-        int iv = pv < w.s.len ? tab[pv >> c.page_shift] : -1;
+        const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
+        int ik = ik_n, iv = iv_n;
         const bool okv = iv >= 0 && iv < c.n_pages;
         if (ik < 0 || ik >= c.n_pages) ik = 0;
         if (!okv) iv = 0;
         nv_n = okv ? min(w.s.len - pv, 16) : 0;
+        look(t + 1);
         // what lies in a page's place that is none of the sequence's may be anything
         ks_n = okv ? c.ks[(int64_t)iv * c.hkv + h] : 0.0f;
         vs_n = okv ? c.vs[(int64_t)iv * c.hkv + h] : 1.0f;
@@ -155,23 +163,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
     f32x4 O[2][DB] = {};
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
+    look(t0);
     fetch(t0);
     stage(lds);
     float ks_c = ks_n, vs_c = vs_n;
     int nv_c = nv_n;
-    if (t0 + 1 < t1) fetch(t0 + 1);
+    fetch(t0 + 1);
     for (int t = t0; t < t1; ++t) {
         wide_barrier();  // tile t is in its buffer, the other one is free
         const half8 *buf = lds + ((t - t0) & 1) * kBuf;
         const float ks = ks_c, vsv = vs_c;
         const int nv = nv_c;
-        if (t + 1 < t1) {
-            stage(lds + ((t + 1 - t0) & 1) * kBuf);
-            ks_c = ks_n;
-            vs_c = vs_n;
-            nv_c = nv_n;
-            if (t + 2 < t1) fetch(t + 2);
-        }
+        stage(lds + ((t + 1 - t0) & 1) * kBuf);
+        ks_c = ks_n;
+        vs_c = vs_n;
+        nv_c = nv_n;
+        fetch(t + 2);
         const int first = (w.tile0 + t) * kTile;
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 }
             }
 
-        const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = 1.0f / vs;
+        const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = __builtin_amdgcn_rcpf(vs);
         // all rows see all of the tile
         const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
                            __all(nv == 16);
@@ -201,7 +208,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = a.softcap * 1.4426950408889634f * tanhf(S[s][i][e] * sc / a.softcap);
+                        S[s][i][e] = softcap_log2(S[s][i][e] * sc, a.softcap);
                 sc = 1.0f;
             }
             if (!clear) {
@@ -221,7 +228,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
             const float top = max_groups(fmaf(hi, sc, lv));
-            if (__any(top > M[s])) {
+            // the maximum may lag by 1: w stays below 2^15
+            if (__any(top > M[s] + 1.0f)) {
                 const float m = fmaxf(M[s], top);
                 const float fac = M[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[s] - m);
                 M[s] = m;

@@ -5,6 +5,8 @@
 
 namespace mgq {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kTile = 64;    // tokens of a tile
 constexpr float kTop = 14.0f;  // the largest w is 2^14
 constexpr float kLeastScale = 0x1p-90f;  // smaller scales of V count as this
@@ -65,6 +67,10 @@ __device__ __forceinline__ float softcap_log2(float x, float cap_log2e) {
     return cap_log2e * (fabsf(x) < 0.35f ? small : big);
 }
 
+__device__ __forceinline__ i32x4 mfma16(i32x4 a, i32x4 b, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
 // A query row's dims grp*KB .. +KB-1 (KB = D/4) as f16 hi + lo pairs of the row
 // times 2^ex, the largest of the row in [2^13, 2^14): 22 bits of every value
 // that is not 2^-24 of the largest. Lanes l, l^16, l^32, l^48 share a row.
@@ -94,6 +100,56 @@ __device__ __forceinline__ float load_query(const float *qp, half8 (&qh)[D / 32]
         ql[i / 8][i % 8] = (_Float16)(x - (float)hi);
     }
     return ldexp2(1.0f, -ex);
+}
+
+// The same row as N signed digits of 8 bits, 16 dims to a register quad: the
+// row times a factor that takes its largest to 0x7F7F.. (all digits 127),
+// rounded to whole numbers; for the int8 matrix cores, whose products with an
+// 8-bit K and their sums are exact. Returns the factor's inverse; a row with a
+// NaN or infinity returns NaN.
+template <int D, int N>
+__device__ __forceinline__ float load_query(const float *qp, i32x4 (&qd)[N][D / 64]) {
+    constexpr int KB = D / 4;
+    constexpr float kMost = (float)(N == 2 ? 0x7F7F : 0x7F7F7F);
+    float v[KB], top = 0.0f, bad = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KB; i += 4) {
+        const f32x4 x = ld_f32x4(qp + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[i + e] = x[e];
+            top = fmaxf(top, fabsf(x[e]));
+            bad += x[e] * 0.0f;
+        }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    bad += __shfl_xor(bad, 16, 64);
+    bad += __shfl_xor(bad, 32, 64);
+    int ex = 0;
+    float mant = 1.0f;  // top = mant * 2^ex
+    if (top > 0.0f && top < 3.4e38f) {
+        ex = __builtin_amdgcn_frexp_expf(top);
+        mant = __builtin_amdgcn_frexp_mantf(top);
+    }
+    const float f = kMost / mant;
+#pragma unroll
+    for (int i = 0; i < KB; i += 4) {
+        uint32_t w[N] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int q = (int)rintf(fminf(fmaxf(ldexp2(v[i + e], -ex) * f, -kMost), kMost));
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int d = n + 1 < N ? (int)(int8_t)q : q;
+                w[n] |= (uint32_t)(d & 0xFF) << (8 * e);
+                q = (q - d) >> 8;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) qd[n][i / 16][i / 4 % 4] = (int)w[n];
+    }
+    return ldexp2(mant / kMost, ex) + bad;
 }
 
 // The first nv of a lane's 16 tokens of V kept, the bytes of the others (they

@@ -69,9 +69,13 @@ __device__ __forceinline__ float max_groups(float x) {
 template <int D, int FMT, bool LO>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks,
                                                                              int splits) {
-    constexpr int KB = D / 4, KS = D / 32, DB = D / 16;
+    // int8 K goes into the int8 matrix cores as it is, q as digits of 8 bits: 16
+    // bits for an f16 result, 24 for f32 (heads of 96 are no multiple of 64)
+    constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
+    constexpr int ND = LO ? 3 : 2;
+    constexpr int KB = D / 4, KS = D / 32, DB = D / 16, KI = D / 64;
     constexpr int VP = DB / 2;               // 8-byte pieces of V that a wavefront stages
-    constexpr int kBuf = 2 * kTile * D / 8;  // 16-byte units of a buffer: K, then V
+    constexpr int kOfK = kTile * D / (I8 ? 16 : 8), kBuf = kOfK + kTile * D / 8;  // 16-byte units of a buffer: K, V
     extern __shared__ half8 lds[];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int page = 1 << c.page_shift;
@@ -89,6 +93,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
 
     // ---- query rows; those past the last repeat it and are not written
     half8 qh[2][KS], ql[2][KS];
+    i32x4 qd[2][ND][D / 64 > 0 ? D / 64 : 1];
     float qs[2];
     int pos[2];
 #pragma unroll
@@ -96,9 +101,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         const int r = min(w.r0 + 32 * wave + 16 * s + col, w.rows - 1);
         const int tq = r / a.group;
         pos[s] = w.s.pos0 + tq;
-        qs[s] = a.scale * load_query<D>(a.q + (int64_t)(w.s.t0 + tq) * a.q_stride +
-                                            (h * a.group + r % a.group) * D + grp * KB,
-                                        qh[s], ql[s]);
+        const float *qp = a.q + (int64_t)(w.s.t0 + tq) * a.q_stride + (h * a.group + r % a.group) * D + grp * KB;
+        if constexpr (I8) qs[s] = a.scale * load_query<D, ND>(qp, qd[s]);
+        else qs[s] = a.scale * load_query<D>(qp, qh[s], ql[s]);
     }
     const bool live = w.r0 + 32 * wave < w.rows;
     // positions of the wavefront's first and last row
@@ -148,16 +153,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         }
     };
     const auto stage = [&](half8 *buf) {
+        if constexpr (I8) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) buf[(wave * KS + k) * 64 + lane] = kv_half8<FMT>(kst[2 * k], kst[2 * k + 1]);
-        half8 *vb = buf + kTile * D / 8;
+            for (int k = 0; k < KI; ++k)
+                reinterpret_cast<u32x4 *>(buf)[(wave * KI + k) * 64 + lane] =
+                    u32x4{kst[4 * k], kst[4 * k + 1], kst[4 * k + 2], kst[4 * k + 3]};
+        } else {
 #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int p = wave * VP + i;  // piece: dims 16 (p/2) .., tokens 8 (p%2) ..
-            u32x2 x = vst[i];
-            if (nv_n < 16) x = kv_keep(x, nv_n, VP % 2 ? p & 1 : i & 1);
-            vb[p * 64 + lane] = kv_half8<FMT>(x[0], x[1]);
+            for (int k = 0; k < KS; ++k) buf[(wave * KS + k) * 64 + lane] = kv_half8<FMT>(kst[2 * k], kst[2 * k + 1]);
         }
+        half8 *vb = buf + kOfK;
+        // piece p: dims 16 (p/2) .., tokens 8 (p%2) ..
+        if (__any(nv_n < 16)) {
+#pragma unroll
+            for (int i = 0; i < VP; ++i) vst[i] = kv_keep(vst[i], nv_n, VP % 2 ? (wave * VP + i) & 1 : i & 1);
+        }
+#pragma unroll
+        for (int i = 0; i < VP; ++i) vb[(wave * VP + i) * 64 + lane] = kv_half8<FMT>(vst[i][0], vst[i][1]);
     };
 
     f32x4 O[2][DB] = {};
@@ -183,17 +195,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
         f32x4 S[2][4] = {};
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
+        if constexpr (I8) {
+            const i32x4 *kb = reinterpret_cast<const i32x4 *>(buf);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const half8 x = buf[(i * KS + k) * 64 + lane];
+                i32x4 x[KI];
+#pragma unroll
+                for (int k = 0; k < KI; ++k) x[k] = kb[(i * KI + k) * 64 + lane];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    S[s][i] = mfma16(x, qh[s][k], S[s][i]);
-                    S[s][i] = mfma16(x, ql[s][k], S[s][i]);
+                    i32x4 d[ND] = {};
+#pragma unroll
+                    for (int k = 0; k < KI; ++k)
+#pragma unroll
+                        for (int n = 0; n < ND; ++n) d[n] = mfma16(x[k], qd[s][n][k], d[n]);
+                    // two digits' sums stay below 2^31; the third joins in f32
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (LO) S[s][i][e] = fmaf((float)(d[2][e] * 256 + d[1][e]), 256.0f, (float)d[0][e]);
+                        else S[s][i][e] = (float)(d[1][e] * 256 + d[0][e]);
+                    }
                 }
             }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const half8 x = buf[(i * KS + k) * 64 + lane];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        S[s][i] = mfma16(x, qh[s][k], S[s][i]);
+                        S[s][i] = mfma16(x, ql[s][k], S[s][i]);
+                    }
+                }
+        }
 
         const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = __builtin_amdgcn_rcpf(vs);
         // all rows see all of the tile
@@ -251,7 +287,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 }
             l[s] += sum * rvs;
         }
-        const half8 *vb = buf + kTile * D / 8;
+        const half8 *vb = buf + kOfK;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -339,7 +375,7 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     int row_blocks, splits;
     wide_plan(a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
-    constexpr size_t kLds = 2 * (2 * kTile * D / 8) * sizeof(half8);
+    constexpr size_t kLds = 2 * (kTile * D / (FMT == kFmtI8 && D % 64 == 0 ? 16 : 8) + kTile * D / 8) * sizeof(half8);
     static std::atomic<int> state[64];
     if (kLds > 64 * 1024) {
         const hipError_t e = allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);

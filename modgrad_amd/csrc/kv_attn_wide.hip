@@ -186,6 +186,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         const half8 *buf = lds + ((t - t0) & 1) * kBuf;
         const float ks = ks_c, vsv = vs_c;
         const int nv = nv_c;
+        i32x4 kx[4][KI > 0 ? KI : 1];
+        if constexpr (I8) {
+            // K's operands on their way while the next tile is staged
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < KI; ++k) kx[i][k] = reinterpret_cast<const i32x4 *>(buf)[(i * KI + k) * 64 + lane];
+            __builtin_amdgcn_sched_barrier(0);
+        }
         stage(lds + ((t + 1 - t0) & 1) * kBuf);
         ks_c = ks_n;
         vs_c = vs_n;
@@ -196,19 +205,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
 
         f32x4 S[2][4] = {};
         if constexpr (I8) {
-            const i32x4 *kb = reinterpret_cast<const i32x4 *>(buf);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                i32x4 x[KI];
-#pragma unroll
-                for (int k = 0; k < KI; ++k) x[k] = kb[(i * KI + k) * 64 + lane];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     i32x4 d[ND] = {};
 #pragma unroll
                     for (int k = 0; k < KI; ++k)
 #pragma unroll
-                        for (int n = 0; n < ND; ++n) d[n] = mfma16(x[k], qd[s][n][k], d[n]);
+                        for (int n = 0; n < ND; ++n) d[n] = mfma16(kx[i][k], qd[s][n][k], d[n]);
                     // two digits' sums stay below 2^31; the third joins in f32
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -231,6 +236,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 }
         }
 
+        constexpr int G = 2;  // blocks of 16 dims read at once
+        const half8 *vb = buf + kOfK;
+        half8 vx[2][2 * G];
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) vx[0][i] = vb[i * 64 + lane];
         const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = __builtin_amdgcn_rcpf(vs);
         // all rows see all of the tile
         const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
@@ -287,18 +297,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 }
             l[s] += sum * rvs;
         }
-        const half8 *vb = buf + kOfK;
+        // V's operands a group ahead of their products
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int g = 0; g < DB / G; ++g) {
+            if (g + 1 < DB / G) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const half8 x = vb[(2 * d + u) * 64 + lane];
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    O[s][d] = mfma16(x, ph[s][u], O[s][d]);
-                    if (LO) O[s][d] = mfma16(x, pl[s][u], O[s][d]);
-                }
+                for (int i = 0; i < 2 * G; ++i) vx[(g + 1) & 1][i] = vb[(2 * G * (g + 1) + i) * 64 + lane];
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int d = g * G + i;
+                        O[s][d] = mfma16(vx[g & 1][2 * i + u], ph[s][u], O[s][d]);
+                        if (LO) O[s][d] = mfma16(vx[g & 1][2 * i + u], pl[s][u], O[s][d]);
+                    }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     if (!live) return;
 

@@ -65,19 +65,37 @@ __device__ __forceinline__ float max_groups(float x) {
     return fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
 }
 
+// Compile-time shape of the kernel. int8 K goes into the int8 matrix cores as it
+// is, q as digits of 8 bits: 16 bits for an f16 result, 24 for f32 (heads of 96
+// are no multiple of the 64 dims of such a product).
+// SETS of 16 query rows a wavefront. One set and 8 wavefronts leave a wavefront
+// few enough registers for 4 (heads of 256: 2) on a SIMD, two sets and 4
+// wavefronts read LDS half as often; which is the faster was measured.
+template <int D, int FMT, bool LO>
+struct WideShape {
+    static constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
+    static constexpr int SETS = D == 256 ? 1 : 2;
+    static constexpr int NW = kWideRows / (16 * SETS);      // wavefronts
+    static constexpr int kThreads = 64 * NW, kPerSimd = (D == 256 ? 1 : 2) * NW / 4;
+    static constexpr bool kAhead = kPerSimd <= 2;           // registers for operands ahead of their use
+    static constexpr int KS = I8 ? D / 64 : D / 32;         // summed steps of S
+    static constexpr int DB = D / 16;                       // blocks of 16 dims of O
+    static constexpr int NK = (4 * KS + NW - 1) / NW;       // pieces of K a wavefront stages: 64 lanes x 16 bytes of LDS
+    static constexpr int NV = (2 * DB + NW - 1) / NW;       // pieces of V
+    static constexpr int kOfV = 4 * KS * 64, kBuf = kOfV + 2 * DB * 64;  // 16-byte units of a buffer: K, then V
+};
+
 // LO: the probabilities as hi + lo pairs.
 template <int D, int FMT, bool LO>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks,
-                                                                             int splits) {
-    // int8 K goes into the int8 matrix cores as it is, q as digits of 8 bits: 16
-    // bits for an f16 result, 24 for f32 (heads of 96 are no multiple of 64)
-    constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
-    constexpr int ND = LO ? 3 : 2;
-    constexpr int KB = D / 4, KS = D / 32, DB = D / 16, KI = D / 64;
-    constexpr int VP = DB / 2;               // 8-byte pieces of V that a wavefront stages
-    constexpr int kOfK = kTile * D / (I8 ? 16 : 8), kBuf = kOfK + kTile * D / 8;  // 16-byte units of a buffer: K, V
+__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
+    typedef WideShape<D, FMT, LO> W;
+    constexpr bool I8 = W::I8;
+    constexpr int SETS = W::SETS, KS = W::KS, DB = W::DB, NK = W::NK, NV = W::NV;
+    constexpr int ND = LO ? 3 : 2;  // digits of q
+    constexpr int KB = D / 4;
     extern __shared__ half8 lds[];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15,
+              grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
     int id = blockIdx.x;
@@ -92,41 +110,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
     if (t0 >= t1) return;
 
     // ---- query rows; those past the last repeat it and are not written
-    half8 qh[2][KS], ql[2][KS];
-    i32x4 qd[2][ND][D / 64 > 0 ? D / 64 : 1];
-    float qs[2];
-    int pos[2];
+    half8 qh[SETS][I8 ? 1 : KS], ql[SETS][I8 ? 1 : KS];
+    i32x4 qd[SETS][ND][I8 ? KS : 1];
+    float qs[SETS];
+    int pos[SETS];
+    const int wr0 = w.r0 + 16 * SETS * wave;  // the wavefront's first row
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int r = min(w.r0 + 32 * wave + 16 * s + col, w.rows - 1);
+    for (int s = 0; s < SETS; ++s) {
+        const int r = min(wr0 + 16 * s + col, w.rows - 1);
         const int tq = r / a.group;
         pos[s] = w.s.pos0 + tq;
         const float *qp = a.q + (int64_t)(w.s.t0 + tq) * a.q_stride + (h * a.group + r % a.group) * D + grp * KB;
         if constexpr (I8) qs[s] = a.scale * load_query<D, ND>(qp, qd[s]);
         else qs[s] = a.scale * load_query<D>(qp, qh[s], ql[s]);
     }
-    const bool live = w.r0 + 32 * wave < w.rows;
+    const bool live = wr0 < w.rows;
     // positions of the wavefront's first and last row
-    const int pos_lo = w.s.pos0 + min(w.r0 + 32 * wave, w.rows - 1) / a.group;
-    const int pos_hi = w.s.pos0 + min(w.r0 + 32 * wave + 31, w.rows - 1) / a.group;
+    const int pos_lo = w.s.pos0 + min(wr0, w.rows - 1) / a.group;
+    const int pos_hi = w.s.pos0 + min(wr0 + 16 * SETS - 1, w.rows - 1) / a.group;
 
-    // ---- staging: block `wave` of K's four, a quarter of V's pieces
+    // ---- staging
     const int kgrp = col >> 2;
     const int *tab = c.table + (int64_t)b * c.max_pages;
-    uint32_t kst[KB / 4];
-    u32x2 vst[VP];
-    float ks_n, vs_n;  // scales and count of the tile in the staging registers
-    int nv_n;
-    // page ids of the tile after it, a tile ahead of their use: -1 past the length
-    int ik_n, iv_n;
     const int last = t1 - 1;
+    // page ids of the tile after the staged one, a tile ahead of their use: -1
+    // past the length
+    int ik_n, iv_n;
     const auto look = [&](int t) {
         const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
         ik_n = pk < w.s.len ? tab[pk >> c.page_shift] : -1;
         iv_n = pv < w.s.len ? tab[pv >> c.page_shift] : -1;
     };
-    // bytes of tile t, whose ids `look` has brought; past the last tile, the last again
-    const auto fetch = [&](int t) {
+    u32x4 kst[NK];  // I8: 16 bytes a piece, else 8
+    u32x2 vst[NV];
+    float ks_n, vs_n;  // scales and count of the tile in the staging registers
+    int nv_n;
+    const auto fetch = [&](int t) {  // past the last tile, the last again
         const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
         int ik = ik_n, iv = iv_n;
         const bool okv = iv >= 0 && iv < c.n_pages;
@@ -137,43 +156,51 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         // what lies in a page's place that is none of the sequence's may be anything
         ks_n = okv ? c.ks[(int64_t)iv * c.hkv + h] : 0.0f;
         vs_n = okv ? c.vs[(int64_t)iv * c.hkv + h] : 1.0f;
-        const uint8_t *kp = c.k + ik * c.page_stride +
-                            ((int64_t)h * page + (pk & (page - 1)) + 4 * wave + (col & 3)) * D + grp * KB;
-#pragma unroll
-        for (int i = 0; i < KB / 8; ++i) {
-            const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 8 * i);
-            kst[2 * i] = x[0];
-            kst[2 * i + 1] = x[1];
-        }
+        const uint8_t *kp = c.k + ik * c.page_stride + ((int64_t)h * page + (pk & (page - 1)) + (col & 3)) * D + grp * KB;
         const uint8_t *vp = c.v + iv * c.page_stride + ((int64_t)h * D + col) * page + (pv & (page - 1));
 #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int p = wave * VP + i, d = VP % 2 ? p >> 1 : wave * (VP / 2) + (i >> 1), u = VP % 2 ? p & 1 : i & 1;
-            vst[i] = *reinterpret_cast<const u32x2 *>(vp + 16 * d * page + 8 * u);
+        for (int i = 0; i < NK; ++i) {
+            const int p = wave * NK + i, bt = p / KS, k = p % KS;
+            if (4 * KS % W::NW == 0 || p < 4 * KS) {
+                if constexpr (I8) {
+                    kst[i] = *reinterpret_cast<const u32x4 *>(kp + 4 * bt * D + 16 * k);
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * bt * D + 8 * k);
+                    kst[i][0] = x[0];
+                    kst[i][1] = x[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int p = wave * NV + i;  // dims 16 (p/2) .., tokens 8 (p%2) ..
+            vst[i] = *reinterpret_cast<const u32x2 *>(vp + 16 * (p >> 1) * page + 8 * (p & 1));
         }
     };
     const auto stage = [&](half8 *buf) {
-        if constexpr (I8) {
 #pragma unroll
-            for (int k = 0; k < KI; ++k)
-                reinterpret_cast<u32x4 *>(buf)[(wave * KI + k) * 64 + lane] =
-                    u32x4{kst[4 * k], kst[4 * k + 1], kst[4 * k + 2], kst[4 * k + 3]};
-        } else {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) buf[(wave * KS + k) * 64 + lane] = kv_half8<FMT>(kst[2 * k], kst[2 * k + 1]);
+        for (int i = 0; i < NK; ++i) {
+            const int p = wave * NK + i;
+            if (4 * KS % W::NW == 0 || p < 4 * KS) {
+                if constexpr (I8) reinterpret_cast<u32x4 *>(buf)[p * 64 + lane] = kst[i];
+                else buf[p * 64 + lane] = kv_half8<FMT>(kst[i][0], kst[i][1]);
+            }
         }
-        half8 *vb = buf + kOfK;
-        // piece p: dims 16 (p/2) .., tokens 8 (p%2) ..
         if (__any(nv_n < 16)) {
 #pragma unroll
-            for (int i = 0; i < VP; ++i) vst[i] = kv_keep(vst[i], nv_n, VP % 2 ? (wave * VP + i) & 1 : i & 1);
+            for (int i = 0; i < NV; ++i) vst[i] = kv_keep(vst[i], nv_n, (wave * NV + i) & 1);
         }
 #pragma unroll
-        for (int i = 0; i < VP; ++i) vb[(wave * VP + i) * 64 + lane] = kv_half8<FMT>(vst[i][0], vst[i][1]);
+        for (int i = 0; i < NV; ++i) buf[W::kOfV + (wave * NV + i) * 64 + lane] = kv_half8<FMT>(vst[i][0], vst[i][1]);
     };
 
-    f32x4 O[2][DB] = {};
-    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    f32x4 O[SETS][DB] = {};
+    float M[SETS], l[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+        M[s] = -INFINITY;
+        l[s] = 0.0f;
+    }
 
     look(t0);
     fetch(t0);
@@ -183,35 +210,39 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
     fetch(t0 + 1);
     for (int t = t0; t < t1; ++t) {
         wide_barrier();  // tile t is in its buffer, the other one is free
-        const half8 *buf = lds + ((t - t0) & 1) * kBuf;
+        const half8 *buf = lds + ((t - t0) & 1) * W::kBuf;
         const float ks = ks_c, vsv = vs_c;
         const int nv = nv_c;
-        i32x4 kx[4][KI > 0 ? KI : 1];
-        if constexpr (I8) {
-            // K's operands on their way while the next tile is staged
+        i32x4 kx[4][I8 ? KS : 1];
+        const auto read_k = [&] {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < KI; ++k) kx[i][k] = reinterpret_cast<const i32x4 *>(buf)[(i * KI + k) * 64 + lane];
+                for (int k = 0; k < KS; ++k) kx[i][k] = reinterpret_cast<const i32x4 *>(buf)[(i * KS + k) * 64 + lane];
+        };
+        if constexpr (I8 && W::kAhead) {
+            // K's operands on their way while the next tile is staged
+            read_k();
             __builtin_amdgcn_sched_barrier(0);
         }
-        stage(lds + ((t + 1 - t0) & 1) * kBuf);
+        stage(lds + ((t + 1 - t0) & 1) * W::kBuf);
+        nv_c = nv_n;
         ks_c = ks_n;
         vs_c = vs_n;
-        nv_c = nv_n;
         fetch(t + 2);
         const int first = (w.tile0 + t) * kTile;
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
-        f32x4 S[2][4] = {};
+        f32x4 S[SETS][4] = {};
         if constexpr (I8) {
+            if (!W::kAhead) read_k();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
+                for (int s = 0; s < SETS; ++s) {
                     i32x4 d[ND] = {};
 #pragma unroll
-                    for (int k = 0; k < KI; ++k)
+                    for (int k = 0; k < KS; ++k)
 #pragma unroll
                         for (int n = 0; n < ND; ++n) d[n] = mfma16(kx[i][k], qd[s][n][k], d[n]);
                     // two digits' sums stay below 2^31; the third joins in f32
@@ -229,15 +260,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
                 for (int i = 0; i < 4; ++i) {
                     const half8 x = buf[(i * KS + k) * 64 + lane];
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    for (int s = 0; s < SETS; ++s) {
                         S[s][i] = mfma16(x, qh[s][k], S[s][i]);
                         S[s][i] = mfma16(x, ql[s][k], S[s][i]);
                     }
                 }
         }
 
-        constexpr int G = 2;  // blocks of 16 dims read at once
-        const half8 *vb = buf + kOfK;
+        constexpr int G = W::kAhead ? 2 : 1;  // blocks of 16 dims read at once
+        const half8 *vb = buf + W::kOfV;
         half8 vx[2][2 * G];
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i) vx[0][i] = vb[i * 64 + lane];
@@ -245,9 +276,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
         // all rows see all of the tile
         const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
                            __all(nv == 16);
-        half8 ph[2][2], pl[2][2];
+        half8 ph[SETS][2], pl[SETS][2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < SETS; ++s) {
             float sc = qs[s] * ks;
             if (a.softcap > 0.0f) {
 #pragma unroll
@@ -310,7 +341,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    for (int s = 0; s < SETS; ++s) {
                         const int d = g * G + i;
                         O[s][d] = mfma16(vx[g & 1][2 * i + u], ph[s][u], O[s][d]);
                         if (LO) O[s][d] = mfma16(vx[g & 1][2 * i + u], pl[s][u], O[s][d]);
@@ -323,11 +354,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvV
     const bool whole = w.chunk >= w.tiles;
     float *st = a.ws + (int64_t)blockIdx.x * state_floats<D>(kWideRows);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < SETS; ++s) {
         float sum = l[s];
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        const int rr = 32 * wave + 16 * s + col, r = w.r0 + rr;
+        const int r = wr0 + 16 * s + col, rr = r - w.r0;
         if (r >= w.rows) continue;
         if (whole) {
             const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -393,13 +424,14 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     int row_blocks, splits;
     wide_plan(a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
-    constexpr size_t kLds = 2 * (kTile * D / (FMT == kFmtI8 && D % 64 == 0 ? 16 : 8) + kTile * D / 8) * sizeof(half8);
+    typedef WideShape<D, FMT, LO> W;
+    constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);
     static std::atomic<int> state[64];
     if (kLds > 64 * 1024) {
         const hipError_t e = allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
         if (e != hipSuccess) return e;
     }
-    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, 256, kLds, stream>>>(c, a, row_blocks, splits);
+    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, row_blocks, splits);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
     kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);

@@ -167,8 +167,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
         const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
         const int pos = live ? q.s.pos0 + tq : -1;
         half8 qh[KS], ql[KS];
-        const float kscale = a.scale * load_query<D>(
-            a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qh, ql);
+        float qv[KB];
+        read_query<D>(a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qv);
+        const float kscale = a.scale * split_query<D>(qv, qh, ql);
 
         f32x4 O[DB] = {};
         float M = -INFINITY, l = 0.0f;

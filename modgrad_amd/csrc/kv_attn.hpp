@@ -71,23 +71,27 @@ __device__ __forceinline__ i32x4 mfma16(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
+// A lane's D/4 floats of a query row.
+template <int D>
+__device__ __forceinline__ void read_query(const float *qp, float (&v)[D / 4]) {
+#pragma unroll
+    for (int i = 0; i < D / 4; i += 4) {
+        const f32x4 x = ld_f32x4(qp + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i + e] = x[e];
+    }
+}
+
 // A query row's dims grp*KB .. +KB-1 (KB = D/4) as f16 hi + lo pairs of the row
 // times 2^ex, the largest of the row in [2^13, 2^14): 22 bits of every value
 // that is not 2^-24 of the largest. Lanes l, l^16, l^32, l^48 share a row.
 // Returns 2^-ex.
 template <int D>
-__device__ __forceinline__ float load_query(const float *qp, half8 (&qh)[D / 32], half8 (&ql)[D / 32]) {
+__device__ __forceinline__ float split_query(const float (&v)[D / 4], half8 (&qh)[D / 32], half8 (&ql)[D / 32]) {
     constexpr int KB = D / 4;
-    float v[KB], top = 0.0f;
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KB; i += 4) {
-        const f32x4 x = ld_f32x4(qp + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[i + e] = x[e];
-            top = fmaxf(top, fabsf(x[e]));
-        }
-    }
+    for (int i = 0; i < KB; ++i) top = fmaxf(top, fabsf(v[i]));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     int ex = 0;
@@ -108,19 +112,14 @@ __device__ __forceinline__ float load_query(const float *qp, half8 (&qh)[D / 32]
 // 8-bit K and their sums are exact. Returns the factor's inverse; a row with a
 // NaN or infinity returns NaN.
 template <int D, int N>
-__device__ __forceinline__ float load_query(const float *qp, i32x4 (&qd)[N][D / 64]) {
+__device__ __forceinline__ float split_query(const float (&v)[D / 4], i32x4 (&qd)[N][D / 64]) {
     constexpr int KB = D / 4;
     constexpr float kMost = (float)(N == 2 ? 0x7F7F : 0x7F7F7F);
-    float v[KB], top = 0.0f, bad = 0.0f;
+    float top = 0.0f, bad = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KB; i += 4) {
-        const f32x4 x = ld_f32x4(qp + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[i + e] = x[e];
-            top = fmaxf(top, fabsf(x[e]));
-            bad += x[e] * 0.0f;
-        }
+    for (int i = 0; i < KB; ++i) {
+        top = fmaxf(top, fabsf(v[i]));
+        bad += v[i] * 0.0f;
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -223,6 +222,18 @@ __device__ __forceinline__ float join_row(int n, int rows, int row, Slot slot, f
         }
     }
     return sum == 0.0f ? 0.0f : o / sum;
+}
+
+// 4 neighbouring values of a result row.
+__device__ __forceinline__ void put_out4(const AttnArgs &a, int64_t token, int head_dim0, f32x4 o) {
+    const int64_t to = token * a.out_stride + head_dim0;
+    if (a.out_f16) {
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+        const half4 x = {(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+        *reinterpret_cast<u32x2_a1 *>(static_cast<_Float16 *>(a.out) + to) = __builtin_bit_cast(u32x2, x);
+    } else {
+        *reinterpret_cast<f32x4_a4 *>(static_cast<float *>(a.out) + to) = o;
+    }
 }
 
 __device__ __forceinline__ void put_out(const AttnArgs &a, int64_t token, int head_dim0, float o) {

@@ -87,7 +87,7 @@ struct WideShape {
 
 // LO: the probabilities as hi + lo pairs.
 template <int D, int FMT, bool LO>
-__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
+__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks, int splits, int turn) {
     typedef WideShape<D, FMT, LO> W;
     constexpr bool I8 = W::I8;
     constexpr int SETS = W::SETS, KS = W::KS, DB = W::DB, NK = W::NK, NV = W::NV;
@@ -98,9 +98,12 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
               grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
-    int id = blockIdx.x;
-    const int h = id % c.hkv;
-    id /= c.hkv;
+    // the second work-groups of the CUs are dealt from the shorter end, beside the
+    // longest ones
+    const int h = blockIdx.x % c.hkv;
+    int id = blockIdx.x / c.hkv;
+    if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
+    const int slot = id * c.hkv + h;
     const int sp = id % splits;
     id /= splits;
     const int b = id % c.n_seqs;
@@ -112,7 +115,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     // ---- query rows; those past the last repeat it and are not written
     half8 qh[SETS][I8 ? 1 : KS], ql[SETS][I8 ? 1 : KS];
     i32x4 qd[SETS][ND][I8 ? KS : 1];
-    float qs[SETS];
+    float qs[SETS], qv[SETS][KB];
     int pos[SETS];
     const int wr0 = w.r0 + 16 * SETS * wave;  // the wavefront's first row
 #pragma unroll
@@ -120,9 +123,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         const int r = min(wr0 + 16 * s + col, w.rows - 1);
         const int tq = r / a.group;
         pos[s] = w.s.pos0 + tq;
-        const float *qp = a.q + (int64_t)(w.s.t0 + tq) * a.q_stride + (h * a.group + r % a.group) * D + grp * KB;
-        if constexpr (I8) qs[s] = a.scale * load_query<D, ND>(qp, qd[s]);
-        else qs[s] = a.scale * load_query<D>(qp, qh[s], ql[s]);
+        read_query<D>(a.q + (int64_t)(w.s.t0 + tq) * a.q_stride + (h * a.group + r % a.group) * D + grp * KB, qv[s]);
     }
     const bool live = wr0 < w.rows;
     // positions of the wavefront's first and last row
@@ -204,6 +205,11 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 
     look(t0);
     fetch(t0);
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+        if constexpr (I8) qs[s] = a.scale * split_query<D, ND>(qv[s], qd[s]);
+        else qs[s] = a.scale * split_query<D>(qv[s], qh[s], ql[s]);
+    }
     stage(lds);
     float ks_c = ks_n, vs_c = vs_n;
     int nv_c = nv_n;
@@ -352,7 +358,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     if (!live) return;
 
     const bool whole = w.chunk >= w.tiles;
-    float *st = a.ws + (int64_t)blockIdx.x * state_floats<D>(kWideRows);
+    float *st = a.ws + (int64_t)slot * state_floats<D>(kWideRows);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         float sum = l[s];
@@ -362,15 +368,9 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         if (r >= w.rows) continue;
         if (whole) {
             const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const int64_t to = (int64_t)(w.s.t0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D + 4 * grp;
+            const int hd = (h * a.group + r % a.group) * D + 4 * grp;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float o = O[s][d][e] * f;
-                    if (a.out_f16) static_cast<_Float16 *>(a.out)[to + 16 * d + e] = (_Float16)o;
-                    else static_cast<float *>(a.out)[to + 16 * d + e] = o;
-                }
+            for (int d = 0; d < DB; ++d) put_out4(a, w.s.t0 + r / a.group, hd + 16 * d, O[s][d] * f);
         } else {
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -431,7 +431,9 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
         const hipError_t e = allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
         if (e != hipSuccess) return e;
     }
-    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, row_blocks, splits);
+    const int cus = device_cus();
+    const int turn = cus % c.hkv == 0 && (int64_t)items * splits >= 2 * cus ? cus / c.hkv : 1 << 29;
+    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, row_blocks, splits, turn);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
     kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);

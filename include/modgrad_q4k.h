@@ -415,8 +415,8 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * into the products with 22 bits; with MGQ_OUT_F16 the probabilities may have
  * 11. Scales of V below 2^-90 count as 2^-90.
  * workspace: device memory, 16-byte aligned, of at least
- * mgq_kv_attention_workspace_bytes bytes; its contents need not be set and do
- * not matter afterwards. Calls that may overlap need distinct ones. */
+ * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);
+ * its contents need not be set and do not matter afterwards. Calls that may overlap need distinct ones. */
 size_t mgq_kv_attention_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads, int max_new);
 hipError_t launch_kv_attention_ex(const mgq_kv_cache *cache, const float *q, int64_t q_stride,
                                   int n_q_heads, void *out, int64_t out_stride, int out_type,

@@ -20,9 +20,9 @@ namespace mgq {
 struct AppendGrid {
     int page_blocks;  // most pages of a sequence that the new tokens touch
     int kv_groups;    // work-groups of the K and V part
-    int q_chunk;      // tokens of a work-group of the query part
     int q_blocks;     // work-groups of a sequence in the query part
 };
+constexpr int kQueryUnits = 4;
 
 // The largest of a work-group's values, on every thread.
 template <int NT>
@@ -52,26 +52,40 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
     const int tid = threadIdx.x;
     const int page = 1 << c.page_shift;
     if ((int)blockIdx.x >= gr.kv_groups) {
-        // ---- queries
+        // ---- queries: 4 units a thread, their loads side by side
         const int w = blockIdx.x - gr.kv_groups, b = w / gr.q_blocks;
         const SeqInfo s = kv_seq(c, b);
-        const int first = (w % gr.q_blocks) * gr.q_chunk;
-        const int n = min(s.n - first, gr.q_chunk);
         const int per_token = kUnits * a.hq;
-        for (int i = tid; i < n * per_token; i += NT) {
-            const int t = first + i / per_token, r = i % per_token, h = r / kUnits;
+        const int64_t units = (int64_t)s.n * per_token, first = (int64_t)(w % gr.q_blocks) * (kQueryUnits * NT) + tid;
+        if (first >= units) return;
+        double v[kQueryUnits][U::N];
+#pragma unroll
+        for (int k = 0; k < kQueryUnits; ++k) {
+            const int64_t i = min(first + k * NT, units - 1);
+            const int t = (int)(i / per_token), r = (int)(i % per_token);
             const U u(r % kUnits, rot, half);
-            double v[U::N];
-            const int64_t row = s.t0 + t;
-            u.load(a.q + row * a.q_stride + h * D, v);
+            u.load(a.q + (s.t0 + t) * a.q_stride + (r / kUnits) * D, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kQueryUnits; ++k) {
+            const int64_t i = min(first + k * NT, units - 1);
+            const int t = (int)(i / per_token), r = (int)(i % per_token);
+            const U u(r % kUnits, rot, half);
             const int p = s.pos0 + t;
             if (p >= 0 && p < n_pos) {
-                u.turn(rope + (int64_t)p * rot, half, v);
+                u.turn(rope + (int64_t)p * rot, half, v[k]);
             } else {
 #pragma unroll
-                for (int e = 0; e < U::N; ++e) v[e] = __builtin_nan("");
+                for (int e = 0; e < U::N; ++e) v[k][e] = __builtin_nan("");
             }
-            u.store(a.q_out + row * a.q_out_stride + h * D, v);
+        }
+#pragma unroll
+        for (int k = 0; k < kQueryUnits; ++k) {
+            const int64_t i = first + k * NT;
+            if (i >= units) break;
+            const int t = (int)(i / per_token), r = (int)(i % per_token);
+            const U u(r % kUnits, rot, half);
+            u.store(a.q_out + (s.t0 + t) * a.q_out_stride + (r / kUnits) * D, v[k]);
         }
         return;
     }
@@ -184,8 +198,8 @@ static hipError_t append_run(const KvView &c, const mgq_rope *rope, const KvAppe
     AppendGrid g;
     g.page_blocks = (c.max_new + page - 2) / page + 1;
     g.kv_groups = c.n_seqs * g.page_blocks * 2 * c.hkv;
-    g.q_chunk = std::min(c.max_new, 4);
-    g.q_blocks = a.q ? (c.max_new + g.q_chunk - 1) / g.q_chunk : 0;
+    const int64_t units = (int64_t)c.max_new * a.hq * (D / RopeUnit<VEC>::N);
+    g.q_blocks = a.q ? (int)((units + kQueryUnits * NT - 1) / (kQueryUnits * NT)) : 0;
     const int64_t grid = g.kv_groups + (int64_t)c.n_seqs * g.q_blocks;
     kv_append_kernel<D, FMT, VEC, NT><<<(unsigned)grid, NT, 0, stream>>>(
         c, a, rope ? rope->table : nullptr, rope ? rope->rot_dim : 0, rope && rope->style == MGQ_ROPE_HALF,

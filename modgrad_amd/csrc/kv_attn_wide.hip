@@ -27,7 +27,7 @@
 namespace mgq {
 
 constexpr int kWideRows = 128;
-constexpr int kWideTarget = 512;  // work-groups worth having: two per CU
+constexpr int kWideChunk = 4;  // least tiles of a split: a work-group's start costs about as much
 
 struct WideBlock {
     SeqInfo s;
@@ -44,7 +44,7 @@ __device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, i
     const int hi = min(w.s.len, max(last + 1, 0));
     w.tile0 = lo / kTile;
     w.tiles = max((hi + kTile - 1) / kTile - w.tile0, 1);  // one, for the zeros of rows that see nothing
-    w.chunk = (w.tiles + splits - 1) / splits;
+    w.chunk = max((w.tiles + splits - 1) / splits, splits > 1 ? kWideChunk : 1);
     return true;
 }
 
@@ -403,18 +403,59 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnAr
         put_out(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
 }
 
-// Row blocks at most, and the splits of each that fill the chip.
-static void wide_plan(int group, int hkv, int n_seqs, int max_new, int64_t cap, int &row_blocks, int &splits) {
-    row_blocks = (max_new * group + kWideRows - 1) / kWideRows;
-    const int64_t items = (int64_t)row_blocks * hkv * n_seqs, tiles = (cap + kTile - 1) / kTile;
-    splits = 1;
-    if (items < kWideTarget)
-        splits = (int)std::max<int64_t>(1, std::min<int64_t>((kWideTarget + items - 1) / items, (tiles + 1) / 2));
+// The same for few splits: D/4 lanes a row, 32 rows a work-group.
+constexpr int kJoinFew = 16;
+template <int D>
+__global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
+    constexpr int L = D / 4, PER = 256 / L, STEPS = kWideRows / 32;
+    int id = blockIdx.x;
+    const int part = id % STEPS;
+    id /= STEPS;
+    const int h = id % c.hkv;
+    id /= c.hkv;
+    const int b = id % c.n_seqs, inv = id / c.n_seqs;
+    WideBlock w;
+    if (!wide_block(c, a, b, row_blocks - 1 - inv, splits, w)) return;
+    if (w.chunk >= w.tiles) return;
+    const int n = (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
+    if ((int)threadIdx.x >= PER * L) return;
+    const float *base = a.ws + (int64_t)((inv * c.n_seqs + b) * splits * c.hkv + h) * state_floats<D>(kWideRows);
+    const int64_t step = (int64_t)c.hkv * state_floats<D>(kWideRows);
+    for (int rr = 32 * part + threadIdx.x / L; rr < 32 * part + 32; rr += PER) {
+        const int r = w.r0 + rr;
+        if (r >= w.rows) break;
+        float M = -INFINITY, l = 0.0f;
+        for (int i = 0; i < n; ++i) M = fmaxf(M, base[i * step + kWideRows * D + 2 * rr]);
+        f32x4 o = {};
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float2 ml = *reinterpret_cast<const float2 *>(base + i * step + kWideRows * D + 2 * rr);
+            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+            l += f * ml.y;
+            o += f * *reinterpret_cast<const f32x4 *>(base + i * step + rr * D + d);
+        }
+        put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    }
 }
 
+// Row blocks at most, and the splits of each that fill the chip once: with
+// n_tokens rows in all, about half of each sequence's last block is there. The
+// grid, which covers what max_new allows, stays within twice that.
+static void wide_plan(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, int &row_blocks,
+                      int &splits) {
+    row_blocks = (max_new * group + kWideRows - 1) / kWideRows;
+    const int64_t slots = dim == 256 ? 256 : 512, items = (int64_t)row_blocks * n_seqs;
+    const int64_t there = std::min(
+        items, ((int64_t)n_tokens * group + (int64_t)n_seqs * (kWideRows / 2) + kWideRows - 1) / kWideRows);
+    const int64_t tiles = (cap + kTile - 1) / kTile;
+    splits = (int)std::max<int64_t>(1, std::min({slots / (there * hkv), 2 * slots / (items * hkv),
+                                                 (tiles + kWideChunk - 1) / kWideChunk}));
+}
+
+// Enough for any n_tokens: fewer rows have more splits, and max_new are the fewest.
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap) {
     int row_blocks, splits;
-    wide_plan(group, hkv, n_seqs, max_new, cap, row_blocks, splits);
+    wide_plan(dim, group, hkv, n_seqs, max_new, max_new, cap, row_blocks, splits);
     if (splits == 1) return 0;
     return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
 }
@@ -422,7 +463,7 @@ size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_n
 template <int D, int FMT, bool LO>
 static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     int row_blocks, splits;
-    wide_plan(a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
+    wide_plan(D, a.group, c.hkv, c.n_seqs, c.n_tokens, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
     typedef WideShape<D, FMT, LO> W;
     constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);
@@ -436,7 +477,10 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, row_blocks, splits, turn);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);
+    if (splits <= kJoinFew)
+        kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 32), 256, 0, stream>>>(c, a, row_blocks, splits);
+    else
+        kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);
     return hipGetLastError();
 }
 

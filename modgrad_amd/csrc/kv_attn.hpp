@@ -53,18 +53,21 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
 __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
 
-// cap * log2 e * tanh(x): a polynomial where the exponential's form would cancel
-// (|x| < 0.35, good to 2^-22 there).
-__device__ __forceinline__ float softcap_log2(float x, float cap_log2e) {
-    const float e = __builtin_amdgcn_exp2f(x * 2.8853900817779268f);  // exp(2x)
-    const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+// tanh(x) for |x| < kCapNear, good to 2^-22: its series.
+constexpr float kCapNear = 0.35f;
+__device__ __forceinline__ float tanh_near(float x) {
     const float y = x * x;
     float p = fmaf(y, -0.008863235529902197f, 0.021869488536155203f);
     p = fmaf(y, p, -0.05396825396825397f);
     p = fmaf(y, p, 0.13333333333333333f);
     p = fmaf(y, p, -0.3333333333333333f);
-    const float small = fmaf(x * y, p, x);
-    return cap_log2e * (fabsf(x) < 0.35f ? small : big);
+    return fmaf(x * y, p, x);
+}
+// cap * log2 e * tanh(x): the series where the exponential's form would cancel.
+__device__ __forceinline__ float softcap_log2(float x, float cap_log2e) {
+    const float e = __builtin_amdgcn_exp2f(x * 2.8853900817779268f);  // exp(2x)
+    const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+    return cap_log2e * (fabsf(x) < kCapNear ? tanh_near(x) : big);
 }
 
 __device__ __forceinline__ i32x4 mfma16(i32x4 a, i32x4 b, i32x4 c) {

@@ -27,6 +27,7 @@
 namespace mgq {
 
 constexpr int kWideRows = 128;
+__host__ __device__ constexpr int wide_slots(int dim) { return dim == 256 ? 256 : 512; }  // resident work-groups
 constexpr int kWideChunk = 4;  // least tiles of a split: a work-group's start costs about as much
 
 struct WideBlock {
@@ -46,6 +47,68 @@ __device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, i
     w.tiles = max((hi + kTile - 1) / kTile - w.tile0, 1);  // one, for the zeros of rows that see nothing
     w.chunk = max((w.tiles + splits - 1) / splits, splits > 1 ? kWideChunk : 1);
     return true;
+}
+
+// Row block `at` of those that are there (sequence by sequence, each from its
+// last, longest one), found by every wavefront for itself; and the splits of
+// every block: as many as fill the chip's slots once, which only the device
+// knows. Work-groups without a block have the last numbers: the dispatcher
+// deals numbers to the shader engines in turn and waits for the one whose turn
+// it is, so empty numbers among the others leave engines idle.
+struct WidePlace {
+    int b, rt;      // rt < 0: none
+    int split, splits;
+    int64_t state;  // number of the block's state, the kv head aside
+    int total;      // row blocks
+};
+template <int D>
+__device__ __forceinline__ WidePlace wide_place(const KvView &c, const AttnArgs &a, int id, int most_splits) {
+    const int lane = threadIdx.x & 63;
+    const auto blocks = [&](int b) { return b < c.n_seqs ? (kv_seq(c, b).n * a.group + kWideRows - 1) / kWideRows : 0; };
+    WidePlace p = {0, -1, 0, 1, 0, 0};
+    if (c.n_seqs == 1) {
+        p.total = blocks(0);
+        p.splits = most_splits;  // made for all its blocks
+        p.split = id / max(1, p.total);
+        if (p.split >= p.splits) return p;
+        p.state = id - p.split * p.total;
+        p.rt = p.total - 1 - (int)p.state;
+        return p;
+    }
+    int n = blocks(lane);
+    if (most_splits > 1) {
+        int sum = n;
+        for (int b = lane + 64; b < c.n_seqs; b += 64) sum += blocks(b);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        p.total = __builtin_amdgcn_readfirstlane(sum);
+        p.splits = max(1, min(most_splits, wide_slots(D) / max(1, p.total * c.hkv)));
+        p.split = id / max(1, p.total);
+        if (p.split >= p.splits) return p;
+        id -= p.split * p.total;
+        p.state = id;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < c.n_seqs; b0 += 64) {
+        if (b0 > 0) n = blocks(b0 + lane);
+        int s = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(s, o, 64);
+            if (lane >= o) s += t;
+        }
+        const uint64_t past = __ballot(before + s > id);  // lanes whose blocks reach beyond id
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            p.b = b0 + l;
+            p.rt = before + __shfl(s, l, 64) - 1 - id;
+            p.b = __builtin_amdgcn_readfirstlane(p.b);
+            p.rt = __builtin_amdgcn_readfirstlane(p.rt);
+            return p;
+        }
+        before += __builtin_amdgcn_readlane(s, 63);
+    }
+    return p;
 }
 
 __device__ __forceinline__ void wide_barrier() {
@@ -74,9 +137,9 @@ __device__ __forceinline__ float max_groups(float x) {
 template <int D, int FMT, bool LO>
 struct WideShape {
     static constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
-    static constexpr int SETS = D == 256 ? 1 : 2;
+    static constexpr int SETS = D == 256 || (D == 128 && LO) ? 1 : 2;
     static constexpr int NW = kWideRows / (16 * SETS);      // wavefronts
-    static constexpr int kThreads = 64 * NW, kPerSimd = (D == 256 ? 1 : 2) * NW / 4;
+    static constexpr int kThreads = 64 * NW, kPerSimd = 2;
     static constexpr bool kAhead = kPerSimd <= 2;           // registers for operands ahead of their use
     static constexpr int KS = I8 ? D / 64 : D / 32;         // summed steps of S
     static constexpr int DB = D / 16;                       // blocks of 16 dims of O
@@ -87,7 +150,7 @@ struct WideShape {
 
 // LO: the probabilities as hi + lo pairs.
 template <int D, int FMT, bool LO>
-__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int row_blocks, int splits, int turn) {
+__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int most_splits, int turn) {
     typedef WideShape<D, FMT, LO> W;
     constexpr bool I8 = W::I8;
     constexpr int SETS = W::SETS, KS = W::KS, DB = W::DB, NK = W::NK, NV = W::NV;
@@ -103,12 +166,11 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     const int h = blockIdx.x % c.hkv;
     int id = blockIdx.x / c.hkv;
     if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
-    const int slot = id * c.hkv + h;
-    const int sp = id % splits;
-    id /= splits;
-    const int b = id % c.n_seqs;
+    const WidePlace place = wide_place<D>(c, a, id, most_splits);
+    if (place.rt < 0) return;
+    const int b = place.b, sp = place.split;
     WideBlock w;
-    if (!wide_block(c, a, b, row_blocks - 1 - id / c.n_seqs, splits, w)) return;
+    if (!wide_block(c, a, b, place.rt, place.splits, w)) return;
     const int t0 = sp * w.chunk, t1 = min(w.tiles, t0 + w.chunk);
     if (t0 >= t1) return;
 
@@ -287,11 +349,32 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         for (int s = 0; s < SETS; ++s) {
             float sc = qs[s] * ks;
             if (a.softcap > 0.0f) {
+                float far = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = softcap_log2(S[s][i][e] * sc, a.softcap);
+                    for (int e = 0; e < 4; ++e) {
+                        S[s][i][e] *= sc;
+                        far = fmaxf(far, fabsf(S[s][i][e]));
+                    }
+                if (!__any(far >= kCapNear)) {  // scores are rarely beyond a third of their bound
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) S[s][i][e] = a.softcap * tanh_near(S[s][i][e]);
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = i == 0 ? S[s][0][e] : i == 1 ? S[s][1][e] : i == 2 ? S[s][2][e] : S[s][3][e];
+                            const float y = softcap_log2(x, a.softcap);
+                            S[s][0][e] = i == 0 ? y : S[s][0][e];
+                            S[s][1][e] = i == 1 ? y : S[s][1][e];
+                            S[s][2][e] = i == 2 ? y : S[s][2][e];
+                            S[s][3][e] = i == 3 ? y : S[s][3][e];
+                        }
+                }
                 sc = 1.0f;
             }
             if (!clear) {
@@ -358,7 +441,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     if (!live) return;
 
     const bool whole = w.chunk >= w.tiles;
-    float *st = a.ws + (int64_t)slot * state_floats<D>(kWideRows);
+    float *st = a.ws + ((place.split * (int64_t)place.total + place.state) * c.hkv + h) * state_floats<D>(kWideRows);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         float sum = l[s];
@@ -382,46 +465,48 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 
 // Joins a split row block: one work-group per (row block, sequence, kv head, row).
 template <int D>
-__global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
+__global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnArgs a, int most_splits) {
     __shared__ float f[kMostStates], red[8 + 256];
     int id = blockIdx.x;
     const int rr = id % kWideRows;
     id /= kWideRows;
     const int h = id % c.hkv;
     id /= c.hkv;
-    const int b = id % c.n_seqs, inv = id / c.n_seqs;
+    const WidePlace place = wide_place<D>(c, a, id, most_splits);
+    if (place.rt < 0 || place.split > 0) return;
     WideBlock w;
-    if (!wide_block(c, a, b, row_blocks - 1 - inv, splits, w)) return;
+    if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
     const int r = w.r0 + rr;
     if (r >= w.rows || w.chunk >= w.tiles) return;
     const int n = (w.tiles + w.chunk - 1) / w.chunk;
     const auto slot = [&](int i) {
-        return a.ws + (int64_t)(((inv * c.n_seqs + b) * splits + i) * c.hkv + h) * state_floats<D>(kWideRows);
+        return a.ws + ((i * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows);
     };
     const float o = join_row<D>(n, kWideRows, rr, slot, f, red);
     if ((int)threadIdx.x < D)
         put_out(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
 }
 
-// The same for few splits: D/4 lanes a row, 32 rows a work-group.
+// The same for few splits: D/4 lanes a row.
 constexpr int kJoinFew = 16;
 template <int D>
-__global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, AttnArgs a, int row_blocks, int splits) {
-    constexpr int L = D / 4, PER = 256 / L, STEPS = kWideRows / 32;
+__global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, AttnArgs a, int most_splits) {
+    constexpr int L = D / 4, PER = 256 / L, R = 8, STEPS = kWideRows / R;  // R rows a work-group
     int id = blockIdx.x;
     const int part = id % STEPS;
     id /= STEPS;
     const int h = id % c.hkv;
     id /= c.hkv;
-    const int b = id % c.n_seqs, inv = id / c.n_seqs;
+    const WidePlace place = wide_place<D>(c, a, id, most_splits);
+    if (place.rt < 0 || place.split > 0) return;
     WideBlock w;
-    if (!wide_block(c, a, b, row_blocks - 1 - inv, splits, w)) return;
+    if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
     if (w.chunk >= w.tiles) return;
     const int n = (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
     if ((int)threadIdx.x >= PER * L) return;
-    const float *base = a.ws + (int64_t)((inv * c.n_seqs + b) * splits * c.hkv + h) * state_floats<D>(kWideRows);
-    const int64_t step = (int64_t)c.hkv * state_floats<D>(kWideRows);
-    for (int rr = 32 * part + threadIdx.x / L; rr < 32 * part + 32; rr += PER) {
+    const float *base = a.ws + ((int64_t)id * c.hkv + h) * state_floats<D>(kWideRows);
+    const int64_t step = (int64_t)place.total * c.hkv * state_floats<D>(kWideRows);
+    for (int rr = R * part + threadIdx.x / L; rr < R * part + R; rr += PER) {
         const int r = w.r0 + rr;
         if (r >= w.rows) break;
         float M = -INFINITY, l = 0.0f;
@@ -438,24 +523,18 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
     }
 }
 
-// Row blocks at most, and the splits of each that fill the chip once: with
-// n_tokens rows in all, about half of each sequence's last block is there. The
-// grid, which covers what max_new allows, stays within twice that.
-static void wide_plan(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, int &row_blocks,
-                      int &splits) {
+// Row blocks of a sequence and splits of a block, both at most: the grid stays
+// within twice the slots, or has no splits.
+static void wide_plan(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, int &row_blocks, int &splits) {
     row_blocks = (max_new * group + kWideRows - 1) / kWideRows;
-    const int64_t slots = dim == 256 ? 256 : 512, items = (int64_t)row_blocks * n_seqs;
-    const int64_t there = std::min(
-        items, ((int64_t)n_tokens * group + (int64_t)n_seqs * (kWideRows / 2) + kWideRows - 1) / kWideRows);
-    const int64_t tiles = (cap + kTile - 1) / kTile;
-    splits = (int)std::max<int64_t>(1, std::min({slots / (there * hkv), 2 * slots / (items * hkv),
-                                                 (tiles + kWideChunk - 1) / kWideChunk}));
+    const int64_t items = (int64_t)row_blocks * n_seqs * hkv, tiles = (cap + kTile - 1) / kTile;
+    splits = (int)std::max<int64_t>(1, std::min(2 * wide_slots(dim) / items, (tiles + kWideChunk - 1) / kWideChunk));
+    splits = std::min(splits, std::max(1, wide_slots(dim) / (row_blocks * hkv)));  // one sequence has all its blocks
 }
 
-// Enough for any n_tokens: fewer rows have more splits, and max_new are the fewest.
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap) {
     int row_blocks, splits;
-    wide_plan(dim, group, hkv, n_seqs, max_new, max_new, cap, row_blocks, splits);
+    wide_plan(dim, group, hkv, n_seqs, max_new, cap, row_blocks, splits);
     if (splits == 1) return 0;
     return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
 }
@@ -463,7 +542,7 @@ size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_n
 template <int D, int FMT, bool LO>
 static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     int row_blocks, splits;
-    wide_plan(D, a.group, c.hkv, c.n_seqs, c.n_tokens, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
+    wide_plan(D, a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
     typedef WideShape<D, FMT, LO> W;
     constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);
@@ -473,14 +552,14 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
         if (e != hipSuccess) return e;
     }
     const int cus = device_cus();
-    const int turn = cus % c.hkv == 0 && (int64_t)items * splits >= 2 * cus ? cus / c.hkv : 1 << 29;
-    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, row_blocks, splits, turn);
+    const int turn = c.n_seqs == 1 && splits == 1 && cus % c.hkv == 0 && (int)items >= 2 * cus ? cus / c.hkv : 1 << 29;
+    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
     if (splits <= kJoinFew)
-        kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 32), 256, 0, stream>>>(c, a, row_blocks, splits);
+        kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
     else
-        kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, row_blocks, splits);
+        kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, splits);
     return hipGetLastError();
 }
 

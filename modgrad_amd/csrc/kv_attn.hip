@@ -28,19 +28,29 @@
 // its f16 hi + lo pair keeps 22 bits down to 2^-24 of the largest. M, l and O
 // are f32.
 //
+// int8 K skips the conversion: q goes in as three digits of 8 bits on the int8
+// matrix cores (v_mfma_i32_16x16x64_i8), whose sums are exact.
+//
+// Loads. K's registers are free for the next tile after S, V's after O, and the
+// page ids are a tile ahead of both: 64 tokens' 16 KiB (D = 128) are on their way
+// for each wavefront while it computes.
+//
 // Split. All (sequence, kv head, 16 query rows) rows of tiles laid end to end
 // are cut into equal runs, one for each work-group, so ragged batches and one
-// long sequence balance alike. The 4 wavefronts of a work-group take tiles in
+// long sequence balance alike. The wavefronts of a work-group take tiles in
 // turn, each with its own softmax state, joined through LDS at the end of a
 // row; a row that a cut goes through leaves partial states in the workspace,
-// which kv_attn_join_kernel joins.
+// which kv_attn_join_kernel joins. Short sequences (no row over kSoloTiles) are
+// not cut: a work-group takes whole rows.
 #include "kv_attn.hpp"
 
 namespace mgq {
 
-constexpr int kRows = 16;       // query rows of a work-group's row of tiles
-constexpr int kAttnGroups = 512;  // work-groups: two per CU
-constexpr int kMinTiles = 4;    // least tiles of a run: one for each wavefront
+constexpr int kRows = 16;         // query rows of a work-group's row of tiles
+constexpr int kAttnGroups = 512;  // work-groups: two of 4 wavefronts per CU
+constexpr int NW = 4;             // wavefronts of a work-group
+// Rows of up to 256 tokens are not cut: the wavefronts have a tile each.
+constexpr int kSoloTiles = NW;
 
 // A row's tiles: rows of (sequence, kv head, row block), kv head and row block
 // within the sequence.
@@ -60,12 +70,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const KvView &c, const AttnArgs &a, 
     r.blocks = (r.s.n * a.group + kRows - 1) / kRows;
     return r;
 }
-__device__ __forceinline__ int attn_units(const KvView &c, const AttnArgs &a, int b) {
-    const AttnSeq r = attn_seq(c, a, b);
-    return r.tiles * r.blocks * c.hkv;
-}
-
-// Sum of v over the work-group (256 threads) and the sum over lower threads.
+// Sum of v over the work-group (NW wavefronts) and the sum over lower threads.
 __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int s = v;
@@ -78,7 +83,7 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
     __syncthreads();
     int before = 0;
     total = 0;
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < NW; ++k) {
         if (k < w) before += part[k];
         total += part[k];
     }
@@ -86,34 +91,62 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
     return before + s - v;
 }
 
-// All units, and where unit `at(total)` lies: its sequence and that one's first
-// unit. One pass over the sequences where they are no more than the threads.
+// The cut: all units, the units of a run, and where this work-group's run lies:
+// its first unit, that one's sequence and the sequence's first unit. With no row
+// over kSoloTiles a unit is a whole row, else a tile. One pass over the
+// sequences where they are no more than the threads.
 struct AttnPlace {
-    int total, b, base;
+    int total, run, at, b, base;
+    bool solo;
+    AttnSeq q;  // the sequence
 };
-template <class At>
-__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int *part, int *found, At at) {
-    AttnPlace p = {0, 0, 0};
+__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int *part, int *found) {
+    constexpr int NT = 64 * NW;
+    AttnPlace p = {0, 0, 0, 0, 0, true, {}};
+    const auto cut = [&](int total) {
+        p.total = total;
+        p.run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+        if (!p.solo) p.run = max(p.run, NW);  // a tile for each wavefront
+        p.at = (int)blockIdx.x * p.run;
+    };
     if (c.n_seqs == 1) {
-        p.total = attn_units(c, a, 0);
+        p.q = attn_seq(c, a, 0);
+        p.solo = p.q.tiles <= kSoloTiles;
+        cut(p.q.blocks * c.hkv * (p.solo ? 1 : p.q.tiles));
         return p;
     }
-    if (c.n_seqs > 256)
-        for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
-            int t;
-            group_scan(b0 + (int)threadIdx.x < c.n_seqs ? attn_units(c, a, b0 + threadIdx.x) : 0, part, t);
-            p.total += t;
+    int rows = 0, tiles = 0, sum_rows = 0, sum_tiles = 0, long_ = 0;
+    for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
+        rows = tiles = 0;
+        if (b0 + (int)threadIdx.x < c.n_seqs) {
+            const AttnSeq q = attn_seq(c, a, b0 + threadIdx.x);
+            rows = q.blocks * c.hkv;
+            tiles = rows * q.tiles;
+            if (rows > 0 && q.tiles > kSoloTiles) long_ = 1;
         }
+        sum_rows += rows;
+        sum_tiles += tiles;
+    }
+    p.solo = __syncthreads_or(long_) == 0;
+    int total;
+    group_scan(p.solo ? sum_rows : sum_tiles, part, total);
+    cut(total);
     int before = 0;
-    for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
+    for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
         const int i = b0 + threadIdx.x;
-        const int u = i < c.n_seqs ? attn_units(c, a, i) : 0;
+        if (c.n_seqs > NT) {
+            rows = tiles = 0;
+            if (i < c.n_seqs) {
+                const AttnSeq q = attn_seq(c, a, i);
+                rows = q.blocks * c.hkv;
+                tiles = rows * q.tiles;
+            }
+        }
+        const int u = p.solo ? rows : tiles;
         int t;
         const int start = before + group_scan(u, part, t);
         before += t;
-        if (c.n_seqs <= 256) p.total = t;
-        const int x = at(p.total);
-        if (x >= start && x < start + u) {
+        if (p.at >= start && p.at < start + u) {
             found[0] = i;
             found[1] = start;
         }
@@ -121,143 +154,198 @@ __device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs 
     __syncthreads();
     p.b = found[0];
     p.base = found[1];
+    if (p.at < p.total) p.q = attn_seq(c, a, p.b);
     return p;
 }
-__device__ __forceinline__ int attn_run(int total, int groups) {
-    return max((total + groups - 1) / groups, kMinTiles);
+
+// Workspace: run w's states, slot 0 for a row begun by an earlier run, slot 1
+// for one that this run begins; then for every row the first and last run of it,
+// written by the first.
+template <int D>
+__device__ __forceinline__ int2 *row_runs(const AttnArgs &a) {
+    return reinterpret_cast<int2 *>(a.ws + (int64_t)kAttnGroups * 2 * state_floats<D>(kRows));
 }
 
-// Workspace of run w: slot 0 for a row begun by an earlier run, slot 1 for one
-// that this run begins.
 template <int D, int FMT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a) {
-    constexpr int KB = D / 4;    // bytes of a token that a lane group has
-    constexpr int KS = D / 32;   // summed steps of S
-    constexpr int DB = D / 16;   // blocks of 16 dims of O
-    constexpr int OP = D + 4;    // LDS row of O
-    __shared__ float sO[4 * kRows * OP];
-    __shared__ float sM[4][kRows], sL[4][kRows];
-    __shared__ int part[4], found[2];
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a, int max_blocks) {
+    constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
+    constexpr int KB = D / 4;               // bytes of a token that a lane group has
+    constexpr int KS = I8 ? D / 64 : D / 32;  // summed steps of S
+    constexpr int DB = D / 16;              // blocks of 16 dims of O
+    constexpr int OP = D + 4;               // LDS row of O
+    constexpr int NT = 64 * NW;
+    __shared__ float sO[NW * kRows * OP];
+    __shared__ float sM[NW][kRows], sL[NW][kRows];
+    __shared__ int part[NW], found[2];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
-    const AttnPlace place = attn_place(
-        c, a, part, found, [&](int total) { return (int)blockIdx.x * attn_run(total, gridDim.x); });
-    const int run = attn_run(place.total, gridDim.x);
-    int at = blockIdx.x * run;
-    const int stop = min(at + run, place.total);
+    const AttnPlace place = attn_place(c, a, part, found);
+    int at = place.at;
+    const int stop = min(at + place.run, place.total);
     if (at >= stop) return;
     int b = place.b, base = place.base;
-    AttnSeq q = attn_seq(c, a, b);
+    AttnSeq q = place.q;
 
     while (at < stop) {
-        while (at - base >= q.tiles * q.blocks * c.hkv) {  // the next sequence with rows
-            base += q.tiles * q.blocks * c.hkv;
+        const auto units = [&] { return q.blocks * c.hkv * (place.solo ? 1 : q.tiles); };
+        while (at - base >= units()) {  // the next sequence with rows
+            base += units();
             q = attn_seq(c, a, ++b);
         }
-        const int row = (at - base) / q.tiles, t0 = (at - base) % q.tiles;
-        const int t1 = min(q.tiles, t0 + stop - at);
-        at += t1 - t0;
-        const int h = row % c.hkv, r0 = (row / c.hkv) * kRows;  // kv head, first query row of the block
+        int row = at - base, t0 = 0, t1 = q.tiles;
+        if (place.solo) {
+            ++at;
+        } else {
+            t0 = row % q.tiles;
+            row /= q.tiles;
+            t1 = min(q.tiles, t0 + stop - at);
+            at += t1 - t0;
+        }
+        const int h = row % c.hkv, blk = row / c.hkv, r0 = blk * kRows;  // kv head, row block, its first query row
         const int rows = q.s.n * a.group;
 
-        // ---- this lane's query row, as hi + lo halves of a normalized row
+        // ---- this lane's query row
         const int r = r0 + col;
         const bool live = r < rows;
         const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
         const int pos = live ? q.s.pos0 + tq : -1;
-        half8 qh[KS], ql[KS];
-        float qv[KB];
-        read_query<D>(a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qv);
-        const float kscale = a.scale * split_query<D>(qv, qh, ql);
-
-        f32x4 O[DB] = {};
-        float M = -INFINITY, l = 0.0f;
-
+        // ---- loads
         const int tile_end = q.tile0 + t1;
         const int kgrp = col >> 2;  // the 16 tokens that this lane's K rows are of
         u32x4 vreg[DB];
-        uint32_t kreg[4][KB / 4];
-        float ksv, vsv;
-        int nv;  // of this lane group's 16 tokens, those that exist
+        u32x4 kreg[4][(KB + 15) / 16];
+        float ks_n = 0.0f, vs_n = 1.0f;
+        int nv_n = 0;         // of this lane group's 16 tokens, those that exist
+        int ik = -1, iv = -1;  // page ids of the next tile to load
         const int *tab = c.table + (int64_t)b * c.max_pages;
-        const auto fetch = [&](int tile) {
-            // a page that the table does not name, or past the length, is read
-            // as page 0 and counts as no tokens
+        const auto look = [&](int tile) {
             const int pk = tile * kTile + 16 * kgrp, pv = tile * kTile + 16 * grp;
-            int ik = pk < q.s.len ? tab[pk >> c.page_shift] : -1;
-            int iv = pv < q.s.len ? tab[pv >> c.page_shift] : -1;
-            const bool okv = iv >= 0 && iv < c.n_pages;
-            if (ik < 0 || ik >= c.n_pages) ik = 0;
-            if (!okv) iv = 0;
-            nv = okv ? min(q.s.len - pv, 16) : 0;
-            ksv = c.ks[(int64_t)iv * c.hkv + h];
-            vsv = c.vs[(int64_t)iv * c.hkv + h];
-            const uint8_t *kp = c.k + ik * c.page_stride + ((int64_t)h * page + (pk & (page - 1)) + (col & 3)) * D + grp * KB;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < KB / 8; ++i) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * t * D + 8 * i);
-                    kreg[t][2 * i] = x[0];
-                    kreg[t][2 * i + 1] = x[1];
-                }
-            const uint8_t *vp = c.v + iv * c.page_stride + ((int64_t)h * D + col) * page + (pv & (page - 1));
-#pragma unroll
-            for (int d = 0; d < DB; ++d) vreg[d] = *reinterpret_cast<const u32x4 *>(vp + (int64_t)16 * d * page);
+            ik = pk < q.s.len ? tab[pk >> c.page_shift] : -1;
+            iv = pv < q.s.len ? tab[pv >> c.page_shift] : -1;
         };
+        // a page that the table does not name, or past the length, is read as
+        // page 0 and counts as no tokens; its scales may be anything
+        const auto load_k = [&](int tile) {
+            const int p = tile * kTile + 16 * kgrp, id = ik < 0 || ik >= c.n_pages ? 0 : ik;
+            const uint8_t *kp = c.k + id * c.page_stride + ((int64_t)h * page + (p & (page - 1)) + (col & 3)) * D + grp * KB;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if constexpr (KB % 16 == 0) {
+#pragma unroll
+                    for (int i = 0; i < KB / 16; ++i)
+                        kreg[t][i] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * D + 16 * i);
+                } else {  // 24 bytes at a multiple of 8
+#pragma unroll
+                    for (int i = 0; i < KB / 8; ++i) {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * t * D + 8 * i);
+                        kreg[t][i / 2][2 * (i % 2)] = x[0];
+                        kreg[t][i / 2][2 * (i % 2) + 1] = x[1];
+                    }
+                }
+            }
+        };
+        const auto load_v = [&](int tile) {
+            const int p = tile * kTile + 16 * grp;
+            const bool ok = iv >= 0 && iv < c.n_pages;
+            const int id = ok ? iv : 0;
+            nv_n = ok ? min(q.s.len - p, 16) : 0;
+            ks_n = ok ? c.ks[(int64_t)id * c.hkv + h] : 0.0f;
+            vs_n = ok ? c.vs[(int64_t)id * c.hkv + h] : 1.0f;
+            const uint8_t *vp = c.v + id * c.page_stride + ((int64_t)h * D + col) * page + (p & (page - 1));
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vreg[d] = *reinterpret_cast<const u32x4 *>(vp + 16 * d * page);
+        };
+        int tile = q.tile0 + t0 + wave;
+        // loads come back in order: the page ids first, which the others wait for
+        look(tile);
+        __builtin_amdgcn_sched_barrier(0);
+        float qv[KB];
+        read_query<D>(a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qv);
+        if (tile < tile_end) {
+            load_k(tile);
+            load_v(tile);
+            look(tile + NW);
+        }
 
-        for (int tile = q.tile0 + t0 + wave; tile < tile_end; tile += 4) {
-            fetch(tile);
+        half8 qh[I8 ? 1 : KS], ql[I8 ? 1 : KS];
+        i32x4 qd[3][I8 ? KS : 1];
+#pragma unroll
+        for (int i = 0; i < KB; ++i) qv[i] = live ? qv[i] : 0.0f;
+        float kscale = a.scale;
+        if constexpr (I8) kscale *= split_query<D, 3>(qv, qd);
+        else kscale *= split_query<D>(qv, qh, ql);
+
+        f32x4 O[DB] = {};
+        float M = -INFINITY, l = 0.0f;
+        for (; tile < tile_end; tile += NW) {
+            const float ks = kscale * ks_n, vs = fmaxf(vs_n, kLeastScale);
+            const int nv = nv_n;
             f32x4 S[4] = {};
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t) {
+                if constexpr (I8) {
+                    i32x4 d[3] = {};
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const half8 x = kv_half8<FMT>(kreg[t][2 * k], kreg[t][2 * k + 1]);
-                    S[t] = mfma16(x, qh[k], S[t]);
-                    S[t] = mfma16(x, ql[k], S[t]);
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int n = 0; n < 3; ++n)
+                            d[n] = mfma16(__builtin_bit_cast(i32x4, kreg[t][k]), qd[n][k], d[n]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        S[t][e] = fmaf((float)(d[2][e] * 256 + d[1][e]), 256.0f, (float)d[0][e]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const half8 x = kv_half8<FMT>(kreg[t][k / 2][2 * (k % 2)], kreg[t][k / 2][2 * (k % 2) + 1]);
+                        S[t] = mfma16(x, qh[k], S[t]);
+                        S[t] = mfma16(x, ql[k], S[t]);
+                    }
                 }
-            // a page of zeros has scale 0: its tokens still count in l
-            const float vs = fmaxf(vsv, kLeastScale);
-            const float lv = __log2f(vs), ks = kscale * ksv;
+            }
+            const bool more = tile + NW < tile_end;
+            if (more) load_k(tile + NW);
+
+            const float lv = __log2f(vs);
             const int first = tile * kTile + 16 * grp;
             const int see = min(pos + 1 - first, nv);  // tokens of the 16 up to the row's own
             const int skip = a.window > 0 ? pos - a.window + 1 - first : 0;
-            float top = M;
+            float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float s = S[t][i] * ks;
                     if (a.softcap > 0.0f) s = softcap_log2(s, a.softcap);
-                    s += lv;
                     const int e = 4 * t + i;
-                    s = (e < see && e >= skip) ? s : -INFINITY;
+                    s = e < see && e >= skip ? s + lv : -INFINITY;
                     S[t][i] = s;
                     top = fmaxf(top, s);
                 }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float ref = top == -INFINITY ? 0.0f : top - kTop;
-            const float fac = M == -INFINITY ? 0.0f : exp2f(M - top);
-            M = top;
+            top = max_groups(top);
+            if (__any(top > M + 1.0f)) {  // the maximum may lag by 1: w stays below 2^15
+                const float m = fmaxf(M, top);
+                const float fac = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
+                M = m;
+                l *= fac;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) O[d] *= fac;
+            }
+            const float ref = M == -INFINITY ? 0.0f : M - kTop;
             float sum = 0.0f;
             half8 ph[2], pl[2];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float w = exp2f(S[t][i] - ref);
+                    const float w = __builtin_amdgcn_exp2f(S[t][i] - ref);
                     sum += w;
                     const _Float16 hi = (_Float16)w;
                     ph[t / 2][4 * (t % 2) + i] = hi;
                     pl[t / 2][4 * (t % 2) + i] = (_Float16)(w - (float)hi);
                 }
-            l = l * fac + sum / vs;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) O[d] *= fac;
-            if (nv < 16) {
+            l += sum * __builtin_amdgcn_rcpf(vs);
+            if (__any(nv < 16)) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -275,39 +363,56 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
                     O[d] = mfma16(x, ph[u], O[d]);
                     O[d] = mfma16(x, pl[u], O[d]);
                 }
+            if (more) {
+                load_v(tile + NW);
+                look(tile + 2 * NW);
+            }
         }
 
-        // ---- the 4 wavefronts' states into one
+        // ---- the wavefronts' states into one
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        __syncthreads();
         if (grp == 0) sM[wave][col] = M;
         __syncthreads();
-        const float all = fmaxf(fmaxf(sM[0][col], sM[1][col]), fmaxf(sM[2][col], sM[3][col]));
-        const float fac = M == -INFINITY ? 0.0f : exp2f(M - all);
-        if (grp == 0) sL[wave][col] = l * fac;
+        float all = sM[0][col];
 #pragma unroll
-        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;
+        for (int w = 1; w < NW; ++w) all = fmaxf(all, sM[w][col]);
+        const float fac = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - all);
+        if (grp == 0) sL[wave][col] = l * fac;
+        if (live) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;
+        }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == q.tiles;
         float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * state_floats<D>(kRows);
-        for (int i = tid; i < kRows * D; i += 256) {
-            const int rr = i / D, d = i % D;
-            if (r0 + rr >= rows) break;
-            float o = 0.0f;
+        const int mine = min(kRows, rows - r0);
+        for (int i = tid; i < mine * (D / 4); i += NT) {
+            const int rr = i / (D / 4), d = 4 * (i % (D / 4));
+            f32x4 o = {};
+            float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) o += sO[(w * kRows + rr) * OP + d];
-            const float s = (sL[0][rr] + sL[1][rr]) + (sL[2][rr] + sL[3][rr]);
+            for (int w = 0; w < NW; ++w) {
+                o += *reinterpret_cast<const f32x4 *>(&sO[(w * kRows + rr) * OP + d]);
+                s += sL[w][rr];
+            }
             if (whole) {
-                put_out(a, q.s.t0 + (r0 + rr) / a.group, (h * a.group + (r0 + rr) % a.group) * D + d,
-                        s == 0.0f ? 0.0f : o / s);
+                put_out4(a, q.s.t0 + (r0 + rr) / a.group, (h * a.group + (r0 + rr) % a.group) * D + d,
+                         o * (s == 0.0f ? 0.0f : 1.0f / s));
             } else {
-                slot[i] = o;
+                *reinterpret_cast<f32x4 *>(slot + rr * D + d) = o;
                 if (d == 0) {
-                    slot[kRows * D + 2 * rr] = fmaxf(fmaxf(sM[0][rr], sM[1][rr]), fmaxf(sM[2][rr], sM[3][rr]));
-                    slot[kRows * D + 2 * rr + 1] = s;
+                    float m = sM[0][rr];
+#pragma unroll
+                    for (int w = 1; w < NW; ++w) m = fmaxf(m, sM[w][rr]);
+                    *reinterpret_cast<float2 *>(slot + kRows * D + 2 * rr) = make_float2(m, s);
                 }
             }
+        }
+        if (tid == 0 && t0 == 0) {
+            // the runs that have the row's other tiles
+            const int last = whole ? 0 : (at - t1 + q.tiles - 1) / place.run - (int)blockIdx.x;
+            row_runs<D>(a)[((int64_t)b * max_blocks + blk) * c.hkv + h] = make_int2(blockIdx.x, blockIdx.x + last);
         }
         __syncthreads();
     }
@@ -316,66 +421,49 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c
 // Joins the partial states of query rows that a cut went through: one
 // work-group per (sequence, row block, kv head, query row).
 template <int D>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int groups, int max_blocks,
-                                                           int block_rows) {
-    __shared__ int part[4], found[2];
-    __shared__ float f[kMostStates], red[8 + 256];
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int max_blocks, int block_rows) {
     int w = blockIdx.x;
     const int rr = w % block_rows;
     w /= block_rows;
     const int h = w % c.hkv;
     w /= c.hkv;
     const int blk = w % max_blocks, b = w / max_blocks;
-    const AttnSeq q = attn_seq(c, a, b);
+    const int2 runs = row_runs<D>(a)[((int64_t)b * max_blocks + blk) * c.hkv + h];
+    const SeqInfo s = kv_seq(c, b);
     const int r = blk * kRows + rr;
-    if (blk >= q.blocks || r >= q.s.n * a.group) return;
-    int total, base = (blk * c.hkv + h) * q.tiles;
-    if (c.n_seqs == 1) {
-        total = q.tiles * q.blocks * c.hkv;
-    } else {
-        total = 0;
-        for (int b0 = 0; b0 < c.n_seqs; b0 += 256) {
-            const int i = b0 + threadIdx.x;
-            int t;
-            const int before = total + group_scan(i < c.n_seqs ? attn_units(c, a, i) : 0, part, t);
-            if (i == b) found[0] = before;
-            total += t;
-        }
-        __syncthreads();
-        base += found[0];
-    }
-    const int run = attn_run(total, groups);
-    const int g0 = base / run, g1 = (base + q.tiles - 1) / run;
+    if (r >= s.n * a.group) return;  // no such row, and nobody has written its runs
+    const int g0 = runs.x, g1 = runs.y;
     if (g0 == g1) return;  // one run had the whole row and has written it
     const auto slot = [&](int i) {
         return a.ws + ((int64_t)(g0 + i) * 2 + (i == 0)) * state_floats<D>(kRows);
     };
-    const float o = join_row<D>(g1 - g0 + 1, kRows, rr, slot, f, red);
-    if ((int)threadIdx.x < D)
-        put_out(a, q.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
+    const f32x4 o = join_row<D>(g1 - g0 + 1, kRows, rr, slot);
+    if ((int)threadIdx.x < D / 4)
+        put_out4(a, s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
 
 // Rows of a kv head above which kv_attn_wide.hip takes the call.
 constexpr int kNarrowRows = 16;
 
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
-    const size_t narrow = (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float);
-    if (max_new * (hq / hkv) <= kNarrowRows) return narrow;
-    return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
+    const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
+    if (rows > kNarrowRows) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
+    return (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float) + (size_t)n_seqs * blocks * hkv * sizeof(int2);
 }
 
 template <int D, int FMT>
 static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     const int max_blocks = (c.max_new * a.group + kRows - 1) / kRows;
-    const int64_t cap = (int64_t)c.max_pages << c.page_shift;
-    const int64_t most = (int64_t)c.n_seqs * c.hkv * max_blocks * ((cap + kTile - 1) / kTile);
-    const int groups = (int)std::min<int64_t>(kAttnGroups, (most + kMinTiles - 1) / kMinTiles);
-    kv_attn_kernel<D, FMT><<<(unsigned)groups, 256, 0, stream>>>(c, a);
+    const int64_t tiles = (((int64_t)c.max_pages << c.page_shift) + kTile - 1) / kTile;
+    const int64_t rows = (int64_t)c.n_seqs * c.hkv * max_blocks;
+    const bool solo = tiles <= kSoloTiles;  // no sequence can be longer
+    const int most = D == 256 ? kAttnGroups / 2 : kAttnGroups;  // resident at once
+    const int groups = (int)std::min<int64_t>(most, solo ? rows : (rows * tiles + NW - 1) / NW);
+    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || groups == 1) return e;
+    if (e != hipSuccess || solo) return e;
     const int block_rows = std::min(kRows, c.max_new * a.group);
-    kv_attn_join_kernel<D><<<(unsigned)(c.n_seqs * max_blocks * c.hkv * block_rows), 256, 0, stream>>>(
-        c, a, groups, max_blocks, block_rows);
+    kv_attn_join_kernel<D><<<(unsigned)(rows * block_rows), 256, 0, stream>>>(c, a, max_blocks, block_rows);
     return hipGetLastError();
 }
 

@@ -53,6 +53,18 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
 __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
 
+// The larger of each of the 4 lanes l, l^16, l^32, l^48.
+__device__ __forceinline__ float max_groups(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];  // a bit cast of an element would take the first
+    x = fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t q0 = q[0], q1 = q[1];
+    return fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+}
+
 // tanh(x) for |x| < kCapNear, good to 2^-22: its series.
 constexpr float kCapNear = 0.35f;
 __device__ __forceinline__ float tanh_near(float x) {
@@ -171,60 +183,53 @@ constexpr int state_floats(int rows) {
     return rows * (D + 2);
 }
 
-// The states of one query row, read from `n` slots (slot(i) -> its first float),
-// joined by a work-group of 256 threads; the row's result on thread d < D.
-// f, red: LDS. n <= kMostStates.
-constexpr int kMostStates = 512;
+// The states of one query row, in `n` slots (slot(i) -> its first float), joined
+// by a work-group of 256 threads: D/4 threads a state, so that (M, l) and O of
+// 1024/D states load at once; each such group of threads joins every 1024/D-th
+// state as it comes, then the groups join through LDS. The row's dims 4d .. on
+// thread d < D/4.
 template <int D, class Slot>
-__device__ __forceinline__ float join_row(int n, int rows, int row, Slot slot, float *f, float *red) {
-    constexpr int W = 256 / D;  // states read at once
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float M = -INFINITY, m[2], l[2];
+__device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
+    constexpr int L = D / 4, W = 256 / L, U = 4;  // threads of a state, states at once, loads ahead
+    __shared__ f32x4 sO[W * L];
+    __shared__ float2 sML[W];
+    const int d = threadIdx.x % L, k = threadIdx.x / L;
+    float M = -INFINITY, l = 0.0f;
+    f32x4 o = {};
+    for (int i0 = k; i0 < n && k < W; i0 += U * W) {
+        float2 ml[U];
+        f32x4 x[U];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = tid + 256 * k;
-        m[k] = -INFINITY;
-        l[k] = 0.0f;
-        if (i < n) {
-            const float2 x = *reinterpret_cast<const float2 *>(slot(i) + rows * D + 2 * row);
-            m[k] = x.x;
-            l[k] = x.y;
+        for (int u = 0; u < U; ++u) {
+            const float *s = slot(min(i0 + u * W, n - 1));
+            ml[u] = *reinterpret_cast<const float2 *>(s + rows * D + 2 * row);
+            x[u] = *reinterpret_cast<const f32x4 *>(s + row * D + 4 * d);
+            if (i0 + u * W >= n) ml[u].x = -INFINITY;
         }
-        M = fmaxf(M, m[k]);
-    }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    if (lane == 0) red[wave] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = tid + 256 * k;
-        const float w = m[k] == -INFINITY ? 0.0f : exp2f(m[k] - M);
-        if (i < n) f[i] = w;
-        sum += w * l[k];
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) red[4 + wave] = sum;
-    __syncthreads();
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
-    const int d = tid % D, k = tid / D;
-    float o = 0.0f;
-    if (k < W) {
-#pragma unroll 8
-        for (int i = k; i < n; i += W) o += f[i] * slot(i)[row * D + d];
-    }
-    if (W > 1) {
-        if (k < W) red[8 + tid] = o;
-        __syncthreads();
-        if (k == 0) {
-#pragma unroll
-            for (int i = 1; i < W; ++i) o += red[8 + i * D + d];
+        for (int u = 0; u < U; ++u) {
+            if (ml[u].x == -INFINITY) continue;  // (M, l, O) of nothing
+            const float m = fmaxf(M, ml[u].x), f = exp2f(M - m), g = exp2f(ml[u].x - m);
+            M = m;
+            l = l * f + ml[u].y * g;
+            o = o * f + x[u] * g;
         }
     }
-    return sum == 0.0f ? 0.0f : o / sum;
+    if (k < W) sO[k * L + d] = o;
+    if (k < W && d == 0) sML[k] = make_float2(M, l);
+    __syncthreads();
+    M = sML[0].x;
+#pragma unroll
+    for (int i = 1; i < W; ++i) M = fmaxf(M, sML[i].x);
+    l = 0.0f;
+    o = f32x4{};
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float f = sML[i].x == -INFINITY ? 0.0f : exp2f(sML[i].x - M);
+        l += sML[i].y * f;
+        o += sO[i * L + d] * f;
+    }
+    return o * (l == 0.0f ? 0.0f : 1.0f / l);
 }
 
 // 4 neighbouring values of a result row.
@@ -237,12 +242,6 @@ __device__ __forceinline__ void put_out4(const AttnArgs &a, int64_t token, int h
     } else {
         *reinterpret_cast<f32x4_a4 *>(static_cast<float *>(a.out) + to) = o;
     }
-}
-
-__device__ __forceinline__ void put_out(const AttnArgs &a, int64_t token, int head_dim0, float o) {
-    const int64_t to = token * a.out_stride + head_dim0;
-    if (a.out_f16) static_cast<_Float16 *>(a.out)[to] = (_Float16)o;
-    else static_cast<float *>(a.out)[to] = o;
 }
 
 }  // namespace mgq

@@ -116,18 +116,6 @@ __device__ __forceinline__ void wide_barrier() {
     __builtin_amdgcn_s_barrier();
 }
 
-// The larger of each of the 4 lanes l, l^16, l^32, l^48.
-__device__ __forceinline__ float max_groups(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    const uint32_t h0 = h[0], h1 = h[1];  // a bit cast of an element would take the first
-    x = fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
-    const uint32_t v = __builtin_bit_cast(uint32_t, x);
-    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    const uint32_t q0 = q[0], q1 = q[1];
-    return fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
-}
-
 // Compile-time shape of the kernel. int8 K goes into the int8 matrix cores as it
 // is, q as digits of 8 bits: 16 bits for an f16 result, 24 for f32 (heads of 96
 // are no multiple of the 64 dims of such a product).
@@ -470,7 +458,6 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 // Joins a split row block: one work-group per (row block, sequence, kv head, row).
 template <int D>
 __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnArgs a, int most_splits) {
-    __shared__ float f[kMostStates], red[8 + 256];
     int id = blockIdx.x;
     const int rr = id % kWideRows;
     id /= kWideRows;
@@ -486,9 +473,9 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnAr
     const auto slot = [&](int i) {
         return a.ws + ((i * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows);
     };
-    const float o = join_row<D>(n, kWideRows, rr, slot, f, red);
-    if ((int)threadIdx.x < D)
-        put_out(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + threadIdx.x, o);
+    const f32x4 o = join_row<D>(n, kWideRows, rr, slot);
+    if ((int)threadIdx.x < D / 4)
+        put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
 
 // The same for few splits: D/4 lanes a row.

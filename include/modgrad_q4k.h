@@ -390,7 +390,7 @@ typedef struct mgq_kv_cache {
  * Tokens past max_pages*page_tokens, or in no page, are not stored. The q_out
  * row of a token at a position outside the table is NaN.
  * hipErrorInvalidValue unless rope->rot_dim <= head_dim and rope->n_pos >=
- * max_pages*page_tokens. */
+ * max_pages*page_tokens, or for max_new*n_q_heads*head_dim >= 2^32. */
 hipError_t launch_kv_append_ex(const mgq_kv_cache *cache, const mgq_rope *rope, const float *k,
                                const float *v, int64_t kv_stride, const float *q,
                                int64_t q_stride, float *q_out, int64_t q_out_stride,

@@ -88,6 +88,8 @@ hipError_t append_check(const mgq_kv_cache *c, const mgq_rope *rope, const float
     }
     // work-groups: pages that new tokens may touch, and chunks of query rows
     const int64_t blocks = ((int64_t)max_new + c->page_tokens - 2) / c->page_tokens + 1;
+    // query pairs of a sequence are counted in 32 bits
+    if (q && (int64_t)max_new * hq * c->head_dim >= (INT64_C(1) << 32)) return hipErrorInvalidValue;
     const int64_t query = q ? (int64_t)max_new * hq * c->head_dim / 512 + 1 : 0;
     const int64_t most = kMaxGrid / c->n_seqs;
     return blocks * 2 * c->n_kv_heads >= most / 2 || query >= most / 2 ? hipErrorInvalidValue : hipSuccess;

@@ -19,7 +19,7 @@ namespace mgq {
 
 struct AppendGrid {
     int page_blocks;  // most pages of a sequence that the new tokens touch
-    int kv_groups;    // work-groups of the K and V part
+    int kv_groups;    // work-groups of the K and V part, which come first
     int q_blocks;     // work-groups of a sequence in the query part
 };
 constexpr int kQueryUnits = 4;
@@ -44,6 +44,18 @@ __device__ __forceinline__ double finite_abs(double v) {
     return a <= 1.7976931348623157e308 ? a : 0.0;  // NaN and inf do not count
 }
 
+// x / s for one s > 0 and many x: the product with the reciprocal, corrected by
+// its remainder, is the rounded quotient (ties of the code to come among them),
+// at a fifth of a division's operations.
+struct Divider {
+    double s, r;
+    __device__ __forceinline__ explicit Divider(float scale) : s(scale), r(1.0 / scale) {}
+    __device__ __forceinline__ double operator()(double x) const {
+        const double q = x * r;
+        return fabs(q) < 1e300 ? fma(fma(-q, s, x), r, q) : q;  // infinities and NaN as they are
+    }
+};
+
 template <int D, int FMT, bool VEC, int NT>
 __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, const float *__restrict__ rope, int rot,
                                                        int half, int n_pos, AppendGrid gr) {
@@ -55,38 +67,34 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
         // ---- queries: 4 units a thread, their loads side by side
         const int w = blockIdx.x - gr.kv_groups, b = w / gr.q_blocks;
         const SeqInfo s = kv_seq(c, b);
-        const int per_token = kUnits * a.hq;
-        const int64_t units = (int64_t)s.n * per_token, first = (int64_t)(w % gr.q_blocks) * (kQueryUnits * NT) + tid;
+        const unsigned per_token = kUnits * a.hq, units = (unsigned)s.n * per_token;
+        const unsigned first = (unsigned)(w % gr.q_blocks) * (kQueryUnits * NT) + tid;
         if (first >= units) return;
+        unsigned t[kQueryUnits], r[kQueryUnits];  // token, unit in it
+#pragma unroll
+        for (int k = 0; k < kQueryUnits; ++k) {
+            const unsigned i = min(first + k * NT, units - 1);
+            t[k] = i / per_token;
+            r[k] = i - t[k] * per_token;
+        }
         double v[kQueryUnits][U::N];
 #pragma unroll
-        for (int k = 0; k < kQueryUnits; ++k) {
-            const int64_t i = min(first + k * NT, units - 1);
-            const int t = (int)(i / per_token), r = (int)(i % per_token);
-            const U u(r % kUnits, rot, half);
-            u.load(a.q + (s.t0 + t) * a.q_stride + (r / kUnits) * D, v[k]);
-        }
+        for (int k = 0; k < kQueryUnits; ++k)
+            U(r[k] % kUnits, rot, half).load(a.q + (s.t0 + (int64_t)t[k]) * a.q_stride + (r[k] / kUnits) * D, v[k]);
 #pragma unroll
         for (int k = 0; k < kQueryUnits; ++k) {
-            const int64_t i = min(first + k * NT, units - 1);
-            const int t = (int)(i / per_token), r = (int)(i % per_token);
-            const U u(r % kUnits, rot, half);
-            const int p = s.pos0 + t;
+            const int p = s.pos0 + (int)t[k];
             if (p >= 0 && p < n_pos) {
-                u.turn(rope + (int64_t)p * rot, half, v[k]);
+                U(r[k] % kUnits, rot, half).turn(rope + (int64_t)p * rot, half, v[k]);
             } else {
 #pragma unroll
                 for (int e = 0; e < U::N; ++e) v[k][e] = __builtin_nan("");
             }
         }
 #pragma unroll
-        for (int k = 0; k < kQueryUnits; ++k) {
-            const int64_t i = first + k * NT;
-            if (i >= units) break;
-            const int t = (int)(i / per_token), r = (int)(i % per_token);
-            const U u(r % kUnits, rot, half);
-            u.store(a.q_out + (s.t0 + t) * a.q_out_stride + (r / kUnits) * D, v[k]);
-        }
+        for (int k = 0; k < kQueryUnits; ++k)
+            if (first + k * NT < units)
+                U(r[k] % kUnits, rot, half).store(a.q_out + (s.t0 + (int64_t)t[k]) * a.q_out_stride + (r[k] / kUnits) * D, v[k]);
         return;
     }
     // ---- one page of one kv head, K or V
@@ -101,43 +109,85 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
     const int begin = max(max(s.pos0, 0), slot << c.page_shift);
     const int end = min(s.pos0 + s.n, (slot + 1) << c.page_shift);
     if (begin >= end) return;
-    const int id = c.table[(int64_t)(w / gr.page_blocks) * c.max_pages + slot];
-    if (id < 0 || id >= c.n_pages) return;
     const int n = end - begin, off = begin & (page - 1);
-    float *sp = (is_v ? c.vs : c.ks) + (int64_t)id * c.hkv + h;
-    uint8_t *blk = (is_v ? c.v : c.k) + id * c.page_stride + (int64_t)h * page * D;
     const float *x = (is_v ? a.v : a.k) + (s.t0 + begin - s.pos0) * a.kv_stride + h * D;
-    const float old = off > 0 ? *sp : 0.0f;
 
+    // K's rotated units tid + e * NT, kBatch of them with their loads side by side:
+    // all of the page's, which then stay in registers, or (`once` false) as many as
+    // there are, one batch after another
+    constexpr int kBatch = VEC ? 4 : NT == 64 ? D / 128 + 1 : 2;
+    const int total = n * kUnits;
+    const bool once = total <= kBatch * NT;
+    double kv[kBatch][U::N];
+    const auto load_keys = [&](int i0) {
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int i = min(i0 + e * NT, total - 1);
+            U(i % kUnits, rot, half).load(x + (int64_t)(i / kUnits) * a.kv_stride, kv[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int i = min(i0 + e * NT, total - 1);
+            U(i % kUnits, rot, half).turn(rope + (int64_t)(begin + i / kUnits) * rot, half, kv[e]);
+        }
+    };
+    const auto each_key = [&](int i0, auto f) {
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const int i = i0 + e * NT;
+            if (i < total) f(i / kUnits, U(i % kUnits, rot, half), kv[e]);
+        }
+    };
+
+    // the page's id loads beside the rows
+    const int id = c.table[(int64_t)(w / gr.page_blocks) * c.max_pages + slot];
     double m = 0.0;
     if (is_v) {
-#pragma unroll 4
-        for (int i = tid; i < n * D; i += NT) m = fmax(m, finite_abs(x[(i / D) * a.kv_stride + i % D]));
-    } else {
-        for (int i = tid; i < n * kUnits; i += NT) {
-            const int t = i / kUnits;
-            const U u(i % kUnits, rot, half);
-            double v[U::N];
-            u.load(x + t * a.kv_stride, v);
-            u.turn(rope + (int64_t)(begin + t) * rot, half, v);
+        constexpr int Q = D / 4, B = 8;
+        float top = 0.0f;
+        for (int i0 = tid; i0 < n * Q; i0 += B * NT) {
+            f32x4 y[B];
 #pragma unroll
-            for (int e = 0; e < U::N; ++e) m = fmax(m, finite_abs(v[e]));
+            for (int e = 0; e < B; ++e) {
+                const int i = min(i0 + e * NT, n * Q - 1);
+                y[e] = ld_f32x4(x + (int64_t)(i / Q) * a.kv_stride + i % Q * 4);
+            }
+#pragma unroll
+            for (int e = 0; e < B; ++e)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float z = fabsf(y[e][k]);
+                    top = z <= 3.4028235e38f && z > top ? z : top;
+                }
+        }
+        m = top;
+    } else {
+        for (int i0 = tid; i0 < total; i0 += kBatch * NT) {
+            load_keys(i0);
+            each_key(i0, [&](int, const U &, const double (&v)[U::N]) {
+#pragma unroll
+                for (int e = 0; e < U::N; ++e) m = fmax(m, finite_abs(v[e]));
+            });
         }
     }
+    if (id < 0 || id >= c.n_pages) return;
+    float *sp = (is_v ? c.vs : c.ks) + (int64_t)id * c.hkv + h;
+    uint8_t *blk = (is_v ? c.v : c.k) + id * c.page_stride + (int64_t)h * page * D;
+    const float old = off > 0 ? *sp : 0.0f;
     m = group_max<NT>(m);
     const float now = fmaxf(old, (float)(m / kv_most<FMT>()));
     if (tid == 0) *sp = now;  // every thread has `old`: group_max's barrier, or one wavefront
-    const double sc = now;
+    const Divider div(now);
 
     if (now > old && off > 0) {  // the held tokens to the new scale
-        const double ratio_top = old;
+        const double held = old;
         if (is_v) {
             const int tg = (off + 3) / 4;
             for (int i = tid; i < D * tg; i += NT) {
                 const int d = i % D, t0 = (i / D) * 4;
                 uint8_t *p = blk + (int64_t)d * page + t0;
                 const int k = min(4, off - t0);
-                for (int e = 0; e < k; ++e) p[e] = (uint8_t)kv_code<FMT>((double)kv_value<FMT>(p[e]) * ratio_top / sc);
+                for (int e = 0; e < k; ++e) p[e] = (uint8_t)kv_code<FMT>(div((double)kv_value<FMT>(p[e]) * held));
             }
         } else {
             for (int i = tid; i < off * (D / 4); i += NT) {
@@ -146,13 +196,13 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
                 uint32_t r = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    r |= kv_code<FMT>((double)kv_value<FMT>((q >> (8 * e)) & 0xFFu) * ratio_top / sc) << (8 * e);
+                    r |= kv_code<FMT>(div((double)kv_value<FMT>((q >> (8 * e)) & 0xFFu) * held)) << (8 * e);
                 *p = r;
             }
         }
     }
 
-    const auto code = [&](double v) { return now > 0.0f ? kv_code<FMT>(v / sc) : 0u; };
+    const auto code = [&](double v) { return now > 0.0f ? kv_code<FMT>(div(v)) : 0u; };
     if (is_v) {
         // a thread has one dim of up to 16 neighbouring tokens: 16 bytes of the
         // [dim][token] block
@@ -174,20 +224,20 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
             }
         }
     } else {
-        for (int i = tid; i < n * kUnits; i += NT) {
-            const int t = i / kUnits;
-            const U u(i % kUnits, rot, half);
-            double v[U::N];
-            u.load(x + t * a.kv_stride, v);
-            u.turn(rope + (int64_t)(begin + t) * rot, half, v);
-            uint8_t *p = blk + (off + t) * D;
-            if constexpr (VEC) {
-                *reinterpret_cast<uint32_t *>(p + u.d0) = code(v[0]) | code(v[1]) << 8 | code(v[2]) << 16 | code(v[3]) << 24;
-                *reinterpret_cast<uint32_t *>(p + u.d1) = code(v[4]) | code(v[5]) << 8 | code(v[6]) << 16 | code(v[7]) << 24;
-            } else {
-                p[u.d0] = (uint8_t)code(v[0]);
-                p[u.d1] = (uint8_t)code(v[1]);
-            }
+        for (int i0 = tid; i0 < total; i0 += kBatch * NT) {
+            if (!once) load_keys(i0);
+            each_key(i0, [&](int t, const U &u, const double (&v)[U::N]) {
+                uint8_t *p = blk + (off + t) * D;
+                if constexpr (VEC) {
+                    *reinterpret_cast<uint32_t *>(p + u.d0) =
+                        code(v[0]) | code(v[1]) << 8 | code(v[2]) << 16 | code(v[3]) << 24;
+                    *reinterpret_cast<uint32_t *>(p + u.d1) =
+                        code(v[4]) | code(v[5]) << 8 | code(v[6]) << 16 | code(v[7]) << 24;
+                } else {
+                    p[u.d0] = (uint8_t)code(v[0]);
+                    p[u.d1] = (uint8_t)code(v[1]);
+                }
+            });
         }
     }
 }

@@ -35,13 +35,15 @@
 // page ids are a tile ahead of both: 64 tokens' 16 KiB (D = 128) are on their way
 // for each wavefront while it computes.
 //
-// Split. All (sequence, kv head, 16 query rows) rows of tiles laid end to end
-// are cut into equal runs, one for each work-group, so ragged batches and one
-// long sequence balance alike. The wavefronts of a work-group take tiles in
-// turn, each with its own softmax state, joined through LDS at the end of a
-// row; a row that a cut goes through leaves partial states in the workspace,
-// which kv_attn_join_kernel joins. Short sequences (no row over kSoloTiles) are
-// not cut: a work-group takes whole rows.
+// Split. The tiles of a (sequence, kv head, 16 query rows) make a row. Much work:
+// all rows laid end to end are cut into equal runs, one for each resident
+// work-group, so ragged batches and one long sequence balance alike. Little work
+// (under kRunTiles tiles a work-group): each row is cut into equal parts by
+// itself, a work-group each, since every further row that a run touches costs its
+// latencies again (~7 us: page ids, loads, join through LDS); rows of kSoloTiles
+// and less are one part. The wavefronts of a work-group take tiles in turn, each
+// with its own softmax state, joined through LDS; a row in several parts leaves
+// their states in the workspace for kv_attn_join_kernel.
 #include "kv_attn.hpp"
 
 namespace mgq {
@@ -49,8 +51,9 @@ namespace mgq {
 constexpr int kRows = 16;         // query rows of a work-group's row of tiles
 constexpr int kAttnGroups = 512;  // work-groups: two of 4 wavefronts per CU
 constexpr int NW = 4;             // wavefronts of a work-group
-// Rows of up to 256 tokens are not cut: the wavefronts have a tile each.
-constexpr int kSoloTiles = NW;
+// A row of 512 tokens is not cut (2 tiles a wavefront cost less than the joining
+// launch), a part has a tile for each wavefront.
+constexpr int kSoloTiles = 2 * NW, kPartTiles = NW, kRunTiles = 4 * NW;
 
 // A row's tiles: rows of (sequence, kv head, row block), kv head and row block
 // within the sequence.
@@ -91,83 +94,90 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
     return before + s - v;
 }
 
-// The cut: all units, the units of a run, and where this work-group's run lies:
-// its first unit, that one's sequence and the sequence's first unit. With no row
-// over kSoloTiles a unit is a whole row, else a tile. One pass over the
-// sequences where they are no more than the threads.
+// The cut. Runs: a unit is a tile, `run` of them a work-group's. Parts: a unit is
+// a part of at most `part` tiles.
 struct AttnPlace {
-    int total, run, at, b, base;
-    bool solo;
-    AttnSeq q;  // the sequence
+    int total, run, part;  // part 0: runs
+    int at, b, base;       // first unit, its sequence, that one's first unit
+    AttnSeq q;             // the sequence
+    __device__ __forceinline__ int parts(const AttnSeq &s) const {
+        return s.tiles <= kSoloTiles ? 1 : (s.tiles + part - 1) / part;
+    }
+    // units of a sequence
+    __device__ __forceinline__ int units(const AttnSeq &s, int hkv) const {
+        return s.blocks * hkv * (part ? parts(s) : s.tiles);
+    }
+    __device__ __forceinline__ void cut(int tiles, int most) {
+        part = tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
+    }
+    __device__ __forceinline__ void deal(int units, int most) {
+        const int groups = part ? (int)gridDim.x : min(most, (int)gridDim.x);
+        total = units;
+        run = (total + groups - 1) / groups;
+        at = (int)blockIdx.x < groups ? (int)blockIdx.x * run : total;
+    }
 };
-__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int *part, int *found) {
+__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int most, int *part, int *found) {
     constexpr int NT = 64 * NW;
-    AttnPlace p = {0, 0, 0, 0, 0, true, {}};
-    const auto cut = [&](int total) {
-        p.total = total;
-        p.run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-        if (!p.solo) p.run = max(p.run, NW);  // a tile for each wavefront
-        p.at = (int)blockIdx.x * p.run;
-    };
+    AttnPlace p = {};
     if (c.n_seqs == 1) {
         p.q = attn_seq(c, a, 0);
-        p.solo = p.q.tiles <= kSoloTiles;
-        cut(p.q.blocks * c.hkv * (p.solo ? 1 : p.q.tiles));
+        p.cut(p.q.blocks * c.hkv * p.q.tiles, most);
+        p.deal(p.units(p.q, c.hkv), most);
         return p;
     }
-    int rows = 0, tiles = 0, sum_rows = 0, sum_tiles = 0, long_ = 0;
+    // all tiles, then all units, then the sequence that `at` lies in; the
+    // sequence of a thread is kept where there are no more than threads
+    AttnSeq q = {};
+    int tiles = 0, units = 0, before = 0, t;
     for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
-        rows = tiles = 0;
-        if (b0 + (int)threadIdx.x < c.n_seqs) {
-            const AttnSeq q = attn_seq(c, a, b0 + threadIdx.x);
-            rows = q.blocks * c.hkv;
-            tiles = rows * q.tiles;
-            if (rows > 0 && q.tiles > kSoloTiles) long_ = 1;
-        }
-        sum_rows += rows;
-        sum_tiles += tiles;
+        q.blocks = 0;
+        if (b0 + (int)threadIdx.x < c.n_seqs) q = attn_seq(c, a, b0 + threadIdx.x);
+        tiles += q.blocks * c.hkv * q.tiles;
     }
-    p.solo = __syncthreads_or(long_) == 0;
-    int total;
-    group_scan(p.solo ? sum_rows : sum_tiles, part, total);
-    cut(total);
-    int before = 0;
+    group_scan(tiles, part, t);
+    p.cut(t, most);
+    int start;
+    if (c.n_seqs <= NT) {
+        units = p.units(q, c.hkv);
+        start = group_scan(units, part, t);
+    } else {
+        for (int b = threadIdx.x; b < c.n_seqs; b += NT) units += p.units(attn_seq(c, a, b), c.hkv);
+        group_scan(units, part, t);
+    }
+    p.deal(t, most);
     for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
-        const int i = b0 + threadIdx.x;
         if (c.n_seqs > NT) {
-            rows = tiles = 0;
-            if (i < c.n_seqs) {
-                const AttnSeq q = attn_seq(c, a, i);
-                rows = q.blocks * c.hkv;
-                tiles = rows * q.tiles;
-            }
+            units = b0 + (int)threadIdx.x < c.n_seqs ? p.units(attn_seq(c, a, b0 + threadIdx.x), c.hkv) : 0;
+            start = before + group_scan(units, part, t);
+            before += t;
         }
-        const int u = p.solo ? rows : tiles;
-        int t;
-        const int start = before + group_scan(u, part, t);
-        before += t;
-        if (p.at >= start && p.at < start + u) {
-            found[0] = i;
+        if (p.at >= start && p.at < start + units) {
+            found[0] = b0 + threadIdx.x;
             found[1] = start;
         }
     }
     __syncthreads();
-    p.b = found[0];
-    p.base = found[1];
-    if (p.at < p.total) p.q = attn_seq(c, a, p.b);
+    if (p.at < p.total) {
+        p.b = found[0];
+        p.base = found[1];
+        p.q = attn_seq(c, a, p.b);
+    }
     return p;
 }
 
-// Workspace: run w's states, slot 0 for a row begun by an earlier run, slot 1
-// for one that this run begins; then for every row the first and last run of it,
-// written by the first.
+// Workspace: states, then for every row its first state's number and how many
+// it has, written by the row's first work-group. Runs: run w has state 2w for a
+// row that an earlier run begins, 2w + 1 for one it begins (the number of states
+// is negative then). Parts: a state has its unit's number.
 template <int D>
-__device__ __forceinline__ int2 *row_runs(const AttnArgs &a) {
-    return reinterpret_cast<int2 *>(a.ws + (int64_t)kAttnGroups * 2 * state_floats<D>(kRows));
+__device__ __forceinline__ int2 *row_states(const AttnArgs &a, int states) {
+    return reinterpret_cast<int2 *>(a.ws + (int64_t)states * state_floats<D>(kRows));
 }
 
 template <int D, int FMT>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a, int max_blocks) {
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a, int max_blocks, int most,
+                                                                               int states) {
     constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
     constexpr int KB = D / 4;               // bytes of a token that a lane group has
     constexpr int KS = I8 ? D / 64 : D / 32;  // summed steps of S
@@ -180,7 +190,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
-    const AttnPlace place = attn_place(c, a, part, found);
+    const AttnPlace place = attn_place(c, a, most, part, found);
     int at = place.at;
     const int stop = min(at + place.run, place.total);
     if (at >= stop) return;
@@ -188,17 +198,19 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
     AttnSeq q = place.q;
 
     while (at < stop) {
-        const auto units = [&] { return q.blocks * c.hkv * (place.solo ? 1 : q.tiles); };
-        while (at - base >= units()) {  // the next sequence with rows
-            base += units();
+        while (at - base >= place.units(q, c.hkv)) {  // the next sequence with rows
+            base += place.units(q, c.hkv);
             q = attn_seq(c, a, ++b);
         }
-        int row = at - base, t0 = 0, t1 = q.tiles;
-        if (place.solo) {
+        const int first_unit = at, cuts = place.part ? place.parts(q) : q.tiles;
+        const int k = (at - base) % cuts, row = (at - base) / cuts;
+        int t0, t1;
+        if (place.part) {
+            t0 = (int)((int64_t)q.tiles * k / cuts);
+            t1 = (int)((int64_t)q.tiles * (k + 1) / cuts);
             ++at;
         } else {
-            t0 = row % q.tiles;
-            row /= q.tiles;
+            t0 = k;
             t1 = min(q.tiles, t0 + stop - at);
             at += t1 - t0;
         }
@@ -385,7 +397,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == q.tiles;
-        float *slot = a.ws + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * state_floats<D>(kRows);
+        float *slot = a.ws + (int64_t)(place.part ? first_unit : 2 * (int)blockIdx.x + (t0 == 0)) * state_floats<D>(kRows);
         const int mine = min(kRows, rows - r0);
         for (int i = tid; i < mine * (D / 4); i += NT) {
             const int rr = i / (D / 4), d = 4 * (i % (D / 4));
@@ -410,9 +422,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
             }
         }
         if (tid == 0 && t0 == 0) {
-            // the runs that have the row's other tiles
-            const int last = whole ? 0 : (at - t1 + q.tiles - 1) / place.run - (int)blockIdx.x;
-            row_runs<D>(a)[((int64_t)b * max_blocks + blk) * c.hkv + h] = make_int2(blockIdx.x, blockIdx.x + last);
+            int2 st = {first_unit, cuts};
+            if (whole) st.y = 1;
+            else if (!place.part) st = {(int)blockIdx.x, (int)blockIdx.x - 1 - (first_unit + q.tiles - 1) / place.run};
+            row_states<D>(a, states)[((int64_t)b * max_blocks + blk) * c.hkv + h] = st;
         }
         __syncthreads();
     }
@@ -421,49 +434,64 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
 // Joins the partial states of query rows that a cut went through: one
 // work-group per (sequence, row block, kv head, query row).
 template <int D>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int max_blocks, int block_rows) {
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a, int max_blocks, int block_rows, int states) {
     int w = blockIdx.x;
     const int rr = w % block_rows;
     w /= block_rows;
     const int h = w % c.hkv;
     w /= c.hkv;
     const int blk = w % max_blocks, b = w / max_blocks;
-    const int2 runs = row_runs<D>(a)[((int64_t)b * max_blocks + blk) * c.hkv + h];
+    const int2 st = row_states<D>(a, states)[((int64_t)b * max_blocks + blk) * c.hkv + h];
     const SeqInfo s = kv_seq(c, b);
     const int r = blk * kRows + rr;
-    if (r >= s.n * a.group) return;  // no such row, and nobody has written its runs
-    const int g0 = runs.x, g1 = runs.y;
-    if (g0 == g1) return;  // one run had the whole row and has written it
+    if (r >= s.n * a.group) return;  // no such row, and nobody has written its states' numbers
+    if (st.y == 1) return;  // the whole row was one work-group's, which has written it
     const auto slot = [&](int i) {
-        return a.ws + ((int64_t)(g0 + i) * 2 + (i == 0)) * state_floats<D>(kRows);
+        return a.ws + (int64_t)(st.y > 0 ? st.x + i : 2 * (st.x + i) + (i == 0)) * state_floats<D>(kRows);
     };
-    const f32x4 o = join_row<D>(g1 - g0 + 1, kRows, rr, slot);
+    const f32x4 o = join_row<D>(abs(st.y), kRows, rr, slot);
     if ((int)threadIdx.x < D / 4)
         put_out4(a, s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
 
-// Rows of a kv head above which kv_attn_wide.hip takes the call.
-constexpr int kNarrowRows = 16;
+// Query rows of a kv head up to which this kernel takes the call, in blocks of
+// 16 that each read the cache, and above which kv_attn_wide.hip does. Measured
+// (28 heads on 4 of 128, int8): 28 rows x 16 sequences of 4000 tokens 29 us here,
+// 46 there; 63 rows x 8 of 8000 56 and 51. Heads of 256: 24 rows 25 and 29, 48
+// rows 57 and 40.
+static int narrow_rows(int dim) { return dim == 256 ? 32 : 48; }
+
+// Most tiles of a row: the table's, or the window's.
+static int64_t most_tiles(int64_t cap, int max_new, int window) {
+    if (window > 0) cap = std::min<int64_t>(cap, (int64_t)window + max_new - 1 + kTile - 1);
+    return (cap + kTile - 1) / kTile;
+}
+
+// States: a run has two, a part one, and with the parts' least size given by
+// `most` there are no more parts than `most` and one for every row.
+static int64_t most_states(int64_t rows) { return kAttnGroups + std::max<int64_t>(rows, kAttnGroups); }
 
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
     const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
-    if (rows > kNarrowRows) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
-    return (size_t)kAttnGroups * 2 * kRows * (dim + 2) * sizeof(float) + (size_t)n_seqs * blocks * hkv * sizeof(int2);
+    if (rows > narrow_rows(dim)) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
+    const int64_t all = (int64_t)n_seqs * blocks * hkv;
+    return (size_t)most_states(all) * kRows * (dim + 2) * sizeof(float) + (size_t)all * sizeof(int2);
 }
 
 template <int D, int FMT>
 static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     const int max_blocks = (c.max_new * a.group + kRows - 1) / kRows;
-    const int64_t tiles = (((int64_t)c.max_pages << c.page_shift) + kTile - 1) / kTile;
+    const int64_t tiles = most_tiles((int64_t)c.max_pages << c.page_shift, c.max_new, a.window);
     const int64_t rows = (int64_t)c.n_seqs * c.hkv * max_blocks;
-    const bool solo = tiles <= kSoloTiles;  // no sequence can be longer
+    const bool solo = tiles <= kSoloTiles;  // no row can be longer
     const int most = D == 256 ? kAttnGroups / 2 : kAttnGroups;  // resident at once
-    const int groups = (int)std::min<int64_t>(most, solo ? rows : (rows * tiles + NW - 1) / NW);
-    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks);
+    const int groups = (int)(solo ? rows : std::min(rows * ((tiles + kPartTiles - 1) / kPartTiles), most + rows));
+    const int states = (int)most_states(rows);
+    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, most, states);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || solo) return e;
     const int block_rows = std::min(kRows, c.max_new * a.group);
-    kv_attn_join_kernel<D><<<(unsigned)(rows * block_rows), 256, 0, stream>>>(c, a, max_blocks, block_rows);
+    kv_attn_join_kernel<D><<<(unsigned)(rows * block_rows), 256, 0, stream>>>(c, a, max_blocks, block_rows, states);
     return hipGetLastError();
 }
 
@@ -479,7 +507,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.softcap = x.softcap * 1.4426950408889634f;
     a.window = x.window;
     a.ws = x.ws;
-    if (c.max_new * a.group > kNarrowRows) return kv_attn_wide_launch(c, dim, fmt, a, stream);
+    if (c.max_new * a.group > narrow_rows(dim)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;
     switch (dim) {
     case 64: return i8 ? attn_run_dim<64, kFmtI8>(c, a, stream) : attn_run_dim<64, kFmtE4M3>(c, a, stream);

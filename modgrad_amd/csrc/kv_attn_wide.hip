@@ -533,7 +533,12 @@ size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_n
 template <int D, int FMT, bool LO>
 static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     int row_blocks, splits;
-    wide_plan(D, a.group, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, row_blocks, splits);
+    const int64_t cap = (int64_t)c.max_pages << c.page_shift;
+    wide_plan(D, a.group, c.hkv, c.n_seqs, c.max_new, cap, row_blocks, splits);
+    if (a.window > 0) {  // a row block's tokens and their windows
+        const int64_t seen = (int64_t)a.window + kWideRows / a.group + 2 * kTile;
+        splits = (int)std::min<int64_t>(splits, (seen / kTile + kWideChunk - 1) / kWideChunk);
+    }
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
     typedef WideShape<D, FMT, LO> W;
     constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);

@@ -115,12 +115,13 @@ class RopeTable:
         self.n_pos, self.rot_dim = table.shape[0], 2 * table.shape[1]
         self.desc = _lib.Rope(table.data_ptr(), self.n_pos, self.rot_dim,
                               _lib.ROPE_HALF if half else _lib.ROPE_INTERLEAVED)
+        self.ref = ctypes.byref(self.desc)
 
     def apply(self, x: int, y: int, pos: int, n_tokens: int, n_heads: int, head_dim: int,
               x_stride: int | None = None, y_stride: int | None = None, stream=None) -> None:
         """y = x, [n_tokens][n_heads][head_dim] f32 turned to positions pos."""
         row = n_heads * head_dim
-        kern.rope(x, y, pos, self.desc, n_tokens, n_heads, head_dim,
+        kern.rope(x, y, pos, self.ref, n_tokens, n_heads, head_dim,
                   row if x_stride is None else x_stride, row if y_stride is None else y_stride,
                   stream)
 
@@ -175,6 +176,8 @@ class KvCache:
         for t in (v, k_scale, v_scale, page_table, seq_len):
             if t.device != self.device:
                 raise BackendError("Runtime", "cache: tensors on different devices")
+        self._devices = torch.cuda.device_count()
+        self._ref = ctypes.byref(self.desc)
         self._free = None
         self._held = [[] for _ in range(self.n_seqs)]
 
@@ -262,7 +265,7 @@ class KvCache:
 
     def _here(self) -> None:
         """Launches go to the current device: it has to be the cache's."""
-        if _torch().cuda.current_device() != self.device.index:
+        if self._devices > 1 and _torch().cuda.current_device() != self.device.index:
             raise BackendError("Runtime", f"the cache is on {self.device}, the current device is "
                                           f"cuda:{_torch().cuda.current_device()}")
 
@@ -274,13 +277,13 @@ class KvCache:
         the cache, k rotated by `rope` (a RopeTable); q, if given, rotated to
         q_out (in place by default)."""
         self._here()
-        kern.kv_append(self.desc, None if rope is None else rope.desc, k, v, kv_stride, q, q_stride,
+        kern.kv_append(self._ref, None if rope is None else rope.ref, k, v, kv_stride, q, q_stride,
                        q if q_out is None else q_out, q_stride if q_out_stride is None else q_out_stride,
                        n_q_heads, n_tokens, max_new, stream)
 
     def attention_workspace(self, n_q_heads: int, n_tokens: int, max_new: int):
         """A device tensor for attend's workspace (any call with these sizes)."""
-        n = kern.kv_attention_workspace_bytes(self.desc, n_q_heads, max_new)
+        n = kern.kv_attention_workspace_bytes(self._ref, n_q_heads, max_new)
         if n == 0 or n_tokens <= 0:
             raise BackendError("Runtime", f"attention of {n_q_heads} heads, {max_new} new tokens")
         return _torch().empty(n, dtype=_torch().uint8, device=self.device)
@@ -296,15 +299,15 @@ class KvCache:
             workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
             if stream is not None:
                 workspace.record_stream(stream)
-        kern.kv_attention(self.desc, q, q_stride, n_q_heads, out, out_stride,
+        kern.kv_attention(self._ref, q, q_stride, n_q_heads, out, out_stride,
                           _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens, max_new,
                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap, window,
-                          workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream)
+                          workspace.data_ptr(), workspace.nbytes, stream)
 
     def dequant(self, pages: int, n: int, k_out: int, v_out: int, stream=None) -> None:
         """n pages (device int32 ids) as f32 [n][kv head][token][dim]."""
         self._here()
-        kern.kv_dequant(self.desc, pages, n, k_out, v_out, stream)
+        kern.kv_dequant(self._ref, pages, n, k_out, v_out, stream)
 
     # -- the same as descriptors of an op chain (q4k.Chain.from_ops) ----------
     def op_append(self, k: int, v: int, kv_stride: int, n_tokens: int, max_new: int, rope=None,

@@ -50,10 +50,9 @@ def _chk(code: int, what: str) -> None:
         raise BackendError("Runtime", f"{what}: hip error {code}")
 
 
-def _stream_ptr(stream) -> ctypes.c_void_p:
-    if stream is None:
-        return ctypes.c_void_p(0)
-    return ctypes.c_void_p(stream.cuda_stream)
+def _stream_ptr(stream):
+    """The hipStream_t of a torch stream; None is the null stream."""
+    return None if stream is None else stream.cuda_stream
 
 
 class HipBuffer:
@@ -353,8 +352,9 @@ class kern:
         _chk(_lib.load().launch_dequant_q4k_ex(q, n_blocks, out, _stream_ptr(stream)),
              "dequant_q4k")
 
-    # rotary positions and the 8-bit key/value cache; modgrad_amd.kvcache holds
-    # the structs (RopeTable.desc, KvCache.desc) these take
+    # rotary positions and the 8-bit key/value cache: `scaling`, `rope` and `cache`
+    # are references (ctypes.byref) to the structs that modgrad_amd.kvcache holds
+    # (RopeScaling.c, RopeTable.desc, KvCache.desc)
     @staticmethod
     def rope_table(table: int, n_pos: int, first_pos: int, rot_dim: int, scaling,
                    stream=None) -> None:
@@ -364,45 +364,42 @@ class kern:
                                               _stream_ptr(stream)), "rope_table")
 
     @staticmethod
-    def rope(x: int, y: int, pos: int, rope: "_lib.Rope", n_tokens: int, n_heads: int,
+    def rope(x: int, y: int, pos: int, rope, n_tokens: int, n_heads: int,
              head_dim: int, x_stride: int, y_stride: int, stream=None) -> None:
         """y = x with every head turned to its token's position."""
-        _chk(_lib.load().launch_rope_ex(x, y, pos, ctypes.byref(rope), n_tokens, n_heads,
+        _chk(_lib.load().launch_rope_ex(x, y, pos, rope, n_tokens, n_heads,
                                         head_dim, x_stride, y_stride, _stream_ptr(stream)),
              "rope")
 
     @staticmethod
-    def kv_append(cache: "_lib.KvCacheDesc", rope: "_lib.Rope | None", k: int, v: int,
+    def kv_append(cache, rope, k: int, v: int,
                   kv_stride: int, q: int, q_stride: int, q_out: int, q_out_stride: int,
                   n_q_heads: int, n_tokens: int, max_new: int, stream=None) -> None:
         """k and v rows into the cache as their sequences' last tokens, k (and
         q, to q_out) rotated."""
         _chk(_lib.load().launch_kv_append_ex(
-            ctypes.byref(cache), None if rope is None else ctypes.byref(rope), k, v, kv_stride,
-            q, q_stride, q_out, q_out_stride, n_q_heads, n_tokens, max_new,
+            cache, rope, k, v, kv_stride, q, q_stride, q_out, q_out_stride, n_q_heads, n_tokens, max_new,
             _stream_ptr(stream)), "kv_append")
 
     @staticmethod
-    def kv_dequant(cache: "_lib.KvCacheDesc", pages: int, n: int, k_out: int, v_out: int,
+    def kv_dequant(cache, pages: int, n: int, k_out: int, v_out: int,
                    stream=None) -> None:
         """n pages of the cache as f32 [n][kv head][token][dim]."""
-        _chk(_lib.load().launch_kv_dequant_ex(ctypes.byref(cache), pages, n, k_out, v_out,
+        _chk(_lib.load().launch_kv_dequant_ex(cache, pages, n, k_out, v_out,
                                               _stream_ptr(stream)), "kv_dequant")
 
     @staticmethod
-    def kv_attention_workspace_bytes(cache: "_lib.KvCacheDesc", n_q_heads: int,
-                                     max_new: int) -> int:
-        return int(_lib.load().mgq_kv_attention_workspace_bytes(ctypes.byref(cache), n_q_heads,
-                                                                max_new))
+    def kv_attention_workspace_bytes(cache, n_q_heads: int, max_new: int) -> int:
+        return int(_lib.load().mgq_kv_attention_workspace_bytes(cache, n_q_heads, max_new))
 
     @staticmethod
-    def kv_attention(cache: "_lib.KvCacheDesc", q: int, q_stride: int, n_q_heads: int, out: int,
+    def kv_attention(cache, q: int, q_stride: int, n_q_heads: int, out: int,
                      out_stride: int, out_type: int, n_tokens: int, max_new: int, scale: float,
                      softcap: float, window: int, workspace: int, workspace_bytes: int,
                      stream=None) -> None:
         """out = softmax(scale q k) v over the cache, per query head."""
         _chk(_lib.load().launch_kv_attention_ex(
-            ctypes.byref(cache), q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens,
+            cache, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens,
             max_new, scale, softcap, window, workspace, workspace_bytes, _stream_ptr(stream)),
             "kv_attention")
 

@@ -378,7 +378,7 @@ typedef struct mgq_kv_cache {
  * kv_stride floats apart) as the last tokens of their sequences, and with
  * `rope` turns k on the way, and q (n_q_heads heads; null: none) from q to
  * q_out (which may be q with the same stride). rope null: k is stored and q
- * copied as they are.
+ * copied as they are. q_out must not overlap k, v or, but for that, q.
  * n_tokens: rows of q, k, v. max_new: no sequence has more new tokens (further
  * ones are left out).
  * For each page, kv head and of K and V: s = max(s_old, f32(amax / M)), amax
@@ -414,6 +414,7 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * and sums are f32. Where out is f32, the queries and the probabilities go
  * into the products with 22 bits; with MGQ_OUT_F16 the probabilities may have
  * 11. Scales of V below 2^-90 count as 2^-90.
+ * out must not overlap q, the cache or the workspace.
  * workspace: device memory, 16-byte aligned, of at least
  * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);
  * its contents need not be set and do not matter afterwards. Calls that may overlap need distinct ones. */
@@ -588,7 +589,7 @@ typedef struct mgq_op_desc {
  * staging), and then no chain is created. */
 hipError_t mgq_chain_create_ops(const mgq_op_desc *ops, int n, void **chain_out);
 
-/* Prepares the current device: sets the GEMV kernels' LDS attributes, which
+/* Prepares the current device: sets the kernels' LDS attributes, which
  * belong to a device (every launcher also does this on its first use on a
  * device), and looks up the device address of the fixed scratch array of
  * launch_matvec_q4k_batched_noalloc. Allocates nothing. Device memory the

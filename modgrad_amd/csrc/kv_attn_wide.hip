@@ -530,6 +530,24 @@ size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_n
     return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
 }
 
+// LDS past 64 KiB has to be allowed, per device.
+template <int D, int FMT, bool LO>
+static hipError_t wide_allow() {
+    typedef WideShape<D, FMT, LO> W;
+    static std::atomic<int> state[64];
+    if (2 * W::kBuf * sizeof(half8) <= 64 * 1024) return hipSuccess;
+    return allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
+}
+
+hipError_t kv_attn_prepare() {
+    hipError_t e = hipSuccess;
+    const auto all = [&](auto... f) { ((e = e == hipSuccess ? f() : e), ...); };
+    all(wide_allow<128, kFmtI8, false>, wide_allow<128, kFmtI8, true>, wide_allow<128, kFmtE4M3, false>,
+        wide_allow<128, kFmtE4M3, true>, wide_allow<256, kFmtI8, false>, wide_allow<256, kFmtI8, true>,
+        wide_allow<256, kFmtE4M3, false>, wide_allow<256, kFmtE4M3, true>);
+    return e;
+}
+
 template <int D, int FMT, bool LO>
 static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     int row_blocks, splits;
@@ -542,11 +560,8 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
     typedef WideShape<D, FMT, LO> W;
     constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);
-    static std::atomic<int> state[64];
-    if (kLds > 64 * 1024) {
-        const hipError_t e = allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
-        if (e != hipSuccess) return e;
-    }
+    const hipError_t allowed = wide_allow<D, FMT, LO>();
+    if (allowed != hipSuccess) return allowed;
     const int cus = device_cus();
     const int turn = c.n_seqs == 1 && splits == 1 && cus % c.hkv == 0 && (int)items >= 2 * cus ? cus / c.hkv : 1 << 29;
     kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);

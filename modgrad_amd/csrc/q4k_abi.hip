@@ -417,6 +417,7 @@ hipError_t mgq_chain_create_ops(const mgq_op_desc *ops, int n, void **chain_out)
         if (e != hipSuccess) return e;
     }
     hipError_t e = mgq::gemv_prepare();  // not allowed to happen mid-capture
+    if (e == hipSuccess) e = mgq::kv_attn_prepare();
     if (e != hipSuccess) return e;
     return chain_record(n, chain_out, [ops](int i, hipStream_t s) { return op_launch(ops[i], s); });
 }
@@ -542,6 +543,7 @@ hipError_t launch_matvec_q4k_glu_ex(const unsigned char *w_gate, const unsigned 
 hipError_t mgq_prepare(void) {
     hipError_t e = mgq::gemv_prepare();
     if (e == hipSuccess) e = mgq::gemm_prepare();
+    if (e == hipSuccess) e = mgq::kv_attn_prepare();
     return e != hipSuccess ? e : mgq::noalloc_prepare();
 }
 

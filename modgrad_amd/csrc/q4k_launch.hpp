@@ -270,6 +270,8 @@ hipError_t chain_persistent_destroy(PersistentChain *p);
 // checks of their argument struct, and the launch (kv_abi.hip).
 hipError_t kv_op_check(int op, const void *args);
 hipError_t kv_op_launch(int op, const void *args, hipStream_t stream);
+// LDS attributes of the prompt attention kernels (safe to call often).
+hipError_t kv_attn_prepare();
 
 hipError_t gemm_f16_launch(const uint8_t *w, const uint16_t *a, float *c, int n, int bpr,
                            int m_tokens, hipStream_t stream);

@@ -8,7 +8,7 @@ C ABI.
   KvCache       pages of 8-bit keys and values, their scales and page tables;
                 append, attend, dequant, and the same as op-chain descriptors
 
-    rope = RopeTable.from_gguf(g, n_pos=8192)
+    rope = RopeTable.from_gguf(g, n_pos=8192, half=True)
     cache = KvCache.new(n_pages=512, page_tokens=64, n_kv_heads=4, head_dim=128,
                         n_seqs=8, max_pages=128)
     cache.set_lengths([n0 + 1, n1 + 1, ...])           # the new tokens included
@@ -22,7 +22,10 @@ from __future__ import annotations
 import ctypes
 import math
 
+import numpy as np
+
 from . import _lib
+from .gguf import GgmlType
 from .q4k import BackendError, _torch, kern
 
 FORMATS = {"i8": _lib.KV_I8, "e4m3": _lib.KV_E4M3}
@@ -79,7 +82,7 @@ class RopeTable:
                 or not scaling.factors.is_contiguous()):
             raise BackendError("Runtime", f"rope factors: {rot_dim // 2} contiguous f32 expected")
         t = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device="cuda")
-        if isinstance(stream, torch.cuda.Stream):
+        if stream is not None:
             t.record_stream(stream)
         kern.rope_table(t.data_ptr(), n_pos, 0, rot_dim, scaling, stream)
         self._hold(t, half)
@@ -95,10 +98,12 @@ class RopeTable:
         return r
 
     @classmethod
-    def from_gguf(cls, g, n_pos: int, half: bool | None = None, factors=None) -> "RopeTable":
+    def from_gguf(cls, g, n_pos: int, half: bool, stream=None) -> "RopeTable":
         """For a GGUF model: its rotated dims (<arch>.rope.dimension_count),
-        scaling, and the pair order (interleaved for llama-family files, which
-        store q and k for it; half otherwise, unless given)."""
+        scaling and, where the file holds them, the divisors of its
+        rope_freqs.weight. Which dims pair up is the architecture's, and no key
+        of the file says it."""
+        torch = _torch()
         arch = g.architecture()
         rot = g.meta_u32(f"{arch}.rope.dimension_count") or g.meta_u32(f"{arch}.attention.key_length")
         if not rot:
@@ -106,9 +111,13 @@ class RopeTable:
             if not emb or not heads:
                 raise BackendError("Runtime", f"missing {arch}.rope.dimension_count")
             rot = emb // heads
-        if half is None:
-            half = arch != "llama"
-        return cls(n_pos, rot, half, RopeScaling.from_gguf(g, factors))
+        factors = None
+        if "rope_freqs.weight" in g.tensors:
+            if g.tensors["rope_freqs.weight"].dtype != GgmlType.F32:
+                raise BackendError("Unsupported", "rope_freqs.weight is not F32")
+            raw = np.frombuffer(g.tensor_bytes("rope_freqs.weight"), np.float32).copy()
+            factors = torch.from_numpy(raw).cuda()
+        return cls(n_pos, rot, half, RopeScaling.from_gguf(g, factors), stream)
 
     def _hold(self, table, half: bool) -> None:
         self.table, self.half = table, bool(half)

@@ -57,6 +57,21 @@ def test_rope_table(n_pos, first, rot, kw):
     assert np.all(np.abs(got[:n_pos] - want) <= 2.0 ** -24 * np.abs(want) + size * (first + n_pos) * 2.0 ** -50)
 
 
+def test_rope_table_from_gguf(tmp_path):
+    from modgrad_amd.gguf import GgmlType, GgufFile, write_gguf
+    from modgrad_amd.kvcache import RopeTable
+    note("rope table of a GGUF file")
+    f = np.linspace(1.0, 4.0, 32).astype(np.float32)
+    path = str(tmp_path / "m.gguf")
+    write_gguf(path, [("general.architecture", 8, "llama"), ("llama.rope.dimension_count", 4, 64),
+                      ("llama.rope.freq_base", 6, 5e5)], [("rope_freqs.weight", [32], GgmlType.F32, f.tobytes())])
+    r = RopeTable.from_gguf(GgufFile.open(path), 100, half=False)
+    a = np.outer(np.arange(100.0), 5e5 ** (-np.arange(32) / 32.0) / f)
+    want = np.stack([np.cos(a), np.sin(a)], 2)
+    assert r.rot_dim == 64 and r.n_pos == 100 and not r.half
+    assert np.all(np.abs(host(r.table) - want) <= 2.0 ** -24 * np.abs(want) + 100 * 2.0 ** -50)
+
+
 # -------------------------------------------------------------------- rope --
 
 @pytest.mark.parametrize("half", [False, True])
@@ -348,6 +363,7 @@ def test_attention_absent_and_shared_pages(fmt, new):
     t[2, :4] = -1
     t[3] = -1
     t[4, 2], t[4, 4] = 10 ** 6, len(both.ref.k)
+    t[4, 1] = t[4, 0]  # the same page twice
     both.gpu.page_table.copy_(torch.from_numpy(t))
     lens, rows = [90, 83, 90, 90, 90], 5 * new
     q = rng.standard_normal((rows, 6, 64)).astype(np.float32)
@@ -434,6 +450,167 @@ def test_attention_one_long_sequence():
         tol = (p * e) @ v[:, :n].abs() + (p * e).sum(-1, keepdim=True) * want.abs()
         diff = (out.double().view(2, 7, 128) - want).abs()
         assert bool((diff <= tol).all()), float((diff / tol).max())
+
+
+def torch_attention(both, q, lens, new, scale, window=0):
+    """In 64 bits on the GPU, with the f32 bound of kv_reference.Cache.attend."""
+    import torch
+    grid = torch.from_numpy(ref.grid(both.gpu.format)).cuda()
+    hq, d = q.shape[1], both.dim
+    g = hq // both.heads
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    t, eps = 0, 2.0 ** -24
+    for b, (n, m) in enumerate(zip(lens, new)):
+        if n and m:
+            ids = torch.from_numpy(both.ref.table[b, :-(-n // both.gpu.page_tokens)]).cuda().long()
+            k = (grid[both.k[ids].long()] * both.ks[ids].double()[..., None, None]).permute(1, 0, 2, 3)
+            v = (grid[both.v[ids].long()] * both.vs[ids].double()[..., None, None]).permute(1, 0, 3, 2)
+            k, v = (y.reshape(both.heads, -1, d)[:, :n].contiguous() for y in (k, v))
+            x = q[t:t + m].double().view(m, both.heads, g, d).permute(1, 2, 0, 3).reshape(both.heads, -1, d)
+            s = scale * (x @ k.transpose(1, 2))
+            ds = (d + 8) * eps * scale * (x.abs() @ k.abs().transpose(1, 2))
+            j = torch.arange(n, device="cuda")
+            pos = n - m + torch.arange(m, device="cuda")
+            hide = j > pos[:, None]
+            if window:
+                hide |= j <= pos[:, None] - window
+            hide = hide.repeat(g, 1)
+            s = s.masked_fill(hide, -torch.inf)
+            p = torch.softmax(s, -1)
+            top = s.amax(-1, keepdim=True)
+            e = ds + ds.amax(-1, keepdim=True) + 2 * eps * (s.abs() + 2 * (top - s) + 34) + 8 * eps + (96 + n / 32) * eps
+            e = torch.where(hide, 0.0, e)
+            o = p @ v
+            w = (p * e) @ v.abs() + (p * e).sum(-1, keepdim=True) * o.abs() + eps * o.abs()
+            back = lambda y: y.view(both.heads, g, m, d).permute(2, 0, 1, 3).reshape(m, hq, d)  # noqa: E731
+            out[t:t + m], tol[t:t + m] = back(o), back(w)
+        t += m
+    return out, tol
+
+
+def random_cache(both, seed):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    for t in (both.k, both.v):
+        x = torch.randn(t.shape, generator=g, device="cuda")
+        t.copy_(x.mul(40).clamp(-127, 127).to(torch.int8).view(torch.uint8) if both.gpu.format == "i8"
+                else x.mul(100).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
+    for s in (both.ks, both.vs):
+        s.copy_(torch.rand(s.shape, generator=g, device="cuda") * 0.02 + 0.005)
+    return g
+
+
+@pytest.mark.parametrize("seqs,most,heads,group,dim,page,new,window,fmt", [
+    (300, 300, 2, 4, 64, 16, 1, 0, "i8"),        # more sequences than a work-group has threads
+    (300, 1500, 1, 3, 128, 32, 2, 700, "e4m3"),
+    (5, 40000, 16, 2, 64, 64, 1, 0, "i8"),       # runs: over 16 tiles for each of the chip's work-groups
+    (40, 9000, 8, 7, 128, 128, 1, 0, "e4m3"),
+    (90, 400, 2, 2, 64, 16, 40, 0, "i8"),        # more sequences than lanes, many query rows
+    (3, 20000, 1, 8, 128, 64, 30, 0, "i8"),      # splits of row blocks, many states
+    (2, 6000, 2, 1, 256, 32, 300, 2500, "e4m3"),
+    (1, 3000, 4, 7, 128, 64, 2100, 0, "i8"),     # over two work-groups a CU, dealt from both ends
+])
+def test_attention_large(seqs, most, heads, group, dim, page, new, window, fmt):
+    import torch
+    note(f"attention large seqs={seqs} most={most} heads={heads}x{group} dim={dim} page={page} new={new} {fmt}")
+    rng = np.random.default_rng(seqs + most)
+    both = Both(rng, seqs, -(-most // page), heads, dim, page, fmt)
+    gen = random_cache(both, most)
+    lens = [int(most * rng.random() ** 2) for _ in range(seqs)]
+    lens[0] = most
+    if seqs > 2:
+        lens[-1] = 0
+    news = [0 if n == 0 and new > 1 else max(1, min(n, int(new * rng.random()) + 1)) for n in lens]
+    news[0] = new
+    if new == 1:
+        news = [1] * seqs
+    rows, hq, scale = sum(news), heads * group, 1.2 / np.sqrt(dim)
+    q = torch.randn(rows, hq, dim, generator=gen, device="cuda") * 2
+    want, tol = torch_attention(both, q, lens, news, scale, window)
+    both.call(lens, news, new == 1)
+    ws = both.gpu.attention_workspace(hq, rows, new)
+    for f16 in (False, True):
+        out = torch.full((rows + 1, hq, dim), 7.0, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+        ws.fill_(255)
+        both.gpu.attend(q.data_ptr(), hq * dim, hq, out.data_ptr(), hq * dim, rows, new, scale=scale, window=window,
+                        out_f16=f16, workspace=ws)
+        check(host(out[:rows]).astype(np.float64), host(want), host(tol), f16)
+        assert bool((out[rows] == 7.0).all())
+
+
+@pytest.mark.parametrize("seqs,page,dim", [(300, 16, 64), (70, 128, 256)])
+def test_append_many_sequences(seqs, page, dim):
+    """One call for hundreds of sequences, single tokens and pieces that pass
+    several pages."""
+    note(f"append {seqs} sequences page={page} dim={dim}")
+    rng = np.random.default_rng(seqs)
+    both = Both(rng, seqs, 4, 1, dim, page, "e4m3")
+    lens = np.zeros(seqs, int)
+    for step in range(3):
+        new = rng.integers(0, 2 if step == 1 else page + page // 2, seqs)
+        lens = lens + new
+        both.call(lens.tolist(), new.tolist())
+        x = rng.standard_normal((int(new.sum()), 2, 1, dim)).astype(np.float32) * (1 + step)
+        xt = dev(x)
+        both.gpu.append(xt.data_ptr(), xt.data_ptr() + 4 * dim, 2 * dim, len(x), int(max(new)))
+        t = 0
+        for b in range(seqs):
+            both.ref.append(b, int(lens[b] - new[b]), x[t:t + new[b], 0].astype(np.float64), x[t:t + new[b], 1].astype(np.float64))
+            t += new[b]
+        both.same()
+
+
+def test_append_exact_ties():
+    """Quotients that lie on a tie of the code exactly, with scales that have no
+    exact reciprocal: largest values 127 s (int8) and 448 s (e4m3), s = 3, 5, 7."""
+    note("append exact ties")
+    rng = np.random.default_rng(15)
+    for fmt in ("i8", "e4m3"):
+        for s in (1, 3, 5, 7, 11):
+            both = Both(rng, 1, 2, 1, 64, 16, fmt)
+            if fmt == "i8":
+                x = (rng.integers(-126, 126, (16, 2, 1, 64)) + 0.5) * s
+            else:
+                g = ref.grid("e4m3")[:126]
+                x = (g[:-1] + g[1:])[rng.integers(0, 125, (16, 2, 1, 64))] / 2 * s
+            x[0] = ref.MOST[fmt] * s
+            x = x.astype(np.float32)
+            xt = dev(x)
+            both.call([16], [16])
+            both.gpu.append(xt.data_ptr(), xt.data_ptr() + 256, 128, 16, 16)
+            both.ref.append(0, 0, x[:, 0].astype(np.float64), x[:, 1].astype(np.float64))
+            both.same()
+
+
+def test_prompt_pieces_recorded_once():
+    """A recorded call with many query rows (splits and their join), replayed with
+    the sequences growing, a dirty workspace and eager work between."""
+    import torch
+    from modgrad_amd.q4k import Chain
+    note("prompt pieces through a chain")
+    rng = np.random.default_rng(16)
+    both = Both(rng, 3, 12, 2, 256, 128, "e4m3")
+    gen = random_cache(both, 5)
+    new, hq = [60, 1, 33], 6
+    rows = sum(new)
+    q = torch.randn(rows, hq, 256, generator=gen, device="cuda")
+    out = torch.empty(rows, hq, 256, device="cuda")
+    lens = [100, 1, 700]
+    both.call(lens, new)
+    ws = both.gpu.attention_workspace(hq, rows, 60)
+    chain = Chain.from_ops([both.gpu.op_attend(q.data_ptr(), hq * 256, hq, out.data_ptr(), hq * 256, rows, 60, ws)])
+    for step in range(5):
+        out.fill_(7.0)
+        ws.fill_(255)
+        both.length.copy_(torch.tensor(lens, dtype=torch.int32))
+        chain.launch()
+        if step % 2:
+            torch.cuda.synchronize()
+        want, tol = torch_attention(both, q, lens, new, 1 / 16)
+        check(host(out).astype(np.float64), host(want), host(tol), False)
+        lens = [n + d for n, d in zip(lens, (177, 64, 130))]
 
 
 def test_cache_past_4_gib():

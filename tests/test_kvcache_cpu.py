@@ -193,3 +193,36 @@ def test_reference_attention_is_a_mean_of_v():
     assert np.allclose(out[0, 1], x[:, 0].mean(0))
     out, _ = c.attend(np.zeros((1, 2, 64)), [20], [1], 1.0, window=5)
     assert np.allclose(out[0, 0], x[15:, 0].mean(0))
+
+
+# ------------------------------------------------------- frequencies by GGUF --
+
+def _gguf(tmp_path, meta):
+    from modgrad_amd.gguf import GgufFile, write_gguf
+    path = str(tmp_path / "m.gguf")
+    write_gguf(path, [("general.architecture", 8, "llama")] + meta, [])
+    return GgufFile.open(path)
+
+
+@pytest.mark.parametrize("meta,want", [
+    ([], dict(base=1e4, freq_scale=1.0, ext_factor=0.0, orig_ctx=0.0)),
+    ([("llama.rope.freq_base", 6, 5e5)], dict(base=5e5, freq_scale=1.0, ext_factor=0.0)),
+    ([("llama.rope.scaling.type", 8, "linear"), ("llama.rope.scaling.factor", 6, 8.0)],
+     dict(base=1e4, freq_scale=0.125, ext_factor=0.0)),
+    ([("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scaling.factor", 6, 4.0),
+      ("llama.rope.scaling.original_context_length", 4, 32768), ("llama.rope.scaling.attn_factor", 6, 1.5)],
+     dict(freq_scale=0.25, ext_factor=1.0, orig_ctx=32768.0, attn_factor=1.5, beta_fast=32.0, beta_slow=1.0)),
+])
+def test_rope_scaling_from_gguf(tmp_path, meta, want):
+    from modgrad_amd.kvcache import RopeScaling
+    c = RopeScaling.from_gguf(_gguf(tmp_path, meta)).c
+    assert {k: getattr(c, k) for k in want} == want and not c.factors
+
+
+def test_rope_scaling_from_gguf_refuses(tmp_path):
+    from modgrad_amd.kvcache import RopeScaling
+    from modgrad_amd.q4k import BackendError
+    for meta in ([("llama.rope.scaling.type", 8, "longer")],
+                 [("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scaling.factor", 6, 4.0)]):
+        with pytest.raises(BackendError):
+            RopeScaling.from_gguf(_gguf(tmp_path, meta))

@@ -95,7 +95,8 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
 }
 
 // The cut. Runs: a unit is a tile, `run` of them a work-group's. Parts: a unit is
-// a part of at most `part` tiles.
+// a part of at most `part` tiles. Where no row can have more than kSoloTiles
+// tiles (`most` 0) every row is one part, however many there are: no join follows.
 struct AttnPlace {
     int total, run, part;  // part 0: runs
     int at, b, base;       // first unit, its sequence, that one's first unit
@@ -108,7 +109,8 @@ struct AttnPlace {
         return s.blocks * hkv * (part ? parts(s) : s.tiles);
     }
     __device__ __forceinline__ void cut(int tiles, int most) {
-        part = tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
+        if (most == 0) part = kSoloTiles;
+        else part = tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
     }
     __device__ __forceinline__ void deal(int units, int most) {
         const int groups = part ? (int)gridDim.x : min(most, (int)gridDim.x);
@@ -487,7 +489,7 @@ static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t s
     const int most = D == 256 ? kAttnGroups / 2 : kAttnGroups;  // resident at once
     const int groups = (int)(solo ? rows : std::min(rows * ((tiles + kPartTiles - 1) / kPartTiles), most + rows));
     const int states = (int)most_states(rows);
-    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, most, states);
+    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || solo) return e;
     const int block_rows = std::min(kRows, c.max_new * a.group);

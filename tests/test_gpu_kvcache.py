@@ -511,6 +511,9 @@ def random_cache(both, seed):
     (3, 20000, 1, 8, 128, 64, 30, 0, "i8"),      # splits of row blocks, many states
     (2, 6000, 2, 1, 256, 32, 300, 2500, "e4m3"),
     (1, 3000, 4, 7, 128, 64, 2100, 0, "i8"),     # over two work-groups a CU, dealt from both ends
+    (500, 512, 8, 1, 64, 64, 1, 0, "i8"),        # rows of at most 8 tiles, far more of them than work-groups
+    (300, 512, 8, 1, 256, 64, 1, 0, "e4m3"),
+    (600, 9000, 8, 2, 64, 32, 1, 300, "i8"),     # the same by a window
 ])
 def test_attention_large(seqs, most, heads, group, dim, page, new, window, fmt):
     import torch

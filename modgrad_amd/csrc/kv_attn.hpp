@@ -204,11 +204,11 @@ __device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
             const float *s = slot(min(i0 + u * W, n - 1));
             ml[u] = *reinterpret_cast<const float2 *>(s + rows * D + 2 * row);
             x[u] = *reinterpret_cast<const f32x4 *>(s + row * D + 4 * d);
-            if (i0 + u * W >= n) ml[u].x = -INFINITY;
+            if (i0 + u * W >= n) ml[u] = make_float2(-INFINITY, 0.0f);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (ml[u].x == -INFINITY) continue;  // (M, l, O) of nothing
+            if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // of nothing; scores of NaN have a NaN l
             const float m = fmaxf(M, ml[u].x), f = exp2f(M - m), g = exp2f(ml[u].x - m);
             M = m;
             l = l * f + ml[u].y * g;

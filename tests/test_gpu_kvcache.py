@@ -452,6 +452,33 @@ def test_attention_one_long_sequence():
         assert bool((diff <= tol).all()), float((diff / tol).max())
 
 
+@pytest.mark.parametrize("seqs,pages,heads,group,dim,new,fmt", [
+    (1, 60, 1, 4, 128, 1, "i8"),      # parts of one row
+    (2, 60, 1, 1, 96, 3, "e4m3"),
+    (1, 60, 1, 2, 128, 100, "i8"),    # few splits of a block of many rows
+    (1, 300, 1, 64, 64, 1, "e4m3"),   # many
+])
+def test_attention_nan_query_over_split_tokens(seqs, pages, heads, group, dim, new, fmt):
+    """A row whose scores are all NaN is NaN however its tokens are split."""
+    import torch
+    note(f"attention of a NaN query seqs={seqs} pages={pages} heads={heads}x{group} dim={dim} new={new} {fmt}")
+    rng = np.random.default_rng(dim + new)
+    both = Both(rng, seqs, pages, heads, dim, 64, fmt)
+    random_cache(both, pages)
+    hq, rows, lens = heads * group, seqs * new, [64 * pages - 3] * seqs
+    q = torch.from_numpy(rng.standard_normal((rows, hq, dim)).astype(np.float32)).cuda()
+    both.call(lens, [new] * seqs, new == 1)
+    outs = []
+    for _ in range(2):
+        out = torch.full((rows, hq, dim), 7.0, device="cuda")
+        both.gpu.attend(q.data_ptr(), hq * dim, hq, out.data_ptr(), hq * dim, rows, new)
+        outs.append(host(out))
+        q[-1, 0, 1] = float("nan")
+    assert np.all(np.isfinite(outs[0])) and np.all(np.isnan(outs[1][-1, 0]))
+    outs[1][-1, 0] = outs[0][-1, 0]
+    assert np.array_equal(*outs)
+
+
 def torch_attention(both, q, lens, new, scale, window=0):
     """In 64 bits on the GPU, with the f32 bound of kv_reference.Cache.attend."""
     import torch

@@ -507,7 +507,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.out_f16 = x.out_f16;
     a.scale = x.softcap > 0.0f ? x.scale / x.softcap : x.scale * 1.4426950408889634f;
     a.softcap = x.softcap * 1.4426950408889634f;
-    a.window = x.window;
+    a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
     a.ws = x.ws;
     if (c.max_new * a.group > narrow_rows(dim)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;

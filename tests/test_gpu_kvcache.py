@@ -452,6 +452,49 @@ def test_attention_one_long_sequence():
         assert bool((diff <= tol).all()), float((diff / tol).max())
 
 
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_lengths_that_do_not_fit_the_rows(new):
+    """Lengths and row starts of any value stay within the call's buffers, with
+    the largest window, and sequences beside them keep their results."""
+    import torch
+    note(f"odd lengths and row starts new={new}")
+    rng = np.random.default_rng(21)
+    big = 2 ** 31 - 1
+    both = Both(rng, 6, 5, 2, 64, 16, "i8")
+    random_cache(both, 3)
+    kv = torch.randn(2 * new, 128, device="cuda")
+    q = torch.randn(2 * new, 4, 64, device="cuda")
+    out = torch.zeros(2 * new, 4, 64, device="cuda")
+    at = lambda lens, cu: (both.length.copy_(torch.tensor(lens, dtype=torch.int32)),  # noqa: E731
+                           both.gpu.use_cu_tokens(torch.tensor(cu, dtype=torch.int32, device="cuda")))
+    attend = lambda window: both.gpu.attend(q.data_ptr(), 256, 4, out.data_ptr(), 256, 2 * new, new, window=window)  # noqa: E731
+    at([75, 0, 0, 0, 0, 80], [0, new, new, new, new, new, 2 * new])
+    attend(0)
+    want = host(out).copy()
+    for lens, cu in (([75, 3, -5, big, -big, 80], [0, new, new, new, new, new, 2 * new]),
+                     ([75, 0, 1, -big, big, 80], [0, new, -big, big, -1, new, 2 * new]),
+                     ([75, 0, 2, 5, -1, 80], [0, new, 2 * new + 9, -3, big, new, 2 * new])):
+        at(lens, cu)
+        for window in (0, big):
+            out.fill_(7.0)
+            attend(window)
+            got = host(out)
+            assert np.array_equal(got[:new], want[:new]) and np.array_equal(got[new:], want[new:])
+    # more rows than tokens: the rows before the first token see nothing and store nothing
+    before = host(both.k).copy()
+    at([75, 0, 0, 0, 0, max(new - 1, 0)], [0, new, new, new, new, new, 2 * new])
+    for window in (0, 1, big):
+        attend(window)
+        got = host(out)
+        assert np.array_equal(got[:new] if window != 1 else want[:new], want[:new])
+        assert np.all(got[new] == 0.0) and np.all(np.isfinite(got))
+    both.gpu.append(kv.data_ptr(), kv.data_ptr(), 128, 2 * new, new)
+    after = host(both.k)
+    held = set(both.ref.table[5, :1 if new < 4 else -(-(new - 1) // 16)]) | set(both.ref.table[0])
+    for p in range(len(before)):
+        assert p in held or np.array_equal(before[p], after[p])
+
+
 @pytest.mark.parametrize("seqs,pages,heads,group,dim,new,fmt", [
     (1, 60, 1, 4, 128, 1, "i8"),      # parts of one row
     (2, 60, 1, 1, 96, 3, "e4m3"),

@@ -383,8 +383,8 @@ typedef struct mgq_kv_cache {
  * ones are left out).
  * For each page, kv head and of K and V: s = max(s_old, f32(amax / M)), amax
  * over the finite new values, M the format's largest, s_old the page's scale
- * if it holds earlier tokens of the sequence, else 0 (as for a NaN). If s > s_old the held
- * values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
+ * if it holds earlier tokens of the sequence, else 0 (as for a NaN). If s > s_old
+ * the held values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
  * nearest even and saturates, NaN becomes 0; all of it in 64 bits. Bytes behind
  * the sequence's last token are left as they are.
  * Tokens past max_pages*page_tokens, or in no page, are not stored. The q_out
@@ -410,14 +410,19 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * s_j = scale * q.k_j, or softcap*tanh(scale * q.k_j / softcap) with
  * softcap > 0. Query head h reads kv head h / (n_q_heads / n_kv_heads). A row
  * that sees nothing is zero. Rows of no sequence are left as they are.
- * q and out: rows of n_q_heads*head_dim values, strides in values. scale >= 0. Statistics
- * and sums are f32. Where out is f32, the queries and the probabilities go
- * into the products with 22 bits; with MGQ_OUT_F16 the probabilities may have
- * 11. Scales of V below 2^-90 count as 2^-90.
+ * q and out: rows of n_q_heads*head_dim values, strides in values. scale >= 0;
+ * hipErrorInvalidValue where 1.4427 * scale, 1.4427 * softcap or scale / softcap
+ * passes f32. A query row with a NaN or infinity gives a row of NaN if it sees
+ * anything. Scales, and values of tokens that a sequence holds, are taken as
+ * finite, as an append leaves them; what lies behind its last token may be
+ * anything. Statistics and sums are f32. Where out is f32, the queries and the
+ * probabilities go into the products with 22 bits; with MGQ_OUT_F16 the
+ * probabilities may have 11. Scales of V below 2^-90 count as 2^-90.
  * out must not overlap q, the cache or the workspace.
  * workspace: device memory, 16-byte aligned, of at least
  * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);
- * its contents need not be set and do not matter afterwards. Calls that may overlap need distinct ones. */
+ * its contents need not be set and do not matter afterwards. Calls that may
+ * overlap, recorded ones too, need distinct ones. */
 size_t mgq_kv_attention_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads, int max_new);
 hipError_t launch_kv_attention_ex(const mgq_kv_cache *cache, const float *q, int64_t q_stride,
                                   int n_q_heads, void *out, int64_t out_stride, int out_type,

@@ -117,7 +117,10 @@ hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq,
     const int64_t row = (int64_t)hq * c->head_dim;
     if (bad4(q) || !out || ((uintptr_t)out & (type == MGQ_OUT_F32 ? 3u : 1u)) || qs < row || os < row)
         return hipErrorInvalidValue;
-    if (!(scale >= 0.0f) || !std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap) || window < 0)
+    if (!(scale >= 0.0f) || !(softcap >= 0.0f) || window < 0) return hipErrorInvalidValue;
+    // as the kernels take them: times log2 e, or scale / softcap
+    if (!std::isfinite(scale * 1.4426950408889634f) || !std::isfinite(softcap * 1.4426950408889634f) ||
+        (softcap > 0.0f && !std::isfinite(scale / softcap)))
         return hipErrorInvalidValue;
     if (bad16(ws) || bytes < mgq_kv_attention_workspace_bytes(c, hq, max_new)) return hipErrorInvalidValue;
     return hipSuccess;

@@ -71,6 +71,12 @@ def test_append_refuses(L, bad):
     assert append(L, cache(), **bad) == INVALID
 
 
+@pytest.mark.parametrize("bad", [dict(scale=3e38), dict(cap=3e38), dict(scale=1e20, cap=1e-20),
+                                 dict(scale=0.1, cap=1e-45)])
+def test_attention_refuses_factors_past_f32(L, bad):
+    assert attend(L, cache(), **bad) == INVALID
+
+
 def test_one_token_each_needs_a_row_each(L):
     c = cache(cu_tokens=None)
     assert append(L, c, n=7, new=1) == INVALID  # 3 sequences

@@ -416,8 +416,8 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * anything. Scales, and values of tokens that a sequence holds, are taken as
  * finite, as an append leaves them; what lies behind its last token may be
  * anything. Statistics and sums are f32. Where out is f32, the queries and the
- * probabilities go into the products with 22 bits; with MGQ_OUT_F16 the
- * probabilities may have 11. Scales of V below 2^-90 count as 2^-90.
+ * probabilities go into the products with 22 bits; with MGQ_OUT_F16 the queries
+ * may have 16 (of the row's largest) and the probabilities 11. Scales of V below 2^-90 count as 2^-90.
  * out must not overlap q, the cache or the workspace.
  * workspace: device memory, 16-byte aligned, of at least
  * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);

@@ -16,6 +16,8 @@ C ABI.
     cache.attend(q, qs, 28, out, 28 * 128, 8, 1)
 
 Addresses are device pointers as in modgrad_amd.q4k.kern; torch only allocates.
+`stream` is a torch stream, None the null stream; page tables and lengths are
+written on it too, so a step's set_lengths is given the stream of its launches.
 """
 from __future__ import annotations
 
@@ -27,6 +29,24 @@ import numpy as np
 from . import _lib
 from .gguf import GgmlType
 from .q4k import BackendError, _torch, kern
+
+
+def _stream(stream):
+    """A context in which torch allocates and writes on the launches' stream:
+    memory freed there is used again behind the launches, not beside them."""
+    cuda = _torch().cuda
+    return cuda.stream(cuda.default_stream() if stream is None else stream)
+
+
+def _on_device(device) -> None:
+    """Launches go to the current device: the tensors have to be there."""
+    cuda = _torch().cuda
+    if device.type != "cuda":
+        raise BackendError("Runtime", f"tensors on {device}")
+    if device.index != cuda.current_device():
+        raise BackendError("Runtime", f"tensors on {device}, the current device is "
+                                      f"cuda:{cuda.current_device()}")
+
 
 FORMATS = {"i8": _lib.KV_I8, "e4m3": _lib.KV_E4M3}
 
@@ -81,9 +101,10 @@ class RopeTable:
                 scaling.factors.numel() != rot_dim // 2 or scaling.factors.dtype != torch.float32
                 or not scaling.factors.is_contiguous()):
             raise BackendError("Runtime", f"rope factors: {rot_dim // 2} contiguous f32 expected")
-        t = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device="cuda")
-        if stream is not None:
-            t.record_stream(stream)
+        if scaling.factors is not None:
+            _on_device(scaling.factors.device)
+        with _stream(stream):
+            t = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device="cuda")
         kern.rope_table(t.data_ptr(), n_pos, 0, rot_dim, scaling, stream)
         self._hold(t, half)
 
@@ -116,7 +137,8 @@ class RopeTable:
             if g.tensors["rope_freqs.weight"].dtype != GgmlType.F32:
                 raise BackendError("Unsupported", "rope_freqs.weight is not F32")
             raw = np.frombuffer(g.tensor_bytes("rope_freqs.weight"), np.float32).copy()
-            factors = torch.from_numpy(raw).cuda()
+            with _stream(stream):
+                factors = torch.from_numpy(raw).cuda()
         return cls(n_pos, rot, half, RopeScaling.from_gguf(g, factors), stream)
 
     def _hold(self, table, half: bool) -> None:
@@ -129,6 +151,7 @@ class RopeTable:
     def apply(self, x: int, y: int, pos: int, n_tokens: int, n_heads: int, head_dim: int,
               x_stride: int | None = None, y_stride: int | None = None, stream=None) -> None:
         """y = x, [n_tokens][n_heads][head_dim] f32 turned to positions pos."""
+        _on_device(self.table.device)
         row = n_heads * head_dim
         kern.rope(x, y, pos, self.ref, n_tokens, n_heads, head_dim,
                   row if x_stride is None else x_stride, row if y_stride is None else y_stride,
@@ -185,7 +208,7 @@ class KvCache:
         for t in (v, k_scale, v_scale, page_table, seq_len):
             if t.device != self.device:
                 raise BackendError("Runtime", "cache: tensors on different devices")
-        self._devices = torch.cuda.device_count()
+        self._own_cu = None
         self._ref = ctypes.byref(self.desc)
         self._free = None
         self._held = [[] for _ in range(self.n_seqs)]
@@ -201,26 +224,29 @@ class KvCache:
 
     @classmethod
     def new(cls, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, n_seqs: int,
-            max_pages: int, fmt: str = "i8") -> "KvCache":
+            max_pages: int, fmt: str = "i8", stream=None) -> "KvCache":
         """An empty cache whose pages reserve() and release() hand out."""
         torch = _torch()
-        try:
-            k = torch.zeros(n_pages, n_kv_heads, page_tokens, head_dim, dtype=torch.uint8, device="cuda")
-            v = torch.zeros(n_pages, n_kv_heads, head_dim, page_tokens, dtype=torch.uint8, device="cuda")
-        except torch.cuda.OutOfMemoryError as e:
-            raise BackendError("OutOfMemory", f"cache of {n_pages} pages") from e
-        c = cls(k, v, torch.zeros(n_pages, n_kv_heads, device="cuda"),
-                torch.zeros(n_pages, n_kv_heads, device="cuda"),
-                torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device="cuda"),
-                torch.zeros(n_seqs, dtype=torch.int32, device="cuda"), None, fmt)
+        with _stream(stream):
+            try:
+                k = torch.zeros(n_pages, n_kv_heads, page_tokens, head_dim, dtype=torch.uint8, device="cuda")
+                v = torch.zeros(n_pages, n_kv_heads, head_dim, page_tokens, dtype=torch.uint8, device="cuda")
+            except torch.cuda.OutOfMemoryError as e:
+                raise BackendError("OutOfMemory", f"cache of {n_pages} pages") from e
+            c = cls(k, v, torch.zeros(n_pages, n_kv_heads, device="cuda"),
+                    torch.zeros(n_pages, n_kv_heads, device="cuda"),
+                    torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device="cuda"),
+                    torch.zeros(n_seqs, dtype=torch.int32, device="cuda"), None, fmt)
         c._free = list(range(n_pages - 1, -1, -1))
         return c
 
     # -- pages and lengths ---------------------------------------------------
-    def reserve(self, seq: int, n_tokens: int) -> None:
+    def reserve(self, seq: int, n_tokens: int, stream=None) -> None:
         """Pages for the first n_tokens positions of slot `seq`."""
         if self._free is None:
             raise BackendError("Unsupported", "reserve: the cache wraps tables of the caller's")
+        if not 0 <= seq < self.n_seqs or n_tokens < 0:
+            raise BackendError("Runtime", f"reserve: {n_tokens} tokens of sequence {seq}")
         held = self._held[seq]
         need = -(-n_tokens // self.page_tokens)
         if need > self.max_pages:
@@ -231,36 +257,46 @@ class KvCache:
                                               f"{len(self._free)} free")
         if need > len(held):
             new = [self._free.pop() for _ in range(need - len(held))]
-            self.page_table[seq, len(held): need] = _torch().tensor(new, dtype=_torch().int32)
+            with _stream(stream):
+                self.page_table[seq, len(held): need] = _torch().tensor(new, dtype=_torch().int32)
             held += new
 
-    def release(self, seq: int) -> None:
+    def release(self, seq: int, stream=None) -> None:
         """Gives the pages of slot `seq` back and leaves it idle."""
         if self._free is None:
             raise BackendError("Unsupported", "release: the cache wraps tables of the caller's")
+        if not 0 <= seq < self.n_seqs:
+            raise BackendError("Runtime", f"release: sequence {seq}")
         self._free += self._held[seq]
         self._held[seq] = []
-        self.page_table[seq] = -1
-        self.seq_len[seq] = 0
+        with _stream(stream):
+            self.page_table[seq] = -1
+            self.seq_len[seq] = 0
 
-    def set_lengths(self, lengths, new=None) -> None:
+    def set_lengths(self, lengths, new=None, stream=None) -> None:
         """Tokens of every slot with the next call's new ones, and how many of
-        them are new (None: one each); pages are reserved for them."""
+        them are new (None: one each); pages are reserved for them. The tensors
+        stay in place, so that recorded calls replay on the new values."""
         torch = _torch()
         lengths = [int(n) for n in lengths]
-        if len(lengths) != self.n_seqs or (new is not None and len(new) != self.n_seqs):
+        counts = None if new is None else [int(n) for n in new]
+        if len(lengths) != self.n_seqs or (counts is not None and len(counts) != self.n_seqs):
             raise BackendError("Runtime", f"set_lengths: {self.n_seqs} sequences")
+        for n, m in zip(lengths, counts or [0] * self.n_seqs):
+            if not 0 <= m <= n < 2 ** 30:
+                raise BackendError("Runtime", f"set_lengths: {n} tokens, {m} of them new")
         if self._free is not None:
             for b, n in enumerate(lengths):
-                self.reserve(b, n)
-        self.seq_len.copy_(torch.tensor(lengths, dtype=torch.int32))
-        if new is None:
-            self.use_cu_tokens(None)
-        else:
-            cu = [0]
-            for n in new:
-                cu.append(cu[-1] + int(n))
-            self.use_cu_tokens(torch.tensor(cu, dtype=torch.int32, device=self.device))
+                self.reserve(b, n, stream)
+        with _stream(stream):
+            self.seq_len.copy_(torch.tensor(lengths, dtype=torch.int32))
+            if counts is None:
+                self.use_cu_tokens(None)
+                return
+            if self._own_cu is None:
+                self._own_cu = torch.empty(self.n_seqs + 1, dtype=torch.int32, device=self.device)
+            self._own_cu.copy_(torch.tensor(np.cumsum([0] + counts), dtype=torch.int32))
+            self.use_cu_tokens(self._own_cu)
 
     def use_cu_tokens(self, cu_tokens) -> None:
         """The device tensor [n_seqs + 1] that says which rows of a call are
@@ -272,12 +308,6 @@ class KvCache:
         self.cu_tokens = cu_tokens
         self.desc.cu_tokens = None if cu_tokens is None else cu_tokens.data_ptr()
 
-    def _here(self) -> None:
-        """Launches go to the current device: it has to be the cache's."""
-        if self._devices > 1 and _torch().cuda.current_device() != self.device.index:
-            raise BackendError("Runtime", f"the cache is on {self.device}, the current device is "
-                                          f"cuda:{_torch().cuda.current_device()}")
-
     # -- operators -----------------------------------------------------------
     def append(self, k: int, v: int, kv_stride: int, n_tokens: int, max_new: int, rope=None,
                q: int = 0, q_stride: int = 0, q_out: int | None = None, q_out_stride: int | None = None,
@@ -285,7 +315,9 @@ class KvCache:
         """Rows of k and v (n_kv_heads*head_dim floats, kv_stride apart) into
         the cache, k rotated by `rope` (a RopeTable); q, if given, rotated to
         q_out (in place by default)."""
-        self._here()
+        _on_device(self.device)
+        if rope is not None and rope.table.device != self.device:
+            raise BackendError("Runtime", f"rope table on {rope.table.device}, cache on {self.device}")
         kern.kv_append(self._ref, None if rope is None else rope.ref, k, v, kv_stride, q, q_stride,
                        q if q_out is None else q_out, q_stride if q_out_stride is None else q_out_stride,
                        n_q_heads, n_tokens, max_new, stream)
@@ -302,12 +334,11 @@ class KvCache:
                window: int = 0, out_f16: bool = False, workspace=None, stream=None) -> None:
         """out = attention of q's rows over the cache (scale: head_dim^-0.5).
         Without a workspace, a fresh one comes from torch's caching allocator,
-        tied to the launch stream."""
-        self._here()
+        of the launch stream."""
+        _on_device(self.device)
         if workspace is None:
-            workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
-            if stream is not None:
-                workspace.record_stream(stream)
+            with _stream(stream):
+                workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
         kern.kv_attention(self._ref, q, q_stride, n_q_heads, out, out_stride,
                           _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens, max_new,
                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap, window,
@@ -315,7 +346,7 @@ class KvCache:
 
     def dequant(self, pages: int, n: int, k_out: int, v_out: int, stream=None) -> None:
         """n pages (device int32 ids) as f32 [n][kv head][token][dim]."""
-        self._here()
+        _on_device(self.device)
         kern.kv_dequant(self._ref, pages, n, k_out, v_out, stream)
 
     # -- the same as descriptors of an op chain (q4k.Chain.from_ops) ----------

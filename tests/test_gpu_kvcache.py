@@ -743,6 +743,95 @@ def test_calls_on_two_streams_and_the_default_workspace():
     check(a.astype(np.float64).reshape(want.shape), want, tol, False)
 
 
+def test_default_workspace_beside_work_on_the_current_stream():
+    """The fresh workspace is the launch stream's: what the current stream
+    allocates and fills meanwhile does not lie in it."""
+    import torch
+    note("default workspace, current stream another one")
+    rng = np.random.default_rng(22)
+    both = Both(rng, 1, 60, 2, 128, 128, "i8")
+    random_cache(both, 5)
+    q = torch.randn(1, 8, 128, device="cuda")
+    both.call([7600], [1], True)
+    outs = torch.zeros(32, 1024, device="cuda")
+    n = both.gpu.attention_workspace(8, 1, 1).nbytes
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for i in range(32):
+            both.gpu.attend(q.data_ptr(), 1024, 8, outs[i].data_ptr(), 1024, 1, 1)  # null stream
+            torch.empty(n, dtype=torch.uint8, device="cuda").fill_(255)
+    torch.cuda.synchronize()
+    got = host(outs)
+    assert np.all(np.isfinite(got)) and np.all(got == got[0])
+
+
+def test_set_lengths_in_place_and_refusals():
+    """New lengths reach a chain that was recorded on the old ones, row starts
+    included; counts that cannot be are refused and leave the cache as it was."""
+    import torch
+    from modgrad_amd.kvcache import KvCache
+    from modgrad_amd.q4k import BackendError, Chain
+    note("set_lengths in place")
+    rng = np.random.default_rng(23)
+    c = KvCache.new(n_pages=40, page_tokens=16, n_kv_heads=1, head_dim=64, n_seqs=2, max_pages=20)
+    sim = None
+    kv = torch.empty(8, 2, 64, device="cuda")
+    q, out = torch.empty(8, 4, 64, device="cuda"), torch.zeros(8, 4, 64, device="cuda")
+    c.set_lengths([5, 3], [5, 3])
+    ws = c.attention_workspace(4, 8, 8)
+    chain = Chain.from_ops([c.op_append(kv.data_ptr(), kv.data_ptr() + 256, 128, 8, 8),
+                            c.op_attend(q.data_ptr(), 256, 4, out.data_ptr(), 256, 8, 8, ws)])
+    lens = [0, 0]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for m in ([5, 3], [1, 7], [8, 0], [0, 8], [4, 4]):
+        lens = [a + b for a, b in zip(lens, m)]
+        with torch.cuda.stream(stream):
+            x, y = rng.standard_normal((8, 2, 64)).astype(np.float32), rng.standard_normal((8, 4, 64)).astype(np.float32)
+            kv.copy_(torch.from_numpy(x))
+            q.copy_(torch.from_numpy(y))
+        c.set_lengths(lens, m, stream=stream)
+        chain.launch(stream)
+        stream.synchronize()
+        ids = host(c.page_table)
+        if sim is None:
+            z = lambda t: np.zeros(tuple(t.shape), host(t).dtype)  # noqa: E731
+            sim = ref.Cache(z(c.k), z(c.v), z(c.k_scale), z(c.v_scale), ids.copy(), "i8")
+        sim.table, t = ids.copy(), 0
+        for b in range(2):
+            sim.append(b, lens[b] - m[b], x[t:t + m[b], :1].astype(np.float64), x[t:t + m[b], 1:].astype(np.float64))
+            t += m[b]
+        want, tol = sim.attend(y, lens, m, 0.125)
+        check(host(out).astype(np.float64), want, tol, False)
+    was = host(c.seq_len).copy()
+    for bad in (dict(lengths=[5]), dict(lengths=[5, -1]), dict(lengths=[5, 3], new=[6, 0]),
+                dict(lengths=[5, 3], new=[1, -1]), dict(lengths=[2 ** 30, 3])):
+        with pytest.raises(BackendError):
+            c.set_lengths(**bad)
+    for f in (lambda: c.release(2), lambda: c.release(-1), lambda: c.reserve(2, 1), lambda: c.reserve(0, -1)):
+        with pytest.raises(BackendError):
+            f()
+    assert np.array_equal(host(c.seq_len), was)
+
+
+def test_tensors_of_the_host_are_refused():
+    import torch
+    from modgrad_amd.kvcache import KvCache, RopeTable
+    from modgrad_amd.q4k import BackendError
+    z = lambda *s, dtype=torch.uint8: torch.zeros(*s, dtype=dtype)  # noqa: E731
+    c = KvCache.wrap(z(4, 2, 16, 64), z(4, 2, 64, 16), z(4, 2, dtype=torch.float32), z(4, 2, dtype=torch.float32),
+                     z(3, 2, dtype=torch.int32), z(3, dtype=torch.int32))
+    p = torch.zeros(1024, device="cuda").data_ptr()
+    rope = RopeTable.wrap(z(32, 32, 2, dtype=torch.float32), True)
+    good = KvCache.new(4, 16, 2, 64, 3, 2)
+    for f in (lambda: c.append(p, p, 128, 3, 1), lambda: c.attend(p, 128, 2, p + 2048, 128, 3, 1),
+              lambda: c.dequant(p, 1, p, p), lambda: rope.apply(p, p, p, 1, 1, 64),
+              lambda: good.append(p, p, 128, 3, 1, rope=rope)):
+        with pytest.raises(BackendError):
+            f()
+
+
 @pytest.mark.parametrize("kind", ["chain", "torch graph"])
 def test_decode_steps_recorded_once(kind):
     """append + attention recorded once and replayed with growing lengths, eager

@@ -38,6 +38,12 @@ def _stream(stream):
     return cuda.stream(cuda.default_stream() if stream is None else stream)
 
 
+def _elsewhere(device) -> bool:
+    """Whether a call has to look (_on_device) if its tensors are on the current
+    device: there is nothing else with one GPU, and looking costs a microsecond."""
+    return device.type != "cuda" or _torch().cuda.device_count() > 1
+
+
 def _on_device(device) -> None:
     """Launches go to the current device: the tensors have to be there."""
     cuda = _torch().cuda
@@ -142,7 +148,8 @@ class RopeTable:
         return cls(n_pos, rot, half, RopeScaling.from_gguf(g, factors), stream)
 
     def _hold(self, table, half: bool) -> None:
-        self.table, self.half = table, bool(half)
+        self.table, self.half, self.device = table, bool(half), table.device
+        self._look = _elsewhere(self.device)
         self.n_pos, self.rot_dim = table.shape[0], 2 * table.shape[1]
         self.desc = _lib.Rope(table.data_ptr(), self.n_pos, self.rot_dim,
                               _lib.ROPE_HALF if half else _lib.ROPE_INTERLEAVED)
@@ -151,7 +158,8 @@ class RopeTable:
     def apply(self, x: int, y: int, pos: int, n_tokens: int, n_heads: int, head_dim: int,
               x_stride: int | None = None, y_stride: int | None = None, stream=None) -> None:
         """y = x, [n_tokens][n_heads][head_dim] f32 turned to positions pos."""
-        _on_device(self.table.device)
+        if self._look:
+            _on_device(self.device)
         row = n_heads * head_dim
         kern.rope(x, y, pos, self.ref, n_tokens, n_heads, head_dim,
                   row if x_stride is None else x_stride, row if y_stride is None else y_stride,
@@ -208,6 +216,7 @@ class KvCache:
         for t in (v, k_scale, v_scale, page_table, seq_len):
             if t.device != self.device:
                 raise BackendError("Runtime", "cache: tensors on different devices")
+        self._look = _elsewhere(self.device)
         self._own_cu = None
         self._ref = ctypes.byref(self.desc)
         self._free = None
@@ -315,9 +324,10 @@ class KvCache:
         """Rows of k and v (n_kv_heads*head_dim floats, kv_stride apart) into
         the cache, k rotated by `rope` (a RopeTable); q, if given, rotated to
         q_out (in place by default)."""
-        _on_device(self.device)
-        if rope is not None and rope.table.device != self.device:
-            raise BackendError("Runtime", f"rope table on {rope.table.device}, cache on {self.device}")
+        if self._look:
+            _on_device(self.device)
+        if rope is not None and (self._look or rope._look) and rope.device != self.device:
+            raise BackendError("Runtime", f"rope table on {rope.device}, cache on {self.device}")
         kern.kv_append(self._ref, None if rope is None else rope.ref, k, v, kv_stride, q, q_stride,
                        q if q_out is None else q_out, q_stride if q_out_stride is None else q_out_stride,
                        n_q_heads, n_tokens, max_new, stream)
@@ -335,7 +345,8 @@ class KvCache:
         """out = attention of q's rows over the cache (scale: head_dim^-0.5).
         Without a workspace, a fresh one comes from torch's caching allocator,
         of the launch stream."""
-        _on_device(self.device)
+        if self._look:
+            _on_device(self.device)
         if workspace is None:
             with _stream(stream):
                 workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
@@ -346,7 +357,8 @@ class KvCache:
 
     def dequant(self, pages: int, n: int, k_out: int, v_out: int, stream=None) -> None:
         """n pages (device int32 ids) as f32 [n][kv head][token][dim]."""
-        _on_device(self.device)
+        if self._look:
+            _on_device(self.device)
         kern.kv_dequant(self._ref, pages, n, k_out, v_out, stream)
 
     # -- the same as descriptors of an op chain (q4k.Chain.from_ops) ----------

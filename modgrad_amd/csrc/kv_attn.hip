@@ -24,9 +24,9 @@
 //
 // Softmax in base 2 with V's scale in the exponent: t_j = s_j log2 e +
 // log2(vs), M the running maximum of t, w_j = 2^(t_j - M + 14) = p_j * vs *
-// const, O += w_j V8_j, l += w_j / vs. So w_j <= 2^14 whatever the scales are:
-// its f16 hi + lo pair keeps 22 bits down to 2^-24 of the largest. M, l and O
-// are f32.
+// const, O += w_j V8_j, l += w_j / vs. M may lag by 1, so w_j < 2^15 whatever the
+// scales are: its f16 hi + lo pair keeps 22 bits down to 2^-24 of the largest. M,
+// l and O are f32.
 //
 // int8 K skips the conversion: q goes in as three digits of 8 bits on the int8
 // matrix cores (v_mfma_i32_16x16x64_i8), whose sums are exact.
@@ -44,6 +44,10 @@
 // and less are one part. The wavefronts of a work-group take tiles in turn, each
 // with its own softmax state, joined through LDS; a row in several parts leaves
 // their states in the workspace for kv_attn_join_kernel.
+//
+// Bound by the cache's bytes (28 heads on 4 of 128): 32 ragged sequences to 32 Ki
+// tokens, e4m3, 380 MB: 81 us + 4.9 for the join, 4.7 TB/s; 200 000 tokens, int8,
+// 205 MB: 42 + 5 us. A sequence of 1000 tokens is latency: 9 + 3 us.
 #include "kv_attn.hpp"
 
 namespace mgq {

@@ -8,7 +8,7 @@ namespace mgq {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;    // tokens of a tile
-constexpr float kTop = 14.0f;  // the largest w is 2^14
+constexpr float kTop = 14.0f;  // w is 2^14 at the running maximum
 constexpr float kLeastScale = 0x1p-90f;  // smaller scales of V count as this
 
 struct AttnArgs {
@@ -51,7 +51,6 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ float ldexp2(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
-
 
 // The larger of each of the 4 lanes l, l^16, l^32, l^48.
 __device__ __forceinline__ float max_groups(float x) {

@@ -341,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                     top = fmaxf(top, s);
                 }
             top = max_groups(top);
-            if (__any(top > M + 1.0f)) {  // the maximum may lag by 1: w stays below 2^15
+            if (__any(outgrown(top, M))) {  // the maximum may lag by 1: w stays below 2^15
                 const float m = fmaxf(M, top);
                 const float fac = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
                 M = m;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
 #pragma unroll
                 for (int d = 0; d < DB; ++d) O[d] *= fac;
             }
-            const float ref = M == -INFINITY ? 0.0f : M - kTop;
+            const float ref = reference_of(M);
             float sum = 0.0f;
             half8 ph[2], pl[2];
 #pragma unroll

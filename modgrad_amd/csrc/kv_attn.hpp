@@ -23,6 +23,15 @@ struct AttnArgs {
     float *ws;
 };
 
+// What a running maximum is compared with and taken from: w = 2^(t - ref). Where
+// numbers as large as M lie 4 and more apart, M - kTop may be off by more than f16 has
+// room for (2^15 to 2^16): ref is M there.
+__device__ __forceinline__ bool outgrown(float top, float M) { return top - M > 1.0f; }
+__device__ __forceinline__ float reference_of(float M) {
+    const float r = M - kTop;
+    return M == -INFINITY ? 0.0f : M - r > kTop + 0.5f ? M : r;
+}
+
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap);

@@ -340,7 +340,10 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         half8 ph[SETS][2], pl[SETS][2];
 #pragma unroll
         for (int s = 0; s < SETS; ++s) {
-            float sc = qs[s] * ks;
+            float sc = qs[s] * ks, add = lv;
+            // scores that may reach 2^19: t is rounded once, below, so that no
+            // w passes the largest
+            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f : __any(sc >= 0x1p-12f));
             if (a.softcap > 0.0f) {
                 float far = 0.0f;
 #pragma unroll
@@ -370,25 +373,26 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                 }
                 sc = 1.0f;
             }
-            if (!clear) {
+            if (exact) {
                 const int at = first + 16 * grp;
                 const int see = min(pos[s] + 1 - at, nv), skip = a.window > 0 ? pos[s] - a.window + 1 - at : 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? S[s][i][e] * sc : -INFINITY;
+                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e], sc, lv) : -INFINITY;
                 sc = 1.0f;
+                add = 0.0f;
             }
-            // the largest of t = S * sc + lv: sc, a lane's own, is not negative
+            // the largest of t = S * sc + add: sc, a lane's own, is not negative
             float hi = S[s][0][0];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
-            const float top = max_groups(fmaf(hi, sc, lv));
+            const float top = max_groups(fmaf(hi, sc, add));
             // the maximum may lag by 1: w stays below 2^15
-            if (__any(top > M[s] + 1.0f)) {
+            if (__any(outgrown(top, M[s]))) {
                 const float m = fmaxf(M[s], top);
                 const float fac = M[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[s] - m);
                 M[s] = m;
@@ -396,7 +400,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int d = 0; d < DB; ++d) O[s][d] *= fac;
             }
-            const float off = lv - (M[s] == -INFINITY ? 0.0f : M[s] - kTop);
+            const float off = add - reference_of(M[s]);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)

@@ -495,6 +495,32 @@ def test_lengths_that_do_not_fit_the_rows(new):
         assert p in held or np.array_equal(before[p], after[p])
 
 
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("new,dim", [(1, 64), (3, 128), (70, 64), (70, 128), (40, 256)])
+def test_attention_of_huge_scores(new, dim, fmt):
+    """Scores from 1e4 to 1e12, where the distance of two f32 numbers passes the
+    room that f16 weights have: results stay within the values attended to."""
+    import torch
+    note(f"attention of huge scores new={new} dim={dim} {fmt}")
+    rng = np.random.default_rng(dim + new)
+    both = Both(rng, 1, 20, 1, dim, 32, fmt)
+    random_cache(both, 9)
+    both.ref.k[:], both.ref.v[:] = host(both.k), host(both.v)
+    both.ref.ks[:], both.ref.vs[:] = host(both.ks), host(both.vs)
+    n = 20 * 32 - 5
+    both.call([n], [new], new == 1)
+    top = max(np.abs(both.ref.read(0, 0, n)[1]).max(), 0.0)
+    q = rng.standard_normal((new, 12, dim)).astype(np.float32)
+    for f in 10.0 ** np.arange(4, 13, 0.5):
+        x = q * np.float32(f)
+        xt = dev(x)
+        for f16 in (False, True):
+            out = torch.full((new, 12, dim), 7.0, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+            both.gpu.attend(xt.data_ptr(), 12 * dim, 12, out.data_ptr(), 12 * dim, new, new, scale=1.0, out_f16=f16)
+            got = host(out).astype(np.float64)
+            assert np.all(np.abs(got) <= top * (1 + 2.0 ** -10)), (f, f16)
+
+
 @pytest.mark.parametrize("seqs,pages,heads,group,dim,new,fmt", [
     (1, 60, 1, 4, 128, 1, "i8"),      # parts of one row
     (2, 60, 1, 1, 96, 3, "e4m3"),

@@ -4,18 +4,18 @@
 //
 // A work-group has 128 query rows of one (sequence, kv head): row r is new token
 // r / group, head r % group of the group, so the rows of a group's heads share
-// the tile. 4 wavefronts of 32 rows (two sets of 16 columns of S^T). Each tile
-// of 64 tokens is converted to f16 ONCE on its way into LDS (a 4-byte word
-// costs 5 operations; each wavefront converts a quarter), as the operands the
-// matrix cores take: 16 bytes of each of 64 lanes one after another, so every
-// LDS access is a contiguous 1 KiB. One operand read feeds four products of S
-// (two sets, q's hi and lo) and two (out f16) or four (out f32) of O.
+// the tile. 4 wavefronts of 32 rows (two sets of 16 columns of S^T), or 8 of 16.
+// Each tile of 64 tokens is converted to f16 ONCE on its way into LDS (V, and K
+// unless it is int8: a 4-byte word costs 5 operations, shared by the wavefronts),
+// as the operands the matrix cores take: 16 bytes of each of 64 lanes one after
+// another, so every LDS access is a contiguous 1 KiB. One operand read feeds a
+// set's two or three digits or halves of q, and one (f16 result) or two (f32) of p.
 //
 // Tile i+2's bytes load into registers and tile i+1's go to the other LDS
 // buffer while tile i multiplies; one barrier a tile, which does not wait for
 // the loads. Bound by the softmax's exponentials and conversions on the vector
 // ALU, which issues in 70 % of the cycles of a 4096-token prompt of 28 heads of
-// 128 on int8 (150 us, 800 TFLOP/s counted as 4 D a pair), beside the matrix
+// 128 on int8 (149 us, 807 TFLOP/s counted as 4 D a pair), beside the matrix
 // cores (34 %): the second wavefront of each SIMD overlaps the two. Pieces of up
 // to 250 tokens over 9000, 16 heads of 256 on e4m3 with f32 results and a softcap: 95
 // + 11 us for the join, the products twice a plain f16 attention's.
@@ -121,9 +121,10 @@ __device__ __forceinline__ void wide_barrier() {
 // Compile-time shape of the kernel. int8 K goes into the int8 matrix cores as it
 // is, q as digits of 8 bits: 16 bits for an f16 result, 24 for f32 (heads of 96
 // are no multiple of the 64 dims of such a product).
-// SETS of 16 query rows a wavefront. One set and 8 wavefronts leave a wavefront
-// few enough registers for 4 (heads of 256: 2) on a SIMD, two sets and 4
-// wavefronts read LDS half as often; which is the faster was measured.
+// SETS of 16 query rows a wavefront: two sets and 4 wavefronts read LDS half as
+// often, one and 8 wavefronts where two spill. Measured: a prompt of heads of 128
+// with f16 results 191 us with two, 220 with one; pieces of heads of 256 with f32
+// results 192 and 126.
 template <int D, int FMT, bool LO>
 struct WideShape {
     static constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
@@ -292,6 +293,14 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
         f32x4 S[SETS][4] = {};
+        // Two digits: their sums (below 2^22 either way) start from the bits of
+        // 1.5 * 2^23, so that as f32 they are that number plus the sum, and the score
+        // is one operation, off by kBias, which goes into the exponent's offset (an
+        // addition and a conversion before: a 4096-token prompt 5 % longer, in turn).
+        // Both that score and the offset are rounded by about half of what q's
+        // digits are off by over 128 dims.
+        constexpr bool kBiased = I8 && !LO;
+        constexpr float kBias = kBiased ? 257.0f * 12582912.0f : 0.0f;
         if constexpr (I8) {
             if (!W::kAhead) read_k();
 #pragma unroll
@@ -299,6 +308,10 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int s = 0; s < SETS; ++s) {
                     i32x4 d[ND] = {};
+                    if (kBiased) {
+#pragma unroll
+                        for (int n = 0; n < ND; ++n) d[n] = i32x4{0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000};
+                    }
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -307,7 +320,10 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (LO) S[s][i][e] = fmaf((float)(d[2][e] * 256 + d[1][e]), 256.0f, (float)d[0][e]);
-                        else S[s][i][e] = (float)(d[1][e] * 256 + d[0][e]);
+                        else {
+                            const int d1 = d[1][e], d0 = d[0][e];
+                            S[s][i][e] = fmaf(__builtin_bit_cast(float, d1), 256.0f, __builtin_bit_cast(float, d0));
+                        }
                     }
                 }
             }
@@ -340,17 +356,18 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         half8 ph[SETS][2], pl[SETS][2];
 #pragma unroll
         for (int s = 0; s < SETS; ++s) {
-            float sc = qs[s] * ks, add = lv;
-            // scores that may reach 2^19: t is rounded once, below, so that no
-            // w passes the largest
-            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f : __any(sc >= 0x1p-12f));
+            float sc = qs[s] * ks, add = lv, bias = kBias;
+            // scores that may reach 2^19 (with kBias, an offset of 2^14): t is rounded
+            // once, below, so that no w passes the largest
+            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f
+                                                           : __any(sc >= (kBiased ? 0x1p-17f : 0x1p-12f)));
             if (a.softcap > 0.0f) {
                 float far = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        S[s][i][e] *= sc;
+                        S[s][i][e] = (S[s][i][e] - kBias) * sc;
                         far = fmaxf(far, fabsf(S[s][i][e]));
                     }
                 if (!__any(far >= kCapNear)) {  // scores are rarely beyond a third of their bound
@@ -372,6 +389,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                         }
                 }
                 sc = 1.0f;
+                bias = 0.0f;
             }
             if (exact) {
                 const int at = first + 16 * grp;
@@ -380,8 +398,9 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e], sc, lv) : -INFINITY;
+                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e] - bias, sc, lv) : -INFINITY;
                 sc = 1.0f;
+                bias = 0.0f;
                 add = 0.0f;
             }
             // the largest of t = S * sc + add: sc, a lane's own, is not negative
@@ -390,7 +409,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
-            const float top = max_groups(fmaf(hi, sc, add));
+            const float top = max_groups(fmaf(hi - bias, sc, add));
             // the maximum may lag by 1: w stays below 2^15
             if (__any(outgrown(top, M[s]))) {
                 const float m = fmaxf(M[s], top);
@@ -400,7 +419,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int d = 0; d < DB; ++d) O[s][d] *= fac;
             }
-            const float off = add - reference_of(M[s]);
+            const float off = fmaf(-bias, sc, add - reference_of(M[s]));
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)

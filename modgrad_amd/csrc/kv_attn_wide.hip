@@ -122,13 +122,14 @@ __device__ __forceinline__ void wide_barrier() {
 // is, q as digits of 8 bits: 16 bits for an f16 result, 24 for f32 (heads of 96
 // are no multiple of the 64 dims of such a product).
 // SETS of 16 query rows a wavefront: two sets and 4 wavefronts read LDS half as
-// often, one and 8 wavefronts where two spill. Measured: a prompt of heads of 128
-// with f16 results 191 us with two, 220 with one; pieces of heads of 256 with f32
-// results 192 and 126.
+// often; one and 8 wavefronts where two spill more than that is worth. Measured
+// (two, one; us for 4096 tokens of 28 heads): heads of 64 to f32 166, 197, on e4m3
+// to f16 129, 157; of 96 156, 198; of 128 on e4m3 to f32 239, 248, on int8 to f32
+// 449, 250; pieces of heads of 256 to f32 192, 126.
 template <int D, int FMT, bool LO>
 struct WideShape {
     static constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
-    static constexpr int SETS = D == 64 || D == 256 || (D == 128 && LO) ? 1 : 2;
+    static constexpr int SETS = D == 256 || (D == 128 && LO && FMT == kFmtI8) ? 1 : 2;
     static constexpr int NW = kWideRows / (16 * SETS);      // wavefronts
     static constexpr int kThreads = 64 * NW, kPerSimd = 2;
     static constexpr bool kAhead = kPerSimd <= 2;           // registers for operands ahead of their use

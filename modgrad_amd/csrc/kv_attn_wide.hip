@@ -294,14 +294,6 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
         f32x4 S[SETS][4] = {};
-        // Two digits: their sums (below 2^22 either way) start from the bits of
-        // 1.5 * 2^23, so that as f32 they are that number plus the sum, and the score
-        // is one operation, off by kBias, which goes into the exponent's offset (an
-        // addition and a conversion before: a 4096-token prompt 5 % longer, in turn).
-        // Both that score and the offset are rounded by about half of what q's
-        // digits are off by over 128 dims.
-        constexpr bool kBiased = I8 && !LO;
-        constexpr float kBias = kBiased ? 257.0f * 12582912.0f : 0.0f;
         if constexpr (I8) {
             if (!W::kAhead) read_k();
 #pragma unroll
@@ -309,22 +301,16 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int s = 0; s < SETS; ++s) {
                     i32x4 d[ND] = {};
-                    if (kBiased) {
-#pragma unroll
-                        for (int n = 0; n < ND; ++n) d[n] = i32x4{0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000};
-                    }
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
                         for (int n = 0; n < ND; ++n) d[n] = mfma16(kx[i][k], qd[s][n][k], d[n]);
-                    // two digits' sums stay below 2^31; the third joins in f32
+                    // two digits' sums stay below 2^31 and join as whole numbers, so that the
+                    // score is rounded once, to f32; the third joins in f32
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (LO) S[s][i][e] = fmaf((float)(d[2][e] * 256 + d[1][e]), 256.0f, (float)d[0][e]);
-                        else {
-                            const int d1 = d[1][e], d0 = d[0][e];
-                            S[s][i][e] = fmaf(__builtin_bit_cast(float, d1), 256.0f, __builtin_bit_cast(float, d0));
-                        }
+                        else S[s][i][e] = (float)(d[1][e] * 256 + d[0][e]);
                     }
                 }
             }
@@ -357,18 +343,17 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         half8 ph[SETS][2], pl[SETS][2];
 #pragma unroll
         for (int s = 0; s < SETS; ++s) {
-            float sc = qs[s] * ks, add = lv, bias = kBias;
-            // scores that may reach 2^19 (with kBias, an offset of 2^14): t is rounded
-            // once, below, so that no w passes the largest
-            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f
-                                                           : __any(sc >= (kBiased ? 0x1p-17f : 0x1p-12f)));
+            float sc = qs[s] * ks, add = lv;
+            // scores that may reach 2^19: t is rounded once, below, so that no w passes
+            // the largest
+            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f : __any(sc >= 0x1p-12f));
             if (a.softcap > 0.0f) {
                 float far = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        S[s][i][e] = (S[s][i][e] - kBias) * sc;
+                        S[s][i][e] *= sc;
                         far = fmaxf(far, fabsf(S[s][i][e]));
                     }
                 if (!__any(far >= kCapNear)) {  // scores are rarely beyond a third of their bound
@@ -390,7 +375,6 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                         }
                 }
                 sc = 1.0f;
-                bias = 0.0f;
             }
             if (exact) {
                 const int at = first + 16 * grp;
@@ -399,9 +383,8 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e] - bias, sc, lv) : -INFINITY;
+                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e], sc, lv) : -INFINITY;
                 sc = 1.0f;
-                bias = 0.0f;
                 add = 0.0f;
             }
             // the largest of t = S * sc + add: sc, a lane's own, is not negative
@@ -410,7 +393,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
-            const float top = max_groups(fmaf(hi - bias, sc, add));
+            const float top = max_groups(fmaf(hi, sc, add));
             // the maximum may lag by 1: w stays below 2^15
             if (__any(outgrown(top, M[s]))) {
                 const float m = fmaxf(M[s], top);
@@ -420,7 +403,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int d = 0; d < DB; ++d) O[s][d] *= fac;
             }
-            const float off = fmaf(-bias, sc, add - reference_of(M[s]));
+            const float off = add - reference_of(M[s]);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)

@@ -355,7 +355,9 @@ hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_ro
  * seq_len and cu_tokens describe a call: sequence b has seq_len[b] tokens,
  * the call's new ones included, and rows cu_tokens[b] .. cu_tokens[b+1]-1 of
  * the call's q, k and v are its last ones. cu_tokens null: row b is the one
- * new token of sequence b. A sequence with seq_len 0 is an idle slot.
+ * new token of sequence b. A sequence with seq_len 0 is an idle slot. Row starts
+ * must not fall; a sequence whose range falls or leaves the call's n_tokens rows
+ * has none, and a row that two ranges hold gets what either sequence writes.
  * These arrays are device memory, read when the kernels run, so a recorded
  * call replays on the lengths of the day. */
 typedef struct mgq_kv_cache {

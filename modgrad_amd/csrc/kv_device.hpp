@@ -24,30 +24,30 @@ struct KvView {
 
 // The new tokens of sequence b: rows t0 .. t0+n-1, at positions pos0 .. ;
 // `len` tokens of the cache are behind the table. cu, len and the table are
-// device data the host has not seen: n is clamped to what the launch covers
-// and to the rows that exist, and pos0 to 2^30 either way (a sequence holds fewer
-// tokens), so that no index leaves a buffer and no position wraps whatever they hold.
+// device data the host has not seen: rows that fall or do not lie in the call's
+// are none (a clamped range could be another sequence's rows too, which both
+// would then write), n is clamped to what the launch covers, and pos0 to 2^30
+// either way (a sequence holds fewer tokens), so that no index leaves a buffer and
+// no position wraps whatever they hold.
 struct SeqInfo {
     int t0, n, pos0, len;
 };
-__device__ __forceinline__ SeqInfo kv_seq(const KvView &c, int b) {
+__host__ __device__ __forceinline__ SeqInfo kv_seq(const KvView &c, int b) {
     SeqInfo s;
     const int len = c.len[b];
     s.t0 = b;
-    int n = 1;
+    int end = b + 1;
     if (c.cu) {
         s.t0 = c.cu[b];
-        n = (int)((unsigned)c.cu[b + 1] - (unsigned)s.t0);
+        end = c.cu[b + 1];
     }
+    int n = s.t0 >= 0 && s.t0 <= end && end <= c.n_tokens ? end - s.t0 : 0;
     const int cap = c.max_pages << c.page_shift;
     constexpr int64_t kFar = INT64_C(1) << 30;
     const int64_t pos = (int64_t)len - n;
     s.pos0 = (int)(pos < -kFar ? -kFar : pos > kFar ? kFar : pos);
     s.len = len < 0 ? 0 : (len < cap ? len : cap);
-    if (n > c.max_new) n = c.max_new;
-    if (s.t0 < 0 || n < 0 || s.t0 >= c.n_tokens) n = 0;
-    else if (n > c.n_tokens - s.t0) n = c.n_tokens - s.t0;
-    s.n = n;
+    s.n = n > c.max_new ? c.max_new : n;
     return s;
 }
 

@@ -345,8 +345,10 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         for (int s = 0; s < SETS; ++s) {
             float sc = qs[s] * ks, add = lv;
             // scores that may reach 2^19: t is rounded once, below, so that no w passes
-            // the largest
-            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f : __any(sc >= 0x1p-12f));
+            // the largest. S is below 2^38 (three digits of q, 256 products with an int8
+            // code), 2^30 (two) or 2^31 (q's halves below 2^14, e4m3 codes to 448).
+            constexpr float kFarScale = !I8 ? 0x1p-12f : LO ? 0x1p-19f : 0x1p-11f;
+            const bool exact = !clear || (a.softcap > 0.0f ? a.softcap > 0x1p19f : __any(sc >= kFarScale));
             if (a.softcap > 0.0f) {
                 float far = 0.0f;
 #pragma unroll

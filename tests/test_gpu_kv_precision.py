@@ -83,3 +83,52 @@ def test_rms_of_the_error(fmt, dim, new, rms):
     # a few hundred weights count, so that the rms of their roundings is its
     # expectation to about 4 %: five times that
     assert err[True] <= 1.2 * float((var / size).sqrt()) + F32, (err, float((var / size).sqrt()))
+
+
+@pytest.mark.parametrize("peak", [False, True])
+@pytest.mark.parametrize("fmt,dim", [("i8", 64), ("i8", 96), ("i8", 128), ("i8", 256), ("e4m3", 128), ("e4m3", 256)])
+def test_scores_at_the_bounds_of_their_sums(fmt, dim, peak):
+    """q constant and K at its largest code, so that the sums of products reach
+    their bounds, over scales that take the scores from 1e3 to 1e9: every token
+    counts alike, or one alone."""
+    import torch
+    note(f"scores at the bounds {fmt} dim={dim} peak={peak}")
+    n, new, page = 330, 60, 32
+    both = Both(np.random.default_rng(dim), 1, -(-n // page), 1, dim, page, fmt)
+    most, less = (127, 100) if fmt == "i8" else (0x7E, 0x7C)  # 448, 384
+    both.k.fill_(less if peak else most)
+    both.k[int(both.ref.table[0, 0]), 0, 10] = most
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    v = torch.randn(both.v.shape, generator=g, device="cuda").mul(40).clamp(-127, 127)
+    both.v.copy_((v.to(torch.int8) if fmt == "i8" else v.to(torch.float8_e4m3fn)).view(torch.uint8))
+    both.ks.fill_(2.0 ** -6)
+    both.vs.fill_(2.0 ** -7)
+    grid = torch.from_numpy(ref.grid(fmt)).cuda()
+    ids = torch.from_numpy(both.ref.table[0]).cuda().long()
+    v = (grid[both.v[ids].long()] * 2.0 ** -7).permute(1, 0, 3, 2).reshape(-1, dim)[:n]
+    count = (n - new + 1 + torch.arange(new, device="cuda", dtype=torch.float64))[:, None]
+    if peak:
+        want, size = v[10].expand(new, dim), v[10].abs().expand(new, dim)
+    else:
+        want, size = (y.cumsum(0)[n - new:] / count for y in (v, v.abs()))
+    both.call([n], [new])
+    q = torch.ones(new, dim, device="cuda")
+    for f16 in (False, True):
+        out = torch.empty(new, dim, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+        top = grid[most].item() * 2.0 ** -6 * dim  # q . k
+        for score in 10.0 ** np.linspace(3, 9, 301):
+            out.fill_(7.0)
+            both.gpu.attend(q.data_ptr(), dim, 1, out.data_ptr(), dim, new, new, scale=score / top, out_f16=f16)
+            off = (out.double() - want).abs()
+            # sums of equal weights in f32, weights of 22 bits. Equal scores t in base 2
+            # have equal weights where each is rounded to f32 by itself. Below 2^19 a tile
+            # that all rows see all of may take t less its reference in one step, and the
+            # other tiles round t first (2^-24 t): its largest (2^-24 t) and its offset
+            # (2^-24 t) are rounded instead, and its weights are off from theirs by
+            # 3 * 2^-24 t ln 2.
+            t = score / np.log(2) + 7
+            e = (96 + n / 32) * 2.0 ** -24 + 2.0 ** -22 + (3 * 2.0 ** -24 * t * np.log(2) if t < 2 ** 19 else 0.0)
+            # f16: weights of 11 bits, all rounded alike, and the result's own rounding
+            most_off = e * (size + want.abs()) + (2.0 ** -10 * want.abs() + 2.0 ** -24 if f16 else 0)
+            assert bool((off <= most_off).all()), (f16, score, float((off / most_off).max()))

@@ -118,7 +118,7 @@ __device__ __forceinline__ float split_query(const float (&v)[D / 4], half8 (&qh
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     int ex = 0;
-    if (top > 0.0f && top < 3.4e38f) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+    if (top > 0.0f && top < INFINITY) ex = 14 - __builtin_amdgcn_frexp_expf(top);
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
         const float x = ldexp2(v[i], ex);
@@ -150,7 +150,7 @@ __device__ __forceinline__ float split_query(const float (&v)[D / 4], i32x4 (&qd
     bad += __shfl_xor(bad, 32, 64);
     int ex = 0;
     float mant = 1.0f;  // top = mant * 2^ex
-    if (top > 0.0f && top < 3.4e38f) {
+    if (top > 0.0f && top < INFINITY) {
         ex = __builtin_amdgcn_frexp_expf(top);
         mant = __builtin_amdgcn_frexp_mantf(top);
     }

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 from tests import kv_reference as ref
-from tests.test_gpu_kvcache import Both, note
+from tests.gpu_util import dev, host
+from tests.test_gpu_kvcache import Both, check, fill, note
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +133,28 @@ def test_scores_at_the_bounds_of_their_sums(fmt, dim, peak):
             # f16: weights of 11 bits, all rounded alike, and the result's own rounding
             most_off = e * (size + want.abs()) + (2.0 ** -10 * want.abs() + 2.0 ** -24 if f16 else 0)
             assert bool((off <= most_off).all()), (f16, score, float((off / most_off).max()))
+
+
+def ends(fmt, dim, new, f16, q, scale):
+    """Attention over 100 tokens in two pages of 64 for these queries, against the reference."""
+    import torch
+    both = Both(np.random.default_rng(3), 1, 2, 1, dim, 64, fmt)
+    fill(both, np.random.default_rng(4), [100])
+    both.call([100], [new], new == 1)
+    out = torch.full((new, 4, dim), 7.0, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+    both.gpu.attend(dev(q).data_ptr(), 4 * dim, 4, out.data_ptr(), 4 * dim, new, new, scale=scale, out_f16=f16)
+    want, tol = both.ref.attend(q, [100], [new], scale)
+    check(host(out).astype(np.float64), want, tol, f16)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("fmt,dim", [("i8", 64), ("i8", 96), ("i8", 128), ("e4m3", 64), ("e4m3", 256)])
+def test_queries_up_to_the_largest_f32(fmt, dim, new, f16):
+    """Rows whose largest value is 3.4e38 to 3.4028e38, finite as all others."""
+    note(f"queries up to the largest f32 {fmt} dim={dim} new={new} f16={f16}")
+    rng = np.random.default_rng(dim + new)
+    q = (rng.uniform(-1, 1, (new, 4, dim)) * 1e38).astype(np.float32)
+    q[:, 0, 3], q[:, 1, 7], q[:, 2, 0] = 3.401e38, -np.finfo(np.float32).max, 3.3999e38
+    q[:, 1, 8:] *= np.float32(0.01)
+    ends(fmt, dim, new, f16, q, 3e-38 / np.sqrt(dim))

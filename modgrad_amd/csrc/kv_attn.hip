@@ -290,9 +290,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         i32x4 qd[3][I8 ? KS : 1];
 #pragma unroll
         for (int i = 0; i < KB; ++i) qv[i] = live ? qv[i] : 0.0f;
-        float kscale = a.scale;
-        if constexpr (I8) kscale *= split_query<D, 3>(qv, qd);
-        else kscale *= split_query<D>(qv, qh, ql);
+        float kscale;
+        if constexpr (I8) kscale = split_query<D, 3>(a.scale, qv, qd);
+        else kscale = split_query<D>(a.scale, qv, qh, ql);
 
         f32x4 O[DB] = {};
         float M = -INFINITY, l = 0.0f;

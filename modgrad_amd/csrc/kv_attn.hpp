@@ -108,9 +108,10 @@ __device__ __forceinline__ void read_query(const float *qp, float (&v)[D / 4]) {
 // A query row's dims grp*KB .. +KB-1 (KB = D/4) as f16 hi + lo pairs of the row
 // times 2^ex, the largest of the row in [2^13, 2^14): 22 bits of every value
 // that is not 2^-24 of the largest. Lanes l, l^16, l^32, l^48 share a row.
-// Returns 2^-ex.
+// Returns scale * 2^-ex: 2^-ex by itself is 0 for the smallest rows.
 template <int D>
-__device__ __forceinline__ float split_query(const float (&v)[D / 4], half8 (&qh)[D / 32], half8 (&ql)[D / 32]) {
+__device__ __forceinline__ float split_query(float scale, const float (&v)[D / 4], half8 (&qh)[D / 32],
+                                             half8 (&ql)[D / 32]) {
     constexpr int KB = D / 4;
     float top = 0.0f;
 #pragma unroll
@@ -126,16 +127,17 @@ __device__ __forceinline__ float split_query(const float (&v)[D / 4], half8 (&qh
         qh[i / 8][i % 8] = hi;
         ql[i / 8][i % 8] = (_Float16)(x - (float)hi);
     }
-    return ldexp2(1.0f, -ex);
+    return ldexp2(scale, -ex);
 }
 
 // The same row as N signed digits of 8 bits, 16 dims to a register quad: the
 // row times a factor that takes its largest to 0x7F7F.. (all digits 127),
 // rounded to whole numbers; for the int8 matrix cores, whose products with an
-// 8-bit K and their sums are exact. Returns the factor's inverse; a row with a
-// NaN or infinity returns NaN.
+// 8-bit K and their sums are exact. Returns scale over the factor (the power of two
+// first, so that neither the smallest nor the largest rows leave f32 on the way); a
+// row with a NaN or infinity returns NaN.
 template <int D, int N>
-__device__ __forceinline__ float split_query(const float (&v)[D / 4], i32x4 (&qd)[N][D / 64]) {
+__device__ __forceinline__ float split_query(float scale, const float (&v)[D / 4], i32x4 (&qd)[N][D / 64]) {
     constexpr int KB = D / 4;
     constexpr float kMost = (float)(N == 2 ? 0x7F7F : 0x7F7F7F);
     float top = 0.0f, bad = 0.0f;
@@ -171,7 +173,8 @@ __device__ __forceinline__ float split_query(const float (&v)[D / 4], i32x4 (&qd
 #pragma unroll
         for (int n = 0; n < N; ++n) qd[n][i / 16][i / 4 % 4] = (int)w[n];
     }
-    return ldexp2(mant / kMost, ex) + bad;
+    constexpr int kBits = 8 * N - 1;  // kMost is just below 2^kBits
+    return ldexp2(scale, ex - kBits) * (mant * ((float)(1 << kBits) / kMost)) + bad;
 }
 
 // The first nv of a lane's 16 tokens of V kept, the bytes of the others (they

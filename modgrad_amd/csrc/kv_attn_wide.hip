@@ -261,8 +261,8 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     fetch(t0);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
-        if constexpr (I8) qs[s] = a.scale * split_query<D, ND>(qv[s], qd[s]);
-        else qs[s] = a.scale * split_query<D>(qv[s], qh[s], ql[s]);
+        if constexpr (I8) qs[s] = split_query<D, ND>(a.scale, qv[s], qd[s]);
+        else qs[s] = split_query<D>(a.scale, qv[s], qh[s], ql[s]);
     }
     stage(lds);
     float ks_c = ks_n, vs_c = vs_n;

@@ -158,3 +158,16 @@ def test_queries_up_to_the_largest_f32(fmt, dim, new, f16):
     q[:, 0, 3], q[:, 1, 7], q[:, 2, 0] = 3.401e38, -np.finfo(np.float32).max, 3.3999e38
     q[:, 1, 8:] *= np.float32(0.01)
     ends(fmt, dim, new, f16, q, 3e-38 / np.sqrt(dim))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size", [1e-36, 1e-38, 1e-40])
+@pytest.mark.parametrize("fmt,dim", [("i8", 64), ("i8", 96), ("i8", 128), ("e4m3", 64), ("e4m3", 256)])
+def test_queries_down_to_the_smallest_f32(fmt, dim, size, new, f16):
+    """Rows near and below the smallest normal number, under scales that bring the
+    scores back."""
+    note(f"queries of {size} {fmt} dim={dim} new={new} f16={f16}")
+    rng = np.random.default_rng(dim + new)
+    q = (rng.uniform(-1, 1, (new, 4, dim)) * size).astype(np.float32)
+    ends(fmt, dim, new, f16, q, min(3.0 / size, 2e38) / np.sqrt(dim))

@@ -72,13 +72,14 @@ class RopeScaling:
     @classmethod
     def from_gguf(cls, g, factors=None) -> "RopeScaling":
         """From an opened GgufFile's <arch>.rope.* keys: freq_base,
-        scaling.type ("none", "linear", "yarn"), scaling.factor,
+        scaling.type ("none", "linear", "yarn"; a factor without a type is
+        linear), scaling.factor (older files: rope.scale_linear),
         scaling.attn_factor, scaling.original_context_length."""
         arch = g.architecture()
         base = g.meta_f32(f"{arch}.rope.freq_base") or 10000.0
         m = g.meta(f"{arch}.rope.scaling.type")
-        kind = m.as_str() if m is not None else "none"
-        factor = g.meta_f32(f"{arch}.rope.scaling.factor") or 1.0
+        kind = m.as_str() if m is not None else "linear"
+        factor = g.meta_f32(f"{arch}.rope.scaling.factor") or g.meta_f32(f"{arch}.rope.scale_linear") or 1.0
         attn = g.meta_f32(f"{arch}.rope.scaling.attn_factor") or 1.0
         if kind not in ("none", "linear", "yarn"):
             raise BackendError("Unsupported", f"rope scaling type {kind!r}")

@@ -232,3 +232,23 @@ def test_rope_scaling_from_gguf_refuses(tmp_path):
                  [("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scaling.factor", 6, 4.0)]):
         with pytest.raises(BackendError):
             RopeScaling.from_gguf(_gguf(tmp_path, meta))
+
+
+@pytest.mark.parametrize("meta,scale", [
+    ([("scaling.factor", 6, 4.0)], 0.25),                                  # a factor without a type is linear
+    ([("scale_linear", 6, 2.0)], 0.5),                                     # the older key
+    ([("scaling.factor", 6, 4.0), ("scale_linear", 6, 2.0)], 0.25),        # the newer one counts
+    ([("scaling.type", 8, "linear"), ("scale_linear", 6, 8.0)], 0.125),
+    ([("scaling.type", 8, "none"), ("scaling.factor", 6, 4.0)], 1.0),
+    ([("scale_linear", 6, 1.0)], 1.0)])
+def test_rope_scaling_from_gguf_without_a_type(tmp_path, meta, scale):
+    from modgrad_amd.kvcache import RopeScaling
+    c = RopeScaling.from_gguf(_gguf(tmp_path, [(f"llama.rope.{k}", t, v) for k, t, v in meta])).c
+    assert (c.freq_scale, c.ext_factor, c.base) == (scale, 0.0, 1e4)
+
+
+def test_rope_scaling_from_gguf_yarn_by_the_older_factor(tmp_path):
+    from modgrad_amd.kvcache import RopeScaling
+    c = RopeScaling.from_gguf(_gguf(tmp_path, [("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scale_linear", 6, 4.0),
+                                               ("llama.rope.scaling.original_context_length", 4, 4096)])).c
+    assert (c.freq_scale, c.ext_factor, c.orig_ctx) == (0.25, 1.0, 4096.0)

@@ -74,19 +74,33 @@ class RopeScaling:
         """From an opened GgufFile's <arch>.rope.* keys: freq_base,
         scaling.type ("none", "linear", "yarn"; a factor without a type is
         linear), scaling.factor (older files: rope.scale_linear),
-        scaling.attn_factor, scaling.original_context_length."""
+        scaling.attn_factor, scaling.original_context_length. Keys that would
+        change the angles in another way (further rope.scaling.* ones of a
+        "yarn" file, numbers of another type) are refused, not passed over."""
         arch = g.architecture()
-        base = g.meta_f32(f"{arch}.rope.freq_base") or 10000.0
+
+        def number(key):
+            m = g.meta(f"{arch}.rope.{key}")
+            x = 0.0 if m is None else m.as_f32()
+            if x is None:
+                raise BackendError("Unsupported", f"{arch}.rope.{key} is not a float")
+            return x
+
+        base = number("freq_base") or 10000.0
         m = g.meta(f"{arch}.rope.scaling.type")
         kind = m.as_str() if m is not None else "linear"
-        factor = g.meta_f32(f"{arch}.rope.scaling.factor") or g.meta_f32(f"{arch}.rope.scale_linear") or 1.0
-        attn = g.meta_f32(f"{arch}.rope.scaling.attn_factor") or 1.0
+        factor = number("scaling.factor") or number("scale_linear") or 1.0
+        attn = number("scaling.attn_factor") or 1.0
         if kind not in ("none", "linear", "yarn"):
             raise BackendError("Unsupported", f"rope scaling type {kind!r}")
         if kind == "none" or factor == 1.0:
             return cls(base, attn_factor=attn, factors=factors)
         if kind == "linear":
             return cls(base, freq_scale=1.0 / factor, attn_factor=attn, factors=factors)
+        known = ("type", "factor", "attn_factor", "original_context_length", "finetuned")
+        for key in g.metadata:
+            if key.startswith(f"{arch}.rope.scaling.") and key.split(".rope.scaling.")[1] not in known:
+                raise BackendError("Unsupported", key)
         orig = g.meta_u32(f"{arch}.rope.scaling.original_context_length")
         if not orig:
             raise BackendError("Runtime", f"missing {arch}.rope.scaling.original_context_length")

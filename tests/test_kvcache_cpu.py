@@ -252,3 +252,24 @@ def test_rope_scaling_from_gguf_yarn_by_the_older_factor(tmp_path):
     c = RopeScaling.from_gguf(_gguf(tmp_path, [("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scale_linear", 6, 4.0),
                                                ("llama.rope.scaling.original_context_length", 4, 4096)])).c
     assert (c.freq_scale, c.ext_factor, c.orig_ctx) == (0.25, 1.0, 4096.0)
+
+
+@pytest.mark.parametrize("meta", [
+    [("scaling.type", 8, "linear"), ("scaling.factor", 4, 4)],             # whole numbers where the format has floats
+    [("freq_base", 4, 500000)],
+    [("scaling.type", 8, "yarn"), ("scaling.factor", 6, 4.0), ("scaling.original_context_length", 4, 4096),
+     ("scaling.yarn_beta_fast", 6, 16.0)],                                 # a ramp of another shape
+])
+def test_rope_scaling_from_gguf_refuses_what_it_would_pass_over(tmp_path, meta):
+    from modgrad_amd.kvcache import RopeScaling
+    from modgrad_amd.q4k import BackendError
+    with pytest.raises(BackendError):
+        RopeScaling.from_gguf(_gguf(tmp_path, [(f"llama.rope.{k}", t, v) for k, t, v in meta]))
+
+
+def test_rope_scaling_from_gguf_takes_the_finetuned_flag(tmp_path):
+    from modgrad_amd.kvcache import RopeScaling
+    c = RopeScaling.from_gguf(_gguf(tmp_path, [
+        ("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scaling.factor", 6, 4.0),
+        ("llama.rope.scaling.original_context_length", 4, 4096), ("llama.rope.scaling.finetuned", 7, True)])).c
+    assert (c.freq_scale, c.ext_factor) == (0.25, 1.0)

@@ -60,7 +60,7 @@ struct Divider {
 
 template <int D, int FMT, bool VEC, int NT>
 __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, const float *__restrict__ rope, int rot,
-                                                       int half, int n_pos, AppendGrid gr) {
+                                                       int half, unsigned last_pos, AppendGrid gr) {
     typedef RopeUnit<VEC> U;
     constexpr int kUnits = D / U::N;
     const int tid = threadIdx.x;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
 #pragma unroll
         for (int k = 0; k < kQueryUnits; ++k) {
             const int p = s.pos0 + (int)t[k];
-            if (p >= 0 && p < n_pos) {
+            if ((unsigned)p <= last_pos) {
                 U(r[k] % kUnits, rot, half).turn(rope + (int64_t)p * rot, half, v[k]);
             } else {
 #pragma unroll
@@ -255,7 +255,7 @@ static hipError_t append_run(const KvView &c, const mgq_rope *rope, const KvAppe
     const int64_t grid = g.kv_groups + (int64_t)c.n_seqs * g.q_blocks;
     kv_append_kernel<D, FMT, VEC, NT><<<(unsigned)grid, NT, 0, stream>>>(
         c, a, rope ? rope->table : nullptr, rope ? rope->rot_dim : 0, rope && rope->style == MGQ_ROPE_HALF,
-        rope ? rope->n_pos : 0x7FFFFFFF, g);
+        rope ? (unsigned)(rope->n_pos - 1) : 0xFFFFFFFFu, g);  // no table: rows are copied, wherever they are
     return hipGetLastError();
 }
 

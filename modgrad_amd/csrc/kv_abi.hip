@@ -99,13 +99,16 @@ bool attn_heads_ok(const mgq_kv_cache *c, int hq) {
     return hq > 0 && hq % c->n_kv_heads == 0 && (int64_t)hq * c->head_dim <= (1 << 24);
 }
 
-// Rows of tiles, whose number the kernels hold in 32 bits.
+// What the kernels count in 32 bits: query rows and work-groups, and where few rows
+// take a call all its tiles.
 bool attn_fits(const mgq_kv_cache *c, int hq, int max_new) {
     const int64_t rows = (int64_t)max_new * (hq / c->n_kv_heads);
     if (rows >= (1 << 28)) return false;
-    const int64_t tiles = ((int64_t)c->max_pages * c->page_tokens + 63) / 64;
     const int64_t lines = (rows + 15) / 16 * c->n_kv_heads;
-    return lines <= kMaxGrid / tiles && lines * tiles <= kMaxGrid / c->n_seqs && lines * c->n_seqs <= kMaxGrid / 16;
+    if (lines * c->n_seqs > kMaxGrid / 16) return false;
+    if (kv_attn_is_wide(c->head_dim, rows)) return true;
+    const int64_t tiles = ((int64_t)c->max_pages * c->page_tokens + 63) / 64;
+    return lines <= kMaxGrid / tiles && lines * tiles <= kMaxGrid / c->n_seqs;
 }
 
 hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq, const void *out, int64_t os, int type,

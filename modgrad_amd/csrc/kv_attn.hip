@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
 // (28 heads on 4 of 128, int8): 28 rows x 16 sequences of 4000 tokens 29 us here,
 // 46 there; 63 rows x 8 of 8000 56 and 51. Heads of 256: 24 rows 25 and 29, 48
 // rows 57 and 40.
-static int narrow_rows(int dim) { return dim == 256 ? 32 : 48; }
+bool kv_attn_is_wide(int dim, int64_t rows) { return rows > (dim == 256 ? 32 : 48); }
 
 // Most tiles of a row: the table's, or the window's.
 static int64_t most_tiles(int64_t cap, int max_new, int window) {
@@ -479,7 +479,7 @@ static int64_t most_states(int64_t rows) { return kAttnGroups + std::max<int64_t
 
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
     const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
-    if (rows > narrow_rows(dim)) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
+    if (kv_attn_is_wide(dim, rows)) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
     const int64_t all = (int64_t)n_seqs * blocks * hkv;
     return (size_t)most_states(all) * kRows * (dim + 2) * sizeof(float) + (size_t)all * sizeof(int2);
 }
@@ -513,7 +513,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.softcap = x.softcap * 1.4426950408889634f;
     a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
     a.ws = x.ws;
-    if (c.max_new * a.group > narrow_rows(dim)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
+    if (kv_attn_is_wide(dim, c.max_new * a.group)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;
     switch (dim) {
     case 64: return i8 ? attn_run_dim<64, kFmtI8>(c, a, stream) : attn_run_dim<64, kFmtE4M3>(c, a, stream);

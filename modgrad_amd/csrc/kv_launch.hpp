@@ -38,6 +38,8 @@ struct KvAttn {
     int window;
     float *ws;
 };
+// Whether this many query rows of a kv head take kv_attn_wide.hip.
+bool kv_attn_is_wide(int dim, int64_t rows);
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity);
 hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &a, hipStream_t stream);
 

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests.gpu_util import dev, host
-from tests.test_gpu_kvcache import Both, note
+from tests.test_gpu_kvcache import Both, check, note, random_cache, torch_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,28 @@ def test_append_copies_the_queries_of_idle_slots(new, place):
     both.gpu.append(kv.data_ptr(), kv.data_ptr() + 256, 128, rows, new, q=qt.data_ptr(), q_stride=128,
                     q_out=out.data_ptr(), q_out_stride=128, n_q_heads=2)
     assert np.array_equal(host(out), q)
+
+
+def test_attention_of_a_large_batch_with_long_tables():
+    """A piece of 2048 tokens beside hundreds of slots whose tables hold 131072
+    tokens: more tiles than 32 bits count, of which few are there."""
+    import torch
+    from modgrad_amd.kvcache import KvCache
+    note("attention of a large batch with long tables")
+    rng = np.random.default_rng(1)
+    both = Both(rng, 3, 40, 2, 64, 64, "i8")
+    gen = random_cache(both, 1)
+    seqs, lens, news = 600, [0] * 600, [0] * 600
+    table = np.full((seqs, 2048), -1, np.int32)
+    for b, at, n, m in ((0, 17, 2100, 2048), (1, 300, 900, 1), (2, 599, 2500, 130)):
+        table[at, :40], lens[at], news[at] = both.ref.table[b], n, m
+    cache = KvCache.wrap(both.k, both.v, both.ks, both.vs, dev(table), dev(np.array(lens, np.int32)),
+                         dev(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)), "i8")
+    rows, hq = sum(news), 16
+    q = torch.randn(rows, hq, 64, generator=gen, device="cuda") * 2
+    want, tol = torch_attention(both, q, [2100, 900, 2500], [2048, 1, 130], 0.125)
+    for f16 in (False, True):
+        out = torch.full((rows + 1, hq, 64), 7.0, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+        cache.attend(q.data_ptr(), hq * 64, hq, out.data_ptr(), hq * 64, rows, 2048, out_f16=f16)
+        check(host(out[:rows]).astype(np.float64), host(want), host(tol), f16)
+        assert bool((out[rows] == 7.0).all())

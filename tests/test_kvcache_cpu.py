@@ -273,3 +273,15 @@ def test_rope_scaling_from_gguf_takes_the_finetuned_flag(tmp_path):
         ("llama.rope.scaling.type", 8, "yarn"), ("llama.rope.scaling.factor", 6, 4.0),
         ("llama.rope.scaling.original_context_length", 4, 4096), ("llama.rope.scaling.finetuned", 7, True)])).c
     assert (c.freq_scale, c.ext_factor) == (0.25, 1.0)
+
+
+def test_attention_takes_large_batches(L):
+    """Long pieces for many sequences of large tables: the number of tiles is no
+    limit where each work-group has rows of one sequence; rows and work-groups are."""
+    size = lambda hq, new, **kw: L.mgq_kv_attention_workspace_bytes(  # noqa: E731
+        ctypes.byref(cache(**kw)), hq, new)
+    big = dict(n_seqs=256, max_pages=131072 // 64, n_kv_heads=8, page_stride=8 * 64 * 128)
+    assert size(64, 2048, **big) > 0 and size(64, 8192, **big) > 0
+    assert size(64, 1, **big) > 0 and size(64, 6, **big) > 0
+    assert size(64, 1 << 26, **big) == 0              # 2^29 rows of a kv head
+    assert size(64, 131072, **{**big, "n_seqs": 4096}) == 0  # 2^31 groups of 16 rows and heads

@@ -414,12 +414,16 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * that sees nothing is zero. Rows of no sequence are left as they are.
  * q and out: rows of n_q_heads*head_dim values, strides in values. scale >= 0;
  * hipErrorInvalidValue where 1.4427 * scale, 1.4427 * softcap or scale / softcap
- * passes f32. A query row with a NaN or infinity gives a row of NaN if it sees
- * anything. Scales, and values of tokens that a sequence holds, are taken as
- * finite, as an append leaves them; what lies behind its last token may be
- * anything. Statistics and sums are f32. Where out is f32, the queries and the
- * probabilities go into the products with 22 bits; with MGQ_OUT_F16 the queries
- * may have 16 (of the row's largest) and the probabilities 11. Scales of V below 2^-90 count as 2^-90.
+ * passes f32, and for sizes that the kernels cannot count: 2^28 and more rows
+ * max_new*n_q_heads/n_kv_heads of a kv head; 2^27 and more groups of 16 of them,
+ * over all kv heads and sequences; and, for up to 48 of them, more than 2^31 - 512
+ * pairs of such a group and 64 tokens with every table full. A query row with a NaN
+ * or infinity gives a row of NaN if it sees anything. Scales, and values of tokens
+ * that a sequence holds, are taken as finite, as an append leaves them; what lies
+ * behind its last token may be anything. Statistics and sums are f32. Where out is
+ * f32, the queries and the probabilities go into the products with 22 bits; with
+ * MGQ_OUT_F16 the queries may have 16 (of the row's largest) and the probabilities
+ * 11. Scales of V below 2^-90 count as 2^-90.
  * out must not overlap q, the cache or the workspace.
  * workspace: device memory, 16-byte aligned, of at least
  * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);

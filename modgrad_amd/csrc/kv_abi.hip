@@ -108,7 +108,9 @@ bool attn_fits(const mgq_kv_cache *c, int hq, int max_new) {
     if (lines * c->n_seqs > kMaxGrid / 16) return false;
     if (kv_attn_is_wide(c->head_dim, rows)) return true;
     const int64_t tiles = ((int64_t)c->max_pages * c->page_tokens + 63) / 64;
-    return lines <= kMaxGrid / tiles && lines * tiles <= kMaxGrid / c->n_seqs;
+    // the runs of the 512 work-groups at most end up to 511 tiles past the last
+    constexpr int64_t kMostTiles = kMaxGrid - 511;
+    return lines <= kMostTiles / tiles && lines * tiles <= kMostTiles / c->n_seqs;
 }
 
 hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq, const void *out, int64_t os, int type,

@@ -285,3 +285,14 @@ def test_attention_takes_large_batches(L):
     assert size(64, 1, **big) > 0 and size(64, 6, **big) > 0
     assert size(64, 1 << 26, **big) == 0              # 2^29 rows of a kv head
     assert size(64, 131072, **{**big, "n_seqs": 4096}) == 0  # 2^31 groups of 16 rows and heads
+
+
+def test_attention_refuses_more_tiles_than_its_runs_can_count(L):
+    """Few query rows: the tiles are cut into 512 equal runs, whose ends are counted
+    in 32 bits."""
+    tiles = (1 << 24) - 1  # of a sequence
+    for seqs, fits in ((127, True), (128, False)):
+        run = -(-seqs * tiles // 512)
+        assert (512 * run < 2 ** 31) == fits and seqs * tiles < 2 ** 31
+        c = cache(n_seqs=seqs, max_pages=tiles, n_kv_heads=1)
+        assert (L.mgq_kv_attention_workspace_bytes(ctypes.byref(c), 1, 1) > 0) == fits

@@ -300,7 +300,9 @@ class KvCache:
     def set_lengths(self, lengths, new=None, stream=None) -> None:
         """Tokens of every slot with the next call's new ones, and how many of
         them are new (None: one each); pages are reserved for them. The tensors
-        stay in place, so that recorded calls replay on the new values."""
+        stay in place, so that recorded calls replay on the new values: one that
+        was recorded with counts takes any that fit its n_tokens and max_new, one
+        that was recorded with one each stays at that."""
         torch = _torch()
         lengths = [int(n) for n in lengths]
         counts = None if new is None else [int(n) for n in new]
@@ -314,13 +316,12 @@ class KvCache:
                 self.reserve(b, n, stream)
         with _stream(stream):
             self.seq_len.copy_(torch.tensor(lengths, dtype=torch.int32))
-            if counts is None:
-                self.use_cu_tokens(None)
-                return
-            if self._own_cu is None:
+            if counts is not None and self._own_cu is None:
                 self._own_cu = torch.empty(self.n_seqs + 1, dtype=torch.int32, device=self.device)
-            self._own_cu.copy_(torch.tensor(np.cumsum([0] + counts), dtype=torch.int32))
-            self.use_cu_tokens(self._own_cu)
+            if self._own_cu is not None:  # one each: for the calls that were recorded with counts
+                starts = np.cumsum([0] + (counts or [1] * self.n_seqs))
+                self._own_cu.copy_(torch.tensor(starts, dtype=torch.int32))
+            self.use_cu_tokens(None if counts is None else self._own_cu)
 
     def use_cu_tokens(self, cu_tokens) -> None:
         """The device tensor [n_seqs + 1] that says which rows of a call are

@@ -51,3 +51,31 @@ def test_attention_of_a_large_batch_with_long_tables():
         cache.attend(q.data_ptr(), hq * 64, hq, out.data_ptr(), hq * 64, rows, 2048, out_f16=f16)
         check(host(out[:rows]).astype(np.float64), host(want), host(tol), f16)
         assert bool((out[rows] == 7.0).all())
+
+
+def test_set_lengths_without_counts_reaches_recorded_calls():
+    """A chain recorded with counts, replayed after lengths were set with one new
+    token each: the rows are those of one each."""
+    import torch
+    from modgrad_amd.kvcache import KvCache
+    from modgrad_amd.q4k import Chain
+    note("set_lengths without counts under a recorded call")
+    rng = np.random.default_rng(2)
+    c, fresh = (KvCache.new(n_pages=8, page_tokens=16, n_kv_heads=1, head_dim=64, n_seqs=2, max_pages=4) for _ in range(2))
+    x = dev(rng.standard_normal((8, 2, 64)).astype(np.float32))
+    q = dev(rng.standard_normal((8, 4, 64)).astype(np.float32))
+    outs = [torch.zeros(8, 4, 64, device="cuda") for _ in range(2)]
+    c.set_lengths([5, 3], [5, 3])
+    ws = c.attention_workspace(4, 8, 8)
+    chain = Chain.from_ops([c.op_append(x.data_ptr(), x.data_ptr() + 256, 128, 8, 8),
+                            c.op_attend(q.data_ptr(), 256, 4, outs[0].data_ptr(), 256, 8, 8, ws)])
+    for lens, new in (([5, 3], [5, 3]), ([6, 4], None), ([7, 5], None), ([9, 11], [2, 6])):
+        c.set_lengths(lens, new)
+        chain.launch()
+        fresh.set_lengths(lens, new)
+        rows, most = (2, 1) if new is None else (8, 6)
+        fresh.append(x.data_ptr(), x.data_ptr() + 256, 128, rows, most)
+        fresh.attend(q.data_ptr(), 256, 4, outs[1].data_ptr(), 256, rows, most)
+        for a, b in ((c.k, fresh.k), (c.v, fresh.v), (c.k_scale, fresh.k_scale), (c.v_scale, fresh.v_scale),
+                     (outs[0][:rows], outs[1][:rows])):
+            assert np.array_equal(host(a), host(b)), (lens, new)

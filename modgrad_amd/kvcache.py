@@ -265,24 +265,30 @@ class KvCache:
         return c
 
     # -- pages and lengths ---------------------------------------------------
+    def _short(self, seq: int, n_tokens: int) -> int:
+        """Pages that slot `seq` lacks for n_tokens positions."""
+        need = -(-n_tokens // self.page_tokens)
+        if need > self.max_pages:
+            raise BackendError("Runtime", f"reserve: {n_tokens} tokens need {need} pages, a "
+                                          f"sequence has {self.max_pages}")
+        return max(0, need - len(self._held[seq]))
+
+    def _afford(self, short: int) -> None:
+        if short > len(self._free):
+            raise BackendError("OutOfMemory", f"reserve: {short} pages, {len(self._free)} free")
+
     def reserve(self, seq: int, n_tokens: int, stream=None) -> None:
         """Pages for the first n_tokens positions of slot `seq`."""
         if self._free is None:
             raise BackendError("Unsupported", "reserve: the cache wraps tables of the caller's")
         if not 0 <= seq < self.n_seqs or n_tokens < 0:
             raise BackendError("Runtime", f"reserve: {n_tokens} tokens of sequence {seq}")
-        held = self._held[seq]
-        need = -(-n_tokens // self.page_tokens)
-        if need > self.max_pages:
-            raise BackendError("Runtime", f"reserve: {n_tokens} tokens need {need} pages, a "
-                                          f"sequence has {self.max_pages}")
-        if need - len(held) > len(self._free):
-            raise BackendError("OutOfMemory", f"reserve: {need - len(held)} pages, "
-                                              f"{len(self._free)} free")
-        if need > len(held):
-            new = [self._free.pop() for _ in range(need - len(held))]
+        short, held = self._short(seq, n_tokens), self._held[seq]
+        self._afford(short)
+        if short:
+            new = [self._free.pop() for _ in range(short)]
             with _stream(stream):
-                self.page_table[seq, len(held): need] = _torch().tensor(new, dtype=_torch().int32)
+                self.page_table[seq, len(held): len(held) + short] = _torch().tensor(new, dtype=_torch().int32)
             held += new
 
     def release(self, seq: int, stream=None) -> None:
@@ -312,6 +318,7 @@ class KvCache:
             if not 0 <= m <= n < 2 ** 30:
                 raise BackendError("Runtime", f"set_lengths: {n} tokens, {m} of them new")
         if self._free is not None:
+            self._afford(sum(self._short(b, n) for b, n in enumerate(lengths)))  # all of them or none
             for b, n in enumerate(lengths):
                 self.reserve(b, n, stream)
         with _stream(stream):

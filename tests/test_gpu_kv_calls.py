@@ -79,3 +79,20 @@ def test_set_lengths_without_counts_reaches_recorded_calls():
         for a, b in ((c.k, fresh.k), (c.v, fresh.v), (c.k_scale, fresh.k_scale), (c.v_scale, fresh.v_scale),
                      (outs[0][:rows], outs[1][:rows])):
             assert np.array_equal(host(a), host(b)), (lens, new)
+
+
+@pytest.mark.parametrize("lens", [[48, 48], [16, 65], [32, 80]])
+def test_set_lengths_that_are_refused_take_no_pages(lens):
+    """More pages than there are, or than a table has: none are taken for the
+    sequences before the one that does not fit."""
+    from modgrad_amd.kvcache import KvCache
+    from modgrad_amd.q4k import BackendError
+    note(f"refused lengths {lens}")
+    c = KvCache.new(n_pages=5, page_tokens=16, n_kv_heads=1, head_dim=64, n_seqs=2, max_pages=4)
+    c.set_lengths([7, 9])
+    was = host(c.page_table).copy()
+    with pytest.raises(BackendError):
+        c.set_lengths(lens)
+    assert len(c._free) == 3 and np.array_equal(host(c.page_table), was) and list(host(c.seq_len)) == [7, 9]
+    c.set_lengths([64, 9])
+    assert len(c._free) == 0

@@ -132,11 +132,11 @@ struct WideShape {
     static constexpr int SETS = D == 256 || (D == 128 && LO && FMT == kFmtI8) ? 1 : 2;
     static constexpr int NW = kWideRows / (16 * SETS);      // wavefronts
     static constexpr int kThreads = 64 * NW, kPerSimd = 2;
-    static constexpr bool kAhead = kPerSimd <= 2;           // registers for operands ahead of their use
     static constexpr int KS = I8 ? D / 64 : D / 32;         // summed steps of S
     static constexpr int DB = D / 16;                       // blocks of 16 dims of O
-    static constexpr int NK = (4 * KS + NW - 1) / NW;       // pieces of K a wavefront stages: 64 lanes x 16 bytes of LDS
-    static constexpr int NV = (2 * DB + NW - 1) / NW;       // pieces of V
+    static constexpr int NK = 4 * KS / NW;                  // pieces of K a wavefront stages: 64 lanes x 16 bytes of LDS
+    static constexpr int NV = 2 * DB / NW;                  // pieces of V
+    static_assert(4 * KS % NW == 0 && 2 * DB % NW == 0, "each wavefront stages as many pieces");
     static constexpr int kOfV = 4 * KS * 64, kBuf = kOfV + 2 * DB * 64;  // 16-byte units of a buffer: K, then V
 };
 
@@ -216,14 +216,12 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             const int p = wave * NK + i, bt = p / KS, k = p % KS;
-            if (4 * KS % W::NW == 0 || p < 4 * KS) {
-                if constexpr (I8) {
-                    kst[i] = *reinterpret_cast<const u32x4 *>(kp + 4 * bt * D + 16 * k);
-                } else {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * bt * D + 8 * k);
-                    kst[i][0] = x[0];
-                    kst[i][1] = x[1];
-                }
+            if constexpr (I8) {
+                kst[i] = *reinterpret_cast<const u32x4 *>(kp + 4 * bt * D + 16 * k);
+            } else {
+                const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * bt * D + 8 * k);
+                kst[i][0] = x[0];
+                kst[i][1] = x[1];
             }
         }
 #pragma unroll
@@ -236,10 +234,8 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             const int p = wave * NK + i;
-            if (4 * KS % W::NW == 0 || p < 4 * KS) {
-                if constexpr (I8) reinterpret_cast<u32x4 *>(buf)[p * 64 + lane] = kst[i];
-                else buf[p * 64 + lane] = kv_half8<FMT>(kst[i][0], kst[i][1]);
-            }
+            if constexpr (I8) reinterpret_cast<u32x4 *>(buf)[p * 64 + lane] = kst[i];
+            else buf[p * 64 + lane] = kv_half8<FMT>(kst[i][0], kst[i][1]);
         }
         if (__any(nv_n < 16)) {
 #pragma unroll
@@ -280,7 +276,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 #pragma unroll
                 for (int k = 0; k < KS; ++k) kx[i][k] = reinterpret_cast<const i32x4 *>(buf)[(i * KS + k) * 64 + lane];
         };
-        if constexpr (I8 && W::kAhead) {
+        if constexpr (I8) {
             // K's operands on their way while the next tile is staged
             read_k();
             __builtin_amdgcn_sched_barrier(0);
@@ -295,7 +291,6 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 
         f32x4 S[SETS][4] = {};
         if constexpr (I8) {
-            if (!W::kAhead) read_k();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -328,7 +323,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                 }
         }
 
-        constexpr int G = W::kAhead ? 2 : 1;  // blocks of 16 dims read at once
+        constexpr int G = 2;  // blocks of 16 dims read at once
         const half8 *vb = buf + W::kOfV;
         half8 vx[2][2 * G];
 #pragma unroll

@@ -195,6 +195,12 @@ def _op(kind: int, args) -> "_lib.OpDesc":
     return d
 
 
+def _workspace(workspace, device) -> None:
+    """A call writes all of its workspace: it has to be memory of the cache's device."""
+    if workspace.device != device or not workspace.is_contiguous():
+        raise BackendError("Runtime", f"workspace: contiguous memory on {device} expected")
+
+
 class KvCache:
     """One layer's paged 8-bit cache and the page tables of n_seqs slots
     (mgq_kv_cache)."""
@@ -373,6 +379,8 @@ class KvCache:
         if workspace is None:
             with _stream(stream):
                 workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
+        else:
+            _workspace(workspace, self.device)
         kern.kv_attention(self._ref, q, q_stride, n_q_heads, out, out_stride,
                           _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens, max_new,
                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap, window,
@@ -397,6 +405,7 @@ class KvCache:
                   n_tokens: int, max_new: int, workspace, scale: float | None = None,
                   softcap: float = 0.0, window: int = 0, out_f16: bool = False) -> "_lib.OpDesc":
         """The workspace has to outlive the chain."""
+        _workspace(workspace, self.device)
         return _op(_lib.OP_KV_ATTENTION, _lib.KvAttentionArgs(
             self.desc, q, out, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             q_stride, out_stride, n_q_heads, _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens,

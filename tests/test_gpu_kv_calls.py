@@ -96,3 +96,20 @@ def test_set_lengths_that_are_refused_take_no_pages(lens):
     assert len(c._free) == 3 and np.array_equal(host(c.page_table), was) and list(host(c.seq_len)) == [7, 9]
     c.set_lengths([64, 9])
     assert len(c._free) == 0
+
+
+def test_workspaces_elsewhere_are_refused():
+    """Memory of the host, and a view that says more bytes than it has."""
+    import torch
+    from modgrad_amd.kvcache import KvCache
+    from modgrad_amd.q4k import BackendError
+    note("workspaces elsewhere")
+    c = KvCache.new(4, 16, 1, 64, 1, 4)
+    c.set_lengths([5])
+    n = c.attention_workspace(1, 1, 1).nbytes
+    p = torch.zeros(64, device="cuda").data_ptr()
+    for ws in (torch.empty(n, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8, device="cuda").expand(n)):
+        with pytest.raises(BackendError):
+            c.attend(p, 64, 1, p, 64, 1, 1, workspace=ws)
+        with pytest.raises(BackendError):
+            c.op_attend(p, 64, 1, p, 64, 1, 1, ws)

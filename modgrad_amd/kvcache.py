@@ -69,6 +69,15 @@ class RopeScaling:
                                   orig_ctx, None if factors is None else factors.data_ptr())
         self.ref = ctypes.byref(self.c)
 
+    def check(self, rot_dim: int) -> None:
+        """The divisors are read as rot_dim/2 floats of the current device."""
+        f = self.factors
+        if f is None:
+            return
+        if f.numel() != rot_dim // 2 or f.dtype != _torch().float32 or not f.is_contiguous():
+            raise BackendError("Runtime", f"rope factors: {rot_dim // 2} contiguous f32 expected")
+        _on_device(f.device)
+
     @classmethod
     def from_gguf(cls, g, factors=None) -> "RopeScaling":
         """From an opened GgufFile's <arch>.rope.* keys: freq_base,
@@ -118,12 +127,6 @@ class RopeTable:
             raise BackendError("Runtime", f"rope table of {n_pos} positions, {rot_dim} dims")
         torch = _torch()
         scaling = scaling or RopeScaling()
-        if scaling.factors is not None and (
-                scaling.factors.numel() != rot_dim // 2 or scaling.factors.dtype != torch.float32
-                or not scaling.factors.is_contiguous()):
-            raise BackendError("Runtime", f"rope factors: {rot_dim // 2} contiguous f32 expected")
-        if scaling.factors is not None:
-            _on_device(scaling.factors.device)
         with _stream(stream):
             t = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device="cuda")
         kern.rope_table(t.data_ptr(), n_pos, 0, rot_dim, scaling, stream)

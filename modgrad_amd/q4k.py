@@ -360,6 +360,7 @@ class kern:
                    stream=None) -> None:
         """[n_pos][rot_dim/2] (cos, sin) of positions first_pos ..; scaling: a
         kvcache.RopeScaling."""
+        scaling.check(rot_dim)
         _chk(_lib.load().launch_rope_table_ex(table, n_pos, first_pos, rot_dim, scaling.ref,
                                               _stream_ptr(stream)), "rope_table")
 

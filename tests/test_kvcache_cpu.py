@@ -296,3 +296,15 @@ def test_attention_refuses_more_tiles_than_its_runs_can_count(L):
         assert (512 * run < 2 ** 31) == fits and seqs * tiles < 2 ** 31
         c = cache(n_seqs=seqs, max_pages=tiles, n_kv_heads=1)
         assert (L.mgq_kv_attention_workspace_bytes(ctypes.byref(c), 1, 1) > 0) == fits
+
+
+@pytest.mark.parametrize("factors", [dict(n=31), dict(n=33), dict(dtype="float64"), dict(step=2), dict()])
+def test_rope_table_refuses_factors(factors):
+    """Too few or too many, of another type, not next to one another, of the host."""
+    import torch
+    from modgrad_amd.kvcache import RopeScaling, kern
+    from modgrad_amd.q4k import BackendError
+    n, step = factors.get("n", 32), factors.get("step", 1)
+    f = torch.ones(n * step, dtype=getattr(torch, factors.get("dtype", "float32")))[::step]
+    with pytest.raises(BackendError, match="factors|tensors on"):  # before the library sees them
+        kern.rope_table(FAKE, 0, 0, 64, RopeScaling(factors=f))

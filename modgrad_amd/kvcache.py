@@ -46,9 +46,9 @@ def _elsewhere(device) -> bool:
 
 def _on_device(device) -> None:
     """Launches go to the current device: the tensors have to be there."""
-    cuda = _torch().cuda
     if device.type != "cuda":
         raise BackendError("Runtime", f"tensors on {device}")
+    cuda = _torch().cuda
     if device.index != cuda.current_device():
         raise BackendError("Runtime", f"tensors on {device}, the current device is "
                                       f"cuda:{cuda.current_device()}")
@@ -74,7 +74,7 @@ class RopeScaling:
         f = self.factors
         if f is None:
             return
-        if f.numel() != rot_dim // 2 or f.dtype != _torch().float32 or not f.is_contiguous():
+        if f.numel() != rot_dim // 2 or str(f.dtype) != "torch.float32" or not f.is_contiguous():
             raise BackendError("Runtime", f"rope factors: {rot_dim // 2} contiguous f32 expected")
         _on_device(f.device)
 

@@ -420,10 +420,11 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * pairs of such a group and 64 tokens with every table full. A query row with a NaN
  * or infinity gives a row of NaN if it sees anything. Scales, and values of tokens
  * that a sequence holds, are taken as finite, as an append leaves them; what lies
- * behind its last token may be anything. Statistics and sums are f32. Where out is
- * f32, the queries and the probabilities go into the products with 22 bits; with
- * MGQ_OUT_F16 the queries may have 16 (of the row's largest) and the probabilities
- * 11. Scales of V below 2^-90 count as 2^-90.
+ * behind its last token may be anything. Statistics and sums are f32. The queries
+ * go into the products with 22 bits, with MGQ_OUT_F16 maybe 16, of the row's largest;
+ * p_j times its page's scale of V with 22 bits, with MGQ_OUT_F16 maybe 11, or to
+ * 2^-38 of the row's largest where that is coarser. Scales of V below 2^-90 count
+ * as 2^-90.
  * out must not overlap q, the cache or the workspace.
  * workspace: device memory, 16-byte aligned, of at least
  * mgq_kv_attention_workspace_bytes bytes (of the same cache, heads and max_new);

@@ -25,8 +25,8 @@
 // Softmax in base 2 with V's scale in the exponent: t_j = s_j log2 e +
 // log2(vs), M the running maximum of t, w_j = 2^(t_j - M + 14) = p_j * vs *
 // const, O += w_j V8_j, l += w_j / vs. M may lag by 1, so w_j < 2^15 whatever the
-// scales are: its f16 hi + lo pair keeps 22 bits down to 2^-24 of the largest. M,
-// l and O are f32.
+// scales are: its f16 hi + lo pair keeps 22 bits down to 2^-17 of the largest, and
+// is off by less than 2^-38 of the largest below. M, l and O are f32.
 //
 // int8 K skips the conversion: q goes in as three digits of 8 bits on the int8
 // matrix cores (v_mfma_i32_16x16x64_i8), whose sums are exact.
@@ -296,6 +296,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
 
         f32x4 O[DB] = {};
         float M = -INFINITY, l = 0.0f;
+        bool loud = false;
         for (; tile < tile_end; tile += NW) {
             const float ks = kscale * ks_n, vs = fmaxf(vs_n, kLeastScale);
             const int nv = nv_n;
@@ -340,14 +341,27 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                     S[t][i] = s;
                     top = fmaxf(top, s);
                 }
+            const float own = top;
+            loud = loud || __any(vs > kLoudScale);
             top = max_groups(top);
-            if (__any(outgrown(top, M))) {  // the maximum may lag by 1: w stays below 2^15
+            float per = __builtin_amdgcn_rcpf(vs);
+            if (loud || __any(outgrown(top, M))) {  // the maximum may lag by 1: w stays below 2^15
                 const float m = fmaxf(M, top);
-                const float fac = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
+                const Exp2 f(M == -INFINITY ? -INFINITY : M - m);
                 M = m;
-                l *= fac;
+                l = f.times(l);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) O[d] *= fac;
+                for (int d = 0; d < DB; ++d) O[d] *= f.f;
+                const float ref = reference_of(m);
+                if (loud && vanishing(own, ref)) {
+                    float near = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) near += __builtin_amdgcn_exp2f(S[t][i] - own);
+                    l += Exp2(own - ref - lv).times(near);
+                    per = 0.0f;
+                }
             }
             const float ref = reference_of(M);
             float sum = 0.0f;
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                     ph[t / 2][4 * (t % 2) + i] = hi;
                     pl[t / 2][4 * (t % 2) + i] = (_Float16)(w - (float)hi);
                 }
-            l += sum * __builtin_amdgcn_rcpf(vs);
+            l += sum * per;
             if (__any(nv < 16)) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -395,8 +409,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         float all = sM[0][col];
 #pragma unroll
         for (int w = 1; w < NW; ++w) all = fmaxf(all, sM[w][col]);
-        const float fac = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - all);
-        if (grp == 0) sL[wave][col] = l * fac;
+        const Exp2 f(M == -INFINITY ? -INFINITY : M - all);
+        const float fac = f.f;
+        if (grp == 0) sL[wave][col] = f.times(l);
         if (live) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;

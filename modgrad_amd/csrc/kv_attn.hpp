@@ -32,6 +32,23 @@ __device__ __forceinline__ float reference_of(float M) {
     return M == -INFINITY ? 0.0f : M - r > kTop + 0.5f ? M : r;
 }
 
+// l = sum of w_j / vs_j = 2^(s_j - ref) moves with V's scales, by 2^211 between a page of
+// 2^121 and one of kLeastScale: more than a power of two in f32, and more than w_j have
+// that vanish below 2^-126. So l is multiplied by the power in two factors, 2^(x/2)
+// each, and
+constexpr float kLoudScale = 0x1p26f;
+struct Exp2 {
+    float h, f;  // f = h * h = 2^x, 0 below f32
+    __device__ __forceinline__ explicit Exp2(float x) : h(__builtin_amdgcn_exp2f(0.5f * x)), f(h * h) {}
+    __device__ __forceinline__ float times(float l) const { return l * h * h; }
+};
+// where the largest t of a lane's tokens is so far below ref, their w are summed
+// relative to that largest. This is looked at once a page above kLoudScale has been
+// seen: without one they are within 2^116 of each other, and what vanishes is below
+// l's own rounding. (4096 tokens of 28 heads with f32 results: heads of 64 4 % longer, of 96
+// 2.5 %, of 128 1.3 %, others the same.)
+__device__ __forceinline__ bool vanishing(float top, float ref) { return top < ref - 100.0f && top > -INFINITY; }
+
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap);
@@ -220,10 +237,11 @@ __device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // of nothing; scores of NaN have a NaN l
-            const float m = fmaxf(M, ml[u].x), f = exp2f(M - m), g = exp2f(ml[u].x - m);
+            const float m = fmaxf(M, ml[u].x);
+            const Exp2 f(M - m), g(ml[u].x - m);
             M = m;
-            l = l * f + ml[u].y * g;
-            o = o * f + x[u] * g;
+            l = f.times(l) + g.times(ml[u].y);
+            o = o * f.f + x[u] * g.f;
         }
     }
     if (k < W) sO[k * L + d] = o;
@@ -236,9 +254,9 @@ __device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
     o = f32x4{};
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float f = sML[i].x == -INFINITY ? 0.0f : exp2f(sML[i].x - M);
-        l += sML[i].y * f;
-        o += sO[i * L + d] * f;
+        const Exp2 f(sML[i].x == -INFINITY ? -INFINITY : sML[i].x - M);
+        l += f.times(sML[i].y);
+        o += sO[i * L + d] * f.f;
     }
     return o * (l == 0.0f ? 0.0f : 1.0f / l);
 }

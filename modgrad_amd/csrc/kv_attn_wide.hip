@@ -247,6 +247,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 
     f32x4 O[SETS][DB] = {};
     float M[SETS], l[SETS];
+    bool loud = false;
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         M[s] = -INFINITY;
@@ -336,6 +337,8 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
                            __all(nv == 16);
         half8 ph[SETS][2], pl[SETS][2];
+        // (an f16 result is infinite before the page that makes others vanish is that loud)
+        if (LO) loud = loud || __any(vs > kLoudScale);
 #pragma unroll
         for (int s = 0; s < SETS; ++s) {
             float sc = qs[s] * ks, add = lv;
@@ -390,17 +393,39 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hi = fmaxf(hi, S[s][i][e]);
-            const float top = max_groups(fmaf(hi, sc, add));
+            const float own = fmaf(hi, sc, add), top = max_groups(own);
             // the maximum may lag by 1: w stays below 2^15
             if (__any(outgrown(top, M[s]))) {
                 const float m = fmaxf(M[s], top);
-                const float fac = M[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[s] - m);
+                float fac;
+                if constexpr (LO) {
+                    const Exp2 f(M[s] == -INFINITY ? -INFINITY : M[s] - m);
+                    fac = f.f;
+                    l[s] = f.times(l[s]);
+                } else {
+                    fac = M[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[s] - m);
+                    l[s] *= fac;
+                }
                 M[s] = m;
-                l[s] *= fac;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) O[s][d] *= fac;
             }
-            const float off = add - reference_of(M[s]);
+            const float ref = reference_of(M[s]), off = add - ref;
+            float per = rvs;
+            if (loud && __any(vanishing(own, ref))) {
+                float near = 0.0f;
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = i == 0 ? S[s][0][e] : i == 1 ? S[s][1][e] : i == 2 ? S[s][2][e] : S[s][3][e];
+                        near += __builtin_amdgcn_exp2f(fmaf(x, sc, add - own));
+                    }
+                if (vanishing(own, ref)) {
+                    l[s] += Exp2(own - ref - lv).times(near);
+                    per = 0.0f;
+                }
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -412,7 +437,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                     ph[s][i / 2][4 * (i % 2) + e] = xh;
                     if (LO) pl[s][i / 2][4 * (i % 2) + e] = (_Float16)(x - (float)xh);
                 }
-            l[s] += sum * rvs;
+            l[s] += sum * per;
         }
         __builtin_amdgcn_s_setprio(0);
         // V's operands a group ahead of their products
@@ -512,9 +537,9 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const float2 ml = *reinterpret_cast<const float2 *>(base + i * step + kWideRows * D + 2 * rr);
-            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-            l += f * ml.y;
-            o += f * *reinterpret_cast<const f32x4 *>(base + i * step + rr * D + d);
+            const Exp2 f(ml.x == -INFINITY ? -INFINITY : ml.x - M);
+            l += f.times(ml.y);
+            o += f.f * *reinterpret_cast<const f32x4 *>(base + i * step + rr * D + d);
         }
         put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
     }

@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+from tests import kv_reference as ref
 from tests.gpu_util import dev, host
-from tests.test_gpu_kvcache import Both, check, note, random_cache, torch_attention
+from tests.test_gpu_kvcache import Both, check, fill, note, random_cache, torch_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +114,39 @@ def test_workspaces_elsewhere_are_refused():
             c.attend(p, 64, 1, p, 64, 1, 1, workspace=ws)
         with pytest.raises(BackendError):
             c.op_attend(p, 64, 1, p, 64, 1, 1, ws)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("new,n", [(1, 100), (1, 1500), (60, 100), (60, 1500)])
+@pytest.mark.parametrize("loud", [0, 2, 5])
+def test_attention_over_pages_of_all_loudness(loud, new, n, dim, fmt):
+    """A page of V whose scale is 2^118 among others of 0.02, 1e-8 and 0: the quiet
+    tokens' values vanish beside it, their part of the probabilities does not."""
+    import torch
+    note(f"pages of all loudness loud={loud} new={new} n={n} dim={dim} {fmt}")
+    rng = np.random.default_rng(loud + dim)
+    both = Both(rng, 1, -(-n // 16), 1, dim, 16, fmt)
+    fill(both, rng, [n])
+    ids = both.ref.table[0]
+    both.ref.vs[ids[1]] *= np.float32(1e-8)
+    both.ref.vs[ids[3]], both.ref.v[ids[3]] = 0, 0
+    both.ref.vs[ids[loud]] = 2.0 ** 118
+    both.vs.copy_(torch.from_numpy(both.ref.vs))
+    both.v.copy_(torch.from_numpy(both.ref.v))
+    q = rng.standard_normal((new, 4, dim)).astype(np.float32)
+    both.call([n], [new], new == 1)
+    out = torch.full((new, 4, dim), 7.0, device="cuda")
+    both.gpu.attend(dev(q).data_ptr(), 4 * dim, 4, out.data_ptr(), 4 * dim, new, new)
+    want, tol = both.ref.attend(q, [n], [new], dim ** -0.5)
+    # A probability goes into the products times its page's scale, as w of 2^14 and
+    # more (or 2^13.5) for the row's largest, in two f16 halves: the second one's step
+    # is 2^-24 at the least, so that w is off by up to 2^-25, 2^-38 of the largest.
+    k, _, _ = both.ref.read(0, 0, n)
+    sc = dim ** -0.5 * q.reshape(-1, dim).astype(np.float64) @ k.T
+    sc[np.arange(n) > n - new + np.arange(new).repeat(4)[:, None]] = -np.inf
+    p = np.exp(sc - sc.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    largest = (p * both.ref.vs[ids, 0].astype(np.float64).repeat(16)[:n]).max(1)
+    tol += (n * 2.0 ** -38 * ref.MOST[fmt] * largest).reshape(new, 4, 1)
+    check(host(out).astype(np.float64), want, tol, False)

@@ -350,7 +350,7 @@ hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_ro
  * Position j of sequence b lies in page page_table[b*max_pages + j/page_tokens].
  * An entry outside 0 .. n_pages-1 names no page: tokens there are not stored,
  * and attention does not see them (pages behind a sliding window may be given
- * back that way). A page that is appended to belongs to one sequence; pages
+ * back that way). A page that is appended to is in one sequence's list, once; pages
  * that are only read may be shared.
  * seq_len and cu_tokens describe a call: sequence b has seq_len[b] tokens,
  * the call's new ones included, and rows cu_tokens[b] .. cu_tokens[b+1]-1 of
@@ -385,8 +385,8 @@ typedef struct mgq_kv_cache {
  * ones are left out).
  * For each page, kv head and of K and V: s = max(s_old, f32(amax / M)), amax
  * over the finite new values, M the format's largest, s_old the page's scale
- * if it holds earlier tokens of the sequence, else 0 (as for a NaN). If s > s_old
- * the held values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
+ * if it holds earlier tokens of the sequence, else 0. A NaN counts as 0, and the
+ * codes under it stay. If s > s_old the held values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
  * nearest even and saturates, NaN becomes 0; all of it in 64 bits. Bytes behind
  * the sequence's last token are left as they are.
  * Tokens past max_pages*page_tokens, or in no page, are not stored. The q_out

@@ -29,7 +29,10 @@
 namespace mgq {
 
 constexpr int kWideRows = 128;
-__host__ __device__ constexpr int wide_slots(int dim) { return dim == 256 ? 256 : 512; }  // resident work-groups
+// Work-groups that a call's splits are made for: those resident at once, of 4 wavefronts
+// two a CU and of 8 one. By the head alone: heads of 128 with one set of rows (int8,
+// f32 results) have 8 wavefronts too and so twice as many splits as fit at once.
+__host__ __device__ constexpr int wide_slots(int dim) { return dim == 256 ? 256 : 512; }
 constexpr int kWideChunk = 4;  // least tiles of a split: a work-group's start costs about as much
 
 struct WideBlock {
@@ -154,7 +157,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     const int page = 1 << c.page_shift;
 
     // the second work-groups of the CUs are dealt from the shorter end, beside the
-    // longest ones
+    // longest ones (where a CU has one at a time they only come in another order)
     const int h = blockIdx.x % c.hkv;
     int id = blockIdx.x / c.hkv;
     if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;

@@ -386,9 +386,9 @@ typedef struct mgq_kv_cache {
  * For each page, kv head and of K and V: s = max(s_old, f32(amax / M)), amax
  * over the finite new values, M the format's largest, s_old the page's scale
  * if it holds earlier tokens of the sequence, else 0. A NaN counts as 0, and the
- * codes under it stay. If s > s_old the held values become Q(held * s_old / s); the new ones are Q(x / s). Q rounds to
- * nearest even and saturates, NaN becomes 0; all of it in 64 bits. Bytes behind
- * the sequence's last token are left as they are.
+ * codes under it stay. If s > s_old the held values become Q(held * s_old / s); the
+ * new ones are Q(x / s). Q rounds to nearest even and saturates, NaN becomes 0; all
+ * of it in 64 bits. Bytes behind the sequence's last token are left as they are.
  * Tokens past max_pages*page_tokens, or in no page, are not stored. The q_out
  * row of a token at a position outside the table is NaN.
  * hipErrorInvalidValue unless rope->rot_dim <= head_dim and rope->n_pos >=

@@ -46,7 +46,7 @@
 // their states in the workspace for kv_attn_join_kernel.
 //
 // Bound by the cache's bytes (28 heads on 4 of 128): 32 ragged sequences to 32 Ki
-// tokens, e4m3, 380 MB: 81 us + 4.9 for the join, 4.7 TB/s; 200 000 tokens, int8,
+// tokens, e4m3, 380 MB: 81 us + 4.8 for the join, 4.7 TB/s; 200 000 tokens, int8,
 // 205 MB: 42 + 5 us. A sequence of 1000 tokens is latency: 9 + 3 us.
 #include "kv_attn.hpp"
 

@@ -14,11 +14,12 @@
 // Tile i+2's bytes load into registers and tile i+1's go to the other LDS
 // buffer while tile i multiplies; one barrier a tile, which does not wait for
 // the loads. Bound by the softmax's exponentials and conversions on the vector
-// ALU, which issues in 70 % of the cycles of a 4096-token prompt of 28 heads of
-// 128 on int8 (149 us, 807 TFLOP/s counted as 4 D a pair), beside the matrix
-// cores (34 %): the second wavefront of each SIMD overlaps the two. Pieces of up
-// to 250 tokens over 9000, 16 heads of 256 on e4m3 with f32 results and a softcap: 95
-// + 11 us for the join, the products twice a plain f16 attention's.
+// ALU, which issues in 71 % of the cycles of a 4096-token prompt of 28 heads of
+// 128 on int8 with f16 results (151 us, 797 TFLOP/s counted as 4 D a pair), beside
+// the matrix cores (34 %): the second wavefront of each SIMD overlaps the two. With f32
+// results, three digits of q and two halves of p, 255 us (66 and 35 %). Pieces of up to 250
+// tokens over 9000, 16 heads of 256 on e4m3 with f32 results and a softcap: 97 us, a
+// tenth of it the join, the products twice a plain f16 attention's (50 and 39 %).
 //
 // Causal work is dealt longest first; work-groups of one kv head are neighbours
 // modulo the number of kv heads, so an XCD's L2 holds few heads' caches. With
@@ -125,8 +126,8 @@ __device__ __forceinline__ void wide_barrier() {
 // is, q as digits of 8 bits: 16 bits for an f16 result, 24 for f32 (heads of 96
 // are no multiple of the 64 dims of such a product).
 // SETS of 16 query rows a wavefront: two sets and 4 wavefronts read LDS half as
-// often; one and 8 wavefronts where two spill more than that is worth. Measured
-// (two, one; us for 4096 tokens of 28 heads): heads of 64 to f32 166, 197, on e4m3
+// often; one and 8 wavefronts where two spill more than that is worth. Measured when
+// it was chosen (two, one; us for 4096 tokens of 28 heads): heads of 64 to f32 166, 197, on e4m3
 // to f16 129, 157; of 96 156, 198; of 128 on e4m3 to f32 239, 248, on int8 to f32
 // 449, 250; pieces of heads of 256 to f32 192, 126.
 template <int D, int FMT, bool LO>

@@ -7,7 +7,7 @@
 // the work-group takes one sine and cosine per pair and run of J positions
 // and turns them on by the angle addition (4 fused operations a step; 32 steps
 // add < 1e-14), which leaves the kernel bound by its stores: 131072 positions of
-// 128 dims, 67 MB, 13 us (5.2 TB/s).
+// 128 dims, 67 MB, 13 us (5.2 TB/s; filling them with one value takes 11).
 #include "kv_device.hpp"
 #include "kv_launch.hpp"
 
@@ -90,8 +90,9 @@ hipError_t rope_table_launch(float *table, int n_pos, int first, int rot_dim, co
 // y = x with the first rot_dim dims of each head turned by the table row of the
 // token's position. Bound by x and y: one thread per unit of dims, a token's
 // heads next to one another, so the row (rot * 4 bytes) comes from the cache
-// for all heads but the first. 4096 tokens of 28 heads of 128: 19 us (6.2 TB/s,
-// part of it from the Infinity Cache).
+// for all heads but the first. 4096 tokens of 28 heads of 128, 118 MB: 24 us from
+// memory (4.9 TB/s, a large copy's rate), 19 where the Infinity Cache holds them (a
+// copy of them 17).
 template <bool VEC>
 __global__ __launch_bounds__(256) void rope_kernel(const float *x, float *y, const int *__restrict__ pos,
                                                    const float *__restrict__ table, int n_pos, int rot_dim, int half,

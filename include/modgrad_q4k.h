@@ -283,6 +283,39 @@ hipError_t launch_matvec_q4k_glu_ex(const unsigned char *w_gate, const unsigned 
                                     float *y, int out_dim, int blocks_per_row,
                                     hipStream_t stream);
 
+/* Result types of launch_block_norm_ex and launch_kv_attention_ex. */
+#define MGQ_OUT_F32 0 /* for the matvecs */
+#define MGQ_OUT_F16 1 /* for launch_gemm_q4k_f16; IEEE half bits */
+
+/* The norms around a block of a layer and what lies between them, in one launch
+ * (no counterpart in the reference as one call: its launch_rms_norm,
+ * launch_scale, launch_residual_add and the next block's launch_rms_norm,
+ * rocm_gemma.rs:429-489). */
+typedef struct mgq_block_norm {
+    const float *post_w; /* hidden weights of the norm of the block's result, or null: none */
+    const float *norm_w; /* hidden weights of the norm of the sum, or null: no y */
+    float h_scale;       /* of the residual stream, 1 */
+    float x_scale;       /* of the block's result, 1 */
+    float eps;           /* >= 0, of both norms */
+    int hidden;
+} mgq_block_norm;
+
+/* For each of `rows` rows of norm->hidden values, with r(a) = 1/sqrt(mean(a^2) + eps):
+ *   z  = x * r(x) * post_w          (post_w null: z = x)
+ *   h' = h_scale*h + x_scale*gate*z (x null: h_scale*h; gate null: 1)
+ *   y  = h' * r(h') * norm_w        as y_type, MGQ_OUT_F32 or MGQ_OUT_F16
+ * h' goes to h_out (null: nowhere), y to y (null: nowhere; not both null). The sums
+ * are 64-bit and h' and y are rounded once from 64-bit products; y is that of the
+ * rounded h'. Values of y past the type's largest are infinite. Strides are in
+ * values, at least hidden; gate_stride 0: one row of gates for all rows. h_out may be
+ * h with the same stride; nothing else that is written may overlap what is read or
+ * written. hipErrorInvalidValue for post_w or gate without x and for y without
+ * norm_w. */
+hipError_t launch_block_norm_ex(const mgq_block_norm *norm, const float *h, int64_t h_stride,
+                                const float *x, int64_t x_stride, const float *gate,
+                                int64_t gate_stride, float *h_out, int64_t h_out_stride, void *y,
+                                int64_t y_stride, int y_type, int rows, hipStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Rotary positions, and attention over a paged key/value cache held in 8 bits
  * (inference; no counterpart in the reference's C ABI except as noted). The
@@ -403,10 +436,6 @@ hipError_t launch_kv_append_ex(const mgq_kv_cache *cache, const mgq_rope *rope, 
 hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int n, float *k_out,
                                 float *v_out, hipStream_t stream);
 
-/* Result types of launch_kv_attention_ex. */
-#define MGQ_OUT_F32 0 /* for the matvecs */
-#define MGQ_OUT_F16 1 /* for launch_gemm_q4k_f16; IEEE half bits */
-
 /* out row t, head h = softmax(s) V over the positions j of t's sequence with
  * j <= pos and, with window > 0, j > pos - window; pos is t's position,
  * s_j = scale * q.k_j, or softcap*tanh(scale * q.k_j / softcap) with
@@ -521,11 +550,12 @@ hipError_t mgq_chain_destroy(void *chain);
  *   MGQ_OP_QUANTIZE_MATVEC_DP4A  the two above in one launch for Q4_K
  *                        (launch_quantize_matvec_q4k_dp4a_ex: y from x, same
  *                        bits; xq/xd/xsum unused).
- * Attention (the arguments in a struct of their own, which w points to in host
+ * Attention and the norms around a block (the arguments in a struct of their own, which w points to in host
  * memory; read when the chain is created, not kept):
  *   MGQ_OP_ROPE          launch_rope_ex of an mgq_rope_args.
  *   MGQ_OP_KV_APPEND     launch_kv_append_ex of an mgq_kv_append_args.
  *   MGQ_OP_KV_ATTENTION  launch_kv_attention_ex of an mgq_kv_attention_args.
+ *   MGQ_OP_BLOCK_NORM    launch_block_norm_ex of an mgq_block_norm_args.
  * No counterpart in the reference's C ABI: its chain is Rust code that
  * launches these kernels one by one; this records them into one graph. */
 #define MGQ_OP_MATVEC 0
@@ -540,7 +570,8 @@ hipError_t mgq_chain_destroy(void *chain);
 #define MGQ_OP_ROPE 9
 #define MGQ_OP_KV_APPEND 10
 #define MGQ_OP_KV_ATTENTION 11
-/* The last three take their arguments from here: mgq_op_desc.w points to one
+#define MGQ_OP_BLOCK_NORM 12
+/* Those from MGQ_OP_ROPE on take their arguments from here: mgq_op_desc.w points to one
  * in host memory. */
 typedef struct mgq_rope_args {
     const float *x;
@@ -567,6 +598,14 @@ typedef struct mgq_kv_attention_args {
     int n_q_heads, out_type, n_tokens, max_new, window;
     float scale, softcap;
 } mgq_kv_attention_args;
+typedef struct mgq_block_norm_args {
+    mgq_block_norm norm;
+    const float *h, *x, *gate;
+    float *h_out;
+    void *y;
+    int64_t h_stride, x_stride, gate_stride, h_out_stride, y_stride;
+    int y_type, rows;
+} mgq_block_norm_args;
 /* GGML tensor types (gguf.rs:9-40) of the quantized weights */
 #define MGQ_DTYPE_Q4_K 12
 #define MGQ_DTYPE_Q5_K 13
@@ -577,7 +616,7 @@ typedef struct mgq_op_desc {
     int layout;               /* MGQ_LAYOUT_* (MGQ_OP_MATVEC on Q4_K) */
     int act;                  /* MGQ_ACT_* (GLU ops) */
     const unsigned char *w;   /* weights (the gate matrix for MGQ_OP_MATVEC_GLU), or
-                                 the host struct of ops 9 to 11 */
+                                 the host struct of ops 9 and up */
     const unsigned char *w2;  /* MGQ_OP_MATVEC_GLU: the up matrix */
     const float *x;           /* input */
     const float *x2;          /* MGQ_OP_GLU: the up vector */

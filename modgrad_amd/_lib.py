@@ -57,6 +57,7 @@ SIGNATURES = {
     "launch_matvec_q4k_rmsnorm_ex": (I, [P, P, P, F, P, I, I, P]),
     "launch_matvec_q6k_rmsnorm_ex": (I, [P, P, P, F, P, I, I, P]),
     "launch_matvec_q4k_glu_ex": (I, [P, P, P, P, F, I, P, I, I, P]),
+    "launch_block_norm_ex": (I, [P, P, L, P, L, P, L, P, L, P, L, I, I, P]),
     "launch_rope_table_ex": (I, [P, I, I, I, P, P]),
     "launch_rope_ex": (I, [P, P, P, P, I, I, I, L, L, P]),
     "launch_kv_append_ex": (I, [P, P, P, P, L, P, L, P, L, I, I, I, P]),
@@ -93,6 +94,7 @@ OP_QUANTIZE_MATVEC_DP4A = 8
 OP_ROPE = 9
 OP_KV_APPEND = 10
 OP_KV_ATTENTION = 11
+OP_BLOCK_NORM = 12
 ROPE_INTERLEAVED = 0
 ROPE_HALF = 1
 KV_I8 = 0
@@ -154,6 +156,17 @@ class KvAttentionArgs(ctypes.Structure):
                 ("workspace_bytes", S), ("q_stride", L), ("out_stride", L), ("n_q_heads", I),
                 ("out_type", I), ("n_tokens", I), ("max_new", I), ("window", I), ("scale", F),
                 ("softcap", F)]
+
+
+class BlockNorm(ctypes.Structure):
+    """mgq_block_norm."""
+    _fields_ = [("post_w", P), ("norm_w", P), ("h_scale", F), ("x_scale", F), ("eps", F), ("hidden", I)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """mgq_block_norm_args (OP_BLOCK_NORM)."""
+    _fields_ = [("norm", BlockNorm), ("h", P), ("x", P), ("gate", P), ("h_out", P), ("y", P), ("h_stride", L),
+                ("x_stride", L), ("gate_stride", L), ("h_out_stride", L), ("y_stride", L), ("y_type", I), ("rows", I)]
 
 
 class HipError(RuntimeError):

@@ -9,6 +9,7 @@
 #include "../../include/modgrad_q4k.h"
 #include "q4k_launch.hpp"
 
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <new>
@@ -308,6 +309,57 @@ static bool q6k_norm_fits(const unsigned char *w, int out_dim, int bpr) {
     return ((uintptr_t)w & 15u) == 0 && ((int64_t)out_dim * bpr * 210) % 16 == 0 && bpr <= 14;
 }
 
+static hipError_t block_norm_check(const mgq_block_norm *n, const mgq_block_norm_args &a) {
+    if (!n || n->hidden <= 0 || n->hidden > (1 << 30) || a.rows <= 0 || bad_f32(a.h)) return hipErrorInvalidValue;
+    for (const float *p : {n->post_w, n->norm_w, a.x, a.gate, static_cast<const float *>(a.h_out)})
+        if (p && misaligned4(p)) return hipErrorInvalidValue;
+    // written so that NaN fails
+    if (!(n->eps >= 0.0f) || !std::isfinite(n->eps) || !std::isfinite(n->h_scale) || !std::isfinite(n->x_scale))
+        return hipErrorInvalidValue;
+    if (a.y_type != MGQ_OUT_F32 && a.y_type != MGQ_OUT_F16) return hipErrorInvalidValue;
+    if (a.y && (!n->norm_w || ((uintptr_t)a.y & (a.y_type == MGQ_OUT_F32 ? 3u : 1u)))) return hipErrorInvalidValue;
+    if (!a.h_out && !a.y) return hipErrorInvalidValue;
+    if (!a.x && (n->post_w || a.gate)) return hipErrorInvalidValue;  // what they are for is missing
+    if (a.h_stride < n->hidden || (a.x && a.x_stride < n->hidden) || (a.h_out && a.h_out_stride < n->hidden) ||
+        (a.y && a.y_stride < n->hidden) || (a.gate && a.gate_stride != 0 && a.gate_stride < n->hidden))
+        return hipErrorInvalidValue;
+    if (a.h == a.h_out && a.h_stride != a.h_out_stride) return hipErrorInvalidValue;
+    const void *out[2] = {a.h_out, a.y};
+    for (const void *o : out)  // the other arrays are read again after these are written
+        if (o && (o == a.x || o == a.gate || o == n->post_w || o == n->norm_w || (o == a.y && (o == a.h || o == a.h_out))))
+            return hipErrorInvalidValue;
+    return hipSuccess;
+}
+
+static hipError_t block_norm_run(const mgq_block_norm *n, const mgq_block_norm_args &a, hipStream_t stream) {
+    const hipError_t e = block_norm_check(n, a);
+    if (e != hipSuccess) return e;
+    return mgq::block_norm_launch({a.h, a.x, a.gate, n->post_w, n->norm_w, a.h_out, a.y, a.h_stride, a.x_stride,
+                                   a.gate_stride, a.h_out_stride, a.y_stride, a.rows, n->hidden,
+                                   a.y_type == MGQ_OUT_F16, n->h_scale, n->x_scale, n->eps},
+                                  stream);
+}
+
+hipError_t launch_block_norm_ex(const mgq_block_norm *norm, const float *h, int64_t h_stride, const float *x,
+                                int64_t x_stride, const float *gate, int64_t gate_stride, float *h_out,
+                                int64_t h_out_stride, void *y, int64_t y_stride, int y_type, int rows,
+                                hipStream_t stream) {
+    mgq_block_norm_args a;
+    a.h = h;
+    a.x = x;
+    a.gate = gate;
+    a.h_out = h_out;
+    a.y = y;
+    a.h_stride = h_stride;
+    a.x_stride = x_stride;
+    a.gate_stride = gate_stride;
+    a.h_out_stride = h_out_stride;
+    a.y_stride = y_stride;
+    a.y_type = y_type;
+    a.rows = rows;
+    return block_norm_run(norm, a, stream);
+}
+
 // Host-side checks of one op descriptor (the launchers check again).
 static hipError_t op_check(const mgq_op_desc &o) {
     switch (o.op) {
@@ -366,6 +418,10 @@ static hipError_t op_check(const mgq_op_desc &o) {
     case MGQ_OP_KV_APPEND:
     case MGQ_OP_KV_ATTENTION:
         return mgq::kv_op_check(o.op, o.w);
+    case MGQ_OP_BLOCK_NORM: {
+        const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);
+        return a ? block_norm_check(&a->norm, *a) : hipErrorInvalidValue;
+    }
     default:
         return hipErrorInvalidValue;
     }
@@ -404,6 +460,10 @@ static hipError_t op_launch(const mgq_op_desc &o, hipStream_t s) {
     case MGQ_OP_KV_APPEND:
     case MGQ_OP_KV_ATTENTION:
         return mgq::kv_op_launch(o.op, o.w, s);
+    case MGQ_OP_BLOCK_NORM: {
+        const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);
+        return block_norm_run(&a->norm, *a, s);
+    }
     default:
         return launch_residual_add_ex(o.y, o.x, o.out_dim, s);
     }

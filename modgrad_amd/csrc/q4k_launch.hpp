@@ -258,6 +258,18 @@ hipError_t glu_launch(const float *gate, const float *up, float *out, int n, int
 hipError_t residual_add_launch(float *h, const float *x, int n, hipStream_t stream);
 hipError_t scale_launch(float *h, float s, int n, hipStream_t stream);
 
+// The norms around a block (block_norm.hip): mgq_block_norm and a call's rows.
+// x null: none; gate, post_w, h_out, norm_w with y: may be null.
+struct BlockNorm {
+    const float *h, *x, *gate, *post_w, *norm_w;
+    float *h_out;
+    void *y;
+    int64_t h_stride, x_stride, gate_stride, h_out_stride, y_stride;
+    int rows, hidden, y_f16;
+    float h_scale, x_scale, eps;
+};
+hipError_t block_norm_launch(const BlockNorm &a, hipStream_t stream);
+
 // Persistent decode-step chain (q4k_chain.hip): one cooperative launch runs
 // a list of row-aligned Q4_K matvecs in order.
 struct PersistentChain;

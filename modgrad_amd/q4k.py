@@ -352,6 +352,14 @@ class kern:
         _chk(_lib.load().launch_dequant_q4k_ex(q, n_blocks, out, _stream_ptr(stream)),
              "dequant_q4k")
 
+    @staticmethod
+    def block_norm(norm, h: int, h_stride: int, x: int, x_stride: int, gate: int, gate_stride: int, h_out: int,
+                   h_out_stride: int, y: int, y_stride: int, y_type: int, rows: int, stream=None) -> None:
+        """h_out = h_scale h + x_scale gate norm(x), y = norm(h_out); `norm`: a
+        reference (ctypes.byref) to a norm.BlockNorm's desc."""
+        _chk(_lib.load().launch_block_norm_ex(norm, h, h_stride, x, x_stride, gate, gate_stride, h_out, h_out_stride,
+                                              y, y_stride, y_type, rows, _stream_ptr(stream)), "block_norm")
+
     # rotary positions and the 8-bit key/value cache: `scaling`, `rope` and `cache`
     # are references (ctypes.byref) to the structs that modgrad_amd.kvcache holds
     # (RopeScaling.c, RopeTable.desc, KvCache.desc)

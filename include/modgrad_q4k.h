@@ -371,6 +371,34 @@ hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_ro
                           int n_tokens, int n_heads, int head_dim, int64_t x_stride,
                           int64_t y_stride, hipStream_t stream);
 
+/* Positions of several axes (time, height, width) for images and video: pair i of
+ * a head turns by the position that the token has on the pair's axis.
+ * MGQ_AXES_BLOCKS: the first sections[0] pairs are axis 0's, the next sections[1]
+ * axis 1's, ... MGQ_AXES_TURNS: the axes have a pair each in turn, one that has its
+ * sections[i] is passed over. The pairs that turn are the first sum(sections) of the
+ * head (rot_dim, in a mgq_rope, is of the table; style says which dims pair up among
+ * the 2*sum(sections) that turn). own 0: pair i has column i of the table, so
+ * rope->rot_dim is 2*sum(sections). own 1: every axis has the table's columns from the
+ * first on, in the order of its pairs (a picture's rows and columns at the same
+ * frequencies), and rope->rot_dim is at least twice the largest section.
+ * Positions are device ints, axis a of row t at pos[a*pos_stride + t]; an axis without
+ * pairs is not read. A position outside 0 .. n_pos-1 gives a row of NaN. */
+#define MGQ_AXES_BLOCKS 0
+#define MGQ_AXES_TURNS 1
+typedef struct mgq_rope_axes {
+    const int *pos;
+    int64_t pos_stride; /* at least the call's rows */
+    int n_axes;         /* 1 .. 4 */
+    int sections[4];    /* pairs of each axis, 0 and more; 1 .. 256 together, within head_dim */
+    int order;          /* MGQ_AXES_* */
+    int own;            /* 0 or 1 */
+} mgq_rope_axes;
+
+/* launch_rope_ex with positions of several axes. */
+hipError_t launch_rope_axes_ex(const float *x, float *y, const mgq_rope_axes *axes,
+                               const mgq_rope *rope, int n_tokens, int n_heads, int head_dim,
+                               int64_t x_stride, int64_t y_stride, hipStream_t stream);
+
 /* 8-bit formats of a cache. */
 #define MGQ_KV_I8 0   /* -127 .. 127 */
 #define MGQ_KV_E4M3 1 /* FP8 E4M3 (OCP), largest 448 */
@@ -430,6 +458,16 @@ hipError_t launch_kv_append_ex(const mgq_kv_cache *cache, const mgq_rope *rope, 
                                const float *v, int64_t kv_stride, const float *q,
                                int64_t q_stride, float *q_out, int64_t q_out_stride,
                                int n_q_heads, int n_tokens, int max_new, hipStream_t stream);
+
+/* launch_kv_append_ex with positions of several axes, which the rows of the call
+ * give (mgq_rope_axes; one for each of the n_tokens rows): where a token lies in the
+ * cache does not depend on them. rope is not null, and of any n_pos. A token with a
+ * position outside the table has a q_out row of NaN, and its key, NaN, counts as 0. */
+hipError_t launch_kv_append_axes_ex(const mgq_kv_cache *cache, const mgq_rope *rope,
+                                    const mgq_rope_axes *axes, const float *k, const float *v,
+                                    int64_t kv_stride, const float *q, int64_t q_stride,
+                                    float *q_out, int64_t q_out_stride, int n_q_heads,
+                                    int n_tokens, int max_new, hipStream_t stream);
 
 /* n pages (device ints) as f32: k_out and v_out [n][n_kv_heads][page_tokens]
  * [head_dim] get value * scale, zeros where the id names no page. */
@@ -555,6 +593,8 @@ hipError_t mgq_chain_destroy(void *chain);
  *   MGQ_OP_ROPE          launch_rope_ex of an mgq_rope_args.
  *   MGQ_OP_KV_APPEND     launch_kv_append_ex of an mgq_kv_append_args.
  *   MGQ_OP_KV_ATTENTION  launch_kv_attention_ex of an mgq_kv_attention_args.
+ *   MGQ_OP_ROPE_AXES     launch_rope_axes_ex of an mgq_rope_axes_args.
+ *   MGQ_OP_KV_APPEND_AXES  launch_kv_append_axes_ex of an mgq_kv_append_axes_args.
  *   MGQ_OP_BLOCK_NORM    launch_block_norm_ex of an mgq_block_norm_args.
  * No counterpart in the reference's C ABI: its chain is Rust code that
  * launches these kernels one by one; this records them into one graph. */
@@ -571,6 +611,8 @@ hipError_t mgq_chain_destroy(void *chain);
 #define MGQ_OP_KV_APPEND 10
 #define MGQ_OP_KV_ATTENTION 11
 #define MGQ_OP_BLOCK_NORM 12
+#define MGQ_OP_ROPE_AXES 13
+#define MGQ_OP_KV_APPEND_AXES 14
 /* Those from MGQ_OP_ROPE on take their arguments from here: mgq_op_desc.w points to one
  * in host memory. */
 typedef struct mgq_rope_args {
@@ -598,6 +640,18 @@ typedef struct mgq_kv_attention_args {
     int n_q_heads, out_type, n_tokens, max_new, window;
     float scale, softcap;
 } mgq_kv_attention_args;
+typedef struct mgq_rope_axes_args {
+    const float *x;
+    float *y;
+    mgq_rope_axes axes;
+    mgq_rope rope;
+    int n_tokens, n_heads, head_dim;
+    int64_t x_stride, y_stride;
+} mgq_rope_axes_args;
+typedef struct mgq_kv_append_axes_args {
+    mgq_kv_append_args append;
+    mgq_rope_axes axes;
+} mgq_kv_append_axes_args;
 typedef struct mgq_block_norm_args {
     mgq_block_norm norm;
     const float *h, *x, *gate;

@@ -60,6 +60,8 @@ SIGNATURES = {
     "launch_block_norm_ex": (I, [P, P, L, P, L, P, L, P, L, P, L, I, I, P]),
     "launch_rope_table_ex": (I, [P, I, I, I, P, P]),
     "launch_rope_ex": (I, [P, P, P, P, I, I, I, L, L, P]),
+    "launch_rope_axes_ex": (I, [P, P, P, P, I, I, I, L, L, P]),
+    "launch_kv_append_axes_ex": (I, [P, P, P, P, P, L, P, L, P, L, I, I, I, P]),
     "launch_kv_append_ex": (I, [P, P, P, P, L, P, L, P, L, I, I, I, P]),
     "launch_kv_dequant_ex": (I, [P, P, I, P, P, P]),
     "mgq_kv_attention_workspace_bytes": (S, [P, I, I]),
@@ -95,6 +97,10 @@ OP_ROPE = 9
 OP_KV_APPEND = 10
 OP_KV_ATTENTION = 11
 OP_BLOCK_NORM = 12
+OP_ROPE_AXES = 13
+OP_KV_APPEND_AXES = 14
+AXES_BLOCKS = 0
+AXES_TURNS = 1
 ROPE_INTERLEAVED = 0
 ROPE_HALF = 1
 KV_I8 = 0
@@ -156,6 +162,22 @@ class KvAttentionArgs(ctypes.Structure):
                 ("workspace_bytes", S), ("q_stride", L), ("out_stride", L), ("n_q_heads", I),
                 ("out_type", I), ("n_tokens", I), ("max_new", I), ("window", I), ("scale", F),
                 ("softcap", F)]
+
+
+class RopeAxes(ctypes.Structure):
+    """mgq_rope_axes."""
+    _fields_ = [("pos", P), ("pos_stride", L), ("n_axes", I), ("sections", I * 4), ("order", I), ("own", I)]
+
+
+class RopeAxesArgs(ctypes.Structure):
+    """mgq_rope_axes_args (OP_ROPE_AXES)."""
+    _fields_ = [("x", P), ("y", P), ("axes", RopeAxes), ("rope", Rope), ("n_tokens", I), ("n_heads", I),
+                ("head_dim", I), ("x_stride", L), ("y_stride", L)]
+
+
+class KvAppendAxesArgs(ctypes.Structure):
+    """mgq_kv_append_axes_args (OP_KV_APPEND_AXES)."""
+    _fields_ = [("append", KvAppendArgs), ("axes", RopeAxes)]
 
 
 class BlockNorm(ctypes.Structure):

@@ -17,14 +17,41 @@ bool bad_rope(const mgq_rope &r, int head_dim) {
            r.rot_dim > head_dim || (r.style != MGQ_ROPE_INTERLEAVED && r.style != MGQ_ROPE_HALF);
 }
 
-hipError_t rope_check(const float *x, const float *y, const int *pos, const mgq_rope *r, int n_tokens, int n_heads,
-                      int head_dim, int64_t xs, int64_t ys) {
-    if (!r || bad4(x) || bad4(y) || bad4(pos) || n_tokens <= 0 || n_heads <= 0 || head_dim <= 0 || head_dim % 2)
-        return hipErrorInvalidValue;
-    if (bad_rope(*r, head_dim)) return hipErrorInvalidValue;
+// Positions of n_tokens rows on several axes, and the table that they take.
+bool bad_axes(const mgq_rope_axes *a, const mgq_rope *r, int head_dim, int64_t n_tokens) {
+    if (!a || !r || bad4(a->pos) || a->n_axes < 1 || a->n_axes > 4 || a->pos_stride < n_tokens) return true;
+    if ((a->order != MGQ_AXES_BLOCKS && a->order != MGQ_AXES_TURNS) || (a->own != 0 && a->own != 1)) return true;
+    int64_t pairs = 0;
+    int most = 0;
+    for (int i = 0; i < a->n_axes; ++i) {
+        if (a->sections[i] < 0) return true;
+        pairs += a->sections[i];
+        most = std::max(most, a->sections[i]);
+    }
+    if (pairs < 1 || pairs > 256 || 2 * pairs > head_dim) return true;
+    if (bad_rope(*r, 512)) return true;  // with own columns the table may be wider than a head
+    return a->own ? 2 * most > r->rot_dim : 2 * pairs != r->rot_dim;
+}
+
+// Heads of a row of tokens, where they come from and go.
+hipError_t turn_check(const float *x, const float *y, int n_tokens, int n_heads, int head_dim, int64_t xs, int64_t ys) {
+    if (bad4(x) || bad4(y) || n_tokens <= 0 || n_heads <= 0 || head_dim <= 0 || head_dim % 2) return hipErrorInvalidValue;
     const int64_t row = (int64_t)n_heads * head_dim;
     if (row > kMaxGrid || xs < row || ys < row || (x == y && xs != ys)) return hipErrorInvalidValue;
     return row * n_tokens / 512 >= kMaxGrid ? hipErrorInvalidValue : hipSuccess;
+}
+
+hipError_t rope_check(const float *x, const float *y, const int *pos, const mgq_rope *r, int n_tokens, int n_heads,
+                      int head_dim, int64_t xs, int64_t ys) {
+    if (!r || bad4(pos)) return hipErrorInvalidValue;
+    const hipError_t e = turn_check(x, y, n_tokens, n_heads, head_dim, xs, ys);
+    return e != hipSuccess ? e : bad_rope(*r, head_dim) ? hipErrorInvalidValue : hipSuccess;
+}
+
+hipError_t rope_axes_check(const float *x, const float *y, const mgq_rope_axes *axes, const mgq_rope *r, int n_tokens,
+                           int n_heads, int head_dim, int64_t xs, int64_t ys) {
+    const hipError_t e = turn_check(x, y, n_tokens, n_heads, head_dim, xs, ys);
+    return e != hipSuccess ? e : bad_axes(axes, r, head_dim, n_tokens) ? hipErrorInvalidValue : hipSuccess;
 }
 
 int page_shift(int tokens) { return tokens == 16 ? 4 : tokens == 32 ? 5 : tokens == 64 ? 6 : tokens == 128 ? 7 : -1; }
@@ -72,12 +99,15 @@ KvView view(const mgq_kv_cache &c, int n_tokens, int max_new) {
     return v;
 }
 
-hipError_t append_check(const mgq_kv_cache *c, const mgq_rope *rope, const float *k, const float *v, int64_t kvs,
-                        const float *q, int64_t qs, const float *qo, int64_t qos, int hq, int n_tokens, int max_new) {
+// axes: null but for positions of several.
+hipError_t append_check(const mgq_kv_cache *c, const mgq_rope *rope, const mgq_rope_axes *axes, const float *k,
+                        const float *v, int64_t kvs, const float *q, int64_t qs, const float *qo, int64_t qos, int hq,
+                        int n_tokens, int max_new) {
     const hipError_t e = call_check(c, n_tokens, max_new);
     if (e != hipSuccess) return e;
     if (bad4(k) || bad4(v) || kvs < (int64_t)c->n_kv_heads * c->head_dim) return hipErrorInvalidValue;
-    if (rope && (bad_rope(*rope, c->head_dim) || rope->n_pos < (int64_t)c->max_pages * c->page_tokens))
+    if (axes ? bad_axes(axes, rope, c->head_dim, n_tokens)
+             : rope && (bad_rope(*rope, c->head_dim) || rope->n_pos < (int64_t)c->max_pages * c->page_tokens))
         return hipErrorInvalidValue;
     if (q) {
         const int64_t row = (int64_t)hq * c->head_dim;
@@ -139,9 +169,19 @@ hipError_t kv_op_check(int op, const void *args) {
         const auto &a = *static_cast<const mgq_rope_args *>(args);
         return rope_check(a.x, a.y, a.pos, &a.rope, a.n_tokens, a.n_heads, a.head_dim, a.x_stride, a.y_stride);
     }
+    if (op == MGQ_OP_ROPE_AXES) {
+        const auto &a = *static_cast<const mgq_rope_axes_args *>(args);
+        return rope_axes_check(a.x, a.y, &a.axes, &a.rope, a.n_tokens, a.n_heads, a.head_dim, a.x_stride, a.y_stride);
+    }
+    if (op == MGQ_OP_KV_APPEND_AXES) {
+        const auto &a = *static_cast<const mgq_kv_append_axes_args *>(args);
+        const mgq_kv_append_args &p = a.append;
+        return append_check(&p.cache, &p.rope, &a.axes, p.k, p.v, p.kv_stride, p.q, p.q_stride, p.q_out,
+                            p.q_out_stride, p.n_q_heads, p.n_tokens, p.max_new);
+    }
     if (op == MGQ_OP_KV_APPEND) {
         const auto &a = *static_cast<const mgq_kv_append_args *>(args);
-        return append_check(&a.cache, a.rope.table ? &a.rope : nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
+        return append_check(&a.cache, a.rope.table ? &a.rope : nullptr, nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
                             a.q_out, a.q_out_stride, a.n_q_heads, a.n_tokens, a.max_new);
     }
     const auto &a = *static_cast<const mgq_kv_attention_args *>(args);
@@ -154,6 +194,17 @@ hipError_t kv_op_launch(int op, const void *args, hipStream_t stream) {
         const auto &a = *static_cast<const mgq_rope_args *>(args);
         return launch_rope_ex(a.x, a.y, a.pos, &a.rope, a.n_tokens, a.n_heads, a.head_dim, a.x_stride, a.y_stride,
                               stream);
+    }
+    if (op == MGQ_OP_ROPE_AXES) {
+        const auto &a = *static_cast<const mgq_rope_axes_args *>(args);
+        return launch_rope_axes_ex(a.x, a.y, &a.axes, &a.rope, a.n_tokens, a.n_heads, a.head_dim, a.x_stride,
+                                   a.y_stride, stream);
+    }
+    if (op == MGQ_OP_KV_APPEND_AXES) {
+        const auto &a = *static_cast<const mgq_kv_append_axes_args *>(args);
+        const mgq_kv_append_args &p = a.append;
+        return launch_kv_append_axes_ex(&p.cache, &p.rope, &a.axes, p.k, p.v, p.kv_stride, p.q, p.q_stride, p.q_out,
+                                        p.q_out_stride, p.n_q_heads, p.n_tokens, p.max_new, stream);
     }
     if (op == MGQ_OP_KV_APPEND) {
         const auto &a = *static_cast<const mgq_kv_append_args *>(args);
@@ -194,14 +245,33 @@ hipError_t launch_rope_ex(const float *x, float *y, const int *pos, const mgq_ro
     return rope_launch(x, y, pos, *rope, n_tokens, n_heads, head_dim, x_stride, y_stride, stream);
 }
 
+hipError_t launch_rope_axes_ex(const float *x, float *y, const mgq_rope_axes *axes, const mgq_rope *rope, int n_tokens,
+                               int n_heads, int head_dim, int64_t x_stride, int64_t y_stride, hipStream_t stream) {
+    const hipError_t e = rope_axes_check(x, y, axes, rope, n_tokens, n_heads, head_dim, x_stride, y_stride);
+    if (e != hipSuccess) return e;
+    return rope_axes_launch(x, y, *axes, *rope, n_tokens, n_heads, head_dim, x_stride, y_stride, stream);
+}
+
 hipError_t launch_kv_append_ex(const mgq_kv_cache *c, const mgq_rope *rope, const float *k, const float *v,
                                int64_t kv_stride, const float *q, int64_t q_stride, float *q_out,
                                int64_t q_out_stride, int n_q_heads, int n_tokens, int max_new, hipStream_t stream) {
-    const hipError_t e = append_check(c, rope, k, v, kv_stride, q, q_stride, q_out, q_out_stride, n_q_heads, n_tokens,
-                                      max_new);
+    const hipError_t e = append_check(c, rope, nullptr, k, v, kv_stride, q, q_stride, q_out, q_out_stride, n_q_heads,
+                                      n_tokens, max_new);
     if (e != hipSuccess) return e;
     const KvAppend a = {k, v, kv_stride, q, q_out, q_stride, q_out_stride, n_q_heads};
-    return kv_append_launch(view(*c, n_tokens, max_new), c->head_dim, c->format, rope, a, stream);
+    return kv_append_launch(view(*c, n_tokens, max_new), c->head_dim, c->format, rope, nullptr, a, stream);
+}
+
+hipError_t launch_kv_append_axes_ex(const mgq_kv_cache *c, const mgq_rope *rope, const mgq_rope_axes *axes,
+                                    const float *k, const float *v, int64_t kv_stride, const float *q,
+                                    int64_t q_stride, float *q_out, int64_t q_out_stride, int n_q_heads, int n_tokens,
+                                    int max_new, hipStream_t stream) {
+    if (!axes) return hipErrorInvalidValue;
+    const hipError_t e = append_check(c, rope, axes, k, v, kv_stride, q, q_stride, q_out, q_out_stride, n_q_heads,
+                                      n_tokens, max_new);
+    if (e != hipSuccess) return e;
+    const KvAppend a = {k, v, kv_stride, q, q_out, q_stride, q_out_stride, n_q_heads};
+    return kv_append_launch(view(*c, n_tokens, max_new), c->head_dim, c->format, rope, axes, a, stream);
 }
 
 hipError_t launch_kv_dequant_ex(const mgq_kv_cache *c, const int *pages, int n, float *k_out, float *v_out,

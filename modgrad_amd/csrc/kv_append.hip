@@ -58,9 +58,9 @@ struct Divider {
     }
 };
 
-template <int D, int FMT, bool VEC, int NT>
-__global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, const float *__restrict__ rope, int rot,
-                                                       int half, unsigned last_pos, AppendGrid gr) {
+template <int D, int FMT, bool VEC, int NT, class Rope>
+__global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, Rope rope, AppendGrid gr) {
+    const int rot = rope.rot, half = rope.half;
     typedef RopeUnit<VEC> U;
     constexpr int kUnits = D / U::N;
     const int tid = threadIdx.x;
@@ -84,15 +84,8 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
         for (int k = 0; k < kQueryUnits; ++k)
             U(r[k] % kUnits, rot, half).load(a.q + (s.t0 + (int64_t)t[k]) * a.q_stride + (r[k] / kUnits) * D, v[k]);
 #pragma unroll
-        for (int k = 0; k < kQueryUnits; ++k) {
-            const int p = s.pos0 + (int)t[k];
-            if ((unsigned)p <= last_pos) {
-                U(r[k] % kUnits, rot, half).turn(rope + (int64_t)p * rot, half, v[k]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < U::N; ++e) v[k][e] = __builtin_nan("");
-            }
-        }
+        for (int k = 0; k < kQueryUnits; ++k)
+            rope.turn(U(r[k] % kUnits, rot, half), s.pos0 + (int)t[k], s.t0 + (int64_t)t[k], v[k]);
 #pragma unroll
         for (int k = 0; k < kQueryUnits; ++k)
             if (first + k * NT < units)
@@ -130,7 +123,8 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
             const int i = min(i0 + e * NT, total - 1);
-            U(i % kUnits, rot, half).turn(rope + (int64_t)(begin + i / kUnits) * rot, half, kv[e]);
+            const int p = begin + i / kUnits;
+            rope.turn_key(U(i % kUnits, rot, half), p, s.t0 + (int64_t)p - s.pos0, kv[e]);
         }
     };
     const auto each_key = [&](int i0, auto f) {
@@ -244,8 +238,8 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvView c, KvAppend a, con
     }
 }
 
-template <int D, int FMT, bool VEC, int NT>
-static hipError_t append_run(const KvView &c, const mgq_rope *rope, const KvAppend &a, hipStream_t stream) {
+template <int D, int FMT, bool VEC, int NT, class Rope>
+static hipError_t append_run(const KvView &c, const Rope &rope, const KvAppend &a, hipStream_t stream) {
     const int page = 1 << c.page_shift;
     AppendGrid g;
     g.page_blocks = (c.max_new + page - 2) / page + 1;
@@ -253,22 +247,20 @@ static hipError_t append_run(const KvView &c, const mgq_rope *rope, const KvAppe
     const int64_t units = (int64_t)c.max_new * a.hq * (D / RopeUnit<VEC>::N);
     g.q_blocks = a.q ? (int)((units + kQueryUnits * NT - 1) / (kQueryUnits * NT)) : 0;
     const int64_t grid = g.kv_groups + (int64_t)c.n_seqs * g.q_blocks;
-    kv_append_kernel<D, FMT, VEC, NT><<<(unsigned)grid, NT, 0, stream>>>(
-        c, a, rope ? rope->table : nullptr, rope ? rope->rot_dim : 0, rope && rope->style == MGQ_ROPE_HALF,
-        rope ? (unsigned)(rope->n_pos - 1) : 0xFFFFFFFFu, g);  // no table: rows are copied, wherever they are
+    kv_append_kernel<D, FMT, VEC, NT, Rope><<<(unsigned)grid, NT, 0, stream>>>(c, a, rope, g);
     return hipGetLastError();
 }
 
-template <int D, int FMT>
-static hipError_t append_dim(const KvView &c, const mgq_rope *rope, const KvAppend &a, hipStream_t stream) {
+template <int D, int FMT, class Rope>
+static hipError_t append_dim(const KvView &c, const Rope &rope, const KvAppend &a, hipStream_t stream) {
     // a single token has one pair for each lane; wide units are for rows of work
     if (c.max_new == 1) return append_run<D, FMT, false, 64>(c, rope, a, stream);
-    if (!rope || rope_wide(D, rope->rot_dim)) return append_run<D, FMT, true, 256>(c, rope, a, stream);
+    if (rope_wide(D, rope.rot)) return append_run<D, FMT, true, 256>(c, rope, a, stream);
     return append_run<D, FMT, false, 256>(c, rope, a, stream);
 }
 
-hipError_t kv_append_launch(const KvView &c, int dim, int fmt, const mgq_rope *rope, const KvAppend &a,
-                            hipStream_t stream) {
+template <class Rope>
+static hipError_t append_any(const KvView &c, int dim, int fmt, const Rope &rope, const KvAppend &a, hipStream_t stream) {
     const bool i8 = fmt == MGQ_KV_I8;
     switch (dim) {
     case 64: return i8 ? append_dim<64, kFmtI8>(c, rope, a, stream) : append_dim<64, kFmtE4M3>(c, rope, a, stream);
@@ -276,6 +268,15 @@ hipError_t kv_append_launch(const KvView &c, int dim, int fmt, const mgq_rope *r
     case 128: return i8 ? append_dim<128, kFmtI8>(c, rope, a, stream) : append_dim<128, kFmtE4M3>(c, rope, a, stream);
     default: return i8 ? append_dim<256, kFmtI8>(c, rope, a, stream) : append_dim<256, kFmtE4M3>(c, rope, a, stream);
     }
+}
+
+hipError_t kv_append_launch(const KvView &c, int dim, int fmt, const mgq_rope *rope, const mgq_rope_axes *axes,
+                            const KvAppend &a, hipStream_t stream) {
+    if (axes) return append_any(c, dim, fmt, rope_many(*rope, *axes), a, stream);
+    // no table: rows are copied, wherever they are
+    RopeLine line = {nullptr, 0, 0, 0xFFFFFFFFu};
+    if (rope) line = {rope->table, rope->rot_dim, rope->style == MGQ_ROPE_HALF, (unsigned)(rope->n_pos - 1)};
+    return append_any(c, dim, fmt, line, a, stream);
 }
 
 // Pages of the cache as f32, K and V both [page][kv head][token][dim]. One

@@ -176,6 +176,93 @@ struct RopeUnit {
     }
 };
 
+// Where a token's rotation comes from: turn() turns a unit of the token in row `row`
+// of the call, at position `pos` of its sequence. A position outside the table makes
+// the whole head NaN.
+//
+// One axis: the table's row of the position. (last: the last position that is looked
+// at; without a table rot is 0 and nothing turns, wherever the token is.)
+struct RopeLine {
+    const float *table;
+    int rot, half;
+    unsigned last;
+    template <bool VEC>
+    __device__ __forceinline__ void turn(const RopeUnit<VEC> &u, int pos, int64_t, double (&v)[RopeUnit<VEC>::N]) const {
+        if ((unsigned)pos <= last) {
+            u.turn(table + (int64_t)pos * rot, half, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < RopeUnit<VEC>::N; ++e) v[e] = __builtin_nan("");
+        }
+    }
+    // a key: its position is in the table
+    template <bool VEC>
+    __device__ __forceinline__ void turn_key(const RopeUnit<VEC> &u, int pos, int64_t, double (&v)[RopeUnit<VEC>::N]) const {
+        u.turn(table + (int64_t)pos * rot, half, v);
+    }
+};
+
+// Several axes: pair i turns by the position of its axis, which the row gives. Which
+// axis that is follows from at most four runs of pairs: from pair `start` on the run's
+// `m` axes (two bits each of `list`) have a pair each in turn; `base` pairs of each of
+// them lie before the run. In blocks a run is an axis.
+struct RopeMany {
+    const float *table;
+    const int *pos;      // [axis][stride]
+    int64_t stride;
+    int rot, half;       // dims that turn: twice the pairs
+    int columns, n_pos;  // of the table
+    int used;            // bits of the axes that have pairs
+    int own;             // the column is the pair's number among its axis's, else among all
+    uint32_t run[4];     // start | m << 9 | list << 12 | base << 20; start 511: none
+    __device__ __forceinline__ void place(int pair, int &axis, int &column) const {
+        uint32_t r = run[0];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) r = pair >= (int)(run[k] & 511u) ? run[k] : r;
+        const int j = pair - (int)(r & 511u), m = (r >> 9) & 7;
+        // j / m for j < 256 by 1024 / m, for m = 3 rounded up: that adds less than a third
+        const int q = (j * (m == 3 ? 342 : 1024 >> (m >> 1))) >> 10;
+        axis = (r >> (12 + 2 * (j - q * m))) & 3;
+        column = own ? q + (int)(r >> 20) : pair;
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void turn(const RopeUnit<VEC> &u, int, int64_t row, double (&v)[RopeUnit<VEC>::N]) const {
+        int p[4];
+        bool ok = true;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            p[a] = used >> a & 1 ? pos[a * stride + row] : 0;
+            ok = ok && (unsigned)p[a] < (unsigned)n_pos;
+        }
+        if (!ok) {
+#pragma unroll
+            for (int e = 0; e < RopeUnit<VEC>::N; ++e) v[e] = __builtin_nan("");
+            return;
+        }
+        if (!u.rot) return;
+        constexpr int H = RopeUnit<VEC>::N / 2;
+        const int first = half ? u.d0 : u.d0 / 2;
+        float2 cs[H];
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+            int axis, column;
+            place(first + e, axis, column);
+            const int at = axis == 0 ? p[0] : axis == 1 ? p[1] : axis == 2 ? p[2] : p[3];
+            const float *c = table + 2 * ((int64_t)at * columns + column);
+            cs[e] = make_float2(c[0], c[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+            if (half) rope_pair(v[e], v[H + e], cs[e].x, cs[e].y);
+            else rope_pair(v[2 * e], v[2 * e + 1], cs[e].x, cs[e].y);
+        }
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void turn_key(const RopeUnit<VEC> &u, int pos_, int64_t row, double (&v)[RopeUnit<VEC>::N]) const {
+        turn(u, pos_, row, v);
+    }
+};
+
 // Whether heads of `dim` with `rot` rotated dims split into wide units.
 __host__ __device__ inline bool rope_wide(int dim, int rot) { return rot % 8 == 0 && dim % 8 == 0; }
 

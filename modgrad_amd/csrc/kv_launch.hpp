@@ -14,6 +14,12 @@ hipError_t rope_table_launch(float *table, int n_pos, int first, int rot_dim, co
 hipError_t rope_launch(const float *x, float *y, const int *pos, const mgq_rope &r, int n_tokens, int heads, int dim,
                        int64_t x_stride, int64_t y_stride, hipStream_t stream);
 
+hipError_t rope_axes_launch(const float *x, float *y, const mgq_rope_axes &axes, const mgq_rope &r, int n_tokens,
+                            int heads, int dim, int64_t x_stride, int64_t y_stride, hipStream_t stream);
+// How the kernels see several axes (kv_rope.hip); all of it checked.
+struct RopeMany;
+RopeMany rope_many(const mgq_rope &r, const mgq_rope_axes &axes);
+
 // k and v rows `kv_stride` floats apart; rope null: stored as they come; q
 // null: no queries. Queries are rotated from q to q_out.
 struct KvAppend {
@@ -24,8 +30,8 @@ struct KvAppend {
     int64_t q_stride, q_out_stride;
     int hq;
 };
-hipError_t kv_append_launch(const KvView &c, int dim, int fmt, const mgq_rope *rope, const KvAppend &a,
-                            hipStream_t stream);
+hipError_t kv_append_launch(const KvView &c, int dim, int fmt, const mgq_rope *rope, const mgq_rope_axes *axes,
+                            const KvAppend &a, hipStream_t stream);
 hipError_t kv_dequant_launch(const KvView &c, int dim, int fmt, const int *pages, int n, float *k_out, float *v_out,
                              hipStream_t stream);
 

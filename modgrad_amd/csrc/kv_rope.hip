@@ -131,4 +131,65 @@ hipError_t rope_launch(const float *x, float *y, const int *pos, const mgq_rope 
     return hipGetLastError();
 }
 
+// The same with positions of several axes, a row of the table for each.
+template <bool VEC>
+__global__ __launch_bounds__(256) void rope_axes_kernel(const float *x, float *y, RopeMany m, int n_tokens, int heads,
+                                                        int dim, int64_t x_stride, int64_t y_stride) {
+    typedef RopeUnit<VEC> U;
+    const unsigned per_head = dim / U::N, per_token = per_head * heads;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (uint64_t)per_token * n_tokens) return;
+    const unsigned t = (unsigned)(i / per_token), r = (unsigned)(i % per_token), h = r / per_head;
+    const U u(r % per_head, m.rot, m.half);
+    double v[U::N];
+    u.load(x + t * x_stride + (int64_t)h * dim, v);
+    m.turn(u, 0, t, v);
+    u.store(y + t * y_stride + (int64_t)h * dim, v);
+}
+
+RopeMany rope_many(const mgq_rope &r, const mgq_rope_axes &a) {
+    RopeMany m;
+    m.table = r.table;
+    m.pos = a.pos;
+    m.stride = a.pos_stride;
+    m.half = r.style == MGQ_ROPE_HALF;
+    m.columns = r.rot_dim / 2;
+    m.n_pos = r.n_pos;
+    m.own = a.own != 0;
+    m.used = 0;
+    int left[4] = {}, pairs = 0;
+    for (int i = 0; i < a.n_axes; ++i) {
+        left[i] = a.sections[i];
+        if (left[i] > 0) m.used |= 1 << i;
+        pairs += left[i];
+    }
+    m.rot = 2 * pairs;
+    for (int k = 0, at = 0, base = 0; k < 4; ++k) {
+        uint32_t list = 0, count = 0;
+        int least = 0;  // of the run's axes, the pairs that the shortest has left
+        for (int i = 0; i < 4; ++i) {
+            if (left[i] == 0 || (a.order == MGQ_AXES_BLOCKS && count > 0)) continue;
+            list |= (uint32_t)i << (2 * count++);
+            least = least ? std::min(least, left[i]) : left[i];
+        }
+        // a run that does not come: past every pair
+        m.run[k] = count ? (uint32_t)at | count << 9 | list << 12 | (uint32_t)base << 20 : 511u | 1u << 9;
+        for (uint32_t j = 0; j < count; ++j) left[list >> (2 * j) & 3] -= least;
+        at += least * (int)count;
+        if (a.order != MGQ_AXES_BLOCKS) base += least;
+    }
+    return m;
+}
+
+hipError_t rope_axes_launch(const float *x, float *y, const mgq_rope_axes &axes, const mgq_rope &r, int n_tokens,
+                            int heads, int dim, int64_t x_stride, int64_t y_stride, hipStream_t stream) {
+    const RopeMany m = rope_many(r, axes);
+    const bool vec = rope_wide(dim, m.rot);
+    const uint64_t units = (uint64_t)n_tokens * heads * (dim / (vec ? 8 : 2));
+    const unsigned grid = (unsigned)((units + 255) / 256);
+    if (vec) rope_axes_kernel<true><<<grid, 256, 0, stream>>>(x, y, m, n_tokens, heads, dim, x_stride, y_stride);
+    else rope_axes_kernel<false><<<grid, 256, 0, stream>>>(x, y, m, n_tokens, heads, dim, x_stride, y_stride);
+    return hipGetLastError();
+}
+
 }  // namespace mgq

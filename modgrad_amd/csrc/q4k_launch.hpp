@@ -278,7 +278,7 @@ hipError_t chain_persistent_launch(PersistentChain *p, hipStream_t stream);
 hipError_t chain_persistent_faults(PersistentChain *p, unsigned *faults);
 hipError_t chain_persistent_destroy(PersistentChain *p);
 
-// MGQ_OP_ROPE, _KV_APPEND and _KV_ATTENTION of an op chain: the host-side
+// MGQ_OP_ROPE, the _KV_ ops and MGQ_OP_ROPE_AXES of an op chain: the host-side
 // checks of their argument struct, and the launch (kv_abi.hip).
 hipError_t kv_op_check(int op, const void *args);
 hipError_t kv_op_launch(int op, const void *args, hipStream_t stream);

@@ -5,6 +5,7 @@ C ABI.
 
   RopeScaling   frequencies of a rotary table, from numbers or GGUF metadata
   RopeTable     a table of (cos, sin) on the device, and its application
+  RopeAxes      positions of several axes (time, height, width) on such a table
   KvCache       pages of 8-bit keys and values, their scales and page tables;
                 append, attend, dequant, and the same as op-chain descriptors
 
@@ -117,6 +118,42 @@ class RopeScaling:
                    orig_ctx=float(orig), factors=factors)
 
 
+class RopeAxes:
+    """How the pairs of a head are shared out among several axes of positions
+    (mgq_rope_axes): sections[a] pairs for axis a, in "blocks" one after another, or in
+    "turns" of one pair for each axis that has some left. own: every axis has the
+    table's columns from the first on (a picture's rows and columns), instead of the
+    pair's. With one, RopeTable.apply and KvCache.append take positions
+    [n_axes][pos_stride]."""
+
+    ORDERS = {"blocks": _lib.AXES_BLOCKS, "turns": _lib.AXES_TURNS}
+
+    def __init__(self, sections, order: str = "blocks", own: bool = False):
+        self.sections = [int(n) for n in sections]
+        if order not in self.ORDERS or not 1 <= len(self.sections) <= 4 or min(self.sections) < 0 \
+                or not 1 <= sum(self.sections) <= 256:
+            raise BackendError("Runtime", f"rope axes: sections {self.sections}, {order!r}")
+        self.order, self.own = order, bool(own)
+
+    @classmethod
+    def from_gguf(cls, g, order: str = "blocks") -> "RopeAxes":
+        """Of a GGUF model's <arch>.rope.dimension_sections. Whether its axes lie in
+        blocks or take turns is the architecture's, and no key of the file says it."""
+        key = f"{g.architecture()}.rope.dimension_sections"
+        m = g.meta(key)
+        values = m.value if m is not None and isinstance(m.value, list) else []
+        sections = [v.value for v in values]
+        if not sections or not all(isinstance(n, int) and not isinstance(n, bool) for n in sections):
+            raise BackendError("Unsupported", f"{key}: whole numbers expected")
+        return cls(sections, order)
+
+    def at(self, pos: int, pos_stride: int) -> "_lib.RopeAxes":
+        """With the positions of a call: device ints, axis a of row t at
+        pos[a * pos_stride + t]."""
+        n = len(self.sections)
+        return _lib.RopeAxes(pos or None, pos_stride, n, (_lib.I * 4)(*self.sections), self.ORDERS[self.order], self.own)
+
+
 class RopeTable:
     """(cos, sin) of positions 0 .. n_pos-1 on the device, f32
     [n_pos][rot_dim/2][2]. half: pairs (i, i + rot_dim/2); else (2i, 2i+1)."""
@@ -174,19 +211,31 @@ class RopeTable:
         self.ref = ctypes.byref(self.desc)
 
     def apply(self, x: int, y: int, pos: int, n_tokens: int, n_heads: int, head_dim: int,
-              x_stride: int | None = None, y_stride: int | None = None, stream=None) -> None:
-        """y = x, [n_tokens][n_heads][head_dim] f32 turned to positions pos."""
+              x_stride: int | None = None, y_stride: int | None = None, stream=None,
+              axes: RopeAxes | None = None, pos_stride: int | None = None) -> None:
+        """y = x, [n_tokens][n_heads][head_dim] f32 turned to positions pos; with
+        axes, pos is [n_axes][pos_stride] (n_tokens by default)."""
         if self._look:
             _on_device(self.device)
         row = n_heads * head_dim
+        if axes is not None:
+            at = axes.at(pos, n_tokens if pos_stride is None else pos_stride)
+            kern.rope_axes(x, y, ctypes.byref(at), self.ref, n_tokens, n_heads, head_dim,
+                           row if x_stride is None else x_stride, row if y_stride is None else y_stride, stream)
+            return
         kern.rope(x, y, pos, self.ref, n_tokens, n_heads, head_dim,
                   row if x_stride is None else x_stride, row if y_stride is None else y_stride,
                   stream)
 
     def op(self, x: int, y: int, pos: int, n_tokens: int, n_heads: int, head_dim: int,
-           x_stride: int | None = None, y_stride: int | None = None) -> "_lib.OpDesc":
+           x_stride: int | None = None, y_stride: int | None = None, axes: RopeAxes | None = None,
+           pos_stride: int | None = None) -> "_lib.OpDesc":
         """apply as a descriptor of an op chain (q4k.Chain.from_ops)."""
         row = n_heads * head_dim
+        if axes is not None:
+            return _op(_lib.OP_ROPE_AXES, _lib.RopeAxesArgs(
+                x, y, axes.at(pos, n_tokens if pos_stride is None else pos_stride), self.desc, n_tokens, n_heads,
+                head_dim, row if x_stride is None else x_stride, row if y_stride is None else y_stride))
         return _op(_lib.OP_ROPE, _lib.RopeArgs(
             x, y, pos, self.desc, n_tokens, n_heads, head_dim,
             row if x_stride is None else x_stride, row if y_stride is None else y_stride))
@@ -352,14 +401,24 @@ class KvCache:
     # -- operators -----------------------------------------------------------
     def append(self, k: int, v: int, kv_stride: int, n_tokens: int, max_new: int, rope=None,
                q: int = 0, q_stride: int = 0, q_out: int | None = None, q_out_stride: int | None = None,
-               n_q_heads: int = 0, stream=None) -> None:
+               n_q_heads: int = 0, stream=None, axes: RopeAxes | None = None, pos: int = 0,
+               pos_stride: int | None = None) -> None:
         """Rows of k and v (n_kv_heads*head_dim floats, kv_stride apart) into
         the cache, k rotated by `rope` (a RopeTable); q, if given, rotated to
-        q_out (in place by default)."""
+        q_out (in place by default). With axes, the rows' positions are pos
+        [n_axes][pos_stride] (n_tokens by default), not their places."""
         if self._look:
             _on_device(self.device)
         if rope is not None and (self._look or rope._look) and rope.device != self.device:
             raise BackendError("Runtime", f"rope table on {rope.device}, cache on {self.device}")
+        if axes is None and pos:
+            raise BackendError("Runtime", "append: positions without axes")
+        if axes is not None:
+            at = axes.at(pos, n_tokens if pos_stride is None else pos_stride)
+            kern.kv_append_axes(self._ref, None if rope is None else rope.ref, ctypes.byref(at), k, v, kv_stride, q,
+                                q_stride, q if q_out is None else q_out,
+                                q_stride if q_out_stride is None else q_out_stride, n_q_heads, n_tokens, max_new, stream)
+            return
         kern.kv_append(self._ref, None if rope is None else rope.ref, k, v, kv_stride, q, q_stride,
                        q if q_out is None else q_out, q_stride if q_out_stride is None else q_out_stride,
                        n_q_heads, n_tokens, max_new, stream)
@@ -398,11 +457,18 @@ class KvCache:
     # -- the same as descriptors of an op chain (q4k.Chain.from_ops) ----------
     def op_append(self, k: int, v: int, kv_stride: int, n_tokens: int, max_new: int, rope=None,
                   q: int = 0, q_stride: int = 0, q_out: int | None = None,
-                  q_out_stride: int | None = None, n_q_heads: int = 0) -> "_lib.OpDesc":
-        return _op(_lib.OP_KV_APPEND, _lib.KvAppendArgs(
+                  q_out_stride: int | None = None, n_q_heads: int = 0, axes: RopeAxes | None = None, pos: int = 0,
+                  pos_stride: int | None = None) -> "_lib.OpDesc":
+        args = _lib.KvAppendArgs(
             self.desc, _lib.Rope() if rope is None else rope.desc, k, v, q or None,
             (q if q_out is None else q_out) or None, kv_stride, q_stride,
-            q_stride if q_out_stride is None else q_out_stride, n_q_heads, n_tokens, max_new))
+            q_stride if q_out_stride is None else q_out_stride, n_q_heads, n_tokens, max_new)
+        if axes is None:
+            if pos:
+                raise BackendError("Runtime", "append: positions without axes")
+            return _op(_lib.OP_KV_APPEND, args)
+        return _op(_lib.OP_KV_APPEND_AXES, _lib.KvAppendAxesArgs(
+            args, axes.at(pos, n_tokens if pos_stride is None else pos_stride)))
 
     def op_attend(self, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int,
                   n_tokens: int, max_new: int, workspace, scale: float | None = None,

@@ -381,6 +381,22 @@ class kern:
              "rope")
 
     @staticmethod
+    def rope_axes(x: int, y: int, axes, rope, n_tokens: int, n_heads: int, head_dim: int, x_stride: int,
+                  y_stride: int, stream=None) -> None:
+        """rope with positions of several axes; `axes`: a reference to a
+        _lib.RopeAxes (kvcache.RopeAxes.at)."""
+        _chk(_lib.load().launch_rope_axes_ex(x, y, axes, rope, n_tokens, n_heads, head_dim, x_stride, y_stride,
+                                             _stream_ptr(stream)), "rope_axes")
+
+    @staticmethod
+    def kv_append_axes(cache, rope, axes, k: int, v: int, kv_stride: int, q: int, q_stride: int, q_out: int,
+                       q_out_stride: int, n_q_heads: int, n_tokens: int, max_new: int, stream=None) -> None:
+        """kv_append with positions of several axes."""
+        _chk(_lib.load().launch_kv_append_axes_ex(
+            cache, rope, axes, k, v, kv_stride, q, q_stride, q_out, q_out_stride, n_q_heads, n_tokens, max_new,
+            _stream_ptr(stream)), "kv_append_axes")
+
+    @staticmethod
     def kv_append(cache, rope, k: int, v: int,
                   kv_stride: int, q: int, q_stride: int, q_out: int, q_out_stride: int,
                   n_q_heads: int, n_tokens: int, max_new: int, stream=None) -> None:

@@ -504,6 +504,18 @@ hipError_t launch_kv_attention_ex(const mgq_kv_cache *cache, const float *q, int
                                   int window, void *workspace, size_t workspace_bytes,
                                   hipStream_t stream);
 
+/* launch_kv_attention_ex where the first `sinks` positions of a sequence stay
+ * visible behind its window: out row t is over the j <= pos with j > pos - window or
+ * j < sinks. With window 0 all of them are visible and sinks changes nothing. Pages
+ * between the first tokens and the window may be given back (-1 in the table). sinks is
+ * not negative; everything else as above, the workspace too. */
+hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *q,
+                                        int64_t q_stride, int n_q_heads, void *out,
+                                        int64_t out_stride, int out_type, int n_tokens,
+                                        int max_new, float scale, float softcap, int window,
+                                        int sinks, void *workspace, size_t workspace_bytes,
+                                        hipStream_t stream);
+
 /* One matvec of a decode-step chain. */
 typedef struct mgq_gemv_desc {
     const unsigned char *w_q4; /* row-aligned Q4_K bytes */
@@ -593,6 +605,8 @@ hipError_t mgq_chain_destroy(void *chain);
  *   MGQ_OP_ROPE          launch_rope_ex of an mgq_rope_args.
  *   MGQ_OP_KV_APPEND     launch_kv_append_ex of an mgq_kv_append_args.
  *   MGQ_OP_KV_ATTENTION  launch_kv_attention_ex of an mgq_kv_attention_args.
+ *   MGQ_OP_KV_ATTENTION_SINKS  launch_kv_attention_sinks_ex of an
+ *                        mgq_kv_attention_sinks_args.
  *   MGQ_OP_ROPE_AXES     launch_rope_axes_ex of an mgq_rope_axes_args.
  *   MGQ_OP_KV_APPEND_AXES  launch_kv_append_axes_ex of an mgq_kv_append_axes_args.
  *   MGQ_OP_BLOCK_NORM    launch_block_norm_ex of an mgq_block_norm_args.
@@ -613,6 +627,7 @@ hipError_t mgq_chain_destroy(void *chain);
 #define MGQ_OP_BLOCK_NORM 12
 #define MGQ_OP_ROPE_AXES 13
 #define MGQ_OP_KV_APPEND_AXES 14
+#define MGQ_OP_KV_ATTENTION_SINKS 15
 /* Those from MGQ_OP_ROPE on take their arguments from here: mgq_op_desc.w points to one
  * in host memory. */
 typedef struct mgq_rope_args {
@@ -640,6 +655,10 @@ typedef struct mgq_kv_attention_args {
     int n_q_heads, out_type, n_tokens, max_new, window;
     float scale, softcap;
 } mgq_kv_attention_args;
+typedef struct mgq_kv_attention_sinks_args {
+    mgq_kv_attention_args attention;
+    int sinks;
+} mgq_kv_attention_sinks_args;
 typedef struct mgq_rope_axes_args {
     const float *x;
     float *y;

@@ -65,6 +65,7 @@ SIGNATURES = {
     "launch_kv_append_ex": (I, [P, P, P, P, L, P, L, P, L, I, I, I, P]),
     "launch_kv_dequant_ex": (I, [P, P, I, P, P, P]),
     "mgq_kv_attention_workspace_bytes": (S, [P, I, I]),
+    "launch_kv_attention_sinks_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, I, P, S, P]),
     "launch_kv_attention_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, P, S, P]),
     "mgq_chain_create": (I, [P, I, P]),
     "mgq_chain_create_ex": (I, [P, I, I, P]),
@@ -99,6 +100,7 @@ OP_KV_ATTENTION = 11
 OP_BLOCK_NORM = 12
 OP_ROPE_AXES = 13
 OP_KV_APPEND_AXES = 14
+OP_KV_ATTENTION_SINKS = 15
 AXES_BLOCKS = 0
 AXES_TURNS = 1
 ROPE_INTERLEAVED = 0
@@ -178,6 +180,11 @@ class RopeAxesArgs(ctypes.Structure):
 class KvAppendAxesArgs(ctypes.Structure):
     """mgq_kv_append_axes_args (OP_KV_APPEND_AXES)."""
     _fields_ = [("append", KvAppendArgs), ("axes", RopeAxes)]
+
+
+class KvAttentionSinksArgs(ctypes.Structure):
+    """mgq_kv_attention_sinks_args (OP_KV_ATTENTION_SINKS)."""
+    _fields_ = [("attention", KvAttentionArgs), ("sinks", I)]
 
 
 class BlockNorm(ctypes.Structure):

@@ -144,7 +144,7 @@ bool attn_fits(const mgq_kv_cache *c, int hq, int max_new) {
 }
 
 hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq, const void *out, int64_t os, int type,
-                      int n_tokens, int max_new, float scale, float softcap, int window, const void *ws, size_t bytes) {
+                      int n_tokens, int max_new, float scale, float softcap, int window, int sinks, const void *ws, size_t bytes) {
     const hipError_t e = call_check(c, n_tokens, max_new);
     if (e != hipSuccess) return e;
     if (!attn_heads_ok(c, hq) || !attn_fits(c, hq, max_new)) return hipErrorInvalidValue;
@@ -152,7 +152,7 @@ hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq,
     const int64_t row = (int64_t)hq * c->head_dim;
     if (bad4(q) || !out || ((uintptr_t)out & (type == MGQ_OUT_F32 ? 3u : 1u)) || qs < row || os < row)
         return hipErrorInvalidValue;
-    if (!(scale >= 0.0f) || !(softcap >= 0.0f) || window < 0) return hipErrorInvalidValue;
+    if (!(scale >= 0.0f) || !(softcap >= 0.0f) || window < 0 || sinks < 0) return hipErrorInvalidValue;
     // as the kernels take them: times log2 e, or scale / softcap
     if (!std::isfinite(scale * 1.4426950408889634f) || !std::isfinite(softcap * 1.4426950408889634f) ||
         (softcap > 0.0f && !std::isfinite(scale / softcap)))
@@ -184,9 +184,15 @@ hipError_t kv_op_check(int op, const void *args) {
         return append_check(&a.cache, a.rope.table ? &a.rope : nullptr, nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
                             a.q_out, a.q_out_stride, a.n_q_heads, a.n_tokens, a.max_new);
     }
+    if (op == MGQ_OP_KV_ATTENTION_SINKS) {
+        const auto &s = *static_cast<const mgq_kv_attention_sinks_args *>(args);
+        const mgq_kv_attention_args &a = s.attention;
+        return attn_check(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens,
+                          a.max_new, a.scale, a.softcap, a.window, s.sinks, a.workspace, a.workspace_bytes);
+    }
     const auto &a = *static_cast<const mgq_kv_attention_args *>(args);
     return attn_check(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens, a.max_new,
-                      a.scale, a.softcap, a.window, a.workspace, a.workspace_bytes);
+                      a.scale, a.softcap, a.window, 0, a.workspace, a.workspace_bytes);
 }
 
 hipError_t kv_op_launch(int op, const void *args, hipStream_t stream) {
@@ -210,6 +216,13 @@ hipError_t kv_op_launch(int op, const void *args, hipStream_t stream) {
         const auto &a = *static_cast<const mgq_kv_append_args *>(args);
         return launch_kv_append_ex(&a.cache, a.rope.table ? &a.rope : nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
                                    a.q_out, a.q_out_stride, a.n_q_heads, a.n_tokens, a.max_new, stream);
+    }
+    if (op == MGQ_OP_KV_ATTENTION_SINKS) {
+        const auto &s = *static_cast<const mgq_kv_attention_sinks_args *>(args);
+        const mgq_kv_attention_args &a = s.attention;
+        return launch_kv_attention_sinks_ex(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type,
+                                            a.n_tokens, a.max_new, a.scale, a.softcap, a.window, s.sinks, a.workspace,
+                                            a.workspace_bytes, stream);
     }
     const auto &a = *static_cast<const mgq_kv_attention_args *>(args);
     return launch_kv_attention_ex(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens,
@@ -291,12 +304,12 @@ size_t mgq_kv_attention_workspace_bytes(const mgq_kv_cache *c, int n_q_heads, in
                              (int64_t)c->max_pages * c->page_tokens);
 }
 
-hipError_t launch_kv_attention_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads, void *out,
-                                  int64_t out_stride, int out_type, int n_tokens, int max_new, float scale,
-                                  float softcap, int window, void *workspace, size_t workspace_bytes,
-                                  hipStream_t stream) {
+hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads,
+                                        void *out, int64_t out_stride, int out_type, int n_tokens, int max_new,
+                                        float scale, float softcap, int window, int sinks, void *workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
     const hipError_t e = attn_check(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale,
-                                    softcap, window, workspace, workspace_bytes);
+                                    softcap, window, sinks, workspace, workspace_bytes);
     if (e != hipSuccess) return e;
     KvAttn a;
     a.q = q;
@@ -308,8 +321,17 @@ hipError_t launch_kv_attention_ex(const mgq_kv_cache *c, const float *q, int64_t
     a.scale = scale;
     a.softcap = softcap;
     a.window = window;
+    a.sinks = sinks;
     a.ws = static_cast<float *>(workspace);
     return kv_attn_launch(view(*c, n_tokens, max_new), c->head_dim, c->format, a, stream);
+}
+
+hipError_t launch_kv_attention_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads, void *out,
+                                  int64_t out_stride, int out_type, int n_tokens, int max_new, float scale,
+                                  float softcap, int window, void *workspace, size_t workspace_bytes,
+                                  hipStream_t stream) {
+    return launch_kv_attention_sinks_ex(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale,
+                                        softcap, window, 0, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

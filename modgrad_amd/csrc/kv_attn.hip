@@ -1,7 +1,7 @@
 // Attention of the new tokens' queries over the paged 8-bit cache.
 //
 //   s_j = scale * q . k_j (or softcap * tanh(s_j / softcap)),
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j), j <= pos, j > pos - window
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j), j <= pos, j > pos - window or j < sinks
 //
 // k_j = ks[page] * K8_j, v_j = vs[page] * V8_j. The 8-bit values of either
 // format are exact in f16, so both products run on the f16 matrix cores with
@@ -63,17 +63,16 @@ constexpr int kSoloTiles = 2 * NW, kPartTiles = NW, kRunTiles = 4 * NW;
 // within the sequence.
 struct AttnSeq {
     SeqInfo s;
-    int tile0, tiles, blocks;  // first tile, tiles of a row, row blocks
+    TileList list;
+    int tiles, blocks;  // tiles of a row, row blocks
 };
 __device__ __forceinline__ AttnSeq attn_seq(const KvView &c, const AttnArgs &a, int b) {
     AttnSeq r;
     r.s = kv_seq(c, b);
-    // tiles that some row sees: from the first one's window to the length
-    const int lo = a.window > 0 ? max(r.s.pos0 - a.window + 1, 0) : 0;
-    r.tile0 = lo / kTile;
+    // tiles that some row sees: the first tokens', from the first one's window to the length
+    r.list = tile_list(a, r.s.pos0);
     const int hi = min(r.s.len, max(r.s.pos0 + r.s.n, 0));
-    // at least one: a row that sees nothing has its zeros written
-    r.tiles = max((hi + kTile - 1) / kTile - r.tile0, 1);
+    r.tiles = r.list.count(hi);
     r.blocks = (r.s.n * a.group + kRows - 1) / kRows;
     return r;
 }
@@ -229,7 +228,6 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
         const int pos = live ? q.s.pos0 + tq : -1;
         // ---- loads
-        const int tile_end = q.tile0 + t1;
         const int kgrp = col >> 2;  // the 16 tokens that this lane's K rows are of
         u32x4 vreg[DB];
         u32x4 kreg[4][(KB + 15) / 16];
@@ -237,34 +235,34 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         int nv_n = 0;         // of this lane group's 16 tokens, those that exist
         int ik = -1, iv = -1;  // page ids of the next tile to load
         const int *tab = c.table + (int64_t)b * c.max_pages;
-        const auto look = [&](int tile) {
-            const int pk = tile * kTile + 16 * kgrp, pv = tile * kTile + 16 * grp;
+        const auto look = [&](int t) {
+            const int at = q.list.at(t) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
             ik = pk < q.s.len ? tab[pk >> c.page_shift] : -1;
             iv = pv < q.s.len ? tab[pv >> c.page_shift] : -1;
         };
         // a page that the table does not name, or past the length, is read as
         // page 0 and counts as no tokens; its scales may be anything
-        const auto load_k = [&](int tile) {
-            const int p = tile * kTile + 16 * kgrp, id = ik < 0 || ik >= c.n_pages ? 0 : ik;
+        const auto load_k = [&](int t) {
+            const int p = q.list.at(t) * kTile + 16 * kgrp, id = ik < 0 || ik >= c.n_pages ? 0 : ik;
             const uint8_t *kp = c.k + id * c.page_stride + ((int64_t)h * page + (p & (page - 1)) + (col & 3)) * D + grp * KB;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int b4 = 0; b4 < 4; ++b4) {
                 if constexpr (KB % 16 == 0) {
 #pragma unroll
                     for (int i = 0; i < KB / 16; ++i)
-                        kreg[t][i] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * D + 16 * i);
+                        kreg[b4][i] = *reinterpret_cast<const u32x4 *>(kp + 4 * b4 * D + 16 * i);
                 } else {  // 24 bytes at a multiple of 8
 #pragma unroll
                     for (int i = 0; i < KB / 8; ++i) {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * t * D + 8 * i);
-                        kreg[t][i / 2][2 * (i % 2)] = x[0];
-                        kreg[t][i / 2][2 * (i % 2) + 1] = x[1];
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + 4 * b4 * D + 8 * i);
+                        kreg[b4][i / 2][2 * (i % 2)] = x[0];
+                        kreg[b4][i / 2][2 * (i % 2) + 1] = x[1];
                     }
                 }
             }
         };
-        const auto load_v = [&](int tile) {
-            const int p = tile * kTile + 16 * grp;
+        const auto load_v = [&](int t) {
+            const int p = q.list.at(t) * kTile + 16 * grp;
             const bool ok = iv >= 0 && iv < c.n_pages;
             const int id = ok ? iv : 0;
             nv_n = ok ? min(q.s.len - p, 16) : 0;
@@ -274,13 +272,13 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
 #pragma unroll
             for (int d = 0; d < DB; ++d) vreg[d] = *reinterpret_cast<const u32x4 *>(vp + 16 * d * page);
         };
-        int tile = q.tile0 + t0 + wave;
+        int tile = t0 + wave;
         // loads come back in order: the page ids first, which the others wait for
         look(tile);
         __builtin_amdgcn_sched_barrier(0);
         float qv[KB];
         read_query<D>(a.q + (int64_t)(q.s.t0 + tq) * a.q_stride + (h * a.group + hd) * D + grp * KB, qv);
-        if (tile < tile_end) {
+        if (tile < t1) {
             load_k(tile);
             load_v(tile);
             look(tile + NW);
@@ -297,7 +295,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         f32x4 O[DB] = {};
         float M = -INFINITY, l = 0.0f;
         bool loud = false;
-        for (; tile < tile_end; tile += NW) {
+        for (; tile < t1; tile += NW) {
             const float ks = kscale * ks_n, vs = fmaxf(vs_n, kLeastScale);
             const int nv = nv_n;
             f32x4 S[4] = {};
@@ -322,13 +320,11 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                     }
                 }
             }
-            const bool more = tile + NW < tile_end;
+            const bool more = tile + NW < t1;
             if (more) load_k(tile + NW);
 
             const float lv = __log2f(vs);
-            const int first = tile * kTile + 16 * grp;
-            const int see = min(pos + 1 - first, nv);  // tokens of the 16 up to the row's own
-            const int skip = a.window > 0 ? pos - a.window + 1 - first : 0;
+            const uint32_t seen = seen_tokens(a, pos, q.list.at(tile) * kTile + 16 * grp, nv);
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -336,8 +332,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                 for (int i = 0; i < 4; ++i) {
                     float s = S[t][i] * ks;
                     if (a.softcap > 0.0f) s = softcap_log2(s, a.softcap);
-                    const int e = 4 * t + i;
-                    s = e < see && e >= skip ? s + lv : -INFINITY;
+                    s = seen >> (4 * t + i) & 1 ? s + lv : -INFINITY;
                     S[t][i] = s;
                     top = fmaxf(top, s);
                 }
@@ -482,10 +477,11 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
 // rows 57 and 40.
 bool kv_attn_is_wide(int dim, int64_t rows) { return rows > (dim == 256 ? 32 : 48); }
 
-// Most tiles of a row: the table's, or the window's.
-static int64_t most_tiles(int64_t cap, int max_new, int window) {
-    if (window > 0) cap = std::min<int64_t>(cap, (int64_t)window + max_new - 1 + kTile - 1);
-    return (cap + kTile - 1) / kTile;
+// Most tiles of a row: the table's, or the window's and those of the first tokens.
+static int64_t most_tiles(int64_t cap, int max_new, const AttnArgs &a) {
+    const int64_t all = (cap + kTile - 1) / kTile;
+    if (a.window == 0) return all;
+    return std::min(all, ((int64_t)a.window + max_new - 1 + kTile - 1 + kTile - 1) / kTile + (a.sinks + kTile - 1) / kTile);
 }
 
 // States: a run has two, a part one, and with the parts' least size given by
@@ -502,7 +498,7 @@ size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int6
 template <int D, int FMT>
 static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     const int max_blocks = (c.max_new * a.group + kRows - 1) / kRows;
-    const int64_t tiles = most_tiles((int64_t)c.max_pages << c.page_shift, c.max_new, a.window);
+    const int64_t tiles = most_tiles((int64_t)c.max_pages << c.page_shift, c.max_new, a);
     const int64_t rows = (int64_t)c.n_seqs * c.hkv * max_blocks;
     const bool solo = tiles <= kSoloTiles;  // no row can be longer
     const int most = D == 256 ? kAttnGroups / 2 : kAttnGroups;  // resident at once
@@ -527,6 +523,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.scale = x.softcap > 0.0f ? x.scale / x.softcap : x.scale * 1.4426950408889634f;
     a.softcap = x.softcap * 1.4426950408889634f;
     a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
+    a.sinks = a.window > 0 ? std::min(x.sinks, 1 << 30) : 0;
     a.ws = x.ws;
     if (kv_attn_is_wide(dim, c.max_new * a.group)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;

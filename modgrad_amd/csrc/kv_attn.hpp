@@ -19,9 +19,33 @@ struct AttnArgs {
     int out_f16;
     // softcap off: scale * log2 e; on: scale / softcap, and softcap * log2 e
     float scale, softcap;
-    int window;
+    int window, sinks;  // sinks: 0 without a window
     float *ws;
 };
+
+// Which tiles a run of query rows goes through, by number: those of the first tokens
+// that stay visible, then from the window of the first row on.
+struct TileList {
+    int head, gap;  // tiles of the first tokens, tiles passed over behind them
+    __device__ __forceinline__ int at(int t) const { return t + (t < head ? 0 : gap); }
+    // tiles up to position `hi`; one at least, so that a row that sees nothing has its zeros written
+    __device__ __forceinline__ int count(int hi) const { return max(max((hi + kTile - 1) / kTile - gap, head), 1); }
+};
+__device__ __forceinline__ TileList tile_list(const AttnArgs &a, int first_pos) {
+    TileList l;
+    const int first = (a.window > 0 ? max(first_pos - a.window + 1, 0) : 0) / kTile;
+    l.head = min((a.sinks + kTile - 1) / kTile, first);
+    l.gap = first - l.head;
+    return l;
+}
+// Which of 16 neighbouring tokens from position `first` on the row at `pos` sees, as
+// bits: those up to its own of the nv that exist, in its window or among the first.
+__device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), 16)) - 1u; }
+__device__ __forceinline__ uint32_t seen_tokens(const AttnArgs &a, int pos, int first, int nv) {
+    uint32_t m = low_bits(min(pos + 1 - first, nv));
+    if (a.window > 0) m &= ~low_bits(pos - a.window + 1 - first) | low_bits(a.sinks - first);
+    return m;
+}
 
 // What a running maximum is compared with and taken from: w = 2^(t - ref). Where
 // numbers as large as M lie 4 and more apart, M - kTop may be off by more than f16 has

@@ -39,7 +39,8 @@ constexpr int kWideChunk = 4;  // least tiles of a split: a work-group's start c
 struct WideBlock {
     SeqInfo s;
     int r0, rows;            // first query row, rows of the sequence
-    int tile0, tiles, chunk; // first tile, tiles, tiles of a split
+    TileList list;
+    int tiles, chunk;        // tiles, tiles of a split
 };
 __device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, int b, int rt, int splits, WideBlock &w) {
     w.s = kv_seq(c, b);
@@ -47,10 +48,9 @@ __device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, i
     w.r0 = rt * kWideRows;
     if (w.r0 >= w.rows) return false;
     const int first = w.s.pos0 + w.r0 / a.group, last = w.s.pos0 + (min(w.r0 + kWideRows, w.rows) - 1) / a.group;
-    const int lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
     const int hi = min(w.s.len, max(last + 1, 0));
-    w.tile0 = lo / kTile;
-    w.tiles = max((hi + kTile - 1) / kTile - w.tile0, 1);  // one, for the zeros of rows that see nothing
+    w.list = tile_list(a, first);
+    w.tiles = w.list.count(hi);
     w.chunk = max((w.tiles + splits - 1) / splits, splits > 1 ? kWideChunk : 1);
     return true;
 }
@@ -196,7 +196,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     // past the length
     int ik_n, iv_n;
     const auto look = [&](int t) {
-        const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
+        const int at = w.list.at(min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
         ik_n = pk < w.s.len ? tab[pk >> c.page_shift] : -1;
         iv_n = pv < w.s.len ? tab[pv >> c.page_shift] : -1;
     };
@@ -205,7 +205,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     float ks_n, vs_n;  // scales and count of the tile in the staging registers
     int nv_n;
     const auto fetch = [&](int t) {  // past the last tile, the last again
-        const int at = (w.tile0 + min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
+        const int at = w.list.at(min(t, last)) * kTile, pk = at + 16 * kgrp, pv = at + 16 * grp;
         int ik = ik_n, iv = iv_n;
         const bool okv = iv >= 0 && iv < c.n_pages;
         if (ik < 0 || ik >= c.n_pages) ik = 0;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         ks_c = ks_n;
         vs_c = vs_n;
         fetch(t + 2);
-        const int first = (w.tile0 + t) * kTile;
+        const int first = w.list.at(t) * kTile;
         if (!live || first > pos_hi) continue;  // no row of the wavefront sees it
 
         f32x4 S[SETS][4] = {};
@@ -338,8 +338,8 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
         __builtin_amdgcn_s_setprio(1);
         const float vs = fmaxf(vsv, kLeastScale), lv = __log2f(vs), rvs = __builtin_amdgcn_rcpf(vs);
         // all rows see all of the tile
-        const bool clear = first + kTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window) &&
-                           __all(nv == 16);
+        const bool clear = first + kTile - 1 <= pos_lo &&
+                           (a.window == 0 || first > pos_hi - a.window || first + kTile <= a.sinks) && __all(nv == 16);
         half8 ph[SETS][2], pl[SETS][2];
         // (an f16 result is infinite before the page that makes others vanish is that loud)
         if (LO) loud = loud || __any(vs > kLoudScale);
@@ -381,13 +381,12 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
                 sc = 1.0f;
             }
             if (exact) {
-                const int at = first + 16 * grp;
-                const int see = min(pos[s] + 1 - at, nv), skip = a.window > 0 ? pos[s] - a.window + 1 - at : 0;
+                const uint32_t seen = seen_tokens(a, pos[s], first + 16 * grp, nv);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        S[s][i][e] = 4 * i + e < see && 4 * i + e >= skip ? fmaf(S[s][i][e], sc, lv) : -INFINITY;
+                        S[s][i][e] = seen >> (4 * i + e) & 1 ? fmaf(S[s][i][e], sc, lv) : -INFINITY;
                 sc = 1.0f;
                 add = 0.0f;
             }
@@ -588,8 +587,8 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     int row_blocks, splits;
     const int64_t cap = (int64_t)c.max_pages << c.page_shift;
     wide_plan(D, a.group, c.hkv, c.n_seqs, c.max_new, cap, row_blocks, splits);
-    if (a.window > 0) {  // a row block's tokens and their windows
-        const int64_t seen = (int64_t)a.window + kWideRows / a.group + 2 * kTile;
+    if (a.window > 0) {  // a row block's tokens, their windows and the first tokens
+        const int64_t seen = (int64_t)a.window + kWideRows / a.group + 2 * kTile + (a.sinks > 0 ? a.sinks + kTile : 0);
         splits = (int)std::min<int64_t>(splits, (seen / kTile + kWideChunk - 1) / kWideChunk);
     }
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);

@@ -41,7 +41,7 @@ struct KvAttn {
     int64_t q_stride, out_stride;
     int hq, out_f16;
     float scale, softcap;
-    int window;
+    int window, sinks;
     float *ws;
 };
 // Whether this many query rows of a kv head take kv_attn_wide.hip.

@@ -419,6 +419,7 @@ static hipError_t op_check(const mgq_op_desc &o) {
     case MGQ_OP_KV_ATTENTION:
     case MGQ_OP_ROPE_AXES:
     case MGQ_OP_KV_APPEND_AXES:
+    case MGQ_OP_KV_ATTENTION_SINKS:
         return mgq::kv_op_check(o.op, o.w);
     case MGQ_OP_BLOCK_NORM: {
         const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);
@@ -463,6 +464,7 @@ static hipError_t op_launch(const mgq_op_desc &o, hipStream_t s) {
     case MGQ_OP_KV_ATTENTION:
     case MGQ_OP_ROPE_AXES:
     case MGQ_OP_KV_APPEND_AXES:
+    case MGQ_OP_KV_ATTENTION_SINKS:
         return mgq::kv_op_launch(o.op, o.w, s);
     case MGQ_OP_BLOCK_NORM: {
         const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);

@@ -432,8 +432,9 @@ class KvCache:
 
     def attend(self, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int,
                n_tokens: int, max_new: int, scale: float | None = None, softcap: float = 0.0,
-               window: int = 0, out_f16: bool = False, workspace=None, stream=None) -> None:
-        """out = attention of q's rows over the cache (scale: head_dim^-0.5).
+               window: int = 0, out_f16: bool = False, workspace=None, stream=None, sinks: int = 0) -> None:
+        """out = attention of q's rows over the cache (scale: head_dim^-0.5); with a
+        window the first `sinks` positions of a sequence stay visible behind it.
         Without a workspace, a fresh one comes from torch's caching allocator,
         of the launch stream."""
         if self._look:
@@ -443,10 +444,14 @@ class KvCache:
                 workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
         else:
             _workspace(workspace, self.device)
-        kern.kv_attention(self._ref, q, q_stride, n_q_heads, out, out_stride,
-                          _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens, max_new,
-                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap, window,
-                          workspace.data_ptr(), workspace.nbytes, stream)
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
+        kind = _lib.OUT_F16 if out_f16 else _lib.OUT_F32
+        if sinks:
+            kern.kv_attention_sinks(self._ref, q, q_stride, n_q_heads, out, out_stride, kind, n_tokens, max_new, scale,
+                                    softcap, window, sinks, workspace.data_ptr(), workspace.nbytes, stream)
+            return
+        kern.kv_attention(self._ref, q, q_stride, n_q_heads, out, out_stride, kind, n_tokens, max_new, scale, softcap,
+                          window, workspace.data_ptr(), workspace.nbytes, stream)
 
     def dequant(self, pages: int, n: int, k_out: int, v_out: int, stream=None) -> None:
         """n pages (device int32 ids) as f32 [n][kv head][token][dim]."""
@@ -472,10 +477,13 @@ class KvCache:
 
     def op_attend(self, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int,
                   n_tokens: int, max_new: int, workspace, scale: float | None = None,
-                  softcap: float = 0.0, window: int = 0, out_f16: bool = False) -> "_lib.OpDesc":
+                  softcap: float = 0.0, window: int = 0, out_f16: bool = False, sinks: int = 0) -> "_lib.OpDesc":
         """The workspace has to outlive the chain."""
         _workspace(workspace, self.device)
-        return _op(_lib.OP_KV_ATTENTION, _lib.KvAttentionArgs(
+        args = _lib.KvAttentionArgs(
             self.desc, q, out, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             q_stride, out_stride, n_q_heads, _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens,
-            max_new, window, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap))
+            max_new, window, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap)
+        if sinks:
+            return _op(_lib.OP_KV_ATTENTION_SINKS, _lib.KvAttentionSinksArgs(args, sinks))
+        return _op(_lib.OP_KV_ATTENTION, args)

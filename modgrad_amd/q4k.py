@@ -428,6 +428,15 @@ class kern:
             max_new, scale, softcap, window, workspace, workspace_bytes, _stream_ptr(stream)),
             "kv_attention")
 
+    @staticmethod
+    def kv_attention_sinks(cache, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int, out_type: int,
+                           n_tokens: int, max_new: int, scale: float, softcap: float, window: int, sinks: int,
+                           workspace: int, workspace_bytes: int, stream=None) -> None:
+        """kv_attention whose first `sinks` positions stay visible behind the window."""
+        _chk(_lib.load().launch_kv_attention_sinks_ex(
+            cache, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap, window, sinks,
+            workspace, workspace_bytes, _stream_ptr(stream)), "kv_attention_sinks")
+
 
 class ops:
     """ops.rs façade for the Q4_K op."""

@@ -516,6 +516,24 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *
                                         int sinks, void *workspace, size_t workspace_bytes,
                                         hipStream_t stream);
 
+/* launch_kv_attention_ex, without a window, for sequences that begin with the same
+ * pages: the first shared_tokens positions of every sequence with rows in the call lie
+ * in the same pages, in the same order. Their whole tiles of 64 tokens are read once
+ * for all rows, the rest sequence by sequence, and the two joined in f32 as the parts
+ * of a long sequence are. A row sees only its own and earlier positions also where
+ * shared_tokens reaches past them; of a prefix that is not as described, what one of the
+ * sequences' pages holds is used for others. shared_tokens is not negative; past
+ * max_pages*page_tokens it counts as that. The workspace is of
+ * mgq_kv_attention_shared_workspace_bytes (0: arguments that the call refuses). */
+size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads,
+                                               int n_tokens, int max_new, int shared_tokens);
+hipError_t launch_kv_attention_shared_ex(const mgq_kv_cache *cache, const float *q,
+                                         int64_t q_stride, int n_q_heads, void *out,
+                                         int64_t out_stride, int out_type, int n_tokens,
+                                         int max_new, float scale, float softcap,
+                                         int shared_tokens, void *workspace,
+                                         size_t workspace_bytes, hipStream_t stream);
+
 /* One matvec of a decode-step chain. */
 typedef struct mgq_gemv_desc {
     const unsigned char *w_q4; /* row-aligned Q4_K bytes */
@@ -607,6 +625,8 @@ hipError_t mgq_chain_destroy(void *chain);
  *   MGQ_OP_KV_ATTENTION  launch_kv_attention_ex of an mgq_kv_attention_args.
  *   MGQ_OP_KV_ATTENTION_SINKS  launch_kv_attention_sinks_ex of an
  *                        mgq_kv_attention_sinks_args.
+ *   MGQ_OP_KV_ATTENTION_SHARED  launch_kv_attention_shared_ex of an
+ *                        mgq_kv_attention_shared_args (window 0).
  *   MGQ_OP_ROPE_AXES     launch_rope_axes_ex of an mgq_rope_axes_args.
  *   MGQ_OP_KV_APPEND_AXES  launch_kv_append_axes_ex of an mgq_kv_append_axes_args.
  *   MGQ_OP_BLOCK_NORM    launch_block_norm_ex of an mgq_block_norm_args.
@@ -628,6 +648,7 @@ hipError_t mgq_chain_destroy(void *chain);
 #define MGQ_OP_ROPE_AXES 13
 #define MGQ_OP_KV_APPEND_AXES 14
 #define MGQ_OP_KV_ATTENTION_SINKS 15
+#define MGQ_OP_KV_ATTENTION_SHARED 16
 /* Those from MGQ_OP_ROPE on take their arguments from here: mgq_op_desc.w points to one
  * in host memory. */
 typedef struct mgq_rope_args {
@@ -659,6 +680,10 @@ typedef struct mgq_kv_attention_sinks_args {
     mgq_kv_attention_args attention;
     int sinks;
 } mgq_kv_attention_sinks_args;
+typedef struct mgq_kv_attention_shared_args {
+    mgq_kv_attention_args attention;
+    int shared_tokens;
+} mgq_kv_attention_shared_args;
 typedef struct mgq_rope_axes_args {
     const float *x;
     float *y;

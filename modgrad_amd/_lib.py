@@ -66,6 +66,8 @@ SIGNATURES = {
     "launch_kv_dequant_ex": (I, [P, P, I, P, P, P]),
     "mgq_kv_attention_workspace_bytes": (S, [P, I, I]),
     "launch_kv_attention_sinks_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, I, P, S, P]),
+    "mgq_kv_attention_shared_workspace_bytes": (S, [P, I, I, I, I]),
+    "launch_kv_attention_shared_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, P, S, P]),
     "launch_kv_attention_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, P, S, P]),
     "mgq_chain_create": (I, [P, I, P]),
     "mgq_chain_create_ex": (I, [P, I, I, P]),
@@ -101,6 +103,7 @@ OP_BLOCK_NORM = 12
 OP_ROPE_AXES = 13
 OP_KV_APPEND_AXES = 14
 OP_KV_ATTENTION_SINKS = 15
+OP_KV_ATTENTION_SHARED = 16
 AXES_BLOCKS = 0
 AXES_TURNS = 1
 ROPE_INTERLEAVED = 0
@@ -185,6 +188,11 @@ class KvAppendAxesArgs(ctypes.Structure):
 class KvAttentionSinksArgs(ctypes.Structure):
     """mgq_kv_attention_sinks_args (OP_KV_ATTENTION_SINKS)."""
     _fields_ = [("attention", KvAttentionArgs), ("sinks", I)]
+
+
+class KvAttentionSharedArgs(ctypes.Structure):
+    """mgq_kv_attention_shared_args (OP_KV_ATTENTION_SHARED)."""
+    _fields_ = [("attention", KvAttentionArgs), ("shared_tokens", I)]
 
 
 class BlockNorm(ctypes.Structure):

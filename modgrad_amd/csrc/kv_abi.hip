@@ -144,7 +144,7 @@ bool attn_fits(const mgq_kv_cache *c, int hq, int max_new) {
 }
 
 hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq, const void *out, int64_t os, int type,
-                      int n_tokens, int max_new, float scale, float softcap, int window, int sinks, const void *ws, size_t bytes) {
+                      int n_tokens, int max_new, float scale, float softcap, int window, int sinks, int shared, const void *ws, size_t bytes) {
     const hipError_t e = call_check(c, n_tokens, max_new);
     if (e != hipSuccess) return e;
     if (!attn_heads_ok(c, hq) || !attn_fits(c, hq, max_new)) return hipErrorInvalidValue;
@@ -152,12 +152,14 @@ hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq,
     const int64_t row = (int64_t)hq * c->head_dim;
     if (bad4(q) || !out || ((uintptr_t)out & (type == MGQ_OUT_F32 ? 3u : 1u)) || qs < row || os < row)
         return hipErrorInvalidValue;
-    if (!(scale >= 0.0f) || !(softcap >= 0.0f) || window < 0 || sinks < 0) return hipErrorInvalidValue;
+    if (!(scale >= 0.0f) || !(softcap >= 0.0f) || window < 0 || sinks < 0 || shared < 0) return hipErrorInvalidValue;
     // as the kernels take them: times log2 e, or scale / softcap
     if (!std::isfinite(scale * 1.4426950408889634f) || !std::isfinite(softcap * 1.4426950408889634f) ||
         (softcap > 0.0f && !std::isfinite(scale / softcap)))
         return hipErrorInvalidValue;
-    if (bad16(ws) || bytes < mgq_kv_attention_workspace_bytes(c, hq, max_new)) return hipErrorInvalidValue;
+    const size_t need = shared > 0 ? mgq_kv_attention_shared_workspace_bytes(c, hq, n_tokens, max_new, shared)
+                                   : mgq_kv_attention_workspace_bytes(c, hq, max_new);
+    if (need == 0 || bad16(ws) || bytes < need) return hipErrorInvalidValue;
     return hipSuccess;
 }
 
@@ -184,15 +186,22 @@ hipError_t kv_op_check(int op, const void *args) {
         return append_check(&a.cache, a.rope.table ? &a.rope : nullptr, nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
                             a.q_out, a.q_out_stride, a.n_q_heads, a.n_tokens, a.max_new);
     }
+    if (op == MGQ_OP_KV_ATTENTION_SHARED) {
+        const auto &s = *static_cast<const mgq_kv_attention_shared_args *>(args);
+        const mgq_kv_attention_args &a = s.attention;
+        if (a.window != 0) return hipErrorInvalidValue;
+        return attn_check(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens,
+                          a.max_new, a.scale, a.softcap, 0, 0, s.shared_tokens, a.workspace, a.workspace_bytes);
+    }
     if (op == MGQ_OP_KV_ATTENTION_SINKS) {
         const auto &s = *static_cast<const mgq_kv_attention_sinks_args *>(args);
         const mgq_kv_attention_args &a = s.attention;
         return attn_check(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens,
-                          a.max_new, a.scale, a.softcap, a.window, s.sinks, a.workspace, a.workspace_bytes);
+                          a.max_new, a.scale, a.softcap, a.window, s.sinks, 0, a.workspace, a.workspace_bytes);
     }
     const auto &a = *static_cast<const mgq_kv_attention_args *>(args);
     return attn_check(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type, a.n_tokens, a.max_new,
-                      a.scale, a.softcap, a.window, 0, a.workspace, a.workspace_bytes);
+                      a.scale, a.softcap, a.window, 0, 0, a.workspace, a.workspace_bytes);
 }
 
 hipError_t kv_op_launch(int op, const void *args, hipStream_t stream) {
@@ -216,6 +225,13 @@ hipError_t kv_op_launch(int op, const void *args, hipStream_t stream) {
         const auto &a = *static_cast<const mgq_kv_append_args *>(args);
         return launch_kv_append_ex(&a.cache, a.rope.table ? &a.rope : nullptr, a.k, a.v, a.kv_stride, a.q, a.q_stride,
                                    a.q_out, a.q_out_stride, a.n_q_heads, a.n_tokens, a.max_new, stream);
+    }
+    if (op == MGQ_OP_KV_ATTENTION_SHARED) {
+        const auto &s = *static_cast<const mgq_kv_attention_shared_args *>(args);
+        const mgq_kv_attention_args &a = s.attention;
+        return launch_kv_attention_shared_ex(&a.cache, a.q, a.q_stride, a.n_q_heads, a.out, a.out_stride, a.out_type,
+                                             a.n_tokens, a.max_new, a.scale, a.softcap, s.shared_tokens, a.workspace,
+                                             a.workspace_bytes, stream);
     }
     if (op == MGQ_OP_KV_ATTENTION_SINKS) {
         const auto &s = *static_cast<const mgq_kv_attention_sinks_args *>(args);
@@ -304,12 +320,12 @@ size_t mgq_kv_attention_workspace_bytes(const mgq_kv_cache *c, int n_q_heads, in
                              (int64_t)c->max_pages * c->page_tokens);
 }
 
-hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads,
-                                        void *out, int64_t out_stride, int out_type, int n_tokens, int max_new,
-                                        float scale, float softcap, int window, int sinks, void *workspace,
-                                        size_t workspace_bytes, hipStream_t stream) {
+static hipError_t attention_run(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads, void *out,
+                                int64_t out_stride, int out_type, int n_tokens, int max_new, float scale,
+                                float softcap, int window, int sinks, int shared_tokens, void *workspace,
+                                size_t workspace_bytes, hipStream_t stream) {
     const hipError_t e = attn_check(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale,
-                                    softcap, window, sinks, workspace, workspace_bytes);
+                                    softcap, window, sinks, shared_tokens, workspace, workspace_bytes);
     if (e != hipSuccess) return e;
     KvAttn a;
     a.q = q;
@@ -323,6 +339,7 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *c, const float *q, i
     a.window = window;
     a.sinks = sinks;
     a.ws = static_cast<float *>(workspace);
+    a.shared_tokens = shared_tokens;
     return kv_attn_launch(view(*c, n_tokens, max_new), c->head_dim, c->format, a, stream);
 }
 
@@ -330,8 +347,34 @@ hipError_t launch_kv_attention_ex(const mgq_kv_cache *c, const float *q, int64_t
                                   int64_t out_stride, int out_type, int n_tokens, int max_new, float scale,
                                   float softcap, int window, void *workspace, size_t workspace_bytes,
                                   hipStream_t stream) {
-    return launch_kv_attention_sinks_ex(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale,
-                                        softcap, window, 0, workspace, workspace_bytes, stream);
+    return attention_run(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap,
+                         window, 0, 0, workspace, workspace_bytes, stream);
+}
+
+hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads,
+                                        void *out, int64_t out_stride, int out_type, int n_tokens, int max_new,
+                                        float scale, float softcap, int window, int sinks, void *workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+    return attention_run(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap,
+                         window, sinks, 0, workspace, workspace_bytes, stream);
+}
+
+size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *c, int n_q_heads, int n_tokens, int max_new,
+                                               int shared_tokens) {
+    if (mgq_kv_attention_workspace_bytes(c, n_q_heads, max_new) == 0 || n_tokens <= 0 || shared_tokens < 0) return 0;
+    // query rows of a kv head, and their blocks and heads, in 32 bits
+    const int64_t rows = (int64_t)n_tokens * (n_q_heads / c->n_kv_heads);
+    if (rows >= (1 << 28) || (rows / 128 + 1) * c->n_kv_heads > kMaxGrid / 512) return 0;
+    return kv_attn_shared_workspace(c->head_dim, n_q_heads, c->n_kv_heads, c->n_seqs, n_tokens, max_new,
+                                    (int64_t)c->max_pages * c->page_tokens, shared_tokens);
+}
+
+hipError_t launch_kv_attention_shared_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads,
+                                         void *out, int64_t out_stride, int out_type, int n_tokens, int max_new,
+                                         float scale, float softcap, int shared_tokens, void *workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+    return attention_run(c, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap, 0, 0,
+                         shared_tokens, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

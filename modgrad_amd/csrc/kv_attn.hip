@@ -70,7 +70,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const KvView &c, const AttnArgs &a, 
     AttnSeq r;
     r.s = kv_seq(c, b);
     // tiles that some row sees: the first tokens', from the first one's window to the length
-    r.list = tile_list(a, r.s.pos0);
+    r.list = tile_list(a, r.s, r.s.pos0);
     const int hi = min(r.s.len, max(r.s.pos0 + r.s.n, 0));
     r.tiles = r.list.count(hi);
     r.blocks = (r.s.n * a.group + kRows - 1) / kRows;
@@ -99,7 +99,8 @@ __device__ __forceinline__ int group_scan(int v, int *part, int &total) {
 
 // The cut. Runs: a unit is a tile, `run` of them a work-group's. Parts: a unit is
 // a part of at most `part` tiles. Where no row can have more than kSoloTiles
-// tiles (`most` 0) every row is one part, however many there are: no join follows.
+// tiles (`most` 0) every row is one part, however many there are: no join follows. Behind a shared
+// prefix there are always parts, so that each state has its own place: all are joined.
 struct AttnPlace {
     int total, run, part;  // part 0: runs
     int at, b, base;       // first unit, its sequence, that one's first unit
@@ -111,9 +112,9 @@ struct AttnPlace {
     __device__ __forceinline__ int units(const AttnSeq &s, int hkv) const {
         return s.blocks * hkv * (part ? parts(s) : s.tiles);
     }
-    __device__ __forceinline__ void cut(int tiles, int most) {
+    __device__ __forceinline__ void cut(int tiles, int most, bool shared) {
         if (most == 0) part = kSoloTiles;
-        else part = tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
+        else part = shared || tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
     }
     __device__ __forceinline__ void deal(int units, int most) {
         const int groups = part ? (int)gridDim.x : min(most, (int)gridDim.x);
@@ -127,7 +128,7 @@ __device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs 
     AttnPlace p = {};
     if (c.n_seqs == 1) {
         p.q = attn_seq(c, a, 0);
-        p.cut(p.q.blocks * c.hkv * p.q.tiles, most);
+        p.cut(p.q.blocks * c.hkv * p.q.tiles, most, a.shared > 0);
         p.deal(p.units(p.q, c.hkv), most);
         return p;
     }
@@ -141,7 +142,7 @@ __device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs 
         tiles += q.blocks * c.hkv * q.tiles;
     }
     group_scan(tiles, part, t);
-    p.cut(t, most);
+    p.cut(t, most, a.shared > 0);
     int start;
     if (c.n_seqs <= NT) {
         units = p.units(q, c.hkv);
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
             for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * kRows + col) * OP + 16 * d + 4 * grp]) = O[d] * fac;
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == q.tiles;
+        const bool whole = t0 == 0 && t1 == q.tiles && a.shared == 0;
         float *slot = a.ws + (int64_t)(place.part ? first_unit : 2 * (int)blockIdx.x + (t0 == 0)) * state_floats<D>(kRows);
         const int mine = min(kRows, rows - r0);
         for (int i = tid; i < mine * (D / 4); i += NT) {
@@ -461,14 +462,22 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
     const SeqInfo s = kv_seq(c, b);
     const int r = blk * kRows + rr;
     if (r >= s.n * a.group) return;  // no such row, and nobody has written its states' numbers
-    if (st.y == 1) return;  // the whole row was one work-group's, which has written it
+    if (st.y == 1 && a.shared == 0) return;  // the whole row was one work-group's, which has written it
+    const int ahead = prefix_parts(a, s);
     const auto slot = [&](int i) {
-        return a.ws + (int64_t)(st.y > 0 ? st.x + i : 2 * (st.x + i) + (i == 0)) * state_floats<D>(kRows);
+        if (i < ahead) return prefix_state<D>(c, a, h, (int64_t)s.t0 * a.group + r, i);
+        i -= ahead;
+        return row_state<D>(a.ws + (int64_t)(st.y > 0 ? st.x + i : 2 * (st.x + i) + (i == 0)) * state_floats<D>(kRows),
+                            kRows, rr);
     };
-    const f32x4 o = join_row<D>(abs(st.y), kRows, rr, slot);
+    const f32x4 o = join_row<D>(ahead + abs(st.y), slot);
     if ((int)threadIdx.x < D / 4)
         put_out4(a, s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
+
+// Work-groups that a prefix's parts are made for, and the least tiles of one.
+static int prefix_slots(int dim) { return dim == 256 ? 256 : 512; }
+constexpr int kPrefixChunk = 4;
 
 // Query rows of a kv head up to which this kernel takes the call, in blocks of
 // 16 that each read the cache, and above which kv_attn_wide.hip does. Measured
@@ -488,11 +497,42 @@ static int64_t most_tiles(int64_t cap, int max_new, const AttnArgs &a) {
 // `most` there are no more parts than `most` and one for every row.
 static int64_t most_states(int64_t rows) { return kAttnGroups + std::max<int64_t>(rows, kAttnGroups); }
 
-size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
+static size_t suffix_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity, bool shared) {
     const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
-    if (kv_attn_is_wide(dim, rows)) return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
+    if (kv_attn_is_wide(dim, rows))
+        return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity, shared));
     const int64_t all = (int64_t)n_seqs * blocks * hkv;
     return (size_t)most_states(all) * kRows * (dim + 2) * sizeof(float) + (size_t)all * sizeof(int2);
+}
+
+size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
+    return suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, false);
+}
+
+// The prefix's part of a call: its tiles, how many a state is over, the states' places.
+// As many parts as fill the chip with blocks of query rows.
+struct PrefixPlan {
+    int tiles, blocks, chunk, parts;
+};
+static PrefixPlan prefix_plan(int dim, int hq, int hkv, int n_tokens, int64_t capacity, int shared_tokens) {
+    PrefixPlan p;
+    p.tiles = (int)(std::min<int64_t>(capacity, shared_tokens) / kTile);
+    p.blocks = (int)(((int64_t)n_tokens * (hq / hkv) + kWideRows - 1) / kWideRows);
+    const int64_t items = (int64_t)p.blocks * hkv;
+    const int most = (p.tiles + kPrefixChunk - 1) / kPrefixChunk;
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(prefix_slots(dim) / items, most));
+    p.chunk = std::max(1, (p.tiles + p.parts - 1) / p.parts);
+    p.parts = (p.tiles + p.chunk - 1) / p.chunk;
+    return p;
+}
+static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t kv_attn_shared_workspace(int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
+                                int shared_tokens) {
+    const PrefixPlan p = prefix_plan(dim, hq, hkv, n_tokens, capacity, shared_tokens);
+    if (p.tiles == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
+    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) +
+           (size_t)p.parts * p.blocks * hkv * kWideRows * (dim + 2) * sizeof(float);
 }
 
 template <int D, int FMT>
@@ -506,7 +546,7 @@ static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t s
     const int states = (int)most_states(rows);
     kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || solo) return e;
+    if (e != hipSuccess || (solo && a.shared == 0)) return e;
     const int block_rows = std::min(kRows, c.max_new * a.group);
     kv_attn_join_kernel<D><<<(unsigned)(rows * block_rows), 256, 0, stream>>>(c, a, max_blocks, block_rows, states);
     return hipGetLastError();
@@ -525,6 +565,19 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
     a.sinks = a.window > 0 ? std::min(x.sinks, 1 << 30) : 0;
     a.ws = x.ws;
+    a.shared = 0;
+    if (x.shared_tokens > 0) {
+        const int64_t cap = (int64_t)c.max_pages << c.page_shift;
+        const PrefixPlan p = prefix_plan(dim, x.hq, c.hkv, c.n_tokens, cap, x.shared_tokens);
+        if (p.tiles > 0) {
+            a.shared = p.tiles;
+            a.prefix_blocks = p.blocks;
+            a.prefix_chunk = p.chunk;
+            a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
+            const hipError_t e = kv_attn_prefix_launch(c, dim, fmt, a, stream);
+            if (e != hipSuccess) return e;
+        }
+    }
     if (kv_attn_is_wide(dim, c.max_new * a.group)) return kv_attn_wide_launch(c, dim, fmt, a, stream);
     const bool i8 = fmt == MGQ_KV_I8;
     switch (dim) {

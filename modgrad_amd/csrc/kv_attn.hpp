@@ -21,7 +21,12 @@ struct AttnArgs {
     float scale, softcap;
     int window, sinks;  // sinks: 0 without a window
     float *ws;
+    // a prefix that the sequences share: its tiles (0: none), and its states: those of
+    // `prefix_blocks` blocks of kWideRows query rows, each over `prefix_chunk` tiles
+    int shared, prefix_blocks, prefix_chunk;
+    float *prefix;
 };
+constexpr int kWideRows = 128;  // query rows that share a tile through LDS
 
 // Which tiles a run of query rows goes through, by number: those of the first tokens
 // that stay visible, then from the window of the first row on.
@@ -31,8 +36,17 @@ struct TileList {
     // tiles up to position `hi`; one at least, so that a row that sees nothing has its zeros written
     __device__ __forceinline__ int count(int hi) const { return max(max((hi + kTile - 1) / kTile - gap, head), 1); }
 };
-__device__ __forceinline__ TileList tile_list(const AttnArgs &a, int first_pos) {
+// Tiles of the prefix that all rows of a sequence see.
+__device__ __forceinline__ int shared_tiles(const AttnArgs &a, const SeqInfo &s) {
+    return min(a.shared, max(s.pos0 + 1, 0) / kTile);
+}
+__device__ __forceinline__ TileList tile_list(const AttnArgs &a, const SeqInfo &s, int first_pos) {
     TileList l;
+    if (a.shared > 0) {
+        l.head = 0;
+        l.gap = shared_tiles(a, s);
+        return l;
+    }
     const int first = (a.window > 0 ? max(first_pos - a.window + 1, 0) : 0) / kTile;
     l.head = min((a.sinks + kTile - 1) / kTile, first);
     l.gap = first - l.head;
@@ -75,7 +89,9 @@ __device__ __forceinline__ bool vanishing(float top, float ref) { return top < r
 
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
-size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap);
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, bool shared);
+// All query rows over the tiles of a prefix that they share.
+hipError_t kv_attn_prefix_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 
 template <int FMT>
 __device__ __forceinline__ half8 kv_half8(uint32_t lo, uint32_t hi) {
@@ -235,13 +251,32 @@ constexpr int state_floats(int rows) {
     return rows * (D + 2);
 }
 
-// The states of one query row, in `n` slots (slot(i) -> its first float), joined
-// by a work-group of 256 threads: D/4 threads a state, so that (M, l) and O of
+// Where a query row's partial state lies.
+struct RowState {
+    const float *o, *ml;
+};
+template <int D>
+__device__ __forceinline__ RowState row_state(const float *state, int rows, int row) {
+    return {state + row * D, state + rows * D + 2 * row};
+}
+// Row `row` of all the call's query rows of a kv head: the state of its i-th part of
+// the prefix.
+template <int D>
+__device__ __forceinline__ RowState prefix_state(const KvView &c, const AttnArgs &a, int h, int64_t row, int i) {
+    const int64_t at = (i * (int64_t)a.prefix_blocks + row / kWideRows) * c.hkv + h;
+    return row_state<D>(a.prefix + at * state_floats<D>(kWideRows), kWideRows, row % kWideRows);
+}
+__device__ __forceinline__ int prefix_parts(const AttnArgs &a, const SeqInfo &s) {
+    return a.shared > 0 ? (shared_tiles(a, s) + a.prefix_chunk - 1) / a.prefix_chunk : 0;
+}
+
+// The states of one query row, `n` of them (slot(i) -> the i-th), joined by a
+// work-group of 256 threads: D/4 threads a state, so that (M, l) and O of
 // 1024/D states load at once; each such group of threads joins every 1024/D-th
 // state as it comes, then the groups join through LDS. The row's dims 4d .. on
 // thread d < D/4.
 template <int D, class Slot>
-__device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
+__device__ __forceinline__ f32x4 join_row(int n, Slot slot) {
     constexpr int L = D / 4, W = 256 / L, U = 4;  // threads of a state, states at once, loads ahead
     __shared__ f32x4 sO[W * L];
     __shared__ float2 sML[W];
@@ -253,9 +288,9 @@ __device__ __forceinline__ f32x4 join_row(int n, int rows, int row, Slot slot) {
         f32x4 x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float *s = slot(min(i0 + u * W, n - 1));
-            ml[u] = *reinterpret_cast<const float2 *>(s + rows * D + 2 * row);
-            x[u] = *reinterpret_cast<const f32x4 *>(s + row * D + 4 * d);
+            const RowState s = slot(min(i0 + u * W, n - 1));
+            ml[u] = *reinterpret_cast<const float2 *>(s.ml);
+            x[u] = *reinterpret_cast<const f32x4 *>(s.o + 4 * d);
             if (i0 + u * W >= n) ml[u] = make_float2(-INFINITY, 0.0f);
         }
 #pragma unroll

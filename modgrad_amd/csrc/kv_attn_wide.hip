@@ -29,7 +29,6 @@
 
 namespace mgq {
 
-constexpr int kWideRows = 128;
 // Work-groups that a call's splits are made for: those resident at once, of 4 wavefronts
 // two a CU and of 8 one. By the head alone: heads of 128 with one set of rows (int8,
 // f32 results) have 8 wavefronts too and so twice as many splits as fit at once.
@@ -49,7 +48,7 @@ __device__ __forceinline__ bool wide_block(const KvView &c, const AttnArgs &a, i
     if (w.r0 >= w.rows) return false;
     const int first = w.s.pos0 + w.r0 / a.group, last = w.s.pos0 + (min(w.r0 + kWideRows, w.rows) - 1) / a.group;
     const int hi = min(w.s.len, max(last + 1, 0));
-    w.list = tile_list(a, first);
+    w.list = tile_list(a, w.s, first);
     w.tiles = w.list.count(hi);
     w.chunk = max((w.tiles + splits - 1) / splits, splits > 1 ? kWideChunk : 1);
     return true;
@@ -117,6 +116,41 @@ __device__ __forceinline__ WidePlace wide_place(const KvView &c, const AttnArgs 
     return p;
 }
 
+// A shared prefix: block rt of all the call's query rows, whichever sequence's they
+// are. A token's rows see as many of its tiles as its sequence does; lim gets them for
+// the block's tokens (0: a row of no sequence). The pages are those of the sequence that
+// sees most (the first such), which the others' lists begin with.
+struct PrefixRows {
+    int lim[kWideRows];
+    unsigned long long best;
+};
+__device__ __forceinline__ void prefix_block(const KvView &c, const AttnArgs &a, int rt, PrefixRows &p, int &b, WideBlock &w) {
+    int *lim = p.lim;
+    unsigned long long &best = p.best;
+    const int threads = blockDim.x;
+    w.rows = c.n_tokens * a.group;
+    w.r0 = rt * kWideRows;
+    const int t0 = w.r0 / a.group, t1 = (min(w.r0 + kWideRows, w.rows) - 1) / a.group + 1;
+    if (threadIdx.x == 0) best = 0;
+    for (int i = threadIdx.x; i < kWideRows; i += threads) lim[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < c.n_seqs; i += threads) {
+        const SeqInfo s = kv_seq(c, i);
+        const int lo = max(s.t0, t0), hi = min(s.t0 + s.n, t1), n = shared_tiles(a, s);
+        for (int t = lo; t < hi; ++t) atomicMax(&lim[t - t0], n);
+        if (lo < hi) atomicMax(&best, (unsigned long long)n << 32 | (0xFFFFFFFFu - (unsigned)i));
+    }
+    __syncthreads();
+    w.tiles = (int)(best >> 32);
+    b = w.tiles > 0 ? (int)(0xFFFFFFFFu - (unsigned)best) : 0;
+    w.s.t0 = 0;
+    w.s.n = c.n_tokens;
+    w.s.pos0 = 0;
+    w.s.len = w.tiles * kTile;
+    w.list = {0, 0};
+    w.chunk = a.prefix_chunk;
+}
+
 __device__ __forceinline__ void wide_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -140,12 +174,17 @@ struct WideShape {
     static constexpr int DB = D / 16;                       // blocks of 16 dims of O
     static constexpr int NK = 4 * KS / NW;                  // pieces of K a wavefront stages: 64 lanes x 16 bytes of LDS
     static constexpr int NV = 2 * DB / NW;                  // pieces of V
+    // of a prefix's kernel, its rows' limits behind the buffers
+    template <bool PREFIX>
+    static constexpr size_t lds_bytes() {
+        return 2 * kBuf * sizeof(half8) + (PREFIX ? sizeof(PrefixRows) : 0);
+    }
     static_assert(4 * KS % NW == 0 && 2 * DB % NW == 0, "each wavefront stages as many pieces");
     static constexpr int kOfV = 4 * KS * 64, kBuf = kOfV + 2 * DB * 64;  // 16-byte units of a buffer: K, then V
 };
 
-// LO: the probabilities as hi + lo pairs.
-template <int D, int FMT, bool LO>
+// LO: the probabilities as hi + lo pairs. PREFIX: over the tiles of a shared prefix.
+template <int D, int FMT, bool LO, bool PREFIX>
 __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int most_splits, int turn) {
     typedef WideShape<D, FMT, LO> W;
     constexpr bool I8 = W::I8;
@@ -161,12 +200,21 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     // longest ones (where a CU has one at a time they only come in another order)
     const int h = blockIdx.x % c.hkv;
     int id = blockIdx.x / c.hkv;
-    if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
-    const WidePlace place = wide_place<D>(c, a, id, most_splits);
-    if (place.rt < 0) return;
-    const int b = place.b, sp = place.split;
+    PrefixRows &rows = *reinterpret_cast<PrefixRows *>(lds + 2 * W::kBuf);  // PREFIX only
+    WidePlace place = {};
+    int b, sp;
     WideBlock w;
-    if (!wide_block(c, a, b, place.rt, place.splits, w)) return;
+    if constexpr (PREFIX) {
+        sp = id / a.prefix_blocks;
+        prefix_block(c, a, id % a.prefix_blocks, rows, b, w);
+    } else {
+        if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
+        place = wide_place<D>(c, a, id, most_splits);
+        if (place.rt < 0) return;
+        b = place.b;
+        sp = place.split;
+        if (!wide_block(c, a, b, place.rt, place.splits, w)) return;
+    }
     const int t0 = sp * w.chunk, t1 = min(w.tiles, t0 + w.chunk);
     if (t0 >= t1) return;
 
@@ -180,13 +228,29 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     for (int s = 0; s < SETS; ++s) {
         const int r = min(wr0 + 16 * s + col, w.rows - 1);
         const int tq = r / a.group;
-        pos[s] = w.s.pos0 + tq;
+        pos[s] = PREFIX ? rows.lim[tq - w.r0 / a.group] * kTile - 1 : w.s.pos0 + tq;
         read_query<D>(a.q + (int64_t)(w.s.t0 + tq) * a.q_stride + (h * a.group + r % a.group) * D + grp * KB, qv[s]);
     }
     const bool live = wr0 < w.rows;
     // positions of the wavefront's first and last row
-    const int pos_lo = w.s.pos0 + min(wr0, w.rows - 1) / a.group;
-    const int pos_hi = w.s.pos0 + min(wr0 + 16 * SETS - 1, w.rows - 1) / a.group;
+    int pos_lo = w.s.pos0 + min(wr0, w.rows - 1) / a.group;
+    int pos_hi = w.s.pos0 + min(wr0 + 16 * SETS - 1, w.rows - 1) / a.group;
+    if constexpr (PREFIX) {  // the least and the most of its rows
+        pos_lo = pos[0];
+        pos_hi = pos[0];
+#pragma unroll
+        for (int s = 1; s < SETS; ++s) {
+            pos_lo = min(pos_lo, pos[s]);
+            pos_hi = max(pos_hi, pos[s]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            pos_lo = min(pos_lo, __shfl_xor(pos_lo, o, 64));
+            pos_hi = max(pos_hi, __shfl_xor(pos_hi, o, 64));
+        }
+        pos_lo = __builtin_amdgcn_readfirstlane(pos_lo);
+        pos_hi = __builtin_amdgcn_readfirstlane(pos_hi);
+    }
 
     // ---- staging
     const int kgrp = col >> 2;
@@ -466,8 +530,9 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     }
     if (!live) return;
 
-    const bool whole = w.chunk >= w.tiles;
-    float *st = a.ws + ((place.split * (int64_t)place.total + place.state) * c.hkv + h) * state_floats<D>(kWideRows);
+    const bool whole = !PREFIX && w.chunk >= w.tiles && a.shared == 0;
+    float *st = PREFIX ? a.prefix + (int64_t)blockIdx.x * state_floats<D>(kWideRows)
+                       : a.ws + ((place.split * (int64_t)place.total + place.state) * c.hkv + h) * state_floats<D>(kWideRows);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         float sum = l[s];
@@ -502,12 +567,14 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnAr
     WideBlock w;
     if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
     const int r = w.r0 + rr;
-    if (r >= w.rows || w.chunk >= w.tiles) return;
-    const int n = (w.tiles + w.chunk - 1) / w.chunk;
+    if (r >= w.rows || (w.chunk >= w.tiles && a.shared == 0)) return;
+    const int n = (w.tiles + w.chunk - 1) / w.chunk, ahead = prefix_parts(a, w.s);
     const auto slot = [&](int i) {
-        return a.ws + ((i * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows);
+        if (i < ahead) return prefix_state<D>(c, a, h, (int64_t)w.s.t0 * a.group + r, i);
+        return row_state<D>(a.ws + (((i - ahead) * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows),
+                            kWideRows, rr);
     };
-    const f32x4 o = join_row<D>(n, kWideRows, rr, slot);
+    const f32x4 o = join_row<D>(ahead + n, slot);
     if ((int)threadIdx.x < D / 4)
         put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
@@ -526,23 +593,28 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
     if (place.rt < 0 || place.split > 0) return;
     WideBlock w;
     if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
-    if (w.chunk >= w.tiles) return;
-    const int n = (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
+    if (w.chunk >= w.tiles && a.shared == 0) return;
+    const int ahead = prefix_parts(a, w.s), n = ahead + (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
     if ((int)threadIdx.x >= PER * L) return;
     const float *base = a.ws + ((int64_t)id * c.hkv + h) * state_floats<D>(kWideRows);
     const int64_t step = (int64_t)place.total * c.hkv * state_floats<D>(kWideRows);
     for (int rr = R * part + threadIdx.x / L; rr < R * part + R; rr += PER) {
         const int r = w.r0 + rr;
         if (r >= w.rows) break;
+        const auto slot = [&](int i) {
+            return i < ahead ? prefix_state<D>(c, a, h, (int64_t)w.s.t0 * a.group + r, i)
+                             : row_state<D>(base + (i - ahead) * step, kWideRows, rr);
+        };
         float M = -INFINITY, l = 0.0f;
-        for (int i = 0; i < n; ++i) M = fmaxf(M, base[i * step + kWideRows * D + 2 * rr]);
+        for (int i = 0; i < n; ++i) M = fmaxf(M, slot(i).ml[0]);
         f32x4 o = {};
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            const float2 ml = *reinterpret_cast<const float2 *>(base + i * step + kWideRows * D + 2 * rr);
+            const RowState s = slot(i);
+            const float2 ml = *reinterpret_cast<const float2 *>(s.ml);
             const Exp2 f(ml.x == -INFINITY ? -INFINITY : ml.x - M);
             l += f.times(ml.y);
-            o += f.f * *reinterpret_cast<const f32x4 *>(base + i * step + rr * D + d);
+            o += f.f * *reinterpret_cast<const f32x4 *>(s.o + d);
         }
         put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
     }
@@ -557,20 +629,20 @@ static void wide_plan(int dim, int group, int hkv, int n_seqs, int max_new, int6
     splits = std::min(splits, std::max(1, wide_slots(dim) / (row_blocks * hkv)));  // one sequence has all its blocks
 }
 
-size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap) {
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, bool shared) {
     int row_blocks, splits;
     wide_plan(dim, group, hkv, n_seqs, max_new, cap, row_blocks, splits);
-    if (splits == 1) return 0;
+    if (splits == 1 && !shared) return 0;
     return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
 }
 
 // LDS past 64 KiB has to be allowed, per device.
-template <int D, int FMT, bool LO>
+template <int D, int FMT, bool LO, bool PREFIX = false>
 static hipError_t wide_allow() {
     typedef WideShape<D, FMT, LO> W;
     static std::atomic<int> state[64];
-    if (2 * W::kBuf * sizeof(half8) <= 64 * 1024) return hipSuccess;
-    return allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
+    if (W::template lds_bytes<PREFIX>() <= 64 * 1024) return hipSuccess;
+    return allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO, PREFIX>), state);
 }
 
 hipError_t kv_attn_prepare() {
@@ -579,6 +651,9 @@ hipError_t kv_attn_prepare() {
     all(wide_allow<128, kFmtI8, false>, wide_allow<128, kFmtI8, true>, wide_allow<128, kFmtE4M3, false>,
         wide_allow<128, kFmtE4M3, true>, wide_allow<256, kFmtI8, false>, wide_allow<256, kFmtI8, true>,
         wide_allow<256, kFmtE4M3, false>, wide_allow<256, kFmtE4M3, true>);
+    all(wide_allow<128, kFmtI8, false, true>, wide_allow<128, kFmtI8, true, true>, wide_allow<128, kFmtE4M3, false, true>,
+        wide_allow<128, kFmtE4M3, true, true>, wide_allow<256, kFmtI8, false, true>, wide_allow<256, kFmtI8, true, true>,
+        wide_allow<256, kFmtE4M3, false, true>, wide_allow<256, kFmtE4M3, true, true>);
     return e;
 }
 
@@ -593,15 +668,16 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     }
     const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
     typedef WideShape<D, FMT, LO> W;
-    constexpr size_t kLds = 2 * W::kBuf * sizeof(half8);
+    constexpr size_t kLds = W::template lds_bytes<false>();
     const hipError_t allowed = wide_allow<D, FMT, LO>();
     if (allowed != hipSuccess) return allowed;
     const int cus = device_cus();
     const int turn = c.n_seqs == 1 && splits == 1 && cus % c.hkv == 0 && (int)items >= 2 * cus ? cus / c.hkv : 1 << 29;
-    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
+    kv_attn_wide_kernel<D, FMT, LO, false><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || splits == 1) return e;
-    if (splits <= kJoinFew)
+    if (e != hipSuccess || (splits == 1 && a.shared == 0)) return e;
+    const int parts = splits + (a.shared > 0 ? (a.shared + a.prefix_chunk - 1) / a.prefix_chunk : 0);
+    if (parts <= kJoinFew)
         kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
     else
         kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, splits);
@@ -621,6 +697,33 @@ hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs
     case 96: return wide_dim<96>(c, fmt, a, stream);
     case 128: return wide_dim<128>(c, fmt, a, stream);
     default: return wide_dim<256>(c, fmt, a, stream);
+    }
+}
+
+template <int D, int FMT, bool LO>
+static hipError_t prefix_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
+    typedef WideShape<D, FMT, LO> W;
+    const hipError_t allowed = wide_allow<D, FMT, LO, true>();
+    if (allowed != hipSuccess) return allowed;
+    const int64_t parts = (a.shared + a.prefix_chunk - 1) / a.prefix_chunk;
+    kv_attn_wide_kernel<D, FMT, LO, true><<<(unsigned)(parts * a.prefix_blocks * c.hkv), W::kThreads,
+                                            W::template lds_bytes<true>(), stream>>>(c, a, 0, 0);
+    return hipGetLastError();
+}
+
+template <int D>
+static hipError_t prefix_dim(const KvView &c, int fmt, const AttnArgs &a, hipStream_t stream) {
+    if (fmt == MGQ_KV_I8)
+        return a.out_f16 ? prefix_run<D, kFmtI8, false>(c, a, stream) : prefix_run<D, kFmtI8, true>(c, a, stream);
+    return a.out_f16 ? prefix_run<D, kFmtE4M3, false>(c, a, stream) : prefix_run<D, kFmtE4M3, true>(c, a, stream);
+}
+
+hipError_t kv_attn_prefix_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream) {
+    switch (dim) {
+    case 64: return prefix_dim<64>(c, fmt, a, stream);
+    case 96: return prefix_dim<96>(c, fmt, a, stream);
+    case 128: return prefix_dim<128>(c, fmt, a, stream);
+    default: return prefix_dim<256>(c, fmt, a, stream);
     }
 }
 

@@ -420,6 +420,7 @@ static hipError_t op_check(const mgq_op_desc &o) {
     case MGQ_OP_ROPE_AXES:
     case MGQ_OP_KV_APPEND_AXES:
     case MGQ_OP_KV_ATTENTION_SINKS:
+    case MGQ_OP_KV_ATTENTION_SHARED:
         return mgq::kv_op_check(o.op, o.w);
     case MGQ_OP_BLOCK_NORM: {
         const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);
@@ -465,6 +466,7 @@ static hipError_t op_launch(const mgq_op_desc &o, hipStream_t s) {
     case MGQ_OP_ROPE_AXES:
     case MGQ_OP_KV_APPEND_AXES:
     case MGQ_OP_KV_ATTENTION_SINKS:
+    case MGQ_OP_KV_ATTENTION_SHARED:
         return mgq::kv_op_launch(o.op, o.w, s);
     case MGQ_OP_BLOCK_NORM: {
         const auto *a = reinterpret_cast<const mgq_block_norm_args *>(o.w);

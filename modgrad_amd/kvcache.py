@@ -253,6 +253,11 @@ def _workspace(workspace, device) -> None:
         raise BackendError("Runtime", f"workspace: contiguous memory on {device} expected")
 
 
+def _without_window(window: int, sinks: int) -> None:
+    if window or sinks:
+        raise BackendError("Unsupported", "attention over a shared prefix with a window")
+
+
 class KvCache:
     """One layer's paged 8-bit cache and the page tables of n_seqs slots
     (mgq_kv_cache)."""
@@ -423,29 +428,40 @@ class KvCache:
                        q if q_out is None else q_out, q_stride if q_out_stride is None else q_out_stride,
                        n_q_heads, n_tokens, max_new, stream)
 
-    def attention_workspace(self, n_q_heads: int, n_tokens: int, max_new: int):
+    def attention_workspace(self, n_q_heads: int, n_tokens: int, max_new: int, shared: int = 0):
         """A device tensor for attend's workspace (any call with these sizes)."""
-        n = kern.kv_attention_workspace_bytes(self._ref, n_q_heads, max_new)
+        if shared:
+            n = kern.kv_attention_shared_workspace_bytes(self._ref, n_q_heads, n_tokens, max_new, shared)
+        else:
+            n = kern.kv_attention_workspace_bytes(self._ref, n_q_heads, max_new)
         if n == 0 or n_tokens <= 0:
             raise BackendError("Runtime", f"attention of {n_q_heads} heads, {max_new} new tokens")
         return _torch().empty(n, dtype=_torch().uint8, device=self.device)
 
     def attend(self, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int,
                n_tokens: int, max_new: int, scale: float | None = None, softcap: float = 0.0,
-               window: int = 0, out_f16: bool = False, workspace=None, stream=None, sinks: int = 0) -> None:
+               window: int = 0, out_f16: bool = False, workspace=None, stream=None, sinks: int = 0,
+               shared: int = 0) -> None:
         """out = attention of q's rows over the cache (scale: head_dim^-0.5); with a
         window the first `sinks` positions of a sequence stay visible behind it.
+        shared: so many first positions of all sequences lie in the same pages, which are
+        read once for all (without a window; the workspace is one for `shared`).
         Without a workspace, a fresh one comes from torch's caching allocator,
         of the launch stream."""
         if self._look:
             _on_device(self.device)
         if workspace is None:
             with _stream(stream):
-                workspace = self.attention_workspace(n_q_heads, n_tokens, max_new)
+                workspace = self.attention_workspace(n_q_heads, n_tokens, max_new, shared)
         else:
             _workspace(workspace, self.device)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
         kind = _lib.OUT_F16 if out_f16 else _lib.OUT_F32
+        if shared:
+            _without_window(window, sinks)
+            kern.kv_attention_shared(self._ref, q, q_stride, n_q_heads, out, out_stride, kind, n_tokens, max_new, scale,
+                                     softcap, shared, workspace.data_ptr(), workspace.nbytes, stream)
+            return
         if sinks:
             kern.kv_attention_sinks(self._ref, q, q_stride, n_q_heads, out, out_stride, kind, n_tokens, max_new, scale,
                                     softcap, window, sinks, workspace.data_ptr(), workspace.nbytes, stream)
@@ -477,13 +493,17 @@ class KvCache:
 
     def op_attend(self, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int,
                   n_tokens: int, max_new: int, workspace, scale: float | None = None,
-                  softcap: float = 0.0, window: int = 0, out_f16: bool = False, sinks: int = 0) -> "_lib.OpDesc":
+                  softcap: float = 0.0, window: int = 0, out_f16: bool = False, sinks: int = 0,
+                  shared: int = 0) -> "_lib.OpDesc":
         """The workspace has to outlive the chain."""
         _workspace(workspace, self.device)
         args = _lib.KvAttentionArgs(
             self.desc, q, out, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             q_stride, out_stride, n_q_heads, _lib.OUT_F16 if out_f16 else _lib.OUT_F32, n_tokens,
             max_new, window, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, softcap)
+        if shared:
+            _without_window(window, sinks)
+            return _op(_lib.OP_KV_ATTENTION_SHARED, _lib.KvAttentionSharedArgs(args, shared))
         if sinks:
             return _op(_lib.OP_KV_ATTENTION_SINKS, _lib.KvAttentionSinksArgs(args, sinks))
         return _op(_lib.OP_KV_ATTENTION, args)

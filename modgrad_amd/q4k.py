@@ -437,6 +437,22 @@ class kern:
             cache, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap, window, sinks,
             workspace, workspace_bytes, _stream_ptr(stream)), "kv_attention_sinks")
 
+    @staticmethod
+    def kv_attention_shared_workspace_bytes(cache, n_q_heads: int, n_tokens: int, max_new: int,
+                                            shared_tokens: int) -> int:
+        return int(_lib.load().mgq_kv_attention_shared_workspace_bytes(cache, n_q_heads, n_tokens, max_new,
+                                                                       shared_tokens))
+
+    @staticmethod
+    def kv_attention_shared(cache, q: int, q_stride: int, n_q_heads: int, out: int, out_stride: int, out_type: int,
+                            n_tokens: int, max_new: int, scale: float, softcap: float, shared_tokens: int,
+                            workspace: int, workspace_bytes: int, stream=None) -> None:
+        """kv_attention of sequences whose first shared_tokens positions lie in the
+        same pages."""
+        _chk(_lib.load().launch_kv_attention_shared_ex(
+            cache, q, q_stride, n_q_heads, out, out_stride, out_type, n_tokens, max_new, scale, softcap, shared_tokens,
+            workspace, workspace_bytes, _stream_ptr(stream)), "kv_attention_shared")
+
 
 class ops:
     """ops.rs façade for the Q4_K op."""

@@ -365,7 +365,7 @@ size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *c, int n_q_he
     // query rows of a kv head, and their blocks and heads, in 32 bits
     const int64_t rows = (int64_t)n_tokens * (n_q_heads / c->n_kv_heads);
     if (rows >= (1 << 28) || (rows / 128 + 1) * c->n_kv_heads > kMaxGrid / 512) return 0;
-    return kv_attn_shared_workspace(c->head_dim, n_q_heads, c->n_kv_heads, c->n_seqs, n_tokens, max_new,
+    return kv_attn_shared_workspace(c->head_dim, c->format, n_q_heads, c->n_kv_heads, c->n_seqs, n_tokens, max_new,
                                     (int64_t)c->max_pages * c->page_tokens, shared_tokens);
 }
 

@@ -463,21 +463,17 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
     const int r = blk * kRows + rr;
     if (r >= s.n * a.group) return;  // no such row, and nobody has written its states' numbers
     if (st.y == 1 && a.shared == 0) return;  // the whole row was one work-group's, which has written it
-    const int ahead = prefix_parts(a, s);
+    const PrefixParts ahead = prefix_parts(a, s, (int64_t)s.t0 * a.group + r);
     const auto slot = [&](int i) {
-        if (i < ahead) return prefix_state<D>(c, a, h, (int64_t)s.t0 * a.group + r, i);
-        i -= ahead;
+        if (i < ahead.n) return ahead.state<D>(c, a, h, i);
+        i -= ahead.n;
         return row_state<D>(a.ws + (int64_t)(st.y > 0 ? st.x + i : 2 * (st.x + i) + (i == 0)) * state_floats<D>(kRows),
                             kRows, rr);
     };
-    const f32x4 o = join_row<D>(ahead + abs(st.y), slot);
+    const f32x4 o = join_row<D>(ahead.n + abs(st.y), slot);
     if ((int)threadIdx.x < D / 4)
         put_out4(a, s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
-
-// Work-groups that a prefix's parts are made for, and the least tiles of one.
-static int prefix_slots(int dim) { return dim == 256 ? 256 : 512; }
-constexpr int kPrefixChunk = 4;
 
 // Query rows of a kv head up to which this kernel takes the call, in blocks of
 // 16 that each read the cache, and above which kv_attn_wide.hip does. Measured
@@ -509,30 +505,43 @@ size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int6
     return suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, false);
 }
 
-// The prefix's part of a call: its tiles, how many a state is over, the states' places.
-// As many parts as fill the chip with blocks of query rows.
+// The prefix's part of a call.
 struct PrefixPlan {
-    int tiles, blocks, chunk, parts;
+    int tiles, blocks, span, run;
+    int64_t runs;  // of a kv head
 };
-static PrefixPlan prefix_plan(int dim, int hq, int hkv, int n_tokens, int64_t capacity, int shared_tokens) {
-    PrefixPlan p;
+static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_tokens, int64_t capacity,
+                              int shared_tokens) {
+    PrefixPlan p = {};
     p.tiles = (int)(std::min<int64_t>(capacity, shared_tokens) / kTile);
     p.blocks = (int)(((int64_t)n_tokens * (hq / hkv) + kWideRows - 1) / kWideRows);
-    const int64_t items = (int64_t)p.blocks * hkv;
-    const int most = (p.tiles + kPrefixChunk - 1) / kPrefixChunk;
-    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(prefix_slots(dim) / items, most));
-    p.chunk = std::max(1, (p.tiles + p.parts - 1) / p.parts);
-    p.parts = (p.tiles + p.chunk - 1) / p.chunk;
+    if (p.tiles == 0) return p;
+    // Runs of equal length over all blocks fill the chip best, but a run with tiles of two
+    // blocks begins twice (rows, page ids, first loads: some 6 us, as long as kTwice
+    // tiles); equal parts of each block are longer where the work-groups are no multiple
+    // of the blocks. 4 blocks of 187 tiles on 63 groups: runs 45 us, parts 37; 33 blocks of
+    // 156 on 128: parts 147, runs 137.
+    constexpr int kTwice = 3;
+    const int64_t groups = std::max(1, kv_attn_prefix_slots(dim, fmt, out_f16) / hkv);
+    const int64_t run = std::min<int64_t>(p.tiles, ((int64_t)p.blocks * p.tiles + groups - 1) / groups);
+    const int64_t parts = std::min<int64_t>(p.tiles, std::max<int64_t>(1, groups / p.blocks));
+    const int64_t part = (p.tiles + parts - 1) / parts;
+    const bool whole = part <= run + kTwice;
+    p.run = (int)(whole ? part : run);
+    p.span = whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
+    p.runs = ((int64_t)p.blocks * p.span + p.run - 1) / p.run;
     return p;
 }
 static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
 
-size_t kv_attn_shared_workspace(int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
+size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
                                 int shared_tokens) {
-    const PrefixPlan p = prefix_plan(dim, hq, hkv, n_tokens, capacity, shared_tokens);
-    if (p.tiles == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
+    int64_t runs = 0;  // for either type of result
+    for (int f16 = 0; f16 < 2; ++f16)
+        runs = std::max(runs, prefix_plan(dim, fmt, f16, hq, hkv, n_tokens, capacity, shared_tokens).runs);
+    if (runs == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
     return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) +
-           (size_t)p.parts * p.blocks * hkv * kWideRows * (dim + 2) * sizeof(float);
+           (size_t)(2 * runs * hkv) * kWideRows * (dim + 2) * sizeof(float);
 }
 
 template <int D, int FMT>
@@ -568,11 +577,12 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.shared = 0;
     if (x.shared_tokens > 0) {
         const int64_t cap = (int64_t)c.max_pages << c.page_shift;
-        const PrefixPlan p = prefix_plan(dim, x.hq, c.hkv, c.n_tokens, cap, x.shared_tokens);
+        const PrefixPlan p = prefix_plan(dim, fmt, x.out_f16, x.hq, c.hkv, c.n_tokens, cap, x.shared_tokens);
         if (p.tiles > 0) {
             a.shared = p.tiles;
             a.prefix_blocks = p.blocks;
-            a.prefix_chunk = p.chunk;
+            a.prefix_span = p.span;
+            a.prefix_run = p.run;
             a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
             const hipError_t e = kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;

@@ -21,9 +21,10 @@ struct AttnArgs {
     float scale, softcap;
     int window, sinks;  // sinks: 0 without a window
     float *ws;
-    // a prefix that the sequences share: its tiles (0: none), and its states: those of
-    // `prefix_blocks` blocks of kWideRows query rows, each over `prefix_chunk` tiles
-    int shared, prefix_blocks, prefix_chunk;
+    // a prefix that the sequences share: its tiles (0: none), the blocks of kWideRows
+    // query rows that go through them, the places that a block has in the row of all
+    // tiles (some at its end may be empty), the tiles of a work-group, and its states
+    int shared, prefix_blocks, prefix_span, prefix_run;
     float *prefix;
 };
 constexpr int kWideRows = 128;  // query rows that share a tile through LDS
@@ -90,7 +91,9 @@ __device__ __forceinline__ bool vanishing(float top, float ref) { return top < r
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, bool shared);
-// All query rows over the tiles of a prefix that they share.
+// All query rows over the tiles of a prefix that they share, and how many of its
+// work-groups are resident at once.
+int kv_attn_prefix_slots(int dim, int fmt, bool out_f16);
 hipError_t kv_attn_prefix_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 
 template <int FMT>
@@ -214,21 +217,24 @@ __device__ __forceinline__ float split_query(float scale, const float (&v)[D / 4
         mant = __builtin_amdgcn_frexp_mantf(top);
     }
     const float f = kMost / mant;
+    // q + 0x80 in every digit's place has the digits, each plus 128, as its bytes: they
+    // are brought together by bytes and lose the 128 by their sign bit
+    constexpr int kBias = N == 2 ? 0x8080 : 0x808080;
 #pragma unroll
     for (int i = 0; i < KB; i += 4) {
-        uint32_t w[N] = {};
+        uint32_t q[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            int q = (int)rintf(fminf(fmaxf(ldexp2(v[i + e], -ex) * f, -kMost), kMost));
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int d = n + 1 < N ? (int)(int8_t)q : q;
-                w[n] |= (uint32_t)(d & 0xFF) << (8 * e);
-                q = (q - d) >> 8;
-            }
+        for (int e = 0; e < 4; ++e)
+            q[e] = (uint32_t)((int)rintf(fminf(fmaxf(ldexp2(v[i + e], -ex) * f, -kMost), kMost)) + kBias);
+        // bytes 0 and 1 of two values each, then of four; perm's bytes 0 to 3 are of its
+        // second operand, 4 to 7 of the first
+        const uint32_t a = __builtin_amdgcn_perm(q[1], q[0], 0x05010400u), b = __builtin_amdgcn_perm(q[3], q[2], 0x05010400u);
+        qd[0][i / 16][i / 4 % 4] = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+        qd[1][i / 16][i / 4 % 4] = (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
+        if constexpr (N == 3) {
+            const uint32_t x = __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0602u), y = __builtin_amdgcn_perm(q[3], q[2], 0x0C0C0602u);
+            qd[2][i / 16][i / 4 % 4] = (int)(__builtin_amdgcn_perm(y, x, 0x05040100u) ^ 0x80808080u);
         }
-#pragma unroll
-        for (int n = 0; n < N; ++n) qd[n][i / 16][i / 4 % 4] = (int)w[n];
     }
     constexpr int kBits = 8 * N - 1;  // kMost is just below 2^kBits
     return ldexp2(scale, ex - kBits) * (mant * ((float)(1 << kBits) / kMost)) + bad;
@@ -259,15 +265,33 @@ template <int D>
 __device__ __forceinline__ RowState row_state(const float *state, int rows, int row) {
     return {state + row * D, state + rows * D + 2 * row};
 }
-// Row `row` of all the call's query rows of a kv head: the state of its i-th part of
-// the prefix.
-template <int D>
-__device__ __forceinline__ RowState prefix_state(const KvView &c, const AttnArgs &a, int h, int64_t row, int i) {
-    const int64_t at = (i * (int64_t)a.prefix_blocks + row / kWideRows) * c.hkv + h;
-    return row_state<D>(a.prefix + at * state_floats<D>(kWideRows), kWideRows, row % kWideRows);
+// A shared prefix's states. Run r of a kv head has state 2r for a row block that an
+// earlier run begins, 2r + 1 for one that it begins.
+inline int64_t prefix_runs(const AttnArgs &a) {
+    return ((int64_t)a.prefix_blocks * a.prefix_span + a.prefix_run - 1) / a.prefix_run;
 }
-__device__ __forceinline__ int prefix_parts(const AttnArgs &a, const SeqInfo &s) {
-    return a.shared > 0 ? (shared_tiles(a, s) + a.prefix_chunk - 1) / a.prefix_chunk : 0;
+template <int D>
+__device__ __forceinline__ float *prefix_slot(const KvView &c, const AttnArgs &a, int h, int run, bool begins) {
+    return a.prefix + ((2 * (int64_t)run + begins) * c.hkv + h) * state_floats<D>(kWideRows);
+}
+// Row `row` of all the call's query rows of a kv head: the runs that its sequence's share
+// of the prefix is over.
+struct PrefixParts {
+    int first, n, row;
+    template <int D>
+    __device__ __forceinline__ RowState state(const KvView &c, const AttnArgs &a, int h, int i) const {
+        return row_state<D>(prefix_slot<D>(c, a, h, first + i, i == 0), kWideRows, row);
+    }
+};
+__device__ __forceinline__ PrefixParts prefix_parts(const AttnArgs &a, const SeqInfo &s, int64_t row) {
+    PrefixParts p = {0, 0, (int)(row % kWideRows)};
+    const int tiles = a.shared > 0 ? shared_tiles(a, s) : 0;
+    if (tiles > 0) {
+        const int64_t at = row / kWideRows * a.prefix_span;
+        p.first = (int)(at / a.prefix_run);
+        p.n = (int)((at + tiles - 1) / a.prefix_run) - p.first + 1;
+    }
+    return p;
 }
 
 // The states of one query row, `n` of them (slot(i) -> the i-th), joined by a

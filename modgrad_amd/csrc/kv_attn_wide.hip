@@ -148,7 +148,7 @@ __device__ __forceinline__ void prefix_block(const KvView &c, const AttnArgs &a,
     w.s.pos0 = 0;
     w.s.len = w.tiles * kTile;
     w.list = {0, 0};
-    w.chunk = a.prefix_chunk;
+    w.chunk = 0;
 }
 
 __device__ __forceinline__ void wide_barrier() {
@@ -183,40 +183,20 @@ struct WideShape {
     static constexpr int kOfV = 4 * KS * 64, kBuf = kOfV + 2 * DB * 64;  // 16-byte units of a buffer: K, then V
 };
 
-// LO: the probabilities as hi + lo pairs. PREFIX: over the tiles of a shared prefix.
+// Tiles t0 .. t1-1 of the rows of one (row block, kv head). LO: the probabilities as hi +
+// lo pairs. PREFIX: over the tiles of a shared prefix, to a state always.
 template <int D, int FMT, bool LO, bool PREFIX>
-__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int most_splits, int turn) {
+__device__ __forceinline__ void wide_rows(const KvView &c, const AttnArgs &a, half8 *lds, const WideBlock &w, int h, int b,
+                                          int t0, int t1, float *st, bool whole) {
     typedef WideShape<D, FMT, LO> W;
     constexpr bool I8 = W::I8;
     constexpr int SETS = W::SETS, KS = W::KS, DB = W::DB, NK = W::NK, NV = W::NV;
     constexpr int ND = LO ? 3 : 2;  // digits of q
     constexpr int KB = D / 4;
-    extern __shared__ half8 lds[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15,
               grp = lane >> 4;
     const int page = 1 << c.page_shift;
-
-    // the second work-groups of the CUs are dealt from the shorter end, beside the
-    // longest ones (where a CU has one at a time they only come in another order)
-    const int h = blockIdx.x % c.hkv;
-    int id = blockIdx.x / c.hkv;
-    PrefixRows &rows = *reinterpret_cast<PrefixRows *>(lds + 2 * W::kBuf);  // PREFIX only
-    WidePlace place = {};
-    int b, sp;
-    WideBlock w;
-    if constexpr (PREFIX) {
-        sp = id / a.prefix_blocks;
-        prefix_block(c, a, id % a.prefix_blocks, rows, b, w);
-    } else {
-        if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
-        place = wide_place<D>(c, a, id, most_splits);
-        if (place.rt < 0) return;
-        b = place.b;
-        sp = place.split;
-        if (!wide_block(c, a, b, place.rt, place.splits, w)) return;
-    }
-    const int t0 = sp * w.chunk, t1 = min(w.tiles, t0 + w.chunk);
-    if (t0 >= t1) return;
+    const PrefixRows &rows = *reinterpret_cast<const PrefixRows *>(lds + 2 * W::kBuf);  // PREFIX only
 
     // ---- query rows; those past the last repeat it and are not written
     half8 qh[SETS][I8 ? 1 : KS], ql[SETS][I8 ? 1 : KS];
@@ -530,9 +510,6 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     }
     if (!live) return;
 
-    const bool whole = !PREFIX && w.chunk >= w.tiles && a.shared == 0;
-    float *st = PREFIX ? a.prefix + (int64_t)blockIdx.x * state_floats<D>(kWideRows)
-                       : a.ws + ((place.split * (int64_t)place.total + place.state) * c.hkv + h) * state_floats<D>(kWideRows);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         float sum = l[s];
@@ -554,6 +531,50 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
     }
 }
 
+template <int D, int FMT, bool LO>
+__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_wide_kernel(KvView c, AttnArgs a, int most_splits, int turn) {
+    extern __shared__ half8 lds[];
+    // the second work-groups of the CUs are dealt from the shorter end, beside the
+    // longest ones (where a CU has one at a time they only come in another order)
+    const int h = blockIdx.x % c.hkv;
+    int id = blockIdx.x / c.hkv;
+    if (id >= turn && id < 2 * turn) id = 3 * turn - 1 - id;
+    const WidePlace place = wide_place<D>(c, a, id, most_splits);
+    if (place.rt < 0) return;
+    WideBlock w;
+    if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
+    const int t0 = place.split * w.chunk, t1 = min(w.tiles, t0 + w.chunk);
+    if (t0 >= t1) return;
+    float *st = a.ws + ((place.split * (int64_t)place.total + place.state) * c.hkv + h) * state_floats<D>(kWideRows);
+    wide_rows<D, FMT, LO, false>(c, a, lds, w, h, place.b, t0, t1, st, w.chunk >= w.tiles && a.shared == 0);
+}
+
+// A shared prefix: the tiles of a kv head's row blocks, laid end to end, are cut into
+// equal runs, a work-group each, whatever the number of blocks. A run is no longer than
+// a block's tiles, so it has the end of one block's and the beginning of the next one's
+// at most, with a state for each.
+template <int D, int FMT, bool LO>
+__global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_prefix_kernel(KvView c, AttnArgs a) {
+    typedef WideShape<D, FMT, LO> W;
+    extern __shared__ half8 lds[];
+    PrefixRows &rows = *reinterpret_cast<PrefixRows *>(lds + 2 * W::kBuf);
+    const int h = blockIdx.x % c.hkv, run = blockIdx.x / c.hkv;
+    const int64_t stop = min((int64_t)(run + 1) * a.prefix_run, (int64_t)a.prefix_blocks * a.prefix_span);
+    for (int64_t at = (int64_t)run * a.prefix_run; at < stop;) {
+        const int rt = (int)(at / a.prefix_span), t0 = (int)(at - (int64_t)rt * a.prefix_span);
+        const int t1 = (int)min((int64_t)a.prefix_span, t0 + stop - at);
+        at += t1 - t0;
+        __syncthreads();  // the run's other block has been read
+        int b;
+        WideBlock w;
+        prefix_block(c, a, rt, rows, b, w);
+        // tiles that no row of the block sees are left out; a state is of those that some does
+        if (t0 < w.tiles)
+            wide_rows<D, FMT, LO, true>(c, a, lds, w, h, b, t0, min(t1, w.tiles),
+                                        prefix_slot<D>(c, a, h, run, t0 == 0), false);
+    }
+}
+
 // Joins a split row block: one work-group per (row block, sequence, kv head, row).
 template <int D>
 __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnArgs a, int most_splits) {
@@ -568,13 +589,14 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnAr
     if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
     const int r = w.r0 + rr;
     if (r >= w.rows || (w.chunk >= w.tiles && a.shared == 0)) return;
-    const int n = (w.tiles + w.chunk - 1) / w.chunk, ahead = prefix_parts(a, w.s);
+    const int n = (w.tiles + w.chunk - 1) / w.chunk;
+    const PrefixParts ahead = prefix_parts(a, w.s, (int64_t)w.s.t0 * a.group + r);
     const auto slot = [&](int i) {
-        if (i < ahead) return prefix_state<D>(c, a, h, (int64_t)w.s.t0 * a.group + r, i);
-        return row_state<D>(a.ws + (((i - ahead) * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows),
+        if (i < ahead.n) return ahead.state<D>(c, a, h, i);
+        return row_state<D>(a.ws + (((i - ahead.n) * (int64_t)place.total + id) * c.hkv + h) * state_floats<D>(kWideRows),
                             kWideRows, rr);
     };
-    const f32x4 o = join_row<D>(ahead + n, slot);
+    const f32x4 o = join_row<D>(ahead.n + n, slot);
     if ((int)threadIdx.x < D / 4)
         put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
@@ -594,16 +616,17 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
     WideBlock w;
     if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
     if (w.chunk >= w.tiles && a.shared == 0) return;
-    const int ahead = prefix_parts(a, w.s), n = ahead + (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
+    const int own = (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
     if ((int)threadIdx.x >= PER * L) return;
     const float *base = a.ws + ((int64_t)id * c.hkv + h) * state_floats<D>(kWideRows);
     const int64_t step = (int64_t)place.total * c.hkv * state_floats<D>(kWideRows);
     for (int rr = R * part + threadIdx.x / L; rr < R * part + R; rr += PER) {
         const int r = w.r0 + rr;
         if (r >= w.rows) break;
+        const PrefixParts ahead = prefix_parts(a, w.s, (int64_t)w.s.t0 * a.group + r);
+        const int n = ahead.n + own;
         const auto slot = [&](int i) {
-            return i < ahead ? prefix_state<D>(c, a, h, (int64_t)w.s.t0 * a.group + r, i)
-                             : row_state<D>(base + (i - ahead) * step, kWideRows, rr);
+            return i < ahead.n ? ahead.state<D>(c, a, h, i) : row_state<D>(base + (i - ahead.n) * step, kWideRows, rr);
         };
         float M = -INFINITY, l = 0.0f;
         for (int i = 0; i < n; ++i) M = fmaxf(M, slot(i).ml[0]);
@@ -639,10 +662,10 @@ size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_n
 // LDS past 64 KiB has to be allowed, per device.
 template <int D, int FMT, bool LO, bool PREFIX = false>
 static hipError_t wide_allow() {
-    typedef WideShape<D, FMT, LO> W;
     static std::atomic<int> state[64];
-    if (W::template lds_bytes<PREFIX>() <= 64 * 1024) return hipSuccess;
-    return allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO, PREFIX>), state);
+    if (WideShape<D, FMT, LO>::template lds_bytes<PREFIX>() <= 64 * 1024) return hipSuccess;
+    if constexpr (PREFIX) return allow_full_lds(reinterpret_cast<const void *>(kv_attn_prefix_kernel<D, FMT, LO>), state);
+    else return allow_full_lds(reinterpret_cast<const void *>(kv_attn_wide_kernel<D, FMT, LO>), state);
 }
 
 hipError_t kv_attn_prepare() {
@@ -673,10 +696,10 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     if (allowed != hipSuccess) return allowed;
     const int cus = device_cus();
     const int turn = c.n_seqs == 1 && splits == 1 && cus % c.hkv == 0 && (int)items >= 2 * cus ? cus / c.hkv : 1 << 29;
-    kv_attn_wide_kernel<D, FMT, LO, false><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
+    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || (splits == 1 && a.shared == 0)) return e;
-    const int parts = splits + (a.shared > 0 ? (a.shared + a.prefix_chunk - 1) / a.prefix_chunk : 0);
+    const int parts = splits + (a.shared > 0 ? (a.shared + a.prefix_run - 1) / a.prefix_run : 0);
     if (parts <= kJoinFew)
         kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
     else
@@ -700,14 +723,32 @@ hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs
     }
 }
 
+// Of 4 wavefronts two a CU, of 8 one: kPerSimd of both.
+template <int D, int FMT, bool LO>
+constexpr int prefix_slots() {
+    return 256 * 4 * WideShape<D, FMT, LO>::kPerSimd / WideShape<D, FMT, LO>::NW;
+}
+template <int D>
+static int prefix_slots_of(int fmt, bool out_f16) {
+    if (fmt == MGQ_KV_I8) return out_f16 ? prefix_slots<D, kFmtI8, false>() : prefix_slots<D, kFmtI8, true>();
+    return out_f16 ? prefix_slots<D, kFmtE4M3, false>() : prefix_slots<D, kFmtE4M3, true>();
+}
+int kv_attn_prefix_slots(int dim, int fmt, bool out_f16) {
+    switch (dim) {
+    case 64: return prefix_slots_of<64>(fmt, out_f16);
+    case 96: return prefix_slots_of<96>(fmt, out_f16);
+    case 128: return prefix_slots_of<128>(fmt, out_f16);
+    default: return prefix_slots_of<256>(fmt, out_f16);
+    }
+}
+
 template <int D, int FMT, bool LO>
 static hipError_t prefix_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     typedef WideShape<D, FMT, LO> W;
     const hipError_t allowed = wide_allow<D, FMT, LO, true>();
     if (allowed != hipSuccess) return allowed;
-    const int64_t parts = (a.shared + a.prefix_chunk - 1) / a.prefix_chunk;
-    kv_attn_wide_kernel<D, FMT, LO, true><<<(unsigned)(parts * a.prefix_blocks * c.hkv), W::kThreads,
-                                            W::template lds_bytes<true>(), stream>>>(c, a, 0, 0);
+    kv_attn_prefix_kernel<D, FMT, LO><<<(unsigned)(prefix_runs(a) * c.hkv), W::kThreads, W::template lds_bytes<true>(),
+                                        stream>>>(c, a);
     return hipGetLastError();
 }
 

@@ -52,7 +52,6 @@
 
 namespace mgq {
 
-constexpr int kRows = 16;         // query rows of a work-group's row of tiles
 constexpr int kAttnGroups = 512;  // work-groups: two of 4 wavefronts per CU
 constexpr int NW = 4;             // wavefronts of a work-group
 // A row of 512 tokens is not cut (2 tiles a wavefront cost less than the joining
@@ -114,22 +113,26 @@ struct AttnPlace {
     }
     __device__ __forceinline__ void cut(int tiles, int most, bool shared) {
         if (most == 0) part = kSoloTiles;
-        else part = shared || tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
+        // many short rows: twice as long parts, so that there are seldom more than work-groups
+        else if (shared) part = max(kPartTiles, (int)((2 * (int64_t)tiles + most - 1) / most));
+        else part = tiles < most * kRunTiles ? max(kPartTiles, (tiles + most - 1) / most) : 0;
     }
-    __device__ __forceinline__ void deal(int units, int most) {
-        const int groups = part ? (int)gridDim.x : min(most, (int)gridDim.x);
+    __device__ __forceinline__ void deal(int units, int most, int group, int of) {
+        const int groups = part ? of : min(most, of);
         total = units;
         run = (total + groups - 1) / groups;
-        at = (int)blockIdx.x < groups ? (int)blockIdx.x * run : total;
+        at = group < groups ? group * run : total;
     }
 };
-__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int most, int *part, int *found) {
+// For work-group `group` of `of`.
+__device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs &a, int most, int group, int of, int *part,
+                                                int *found) {
     constexpr int NT = 64 * NW;
     AttnPlace p = {};
     if (c.n_seqs == 1) {
         p.q = attn_seq(c, a, 0);
         p.cut(p.q.blocks * c.hkv * p.q.tiles, most, a.shared > 0);
-        p.deal(p.units(p.q, c.hkv), most);
+        p.deal(p.units(p.q, c.hkv), most, group, of);
         return p;
     }
     // all tiles, then all units, then the sequence that `at` lies in; the
@@ -151,7 +154,7 @@ __device__ __forceinline__ AttnPlace attn_place(const KvView &c, const AttnArgs 
         for (int b = threadIdx.x; b < c.n_seqs; b += NT) units += p.units(attn_seq(c, a, b), c.hkv);
         group_scan(units, part, t);
     }
-    p.deal(t, most);
+    p.deal(t, most, group, of);
     for (int b0 = 0; b0 < c.n_seqs; b0 += NT) {
         if (c.n_seqs > NT) {
             units = b0 + (int)threadIdx.x < c.n_seqs ? p.units(attn_seq(c, a, b0 + threadIdx.x), c.hkv) : 0;
@@ -181,7 +184,8 @@ __device__ __forceinline__ int2 *row_states(const AttnArgs &a, int states) {
     return reinterpret_cast<int2 *>(a.ws + (int64_t)states * state_floats<D>(kRows));
 }
 
-template <int D, int FMT>
+// SHARED: the first work-groups have a shared prefix's parts, for few rows.
+template <int D, int FMT, bool SHARED>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvView c, AttnArgs a, int max_blocks, int most,
                                                                                int states) {
     constexpr bool I8 = FMT == kFmtI8 && D % 64 == 0;
@@ -196,22 +200,52 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int page = 1 << c.page_shift;
 
-    const AttnPlace place = attn_place(c, a, most, part, found);
-    int at = place.at;
-    const int stop = min(at + place.run, place.total);
-    if (at >= stop) return;
-    int b = place.b, base = place.base;
-    AttnSeq q = place.q;
+    __shared__ int lim[SHARED ? kRows : 1];
+    __shared__ unsigned long long best;
+    const int ahead = SHARED ? a.prefix_cuts * a.prefix_blocks * c.hkv : 0;
+    const bool of_prefix = SHARED && (int)blockIdx.x < ahead;
+    AttnPlace place = {};
+    int at = 0, stop = 1, b = 0, base = 0;
+    AttnSeq q = {};
+    if (of_prefix) {
+        q.s = {0, c.n_tokens, 0, a.shared * kTile};
+        q.tiles = a.shared;
+        q.blocks = a.prefix_blocks;
+    } else {
+        place = attn_place(c, a, most, (int)blockIdx.x - ahead, (int)gridDim.x - ahead, part, found);
+        at = place.at;
+        stop = min(at + place.run, place.total);
+        if (at >= stop) return;
+        b = place.b;
+        base = place.base;
+        q = place.q;
+    }
 
     while (at < stop) {
-        while (at - base >= place.units(q, c.hkv)) {  // the next sequence with rows
+        while (!of_prefix && at - base >= place.units(q, c.hkv)) {  // the next sequence with rows
             base += place.units(q, c.hkv);
             q = attn_seq(c, a, ++b);
         }
-        const int first_unit = at, cuts = place.part ? place.parts(q) : q.tiles;
-        const int k = (at - base) % cuts, row = (at - base) / cuts;
-        int t0, t1;
-        if (place.part) {
+        const int first_unit = at;
+        int cuts, k, row, t0, t1;
+        if (of_prefix) {  // parts of one kv head that many blocks go through are dealt together
+            cuts = a.prefix_cuts;
+            k = (int)blockIdx.x / c.hkv % cuts;
+            row = (int)blockIdx.x / c.hkv / cuts * c.hkv + (int)blockIdx.x % c.hkv;
+        } else {
+            cuts = place.part ? place.parts(q) : q.tiles;
+            k = (at - base) % cuts;
+            row = (at - base) / cuts;
+        }
+        if (of_prefix) {
+            const int first = row / c.hkv * kRows;
+            prefix_limits(c, a, first / a.group, (min(first + kRows, q.s.n * a.group) - 1) / a.group + 1, NT, lim, best);
+            t0 = k * a.prefix_run;
+            t1 = min((int)(best >> 32), t0 + a.prefix_run);
+            if (t0 >= t1) return;  // no row of the block sees them, nor asks for their state
+            b = (int)(0xFFFFFFFFu - (unsigned)best);
+            ++at;
+        } else if (place.part) {
             t0 = (int)((int64_t)q.tiles * k / cuts);
             t1 = (int)((int64_t)q.tiles * (k + 1) / cuts);
             ++at;
@@ -227,7 +261,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         const int r = r0 + col;
         const bool live = r < rows;
         const int tq = live ? r / a.group : 0, hd = live ? r % a.group : 0;
-        const int pos = live ? q.s.pos0 + tq : -1;
+        const int pos = !live ? -1 : of_prefix ? lim[tq - r0 / a.group] * kTile - 1 : q.s.pos0 + tq;
         // ---- loads
         const int kgrp = col >> 2;  // the 16 tokens that this lane's K rows are of
         u32x4 vreg[DB];
@@ -414,7 +448,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == q.tiles && a.shared == 0;
-        float *slot = a.ws + (int64_t)(place.part ? first_unit : 2 * (int)blockIdx.x + (t0 == 0)) * state_floats<D>(kRows);
+        float *slot = of_prefix ? prefix_part<D>(c, a, h, blk, k)
+                                : a.ws + (int64_t)(place.part ? first_unit : 2 * (int)blockIdx.x + (t0 == 0)) * state_floats<D>(kRows);
         const int mine = min(kRows, rows - r0);
         for (int i = tid; i < mine * (D / 4); i += NT) {
             const int rr = i / (D / 4), d = 4 * (i % (D / 4));
@@ -438,7 +473,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void kv_attn_kernel(KvVi
                 }
             }
         }
-        if (tid == 0 && t0 == 0) {
+        if (tid == 0 && t0 == 0 && !of_prefix) {
             int2 st = {first_unit, cuts};
             if (whole) st.y = 1;
             else if (!place.part) st = {(int)blockIdx.x, (int)blockIdx.x - 1 - (first_unit + q.tiles - 1) / place.run};
@@ -475,6 +510,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
         put_out4(a, s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
 
+// Work-groups that are resident at once.
+static int attn_slots(int dim) { return dim == 256 ? kAttnGroups / 2 : kAttnGroups; }
+// Query rows of all sequences, of a kv head, up to which a shared prefix is gone through in
+// blocks of kRows beside the sequences' own tiles.
+constexpr int64_t kThinRows = 448, kThinTiles = 15000;
+
 // Query rows of a kv head up to which this kernel takes the call, in blocks of
 // 16 that each read the cache, and above which kv_attn_wide.hip does. Measured
 // (28 heads on 4 of 128, int8): 28 rows x 16 sequences of 4000 tokens 29 us here,
@@ -482,9 +523,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
 // rows 57 and 40.
 bool kv_attn_is_wide(int dim, int64_t rows) { return rows > (dim == 256 ? 32 : 48); }
 
-// Most tiles of a row: the table's, or the window's and those of the first tokens.
+// Most tiles of a row: the table's, or the window's and those of the first tokens, or what
+// is behind a shared prefix (a sequence that does not see all of it has only its new
+// tokens behind what it sees).
 static int64_t most_tiles(int64_t cap, int max_new, const AttnArgs &a) {
     const int64_t all = (cap + kTile - 1) / kTile;
+    if (a.shared > 0) return std::min(all, std::max(all - a.shared, ((int64_t)max_new + kTile - 1) / kTile + 1));
     if (a.window == 0) return all;
     return std::min(all, ((int64_t)a.window + max_new - 1 + kTile - 1 + kTile - 1) / kTile + (a.sinks + kTile - 1) / kTile);
 }
@@ -507,15 +551,57 @@ size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int6
 
 // The prefix's part of a call.
 struct PrefixPlan {
-    int tiles, blocks, span, run;
-    int64_t runs;  // of a kv head
+    int tiles, blocks, span, run, cuts;
+    int64_t states;  // of a kv head
+    int rows;        // of a state
 };
-static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_tokens, int64_t capacity,
-                              int shared_tokens) {
+// Tiles of a part of a prefix, for few rows: `rows` blocks of them, `own` rows of the
+// sequences' own tiles in the same launch. By the time until all are done, in steps of a
+// tile for each wavefront (some 2.5 us): a work-group's start takes kStart, a
+// sequence's own tiles are taken as two steps; the parts, which begin first, are as many
+// as end together with what finds room beside them.
+static int thin_run(int dim, int tiles, int64_t rows, int64_t own) {
+    constexpr int kStart = 3, kOwn = kStart + 2;
+    const int64_t slots = attn_slots(dim);
+    int best = tiles;
+    int64_t least = INT64_MAX;
+    for (int run = kPartTiles;; run += kPartTiles) {
+        run = std::min(run, tiles);
+        const int64_t parts = rows * ((tiles + run - 1) / run), step = kStart + (run + NW - 1) / NW;
+        const int64_t rounds = (parts + slots - 1) / slots, beside = rounds * slots - parts;
+        const int64_t left = std::max<int64_t>(0, own - beside * (step / kOwn));
+        const int64_t all = rounds * step + (left + slots - 1) / slots * kOwn;
+        if (all < least) {
+            least = all;
+            best = run;
+        }
+        if (run == tiles) return best;
+    }
+}
+static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
+                              int64_t capacity, int shared_tokens) {
     PrefixPlan p = {};
     p.tiles = (int)(std::min<int64_t>(capacity, shared_tokens) / kTile);
-    p.blocks = (int)(((int64_t)n_tokens * (hq / hkv) + kWideRows - 1) / kWideRows);
     if (p.tiles == 0) return p;
+    const int64_t rows = (int64_t)n_tokens * (hq / hkv), each = (int64_t)max_new * (hq / hkv);
+    // a prefix of less than two tiles for each work-group when every sequence reads it by
+    // itself: that costs less than the further states (4 tokens behind 2000, 28 heads on
+    // 4: 14.0 and 16.3 us; 32 behind 500: 18.5 and 17.4)
+    if ((int64_t)n_seqs * hkv * ((each + kRows - 1) / kRows) * p.tiles < 2 * attn_slots(dim)) {
+        p.tiles = 0;
+        return p;
+    }
+    if (rows <= kThinRows && (rows + kRows - 1) / kRows * hkv * p.tiles <= kThinTiles && !kv_attn_is_wide(dim, each)) {
+        p.blocks = (int)((rows + kRows - 1) / kRows);
+        p.run = thin_run(dim, p.tiles, (int64_t)p.blocks * hkv,
+                         (int64_t)n_seqs * hkv * (((int64_t)max_new * (hq / hkv) + kRows - 1) / kRows));
+        p.cuts = (p.tiles + p.run - 1) / p.run;
+        p.states = (int64_t)p.blocks * p.cuts;
+        p.rows = kRows;
+        return p;
+    }
+    p.blocks = (int)((rows + kWideRows - 1) / kWideRows);
+    p.rows = kWideRows;
     // Runs of equal length over all blocks fill the chip best, but a run with tiles of two
     // blocks begins twice (rows, page ids, first loads: some 6 us, as long as kTwice
     // tiles); equal parts of each block are longer where the work-groups are no multiple
@@ -529,19 +615,20 @@ static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, in
     const bool whole = part <= run + kTwice;
     p.run = (int)(whole ? part : run);
     p.span = whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
-    p.runs = ((int64_t)p.blocks * p.span + p.run - 1) / p.run;
+    p.states = 2 * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
     return p;
 }
 static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
                                 int shared_tokens) {
-    int64_t runs = 0;  // for either type of result
-    for (int f16 = 0; f16 < 2; ++f16)
-        runs = std::max(runs, prefix_plan(dim, fmt, f16, hq, hkv, n_tokens, capacity, shared_tokens).runs);
-    if (runs == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
-    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) +
-           (size_t)(2 * runs * hkv) * kWideRows * (dim + 2) * sizeof(float);
+    size_t floats = 0;  // for either type of result
+    for (int f16 = 0; f16 < 2; ++f16) {
+        const PrefixPlan p = prefix_plan(dim, fmt, f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
+        floats = std::max(floats, (size_t)(p.states * hkv) * p.rows * (dim + 2));
+    }
+    if (floats == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
+    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) + floats * sizeof(float);
 }
 
 template <int D, int FMT>
@@ -550,10 +637,14 @@ static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t s
     const int64_t tiles = most_tiles((int64_t)c.max_pages << c.page_shift, c.max_new, a);
     const int64_t rows = (int64_t)c.n_seqs * c.hkv * max_blocks;
     const bool solo = tiles <= kSoloTiles;  // no row can be longer
-    const int most = D == 256 ? kAttnGroups / 2 : kAttnGroups;  // resident at once
+    const int most = attn_slots(D);
     const int groups = (int)(solo ? rows : std::min(rows * ((tiles + kPartTiles - 1) / kPartTiles), most + rows));
     const int states = (int)most_states(rows);
-    kv_attn_kernel<D, FMT><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
+    const int ahead = a.prefix_cuts * a.prefix_blocks * c.hkv;
+    if (ahead > 0)
+        kv_attn_kernel<D, FMT, true><<<(unsigned)(ahead + groups), 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
+    else
+        kv_attn_kernel<D, FMT, false><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || (solo && a.shared == 0)) return e;
     const int block_rows = std::min(kRows, c.max_new * a.group);
@@ -574,17 +665,19 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
     a.sinks = a.window > 0 ? std::min(x.sinks, 1 << 30) : 0;
     a.ws = x.ws;
-    a.shared = 0;
+    a.shared = a.prefix_cuts = a.prefix_blocks = 0;
     if (x.shared_tokens > 0) {
         const int64_t cap = (int64_t)c.max_pages << c.page_shift;
-        const PrefixPlan p = prefix_plan(dim, fmt, x.out_f16, x.hq, c.hkv, c.n_tokens, cap, x.shared_tokens);
+        const PrefixPlan p = prefix_plan(dim, fmt, x.out_f16, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap,
+                                         x.shared_tokens);
         if (p.tiles > 0) {
             a.shared = p.tiles;
             a.prefix_blocks = p.blocks;
             a.prefix_span = p.span;
             a.prefix_run = p.run;
             a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
-            const hipError_t e = kv_attn_prefix_launch(c, dim, fmt, a, stream);
+            a.prefix_cuts = p.cuts;
+            const hipError_t e = p.cuts > 0 ? hipSuccess : kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;
         }
     }

@@ -25,8 +25,12 @@ struct AttnArgs {
     // query rows that go through them, the places that a block has in the row of all
     // tiles (some at its end may be empty), the tiles of a work-group, and its states
     int shared, prefix_blocks, prefix_span, prefix_run;
+    // few query rows: blocks of kRows of them, each block's tiles in `prefix_cuts` parts of
+    // prefix_run tiles (0: many rows)
+    int prefix_cuts;
     float *prefix;
 };
+constexpr int kRows = 16;       // query rows of a work-group's row of tiles
 constexpr int kWideRows = 128;  // query rows that share a tile through LDS
 
 // Which tiles a run of query rows goes through, by number: those of the first tokens
@@ -265,8 +269,8 @@ template <int D>
 __device__ __forceinline__ RowState row_state(const float *state, int rows, int row) {
     return {state + row * D, state + rows * D + 2 * row};
 }
-// A shared prefix's states. Run r of a kv head has state 2r for a row block that an
-// earlier run begins, 2r + 1 for one that it begins.
+// A shared prefix's states. Many rows: run r of a kv head has state 2r for a row block
+// that an earlier run begins, 2r + 1 for one that it begins. Few: every part has one.
 inline int64_t prefix_runs(const AttnArgs &a) {
     return ((int64_t)a.prefix_blocks * a.prefix_span + a.prefix_run - 1) / a.prefix_run;
 }
@@ -274,24 +278,49 @@ template <int D>
 __device__ __forceinline__ float *prefix_slot(const KvView &c, const AttnArgs &a, int h, int run, bool begins) {
     return a.prefix + ((2 * (int64_t)run + begins) * c.hkv + h) * state_floats<D>(kWideRows);
 }
-// Row `row` of all the call's query rows of a kv head: the runs that its sequence's share
-// of the prefix is over.
+template <int D>
+__device__ __forceinline__ float *prefix_part(const KvView &c, const AttnArgs &a, int h, int block, int k) {
+    return a.prefix + (((int64_t)block * a.prefix_cuts + k) * c.hkv + h) * state_floats<D>(kRows);
+}
+// Row `row` of all the call's query rows of a kv head: the states that its sequence's
+// share of the prefix is in.
 struct PrefixParts {
-    int first, n, row;
+    int first, n;  // many rows: the first run
+    int64_t row;
     template <int D>
     __device__ __forceinline__ RowState state(const KvView &c, const AttnArgs &a, int h, int i) const {
-        return row_state<D>(prefix_slot<D>(c, a, h, first + i, i == 0), kWideRows, row);
+        if (a.prefix_cuts > 0)
+            return row_state<D>(prefix_part<D>(c, a, h, (int)(row / kRows), i), kRows, (int)(row % kRows));
+        return row_state<D>(prefix_slot<D>(c, a, h, first + i, i == 0), kWideRows, (int)(row % kWideRows));
     }
 };
 __device__ __forceinline__ PrefixParts prefix_parts(const AttnArgs &a, const SeqInfo &s, int64_t row) {
-    PrefixParts p = {0, 0, (int)(row % kWideRows)};
+    PrefixParts p = {0, 0, row};
     const int tiles = a.shared > 0 ? shared_tiles(a, s) : 0;
     if (tiles > 0) {
-        const int64_t at = row / kWideRows * a.prefix_span;
+        const int64_t at = a.prefix_cuts > 0 ? 0 : row / kWideRows * a.prefix_span;
         p.first = (int)(at / a.prefix_run);
         p.n = (int)((at + tiles - 1) / a.prefix_run) - p.first + 1;
     }
     return p;
+}
+// What tokens t0 .. t1-1 of the call, whichever sequence's they are, see of the prefix:
+// lim gets the tiles of each (0: a row of no sequence), for a work-group of `threads`.
+// The pages are those of the sequence that sees most (the first such), which the others'
+// lists begin with: `best` has its tiles, and its number's complement.
+__device__ __forceinline__ void prefix_limits(const KvView &c, const AttnArgs &a, int t0, int t1, int threads, int *lim,
+                                              unsigned long long &best) {
+    if (threadIdx.x == 0) best = 0;
+    for (int i = threadIdx.x; i < t1 - t0; i += threads) lim[i] = 0;
+    __syncthreads();
+    // without row starts a token is its own sequence's
+    for (int i = threadIdx.x + (c.cu ? 0 : t0); i < (c.cu ? c.n_seqs : t1); i += threads) {
+        const SeqInfo s = kv_seq(c, i);
+        const int lo = max(s.t0, t0), hi = min(s.t0 + s.n, t1), n = shared_tiles(a, s);
+        for (int t = lo; t < hi; ++t) atomicMax(&lim[t - t0], n);
+        if (lo < hi) atomicMax(&best, (unsigned long long)n << 32 | (0xFFFFFFFFu - (unsigned)i));
+    }
+    __syncthreads();
 }
 
 // The states of one query row, `n` of them (slot(i) -> the i-th), joined by a

@@ -116,37 +116,18 @@ __device__ __forceinline__ WidePlace wide_place(const KvView &c, const AttnArgs 
     return p;
 }
 
-// A shared prefix: block rt of all the call's query rows, whichever sequence's they
-// are. A token's rows see as many of its tiles as its sequence does; lim gets them for
-// the block's tokens (0: a row of no sequence). The pages are those of the sequence that
-// sees most (the first such), which the others' lists begin with.
+// A shared prefix: block rt of all the call's query rows.
 struct PrefixRows {
     int lim[kWideRows];
     unsigned long long best;
 };
 __device__ __forceinline__ void prefix_block(const KvView &c, const AttnArgs &a, int rt, PrefixRows &p, int &b, WideBlock &w) {
-    int *lim = p.lim;
-    unsigned long long &best = p.best;
-    const int threads = blockDim.x;
     w.rows = c.n_tokens * a.group;
     w.r0 = rt * kWideRows;
-    const int t0 = w.r0 / a.group, t1 = (min(w.r0 + kWideRows, w.rows) - 1) / a.group + 1;
-    if (threadIdx.x == 0) best = 0;
-    for (int i = threadIdx.x; i < kWideRows; i += threads) lim[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < c.n_seqs; i += threads) {
-        const SeqInfo s = kv_seq(c, i);
-        const int lo = max(s.t0, t0), hi = min(s.t0 + s.n, t1), n = shared_tiles(a, s);
-        for (int t = lo; t < hi; ++t) atomicMax(&lim[t - t0], n);
-        if (lo < hi) atomicMax(&best, (unsigned long long)n << 32 | (0xFFFFFFFFu - (unsigned)i));
-    }
-    __syncthreads();
-    w.tiles = (int)(best >> 32);
-    b = w.tiles > 0 ? (int)(0xFFFFFFFFu - (unsigned)best) : 0;
-    w.s.t0 = 0;
-    w.s.n = c.n_tokens;
-    w.s.pos0 = 0;
-    w.s.len = w.tiles * kTile;
+    prefix_limits(c, a, w.r0 / a.group, (min(w.r0 + kWideRows, w.rows) - 1) / a.group + 1, blockDim.x, p.lim, p.best);
+    w.tiles = (int)(p.best >> 32);
+    b = w.tiles > 0 ? (int)(0xFFFFFFFFu - (unsigned)p.best) : 0;
+    w.s = {0, c.n_tokens, 0, w.tiles * kTile};
     w.list = {0, 0};
     w.chunk = 0;
 }

@@ -305,8 +305,8 @@ typedef struct mgq_block_norm {
  *   h' = h_scale*h + x_scale*gate*z (x null: h_scale*h; gate null: 1)
  *   y  = h' * r(h') * norm_w        as y_type, MGQ_OUT_F32 or MGQ_OUT_F16
  * h' goes to h_out (null: nowhere), y to y (null: nowhere; not both null). The sums
- * are 64-bit and h' and y are rounded once from 64-bit products; y is that of the
- * rounded h'. Values of y past the type's largest are infinite. Strides are in
+ * of squares are 64-bit, r(a) may be of any size, the products are f32; y is that of
+ * the rounded h'. Values of y past the type's largest are infinite. Strides are in
  * values, at least hidden; gate_stride 0: one row of gates for all rows. h_out may be
  * h with the same stride; nothing else that is written may overlap what is read or
  * written. hipErrorInvalidValue for post_w or gate without x and for y without

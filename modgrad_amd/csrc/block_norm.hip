@@ -2,34 +2,36 @@
 //
 //   z  = x * r(x) * post_w   (post_w null: x),   r(a) = 1 / sqrt(mean(a^2) + eps)
 //   h' = h_scale * h + x_scale * gate * z
-//   y  = h' * r(h') * norm_w, f32 or f16
+//   y  = h' * r(h') * norm_w, f32 or f16; of the h' that was stored
 //
-// in one pass: a row of x and h is read once and stays in registers over both
-// sums. The squares are summed in 64 bits (a row of 1e20 has a square that f32 does
-// not), each product of factors is taken in 64 bits and rounded once, to h' and to
-// y; y is that of the h' that was stored. The conversions and 64-bit operations,
-// some 12 a value, take a tenth of the time that its 16 bytes do.
+// in one pass: a row of x and h is read once and stays in registers over both sums. The
+// squares are summed in 64 bits (a row of 1e25 has squares that f32 does not), the
+// factor r is a mantissa and a power of two, and everything else is f32: with its
+// products in 64 bits too, a value took 12 conversions at a quarter of the rate.
 #include "q4k_device.hpp"
 #include "q4k_launch.hpp"
+
+#include <climits>
 
 namespace mgq {
 
 constexpr int kNormThreads = 256;
 
-// NT threads a row (64: a wavefront each, kNormThreads / 64 rows a work-group), V
-// quads of neighbouring values a thread.
-__device__ __forceinline__ double wave_sum(double v) {
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-template <int NT>
-__device__ __forceinline__ double row_sum(double v, double *part) {
+// The sum of a row's NT threads, on each (64: a wavefront each, kNormThreads / 64 rows a
+// work-group).
+template <int NT, class T>
+__device__ __forceinline__ T row_sum(T v, T *part) {
     v = wave_sum(v);
     if constexpr (NT > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.0;
+        v = 0;
 #pragma unroll
         for (int w = 0; w < NT / 64; ++w) v += part[w];
     }
@@ -41,6 +43,13 @@ __device__ __forceinline__ double inv_sqrt(double s) {
     const double r = __builtin_amdgcn_rsq(s), e = fma(-s * r, r, 1.0);
     return fabs(e) < 1.0 ? fma(0.5 * e, r, r) : r;
 }
+// A factor of any size on f32 values.
+struct Factor {
+    float m;
+    int e;
+    __device__ __forceinline__ explicit Factor(double r) : m((float)__builtin_amdgcn_frexp_mant(r)), e(__builtin_amdgcn_frexp_exp(r)) {}
+    __device__ __forceinline__ float operator*(float x) const { return __builtin_amdgcn_ldexpf(x, e) * m; }
+};
 
 // Quad c of a row of n values; values past the row's end are 0.
 __device__ __forceinline__ f32x4 ld_quad(const float *row, int c, int n) {
@@ -51,16 +60,16 @@ __device__ __forceinline__ f32x4 ld_quad(const float *row, int c, int n) {
         if (4 * c + e < n) v[e] = row[4 * c + e];
     return v;
 }
-__device__ __forceinline__ void st_quad(float *row, int c, int n, const float (&v)[4]) {
+__device__ __forceinline__ void st_quad(float *row, int c, int n, f32x4 v) {
     if (4 * c + 4 <= n) {
-        *reinterpret_cast<f32x4_a4 *>(row + 4 * c) = f32x4_a4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_a4 *>(row + 4 * c) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (4 * c + e < n) row[4 * c + e] = v[e];
     }
 }
-__device__ __forceinline__ void st_quad(_Float16 *row, int c, int n, const float (&v)[4]) {
+__device__ __forceinline__ void st_quad(_Float16 *row, int c, int n, f32x4 v) {
     typedef _Float16 half4 __attribute__((ext_vector_type(4)));
     const half4 x = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     if (4 * c + 4 <= n) {
@@ -71,84 +80,89 @@ __device__ __forceinline__ void st_quad(_Float16 *row, int c, int n, const float
             if (4 * c + e < n) row[4 * c + e] = x[e];
     }
 }
-
-template <int NT, int V>
+// V quads of neighbouring values a thread; TAIL: rows end inside a quad.
+template <int NT, int V, bool TAIL>
 __global__ __launch_bounds__(NT < kNormThreads ? kNormThreads : NT) void block_norm_kernel(BlockNorm a) {
     constexpr int ROWS = NT < kNormThreads ? kNormThreads / NT : 1;
     // of this row and the one before, which a slower wavefront may still be reading
     __shared__ double part[2][2][NT / 64];
     const int tid = threadIdx.x % NT, n = a.hidden;
-    f32x4 pv[V], nv[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        pv[i] = a.post_w ? ld_quad(a.post_w, tid + i * NT, n) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
-        nv[i] = a.norm_w ? ld_quad(a.norm_w, tid + i * NT, n) : f32x4{};
-    }
+    const auto get = [&](const float *row, int i) {
+        const int c = tid + i * NT;
+        if (TAIL) return ld_quad(row, c, n);
+        return 4 * c < n ? ld_f32x4(row + 4 * c) : f32x4{};
+    };
+    const auto put = [&](auto *row, int i, f32x4 v) {
+        const int c = tid + i * NT;
+        if (TAIL || 4 * c < n) st_quad(row, c, TAIL ? n : INT_MAX, v);
+    };
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+        turn ^= 1;
         const float *h = a.h + row * a.h_stride, *x = a.x ? a.x + row * a.x_stride : nullptr;
         const float *gate = a.gate ? a.gate + row * a.gate_stride : nullptr;
-        f32x4 xv[V], hv[V], gv[V];
+        f32x4 xv[V], hv[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = tid + i * NT;
-            xv[i] = x ? ld_quad(x, c, n) : f32x4{};
-            hv[i] = ld_quad(h, c, n);
-            gv[i] = gate ? ld_quad(gate, c, n) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
-        }
-        double r = a.x_scale;
+        for (int i = 0; i < V; ++i) xv[i] = x ? get(x, i) : f32x4{};
+#pragma unroll
+        for (int i = 0; i < V; ++i) hv[i] = get(h, i);
         if (a.post_w) {
             double s = 0.0;
 #pragma unroll
             for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s = fma((double)xv[i][e], (double)xv[i][e], s);
-            r *= inv_sqrt(row_sum<NT>(s, part[turn][0]) / n + a.eps);
+            const Factor r(inv_sqrt(row_sum<NT>(s, part[turn][0]) / n + a.eps));
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const f32x4 w = get(a.post_w, i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xv[i][e] = r * xv[i][e] * w[e];
+            }
+        }
+        if (gate) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) xv[i] *= get(gate, i);
         }
         double s = 0.0;
         float *ho = a.h_out ? a.h_out + row * a.h_out_stride : nullptr;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = tid + i * NT;
-            float o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const double z = (double)xv[i][e] * r * pv[i][e] * gv[i][e];
-                o[e] = (float)(x ? fma((double)a.h_scale, (double)hv[i][e], z) : (double)a.h_scale * hv[i][e]);
-                hv[i][e] = o[e];
-                s = fma((double)o[e], (double)o[e], s);
+                hv[i][e] = a.h_scale * hv[i][e];
+                if (x) hv[i][e] = fmaf(xv[i][e], a.x_scale, hv[i][e]);
+                s = fma((double)hv[i][e], (double)hv[i][e], s);
             }
-            if (ho) st_quad(ho, c, n, o);
+            if (ho) put(ho, i, hv[i]);
         }
-        if (a.y) {
-            r = inv_sqrt(row_sum<NT>(s, part[turn][1]) / n + a.eps);
+        if (!a.y) continue;
+        const Factor r(inv_sqrt(row_sum<NT>(s, part[turn][1]) / n + a.eps));
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int c = tid + i * NT;
-                float o[4];
+        for (int i = 0; i < V; ++i) {
+            const f32x4 w = get(a.norm_w, i);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (float)((double)hv[i][e] * r * nv[i][e]);
-                if (a.y_f16) st_quad(static_cast<_Float16 *>(a.y) + row * a.y_stride, c, n, o);
-                else st_quad(static_cast<float *>(a.y) + row * a.y_stride, c, n, o);
-            }
+            for (int e = 0; e < 4; ++e) hv[i][e] = r * hv[i][e] * w[e];
+            if (a.y_f16) put(static_cast<_Float16 *>(a.y) + row * a.y_stride, i, hv[i]);
+            else put(static_cast<float *>(a.y) + row * a.y_stride, i, hv[i]);
         }
-        turn ^= 1;
     }
 }
 
-// Rows that no work-group's registers hold: each thread goes through its quads three
-// times (h' through h_out, or computed again where it is not kept).
+// Rows that no work-group's registers hold: each thread goes through its own quads three
+// times; h' comes back through h_out, or is computed again where it is not kept.
 constexpr int kLongThreads = 1024;
-
 __global__ __launch_bounds__(kLongThreads) void block_norm_long_kernel(BlockNorm a) {
     constexpr int NT = kLongThreads;
     __shared__ double part[2][2][NT / 64];
     const int tid = threadIdx.x, n = a.hidden, quads = (n + 3) / 4;
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        turn ^= 1;
         const float *h = a.h + row * a.h_stride, *x = a.x ? a.x + row * a.x_stride : nullptr;
         const float *gate = a.gate ? a.gate + row * a.gate_stride : nullptr;
-        double r = a.x_scale;
+        float *ho = a.h_out ? a.h_out + row * a.h_out_stride : nullptr;
+        double mean = 1.0;
         if (a.post_w) {
             double s = 0.0;
 #pragma unroll 4
@@ -157,55 +171,42 @@ __global__ __launch_bounds__(kLongThreads) void block_norm_long_kernel(BlockNorm
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s = fma((double)v[e], (double)v[e], s);
             }
-            r *= inv_sqrt(row_sum<NT>(s, part[turn][0]) / n + a.eps);
+            mean = row_sum<NT>(s, part[turn][0]) / n + a.eps;
         }
-        const auto value = [&](int c, float (&o)[4]) {
-            const f32x4 hv = ld_quad(h, c, n);
-            if (!x) {
+        const Factor rx(a.post_w ? inv_sqrt(mean) : 1.0);
+        const auto value = [&](int c) {
+            f32x4 o = a.h_scale * ld_quad(h, c, n);
+            if (!x) return o;
+            f32x4 z = ld_quad(x, c, n);
+            if (a.post_w) {
+                const f32x4 w = ld_quad(a.post_w, c, n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (float)((double)a.h_scale * hv[e]);
-                return;
+                for (int e = 0; e < 4; ++e) z[e] = rx * z[e] * w[e];
             }
-            const f32x4 one = {1.0f, 1.0f, 1.0f, 1.0f}, xv = ld_quad(x, c, n);
-            const f32x4 pv = a.post_w ? ld_quad(a.post_w, c, n) : one, gv = gate ? ld_quad(gate, c, n) : one;
+            if (gate) z *= ld_quad(gate, c, n);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double z = (double)xv[e] * r * pv[e] * gv[e];
-                o[e] = (float)fma((double)a.h_scale, (double)hv[e], z);
-            }
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(z[e], a.x_scale, o[e]);
+            return o;
         };
-        float *ho = a.h_out ? a.h_out + row * a.h_out_stride : nullptr;
         double s = 0.0;
 #pragma unroll 2
         for (int c = tid; c < quads; c += NT) {
-            float o[4];
-            value(c, o);
+            const f32x4 o = value(c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s = fma((double)o[e], (double)o[e], s);
             if (ho) st_quad(ho, c, n, o);
         }
-        if (!a.y) {
-            turn ^= 1;
-            continue;
-        }
-        const double ry = inv_sqrt(row_sum<NT>(s, part[turn][1]) / n + a.eps);
+        if (!a.y) continue;
+        const Factor r(inv_sqrt(row_sum<NT>(s, part[turn][1]) / n + a.eps));
 #pragma unroll 2
         for (int c = tid; c < quads; c += NT) {
-            float o[4];
-            if (ho) {  // what this thread has stored (h may be h_out)
-                const f32x4 v = ld_quad(ho, c, n);
+            f32x4 o = ho ? ld_quad(ho, c, n) : value(c);
+            const f32x4 w = ld_quad(a.norm_w, c, n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = v[e];
-            } else {
-                value(c, o);
-            }
-            const f32x4 nv = ld_quad(a.norm_w, c, n);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (float)((double)o[e] * ry * nv[e]);
+            for (int e = 0; e < 4; ++e) o[e] = r * o[e] * w[e];
             if (a.y_f16) st_quad(static_cast<_Float16 *>(a.y) + row * a.y_stride, c, n, o);
             else st_quad(static_cast<float *>(a.y) + row * a.y_stride, c, n, o);
         }
-        turn ^= 1;
     }
 }
 
@@ -216,7 +217,9 @@ static unsigned norm_grid(int64_t groups) { return (unsigned)std::min<int64_t>(g
 template <int NT, int V>
 static hipError_t norm_run(const BlockNorm &a, hipStream_t stream) {
     constexpr int ROWS = NT < kNormThreads ? kNormThreads / NT : 1, THREADS = NT * ROWS;
-    block_norm_kernel<NT, V><<<norm_grid(((int64_t)a.rows + ROWS - 1) / ROWS), THREADS, 0, stream>>>(a);
+    const unsigned grid = norm_grid(((int64_t)a.rows + ROWS - 1) / ROWS);
+    if (a.hidden % 4) block_norm_kernel<NT, V, true><<<grid, THREADS, 0, stream>>>(a);
+    else block_norm_kernel<NT, V, false><<<grid, THREADS, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -226,6 +229,7 @@ hipError_t block_norm_launch(const BlockNorm &a, hipStream_t stream) {
     if (few ? quads <= 64 : quads <= 256) return quads <= 64 ? norm_run<64, 1>(a, stream) : norm_run<64, 4>(a, stream);
     if (few ? quads <= 256 : quads <= 1024) return quads <= 256 ? norm_run<256, 1>(a, stream) : norm_run<256, 4>(a, stream);
     if (quads <= 1024) return norm_run<1024, 1>(a, stream);
+    if (quads <= 2048) return norm_run<1024, 2>(a, stream);
     if (quads <= 4096) return norm_run<1024, 4>(a, stream);
     block_norm_long_kernel<<<norm_grid(a.rows), kLongThreads, 0, stream>>>(a);
     return hipGetLastError();

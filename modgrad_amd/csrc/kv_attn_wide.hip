@@ -91,8 +91,8 @@ __device__ __forceinline__ WidePlace wide_place(const KvView &c, const AttnArgs 
         p.split = id / max(1, p.total);
         if (p.split >= p.splits) return p;
         id -= p.split * p.total;
-        p.state = id;
     }
+    p.state = id;
     int before = 0;
     for (int b0 = 0; b0 < c.n_seqs; b0 += 64) {
         if (b0 > 0) n = blocks(b0 + lane);

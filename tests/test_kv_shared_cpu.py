@@ -66,3 +66,16 @@ def test_refuses_null(L):
                                            None) == INVALID
     d, chain = _lib.OpDesc(op=_lib.OP_KV_ATTENTION_SHARED), ctypes.c_void_p()
     assert L.mgq_chain_create_ops(ctypes.byref(d), 1, ctypes.byref(chain)) == INVALID
+
+
+def test_sizes_that_go_through_the_prefix_once(L):
+    """The GPU tests of those paths are of sizes that take them: room for their states."""
+    from tests.test_gpu_kv_shared_paths import CASES, WAYS
+    cases = [(prefix, seqs, new, heads, group, dim, page) for prefix, seqs, _, new, heads, group, dim, page, _ in
+             CASES.values()] + [(1024, seqs, new, 4, group, 64, 16) for seqs, new, group in WAYS.values()]
+    for prefix, seqs, new, heads, group, dim, page in cases:
+        for fmt in (0, 1):
+            c = cache(page_stride=heads * page * dim, page_tokens=page, n_kv_heads=heads, head_dim=dim, format=fmt,
+                      n_seqs=seqs, max_pages=prefix // page + 100)
+            plain = L.mgq_kv_attention_workspace_bytes(ctypes.byref(c), heads * group, new)
+            assert size(L, c, hq=heads * group, n=seqs * new, new=new, shared=prefix) > plain

@@ -46,13 +46,14 @@ def test_refuses(L, bad):
 
 
 def test_workspace(L):
-    c = cache(max_pages=40)
+    c, big = cache(max_pages=40, n_seqs=64), dict(n=320, shared=1024)
     plain = L.mgq_kv_attention_workspace_bytes(ctypes.byref(c), 4, 5)
-    need = size(L, c)
+    need = size(L, c, **big)
     assert need > plain > 0 and need % 16 == 0
-    assert attend(L, c, nbytes=need - 1) == INVALID
-    assert size(L, c, shared=63) == plain  # no whole tile of 64 tokens: the plain call
-    assert size(L, c, shared=2 ** 31 - 1) == size(L, c, shared=40 * 64)
+    assert attend(L, c, nbytes=need - 1, **big) == INVALID
+    # no whole tile of 64 tokens, or so few that every sequence reads them: the plain call's
+    assert size(L, c, n=320, shared=63) == plain and size(L, c, n=320, shared=64) == plain
+    assert size(L, c, n=320, shared=2 ** 31 - 1) == size(L, c, n=320, shared=40 * 64)
     for bad in (dict(hq=3), dict(n=0), dict(n=-1), dict(new=0), dict(shared=-1), dict(n=1 << 28)):
         assert size(L, c, **bad) == 0
     # room for the states of every block of 128 query rows and its parts of the prefix

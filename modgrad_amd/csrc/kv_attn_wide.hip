@@ -582,9 +582,10 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_kernel(KvView c, AttnAr
         put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + 4 * threadIdx.x, o);
 }
 
-// The same for few splits: D/4 lanes a row.
+// The same for few splits: D/4 lanes a row. Behind a shared prefix every row is joined:
+// latency bounds it, so that 4 states load at once, and the sum moves with the maximum.
 constexpr int kJoinFew = 16;
-template <int D>
+template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, AttnArgs a, int most_splits) {
     constexpr int L = D / 4, PER = 256 / L, R = 8, STEPS = kWideRows / R;  // R rows a work-group
     int id = blockIdx.x;
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
     if (place.rt < 0 || place.split > 0) return;
     WideBlock w;
     if (!wide_block(c, a, place.b, place.rt, place.splits, w)) return;
-    if (w.chunk >= w.tiles && a.shared == 0) return;
+    if (w.chunk >= w.tiles && !SHARED) return;
     const int own = (w.tiles + w.chunk - 1) / w.chunk, d = 4 * (threadIdx.x % L);
     if ((int)threadIdx.x >= PER * L) return;
     const float *base = a.ws + ((int64_t)id * c.hkv + h) * state_floats<D>(kWideRows);
@@ -604,14 +605,40 @@ __global__ __launch_bounds__(256) void kv_attn_wide_join_few_kernel(KvView c, At
     for (int rr = R * part + threadIdx.x / L; rr < R * part + R; rr += PER) {
         const int r = w.r0 + rr;
         if (r >= w.rows) break;
-        const PrefixParts ahead = prefix_parts(a, w.s, (int64_t)w.s.t0 * a.group + r);
+        PrefixParts ahead = {};
+        if (SHARED) ahead = prefix_parts(a, w.s, (int64_t)w.s.t0 * a.group + r);
         const int n = ahead.n + own;
         const auto slot = [&](int i) {
-            return i < ahead.n ? ahead.state<D>(c, a, h, i) : row_state<D>(base + (i - ahead.n) * step, kWideRows, rr);
+            return SHARED && i < ahead.n ? ahead.state<D>(c, a, h, i) : row_state<D>(base + (i - ahead.n) * step, kWideRows, rr);
         };
         float M = -INFINITY, l = 0.0f;
-        for (int i = 0; i < n; ++i) M = fmaxf(M, slot(i).ml[0]);
         f32x4 o = {};
+        if constexpr (SHARED) {
+            constexpr int U = 4;
+            for (int i0 = 0; i0 < n; i0 += U) {
+                float2 ml[U];
+                f32x4 x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const RowState s = slot(min(i0 + u, n - 1));
+                    ml[u] = *reinterpret_cast<const float2 *>(s.ml);
+                    x[u] = *reinterpret_cast<const f32x4 *>(s.o + d);
+                    if (i0 + u >= n) ml[u] = make_float2(-INFINITY, 0.0f);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // of nothing; scores of NaN have a NaN l
+                    const float m = fmaxf(M, ml[u].x);
+                    const Exp2 f(M == -INFINITY ? -INFINITY : M - m), g(ml[u].x == -INFINITY ? -INFINITY : ml[u].x - m);
+                    M = m;
+                    l = f.times(l) + g.times(ml[u].y);
+                    o = o * f.f + x[u] * g.f;
+                }
+            }
+            put_out4(a, w.s.t0 + r / a.group, (h * a.group + r % a.group) * D + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
+            continue;
+        }
+        for (int i = 0; i < n; ++i) M = fmaxf(M, slot(i).ml[0]);
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const RowState s = slot(i);
@@ -681,8 +708,10 @@ static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t strea
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || (splits == 1 && a.shared == 0)) return e;
     const int parts = splits + (a.shared > 0 ? (a.shared + a.prefix_run - 1) / a.prefix_run : 0);
-    if (parts <= kJoinFew)
-        kv_attn_wide_join_few_kernel<D><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
+    if (parts <= kJoinFew && a.shared > 0)
+        kv_attn_wide_join_few_kernel<D, true><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
+    else if (parts <= kJoinFew)
+        kv_attn_wide_join_few_kernel<D, false><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
     else
         kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, splits);
     return hipGetLastError();

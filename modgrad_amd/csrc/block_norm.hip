@@ -7,7 +7,13 @@
 // in one pass: a row of x and h is read once and stays in registers over both sums. The
 // squares are summed in 64 bits (a row of 1e25 has squares that f32 does not), the
 // factor r is a mantissa and a power of two, and everything else is f32: with its
-// products in 64 bits too, a value took 12 conversions at a quarter of the rate.
+// products in 64 bits too, a value took 12 conversions at a quarter of the rate (4096
+// rows of 3584, f16 results: 55 us, 46 so).
+//
+// Many rows are bound by their bytes: 256 threads of 4 quads a row of 3584 (206 MB, 46 us,
+// 4.5 TB/s; a copy reaches 5.1), a wavefront a row up to 1024 values (16384 rows of 896:
+// 4.8 TB/s). 512 threads of 2 quads: 50 us; registers for 5 or 6 wavefronts a SIMD
+// instead of 4: 65 and 104 (spills). Few rows are bound by latency: a quad a thread.
 #include "q4k_device.hpp"
 #include "q4k_launch.hpp"
 

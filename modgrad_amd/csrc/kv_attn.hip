@@ -45,6 +45,11 @@
 // with its own softmax state, joined through LDS; a row in several parts leaves
 // their states in the workspace for kv_attn_join_kernel.
 //
+// Few query rows behind a shared prefix: the launch's first work-groups go through it for
+// blocks of 16 rows of whichever sequences, the others through what is each sequence's
+// own, and a row's states of both are joined. 6 tokens of 14 heads behind 1472: 11.6 us;
+// 16 of 28 heads behind 8000: 22, every sequence by itself 34.
+//
 // Bound by the cache's bytes (28 heads on 4 of 128): 32 ragged sequences to 32 Ki
 // tokens, e4m3, 380 MB: 81 us + 4.8 for the join, 4.7 TB/s; 200 000 tokens, int8,
 // 205 MB: 42 + 5 us. A sequence of 1000 tokens is latency: 9 + 3 us.
@@ -513,7 +518,11 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvView c, AttnArgs a,
 // Work-groups that are resident at once.
 static int attn_slots(int dim) { return dim == 256 ? kAttnGroups / 2 : kAttnGroups; }
 // Query rows of all sequences, of a kv head, up to which a shared prefix is gone through in
-// blocks of kRows beside the sequences' own tiles.
+// blocks of kRows beside the sequences' own tiles, in one launch, and tiles of those blocks,
+// over all kv heads. Above, kv_attn_prefix_kernel has fewer, dearer tiles and a launch of
+// its own. Measured (28 heads on 4 of 128, here and there; us a call): 16 tokens behind
+// 12000 28 and 38, 32 behind 12000 37 and 45, 48 behind 12000 (15700 tiles) 52 and 48, 64
+// behind 12000 63 and 59.
 constexpr int64_t kThinRows = 448, kThinTiles = 15000;
 
 // Query rows of a kv head up to which this kernel takes the call, in blocks of

@@ -131,7 +131,10 @@ hipError_t rope_launch(const float *x, float *y, const int *pos, const mgq_rope 
     return hipGetLastError();
 }
 
-// The same with positions of several axes, a row of the table for each.
+// The same with positions of several axes: each pair's entry by its axis's position, which
+// a few operations on the pair's number name, so that no map is read. Bound by x and y as
+// above: 4900 tokens of 16 heads of 80, 52 MB, 11.3 us (4.6 TB/s, inputs in the Infinity
+// Cache); 7 tokens 3.0-3.3 us, a launch.
 template <bool VEC>
 __global__ __launch_bounds__(256) void rope_axes_kernel(const float *x, float *y, RopeMany m, int n_tokens, int heads,
                                                         int dim, int64_t x_stride, int64_t y_stride) {

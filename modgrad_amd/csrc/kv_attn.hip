@@ -47,8 +47,8 @@
 //
 // Few query rows behind a shared prefix: the launch's first work-groups go through it for
 // blocks of 16 rows of whichever sequences, the others through what is each sequence's
-// own, and a row's states of both are joined. 6 tokens of 14 heads behind 1472: 11.6 us;
-// 16 of 28 heads behind 8000: 22, every sequence by itself 34.
+// own, and a row's states of both are joined. 16 tokens of 28 heads on 4 of 128 behind
+// 8000: 22 us, every sequence by itself 34; 4 behind 8000 17 and 19.
 //
 // Bound by the cache's bytes (28 heads on 4 of 128): 32 ragged sequences to 32 Ki
 // tokens, e4m3, 380 MB: 81 us + 4.8 for the join, 4.7 TB/s; 200 000 tokens, int8,
@@ -572,20 +572,25 @@ struct PrefixPlan {
 static int thin_run(int dim, int tiles, int64_t rows, int64_t own) {
     constexpr int kStart = 3, kOwn = kStart + 2;
     const int64_t slots = attn_slots(dim);
+    const int64_t most = (tiles + kPartTiles - 1) / kPartTiles, all = std::max<int64_t>(1, std::min(slots / rows, most));
     int best = tiles;
     int64_t least = INT64_MAX;
-    for (int run = kPartTiles;; run += kPartTiles) {
-        run = std::min(run, tiles);
+    // as many parts as there are work-groups for, some fewer, and as many as leave every
+    // own row a place in one round or two
+    for (int i = 0; i < 12; ++i) {
+        const int64_t cuts = i < 9 ? all - i : i == 9 ? (slots - own) / rows : i == 10 ? 2 * slots / rows : (2 * slots - own) / rows;
+        if (cuts < 1 || cuts > most) continue;
+        const int run = (int)((tiles + cuts - 1) / cuts);
         const int64_t parts = rows * ((tiles + run - 1) / run), step = kStart + (run + NW - 1) / NW;
         const int64_t rounds = (parts + slots - 1) / slots, beside = rounds * slots - parts;
         const int64_t left = std::max<int64_t>(0, own - beside * (step / kOwn));
-        const int64_t all = rounds * step + (left + slots - 1) / slots * kOwn;
-        if (all < least) {
-            least = all;
+        const int64_t time = rounds * step + (left + slots - 1) / slots * kOwn;
+        if (time < least) {
+            least = time;
             best = run;
         }
-        if (run == tiles) return best;
     }
+    return best;
 }
 static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
                               int64_t capacity, int shared_tokens) {

@@ -534,6 +534,23 @@ hipError_t launch_kv_attention_shared_ex(const mgq_kv_cache *cache, const float 
                                          int shared_tokens, void *workspace,
                                          size_t workspace_bytes, hipStream_t stream);
 
+/* How such a call goes through the prefix (host only, launches nothing);
+ * hipErrorInvalidValue where the workspace's size is 0. */
+#define MGQ_SHARED_PLAIN 0 /* every sequence reads it by itself */
+#define MGQ_SHARED_FEW 1   /* once for 16 query rows of a kv head, beside the sequences' own tiles */
+#define MGQ_SHARED_PARTS 2 /* once for 128, in equal parts of each such row block */
+#define MGQ_SHARED_RUNS 3  /* once for 128, in equal runs, which may go on into the next block */
+typedef struct mgq_kv_shared_plan {
+    int way;             /* MGQ_SHARED_* */
+    int tiles;           /* of 64 tokens that are gone through so; 0 for MGQ_SHARED_PLAIN */
+    int blocks, run;     /* row blocks of a kv head; tiles of a part or a run */
+    int64_t own_groups;  /* work-groups on what each sequence reads by itself, */
+    int64_t join_groups; /* and of the launch that joins; 0: none */
+} mgq_kv_shared_plan;
+hipError_t mgq_kv_attention_shared_plan(const mgq_kv_cache *cache, int n_q_heads, int out_type,
+                                        int n_tokens, int max_new, int shared_tokens,
+                                        mgq_kv_shared_plan *plan);
+
 /* One matvec of a decode-step chain. */
 typedef struct mgq_gemv_desc {
     const unsigned char *w_q4; /* row-aligned Q4_K bytes */

@@ -67,6 +67,7 @@ SIGNATURES = {
     "mgq_kv_attention_workspace_bytes": (S, [P, I, I]),
     "launch_kv_attention_sinks_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, I, P, S, P]),
     "mgq_kv_attention_shared_workspace_bytes": (S, [P, I, I, I, I]),
+    "mgq_kv_attention_shared_plan": (I, [P, I, I, I, I, I, P]),
     "launch_kv_attention_shared_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, P, S, P]),
     "launch_kv_attention_ex": (I, [P, P, L, I, P, L, I, I, I, F, F, I, P, S, P]),
     "mgq_chain_create": (I, [P, I, P]),
@@ -104,6 +105,10 @@ OP_ROPE_AXES = 13
 OP_KV_APPEND_AXES = 14
 OP_KV_ATTENTION_SINKS = 15
 OP_KV_ATTENTION_SHARED = 16
+SHARED_PLAIN = 0
+SHARED_FEW = 1
+SHARED_PARTS = 2
+SHARED_RUNS = 3
 AXES_BLOCKS = 0
 AXES_TURNS = 1
 ROPE_INTERLEAVED = 0
@@ -193,6 +198,11 @@ class KvAttentionSinksArgs(ctypes.Structure):
 class KvAttentionSharedArgs(ctypes.Structure):
     """mgq_kv_attention_shared_args (OP_KV_ATTENTION_SHARED)."""
     _fields_ = [("attention", KvAttentionArgs), ("shared_tokens", I)]
+
+
+class KvSharedPlan(ctypes.Structure):
+    """mgq_kv_shared_plan."""
+    _fields_ = [("way", I), ("tiles", I), ("blocks", I), ("run", I), ("own_groups", L), ("join_groups", L)]
 
 
 class BlockNorm(ctypes.Structure):

@@ -369,6 +369,16 @@ size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *c, int n_q_he
                                     (int64_t)c->max_pages * c->page_tokens, shared_tokens);
 }
 
+hipError_t mgq_kv_attention_shared_plan(const mgq_kv_cache *c, int n_q_heads, int out_type, int n_tokens, int max_new,
+                                        int shared_tokens, mgq_kv_shared_plan *plan) {
+    if (!plan || (out_type != MGQ_OUT_F32 && out_type != MGQ_OUT_F16)) return hipErrorInvalidValue;
+    if (mgq_kv_attention_shared_workspace_bytes(c, n_q_heads, n_tokens, max_new, shared_tokens) == 0)
+        return hipErrorInvalidValue;
+    *plan = kv_attn_shared_plan(c->head_dim, c->format, out_type == MGQ_OUT_F16, n_q_heads, c->n_kv_heads, c->n_seqs,
+                                n_tokens, max_new, (int64_t)c->max_pages * c->page_tokens, shared_tokens);
+    return hipSuccess;
+}
+
 hipError_t launch_kv_attention_shared_ex(const mgq_kv_cache *c, const float *q, int64_t q_stride, int n_q_heads,
                                          void *out, int64_t out_stride, int out_type, int n_tokens, int max_new,
                                          float scale, float softcap, int shared_tokens, void *workspace,

@@ -563,7 +563,16 @@ struct PrefixPlan {
     int tiles, blocks, span, run, cuts;
     int64_t states;  // of a kv head
     int rows;        // of a state
+    bool whole;      // many rows: equal parts of each block, not runs over all
 };
+// ... as the kernels and the grids see it, but for where its states lie.
+static void use_plan(AttnArgs &a, const PrefixPlan &p) {
+    a.shared = p.tiles;
+    a.prefix_blocks = p.blocks;
+    a.prefix_span = p.span;
+    a.prefix_run = p.run;
+    a.prefix_cuts = p.cuts;
+}
 // Tiles of a part of a prefix, for few rows: `rows` blocks of them, `own` rows of the
 // sequences' own tiles in the same launch. By the time until all are done, in steps of a
 // tile for each wavefront (some 2.5 us): a work-group's start takes kStart, a
@@ -626,9 +635,9 @@ static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, in
     const int64_t run = std::min<int64_t>(p.tiles, ((int64_t)p.blocks * p.tiles + groups - 1) / groups);
     const int64_t parts = std::min<int64_t>(p.tiles, std::max<int64_t>(1, groups / p.blocks));
     const int64_t part = (p.tiles + parts - 1) / parts;
-    const bool whole = part <= run + kTwice;
-    p.run = (int)(whole ? part : run);
-    p.span = whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
+    p.whole = part <= run + kTwice;
+    p.run = (int)(p.whole ? part : run);
+    p.span = p.whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
     p.states = 2 * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
     return p;
 }
@@ -645,25 +654,57 @@ size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, i
     return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) + floats * sizeof(float);
 }
 
+// The launches of a call of few query rows of a sequence.
+struct TokenGrid {
+    int max_blocks, block_rows, states;  // row blocks of a sequence, rows of a block, states in the workspace
+    bool solo;                           // no row can be longer than kSoloTiles
+    int64_t groups, join;                // work-groups on the sequences' own tiles, and of the join (0: none)
+};
+static TokenGrid token_grid(int dim, int hkv, int n_seqs, int max_new, int64_t cap, const AttnArgs &a) {
+    TokenGrid g;
+    g.max_blocks = (max_new * a.group + kRows - 1) / kRows;
+    g.block_rows = std::min(kRows, max_new * a.group);
+    const int64_t tiles = most_tiles(cap, max_new, a), rows = (int64_t)n_seqs * hkv * g.max_blocks;
+    g.states = (int)most_states(rows);
+    g.solo = tiles <= kSoloTiles;
+    g.groups = g.solo ? rows : std::min(rows * ((tiles + kPartTiles - 1) / kPartTiles), attn_slots(dim) + rows);
+    g.join = g.solo && a.shared == 0 ? 0 : rows * g.block_rows;
+    return g;
+}
+
 template <int D, int FMT>
 static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
-    const int max_blocks = (c.max_new * a.group + kRows - 1) / kRows;
-    const int64_t tiles = most_tiles((int64_t)c.max_pages << c.page_shift, c.max_new, a);
-    const int64_t rows = (int64_t)c.n_seqs * c.hkv * max_blocks;
-    const bool solo = tiles <= kSoloTiles;  // no row can be longer
-    const int most = attn_slots(D);
-    const int groups = (int)(solo ? rows : std::min(rows * ((tiles + kPartTiles - 1) / kPartTiles), most + rows));
-    const int states = (int)most_states(rows);
+    const TokenGrid g = token_grid(D, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, a);
+    const int most = g.solo ? 0 : attn_slots(D);
     const int ahead = a.prefix_cuts * a.prefix_blocks * c.hkv;
     if (ahead > 0)
-        kv_attn_kernel<D, FMT, true><<<(unsigned)(ahead + groups), 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
+        kv_attn_kernel<D, FMT, true><<<(unsigned)(ahead + g.groups), 64 * NW, 0, stream>>>(c, a, g.max_blocks, most, g.states);
     else
-        kv_attn_kernel<D, FMT, false><<<(unsigned)groups, 64 * NW, 0, stream>>>(c, a, max_blocks, solo ? 0 : most, states);
+        kv_attn_kernel<D, FMT, false><<<(unsigned)g.groups, 64 * NW, 0, stream>>>(c, a, g.max_blocks, most, g.states);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (solo && a.shared == 0)) return e;
-    const int block_rows = std::min(kRows, c.max_new * a.group);
-    kv_attn_join_kernel<D><<<(unsigned)(rows * block_rows), 256, 0, stream>>>(c, a, max_blocks, block_rows, states);
+    if (e != hipSuccess || g.join == 0) return e;
+    kv_attn_join_kernel<D><<<(unsigned)g.join, 256, 0, stream>>>(c, a, g.max_blocks, g.block_rows, g.states);
     return hipGetLastError();
+}
+
+SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
+                               int64_t capacity, int shared_tokens) {
+    const PrefixPlan p = prefix_plan(dim, fmt, out_f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
+    AttnArgs a = {};
+    a.group = hq / hkv;
+    use_plan(a, p);
+    SharedPlan s = {p.tiles == 0 ? MGQ_SHARED_PLAIN : p.cuts > 0 ? MGQ_SHARED_FEW : p.whole ? MGQ_SHARED_PARTS : MGQ_SHARED_RUNS,
+                    p.tiles, p.blocks, p.run, 0, 0};
+    if (kv_attn_is_wide(dim, (int64_t)max_new * a.group)) {
+        const WideGrid g = kv_attn_wide_grid(dim, hkv, n_seqs, max_new, capacity, a);
+        s.own_groups = g.items * g.splits;
+        s.join_groups = g.join;
+    } else {
+        const TokenGrid g = token_grid(dim, hkv, n_seqs, max_new, capacity, a);
+        s.own_groups = g.groups;
+        s.join_groups = g.join;
+    }
+    return s;
 }
 
 hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hipStream_t stream) {
@@ -685,12 +726,8 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
         const PrefixPlan p = prefix_plan(dim, fmt, x.out_f16, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap,
                                          x.shared_tokens);
         if (p.tiles > 0) {
-            a.shared = p.tiles;
-            a.prefix_blocks = p.blocks;
-            a.prefix_span = p.span;
-            a.prefix_run = p.run;
+            use_plan(a, p);
             a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
-            a.prefix_cuts = p.cuts;
             const hipError_t e = p.cuts > 0 ? hipSuccess : kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;
         }

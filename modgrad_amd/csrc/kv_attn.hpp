@@ -95,6 +95,15 @@ __device__ __forceinline__ bool vanishing(float top, float ref) { return top < r
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
 size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, bool shared);
+// Its launches: row blocks of all kv heads, splits of each, work-groups of the join (0: none)
+// and which of the two joins that is.
+struct WideGrid {
+    int64_t items;
+    int splits;
+    int64_t join;
+    bool few;
+};
+WideGrid kv_attn_wide_grid(int dim, int hkv, int n_seqs, int max_new, int64_t cap, const AttnArgs &a);
 // All query rows over the tiles of a prefix that they share, and how many of its
 // work-groups are resident at once.
 int kv_attn_prefix_slots(int dim, int fmt, bool out_f16);

@@ -693,32 +693,35 @@ hipError_t kv_attn_prepare() {
     return e;
 }
 
-template <int D, int FMT, bool LO>
-static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
-    int row_blocks, splits;
-    const int64_t cap = (int64_t)c.max_pages << c.page_shift;
-    wide_plan(D, a.group, c.hkv, c.n_seqs, c.max_new, cap, row_blocks, splits);
+WideGrid kv_attn_wide_grid(int dim, int hkv, int n_seqs, int max_new, int64_t cap, const AttnArgs &a) {
+    WideGrid g;
+    int row_blocks;
+    wide_plan(dim, a.group, hkv, n_seqs, max_new, cap, row_blocks, g.splits);
     if (a.window > 0) {  // a row block's tokens, their windows and the first tokens
         const int64_t seen = (int64_t)a.window + kWideRows / a.group + 2 * kTile + (a.sinks > 0 ? a.sinks + kTile : 0);
-        splits = (int)std::min<int64_t>(splits, (seen / kTile + kWideChunk - 1) / kWideChunk);
+        g.splits = (int)std::min<int64_t>(g.splits, (seen / kTile + kWideChunk - 1) / kWideChunk);
     }
-    const unsigned items = (unsigned)(row_blocks * c.hkv * c.n_seqs);
+    g.items = (int64_t)row_blocks * hkv * n_seqs;
+    g.few = g.splits + (a.shared > 0 ? (a.shared + a.prefix_run - 1) / a.prefix_run : 0) <= kJoinFew;
+    g.join = g.splits == 1 && a.shared == 0 ? 0 : g.items * (g.few ? kWideRows / 8 : kWideRows);
+    return g;
+}
+
+template <int D, int FMT, bool LO>
+static hipError_t wide_run(const KvView &c, const AttnArgs &a, hipStream_t stream) {
+    const WideGrid g = kv_attn_wide_grid(D, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, a);
     typedef WideShape<D, FMT, LO> W;
     constexpr size_t kLds = W::template lds_bytes<false>();
     const hipError_t allowed = wide_allow<D, FMT, LO>();
     if (allowed != hipSuccess) return allowed;
     const int cus = device_cus();
-    const int turn = c.n_seqs == 1 && splits == 1 && cus % c.hkv == 0 && (int)items >= 2 * cus ? cus / c.hkv : 1 << 29;
-    kv_attn_wide_kernel<D, FMT, LO><<<items * splits, W::kThreads, kLds, stream>>>(c, a, splits, turn);
+    const int turn = c.n_seqs == 1 && g.splits == 1 && cus % c.hkv == 0 && g.items >= 2 * cus ? cus / c.hkv : 1 << 29;
+    kv_attn_wide_kernel<D, FMT, LO><<<(unsigned)(g.items * g.splits), W::kThreads, kLds, stream>>>(c, a, g.splits, turn);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (splits == 1 && a.shared == 0)) return e;
-    const int parts = splits + (a.shared > 0 ? (a.shared + a.prefix_run - 1) / a.prefix_run : 0);
-    if (parts <= kJoinFew && a.shared > 0)
-        kv_attn_wide_join_few_kernel<D, true><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
-    else if (parts <= kJoinFew)
-        kv_attn_wide_join_few_kernel<D, false><<<items * (kWideRows / 8), 256, 0, stream>>>(c, a, splits);
-    else
-        kv_attn_wide_join_kernel<D><<<items * kWideRows, 256, 0, stream>>>(c, a, splits);
+    if (e != hipSuccess || g.join == 0) return e;
+    if (g.few && a.shared > 0) kv_attn_wide_join_few_kernel<D, true><<<(unsigned)g.join, 256, 0, stream>>>(c, a, g.splits);
+    else if (g.few) kv_attn_wide_join_few_kernel<D, false><<<(unsigned)g.join, 256, 0, stream>>>(c, a, g.splits);
+    else kv_attn_wide_join_kernel<D><<<(unsigned)g.join, 256, 0, stream>>>(c, a, g.splits);
     return hipGetLastError();
 }
 

@@ -522,8 +522,9 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *
  * for all rows, the rest sequence by sequence, and the two joined in f32 as the parts
  * of a long sequence are. A row sees only its own and earlier positions also where
  * shared_tokens reaches past them; of a prefix that is not as described, what one of the
- * sequences' pages holds is used for others. shared_tokens is not negative; past
- * max_pages*page_tokens it counts as that. The workspace is of
+ * sequences' pages holds is used for others. Where row starts fall, so that ranges
+ * overlap, rows of ranges past the first n_tokens rows' worth may be left as they are.
+ * shared_tokens is not negative; past max_pages*page_tokens it counts as that. The workspace is of
  * mgq_kv_attention_shared_workspace_bytes (0: arguments that the call refuses). */
 size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads,
                                                int n_tokens, int max_new, int shared_tokens);

@@ -55,6 +55,8 @@
 // 205 MB: 42 + 5 us. A sequence of 1000 tokens is latency: 9 + 3 us.
 #include "kv_attn.hpp"
 
+#include <climits>
+
 namespace mgq {
 
 constexpr int kAttnGroups = 512;  // work-groups: two of 4 wavefronts per CU
@@ -566,7 +568,8 @@ struct PrefixPlan {
     bool whole;      // many rows: equal parts of each block, not runs over all
 };
 // ... as the kernels and the grids see it, but for where its states lie.
-static void use_plan(AttnArgs &a, const PrefixPlan &p) {
+static void use_plan(AttnArgs &a, const PrefixPlan &p, int n_seqs, int n_tokens, int max_new) {
+    a.row_blocks = p.tiles > 0 ? (int)std::min<int64_t>(INT_MAX, most_row_blocks(a.group, n_seqs, n_tokens, max_new)) : INT_MAX;
     a.shared = p.tiles;
     a.prefix_blocks = p.blocks;
     a.prefix_span = p.span;
@@ -601,8 +604,8 @@ static int thin_run(int dim, int tiles, int64_t rows, int64_t own) {
     }
     return best;
 }
-static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
-                              int64_t capacity, int shared_tokens) {
+static PrefixPlan prefix_cut(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
+                             int64_t capacity, int shared_tokens) {
     PrefixPlan p = {};
     p.tiles = (int)(std::min<int64_t>(capacity, shared_tokens) / kTile);
     if (p.tiles == 0) return p;
@@ -641,19 +644,6 @@ static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, in
     p.states = 2 * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
     return p;
 }
-static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
-
-size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
-                                int shared_tokens) {
-    size_t floats = 0;  // for either type of result
-    for (int f16 = 0; f16 < 2; ++f16) {
-        const PrefixPlan p = prefix_plan(dim, fmt, f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
-        floats = std::max(floats, (size_t)(p.states * hkv) * p.rows * (dim + 2));
-    }
-    if (floats == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
-    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) + floats * sizeof(float);
-}
-
 // The launches of a call of few query rows of a sequence.
 struct TokenGrid {
     int max_blocks, block_rows, states;  // row blocks of a sequence, rows of a block, states in the workspace
@@ -672,6 +662,51 @@ static TokenGrid token_grid(int dim, int hkv, int n_seqs, int max_new, int64_t c
     return g;
 }
 
+// Work-groups on the sequences' own tiles, and of the join, of a call with such a plan.
+struct OwnGrid {
+    int64_t groups, join;
+};
+static OwnGrid own_grid(const PrefixPlan &p, int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap) {
+    AttnArgs a = {};
+    a.group = hq / hkv;
+    use_plan(a, p, n_seqs, n_tokens, max_new);
+    if (kv_attn_is_wide(dim, (int64_t)max_new * a.group)) {
+        const WideGrid g = kv_attn_wide_grid(dim, hkv, n_seqs, max_new, cap, a);
+        return {g.items * g.splits, g.join};
+    }
+    const TokenGrid g = token_grid(dim, hkv, n_seqs, max_new, cap, a);
+    return {g.groups, g.join};
+}
+// The plan of a call. Where its join would have the 2^32 threads that no launch has, every
+// sequence reads the prefix by itself, and few row blocks or none are joined.
+static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
+                              int64_t capacity, int shared_tokens) {
+    const PrefixPlan p = prefix_cut(dim, fmt, out_f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
+    const bool fits = own_grid(p, dim, hq, hkv, n_seqs, n_tokens, max_new, capacity).join < (INT64_C(1) << 32) / 256;
+    return fits ? p : PrefixPlan{};
+}
+
+SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
+                               int64_t capacity, int shared_tokens) {
+    const PrefixPlan p = prefix_plan(dim, fmt, out_f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
+    const OwnGrid g = own_grid(p, dim, hq, hkv, n_seqs, n_tokens, max_new, capacity);
+    return {p.tiles == 0 ? MGQ_SHARED_PLAIN : p.cuts > 0 ? MGQ_SHARED_FEW : p.whole ? MGQ_SHARED_PARTS : MGQ_SHARED_RUNS,
+            p.tiles, p.blocks, p.run, g.groups, g.join};
+}
+
+static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
+                                int shared_tokens) {
+    size_t floats = 0;  // for either type of result
+    for (int f16 = 0; f16 < 2; ++f16) {
+        const PrefixPlan p = prefix_plan(dim, fmt, f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
+        floats = std::max(floats, (size_t)(p.states * hkv) * p.rows * (dim + 2));
+    }
+    if (floats == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
+    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) + floats * sizeof(float);
+}
+
 template <int D, int FMT>
 static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t stream) {
     const TokenGrid g = token_grid(D, c.hkv, c.n_seqs, c.max_new, (int64_t)c.max_pages << c.page_shift, a);
@@ -687,26 +722,6 @@ static hipError_t attn_run_dim(const KvView &c, const AttnArgs &a, hipStream_t s
     return hipGetLastError();
 }
 
-SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
-                               int64_t capacity, int shared_tokens) {
-    const PrefixPlan p = prefix_plan(dim, fmt, out_f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
-    AttnArgs a = {};
-    a.group = hq / hkv;
-    use_plan(a, p);
-    SharedPlan s = {p.tiles == 0 ? MGQ_SHARED_PLAIN : p.cuts > 0 ? MGQ_SHARED_FEW : p.whole ? MGQ_SHARED_PARTS : MGQ_SHARED_RUNS,
-                    p.tiles, p.blocks, p.run, 0, 0};
-    if (kv_attn_is_wide(dim, (int64_t)max_new * a.group)) {
-        const WideGrid g = kv_attn_wide_grid(dim, hkv, n_seqs, max_new, capacity, a);
-        s.own_groups = g.items * g.splits;
-        s.join_groups = g.join;
-    } else {
-        const TokenGrid g = token_grid(dim, hkv, n_seqs, max_new, capacity, a);
-        s.own_groups = g.groups;
-        s.join_groups = g.join;
-    }
-    return s;
-}
-
 hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hipStream_t stream) {
     AttnArgs a;
     a.q = x.q;
@@ -720,13 +735,13 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
     a.sinks = a.window > 0 ? std::min(x.sinks, 1 << 30) : 0;
     a.ws = x.ws;
-    a.shared = a.prefix_cuts = a.prefix_blocks = 0;
+    use_plan(a, PrefixPlan{}, c.n_seqs, c.n_tokens, c.max_new);
     if (x.shared_tokens > 0) {
         const int64_t cap = (int64_t)c.max_pages << c.page_shift;
         const PrefixPlan p = prefix_plan(dim, fmt, x.out_f16, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap,
                                          x.shared_tokens);
         if (p.tiles > 0) {
-            use_plan(a, p);
+            use_plan(a, p, c.n_seqs, c.n_tokens, c.max_new);
             a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
             const hipError_t e = p.cuts > 0 ? hipSuccess : kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;

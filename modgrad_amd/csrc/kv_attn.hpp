@@ -29,6 +29,7 @@ struct AttnArgs {
     // prefix_run tiles (0: many rows)
     int prefix_cuts;
     float *prefix;
+    int row_blocks;  // of kWideRows, of all sequences, that the call's rows can make (no prefix: any number)
 };
 constexpr int kRows = 16;       // query rows of a work-group's row of tiles
 constexpr int kWideRows = 128;  // query rows that share a tile through LDS
@@ -103,6 +104,12 @@ struct WideGrid {
     int64_t join;
     bool few;
 };
+// Row blocks that the sequences' rows make at most, where their ranges do not overlap: each
+// begins at most one that is not full.
+inline int64_t most_row_blocks(int group, int n_seqs, int n_tokens, int max_new) {
+    const int64_t each = ((int64_t)max_new * group + kWideRows - 1) / kWideRows;
+    return std::min(each * n_seqs, (int64_t)n_tokens * group / kWideRows + n_seqs);
+}
 WideGrid kv_attn_wide_grid(int dim, int hkv, int n_seqs, int max_new, int64_t cap, const AttnArgs &a);
 // All query rows over the tiles of a prefix that they share, and how many of its
 // work-groups are resident at once.

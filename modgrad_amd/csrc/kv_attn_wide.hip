@@ -86,7 +86,7 @@ __device__ __forceinline__ WidePlace wide_place(const KvView &c, const AttnArgs 
         for (int b = lane + 64; b < c.n_seqs; b += 64) sum += blocks(b);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        p.total = __builtin_amdgcn_readfirstlane(sum);
+        p.total = min(__builtin_amdgcn_readfirstlane(sum), a.row_blocks);  // overlapping ranges: those that have a place
         p.splits = max(1, min(most_splits, wide_slots(D) / max(1, p.total * c.hkv)));
         p.split = id / max(1, p.total);
         if (p.split >= p.splits) return p;
@@ -701,7 +701,9 @@ WideGrid kv_attn_wide_grid(int dim, int hkv, int n_seqs, int max_new, int64_t ca
         const int64_t seen = (int64_t)a.window + kWideRows / a.group + 2 * kTile + (a.sinks > 0 ? a.sinks + kTile : 0);
         g.splits = (int)std::min<int64_t>(g.splits, (seen / kTile + kWideChunk - 1) / kWideChunk);
     }
-    g.items = (int64_t)row_blocks * hkv * n_seqs;
+    // behind a prefix every block is joined: the grid is of those that the rows can make
+    // (64 sequences, one with 2048 tokens: 716 pairs of 28672), and of blocks that have a state
+    g.items = (a.shared > 0 ? a.row_blocks : (int64_t)row_blocks * n_seqs) * hkv;
     g.few = g.splits + (a.shared > 0 ? (a.shared + a.prefix_run - 1) / a.prefix_run : 0) <= kJoinFew;
     g.join = g.splits == 1 && a.shared == 0 ? 0 : g.items * (g.few ? kWideRows / 8 : kWideRows);
     return g;

@@ -1,0 +1,35 @@
+"""Attention behind a shared prefix launches and asks for no more than the call's rows can
+need, however ragged the batch (host only, no GPU)."""
+import pytest
+
+from modgrad_amd import _lib
+from tests.test_kv_shared_plan_cpu import ask, cache_of
+
+LAUNCH = (2 ** 32 - 1) // 256  # work-groups of 256 threads that one launch counts
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_launches_are_of_the_rows(fmt, kind):
+    """One piece of 2048 tokens among 63 single tokens: 116 row blocks of 128 and 63 that are
+    not full at most, of 4 heads; not 64 times those of the piece."""
+    c = cache_of(64, 4, 128, 64, fmt, 400)
+    p = ask(c, 28, 2111, 2048, 12000, kind)
+    assert p.way != _lib.SHARED_PLAIN
+    pairs = (2111 * 7 // 128 + 64) * 4
+    assert p.own_groups <= pairs and p.join_groups <= 128 * pairs
+    even = ask(c, 28, 64 * 2048, 2048, 12000, kind)  # all of them as long
+    assert even.own_groups == 64 * 112 * 4
+
+
+@pytest.mark.parametrize("seqs,heads,hq,n,new,shared", [
+    (256, 8, 64, 8447, 8192, 12032), (256, 8, 64, 256 * 8192, 8192, 12032), (256, 8, 64, 256 * 4096, 4096, 20000),
+    (1024, 8, 128, 1024 * 900, 900, 200000), (1 << 18, 8, 8, 1 << 18, 1, 20000), (1 << 16, 16, 256, 1 << 16, 1, 64000),
+    (1 << 20, 1, 16, 1 << 20, 1, 8000), (512, 64, 64, 512 * 700, 700, 4096)])
+def test_launches_are_counted(seqs, heads, hq, n, new, shared):
+    for dim in (64, 128, 256):
+        for kind in (0, 1):
+            c = cache_of(seqs, heads, dim, 64, 0, -(-(shared + new) // 64) + 1)
+            p = ask(c, hq, n, new, shared, kind)
+            if p is not None and p.way != _lib.SHARED_PLAIN:
+                assert 0 < p.join_groups <= LAUNCH and 0 < p.own_groups <= LAUNCH

@@ -548,16 +548,17 @@ static int64_t most_tiles(int64_t cap, int max_new, const AttnArgs &a) {
 // `most` there are no more parts than `most` and one for every row.
 static int64_t most_states(int64_t rows) { return kAttnGroups + std::max<int64_t>(rows, kAttnGroups); }
 
-static size_t suffix_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity, bool shared) {
+// Room for the states of the sequences' own tiles; n_tokens counts behind a shared prefix.
+static size_t own_workspace(int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity, bool shared) {
     const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
     if (kv_attn_is_wide(dim, rows))
-        return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity, shared));
+        return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, n_tokens, max_new, capacity, shared));
     const int64_t all = (int64_t)n_seqs * blocks * hkv;
     return (size_t)most_states(all) * kRows * (dim + 2) * sizeof(float) + (size_t)all * sizeof(int2);
 }
 
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
-    return suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, false);
+    return own_workspace(dim, hq, hkv, n_seqs, 0, max_new, capacity, false);
 }
 
 // The prefix's part of a call.
@@ -704,7 +705,7 @@ size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, i
         floats = std::max(floats, (size_t)(p.states * hkv) * p.rows * (dim + 2));
     }
     if (floats == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
-    return whole16(suffix_workspace(dim, hq, hkv, n_seqs, max_new, capacity, true)) + floats * sizeof(float);
+    return whole16(own_workspace(dim, hq, hkv, n_seqs, n_tokens, max_new, capacity, true)) + floats * sizeof(float);
 }
 
 template <int D, int FMT>
@@ -742,7 +743,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
                                          x.shared_tokens);
         if (p.tiles > 0) {
             use_plan(a, p, c.n_seqs, c.n_tokens, c.max_new);
-            a.prefix = x.ws + whole16(suffix_workspace(dim, x.hq, c.hkv, c.n_seqs, c.max_new, cap, true)) / sizeof(float);
+            a.prefix = x.ws + whole16(own_workspace(dim, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap, true)) / sizeof(float);
             const hipError_t e = p.cuts > 0 ? hipSuccess : kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;
         }

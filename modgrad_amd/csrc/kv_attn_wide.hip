@@ -665,11 +665,13 @@ static void wide_plan(int dim, int group, int hkv, int n_seqs, int max_new, int6
     splits = std::min(splits, std::max(1, wide_slots(dim) / (row_blocks * hkv)));  // one sequence has all its blocks
 }
 
-size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap, bool shared) {
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, bool shared) {
     int row_blocks, splits;
     wide_plan(dim, group, hkv, n_seqs, max_new, cap, row_blocks, splits);
     if (splits == 1 && !shared) return 0;
-    return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
+    // behind a prefix every block has a state: as many as there are work-groups for
+    const int64_t blocks = shared ? most_row_blocks(group, n_seqs, n_tokens, max_new) : (int64_t)row_blocks * n_seqs;
+    return (size_t)(blocks * hkv * splits) * kWideRows * (dim + 2) * sizeof(float);
 }
 
 // LDS past 64 KiB has to be allowed, per device.

@@ -1,5 +1,7 @@
 """Attention behind a shared prefix launches and asks for no more than the call's rows can
 need, however ragged the batch (host only, no GPU)."""
+import ctypes
+
 import pytest
 
 from modgrad_amd import _lib
@@ -33,3 +35,18 @@ def test_launches_are_counted(seqs, heads, hq, n, new, shared):
             p = ask(c, hq, n, new, shared, kind)
             if p is not None and p.way != _lib.SHARED_PLAIN:
                 assert 0 < p.join_groups <= LAUNCH and 0 < p.own_groups <= LAUNCH
+
+
+def room(c, hq, n, new, shared):
+    return _lib.load().mgq_kv_attention_shared_workspace_bytes(ctypes.byref(c), hq, n, new, shared)
+
+
+def test_room_is_of_the_rows():
+    """The same batch: own states of its row blocks (47.7 MB) and the prefix's (62 MB at two
+    for each of 116 blocks), not the 1.9 GB of 64 such pieces."""
+    c = cache_of(64, 4, 128, 64, 0, 400)
+    assert room(c, 28, 2111, 2048, 12000) < 2.5e8
+    # a sequence's last block is seldom full: no less than the rows take
+    assert room(c, 28, 64 * 2048, 2048, 12000) >= 2 * 64 * 2048 * 28 * 130 * 4
+    c = cache_of(256, 8, 128, 64, 0, 400)
+    assert room(c, 64, 8447, 8192, 12032) < 1e9

@@ -576,6 +576,7 @@ static void use_plan(AttnArgs &a, const PrefixPlan &p, int n_seqs, int n_tokens,
     a.prefix_span = p.span;
     a.prefix_run = p.run;
     a.prefix_cuts = p.cuts;
+    a.prefix_two = !p.whole;
 }
 // Tiles of a part of a prefix, for few rows: `rows` blocks of them, `own` rows of the
 // sequences' own tiles in the same launch. By the time until all are done, in steps of a
@@ -642,7 +643,7 @@ static PrefixPlan prefix_cut(int dim, int fmt, int out_f16, int hq, int hkv, int
     p.whole = part <= run + kTwice;
     p.run = (int)(p.whole ? part : run);
     p.span = p.whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
-    p.states = 2 * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
+    p.states = (p.whole ? 1 : 2) * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
     return p;
 }
 // The launches of a call of few query rows of a sequence.

@@ -28,6 +28,7 @@ struct AttnArgs {
     // few query rows: blocks of kRows of them, each block's tiles in `prefix_cuts` parts of
     // prefix_run tiles (0: many rows)
     int prefix_cuts;
+    int prefix_two;  // whether a run may have tiles of two blocks, and so two states
     float *prefix;
     int row_blocks;  // of kWideRows, of all sequences, that the call's rows can make (no prefix: any number)
 };
@@ -286,13 +287,14 @@ __device__ __forceinline__ RowState row_state(const float *state, int rows, int 
     return {state + row * D, state + rows * D + 2 * row};
 }
 // A shared prefix's states. Many rows: run r of a kv head has state 2r for a row block
-// that an earlier run begins, 2r + 1 for one that it begins. Few: every part has one.
+// that an earlier run begins, 2r + 1 for one that it begins, and state r where runs are
+// parts of one block. Few: every part has one.
 inline int64_t prefix_runs(const AttnArgs &a) {
     return ((int64_t)a.prefix_blocks * a.prefix_span + a.prefix_run - 1) / a.prefix_run;
 }
 template <int D>
 __device__ __forceinline__ float *prefix_slot(const KvView &c, const AttnArgs &a, int h, int run, bool begins) {
-    return a.prefix + ((2 * (int64_t)run + begins) * c.hkv + h) * state_floats<D>(kWideRows);
+    return a.prefix + ((a.prefix_two ? 2 * (int64_t)run + begins : run) * c.hkv + h) * state_floats<D>(kWideRows);
 }
 template <int D>
 __device__ __forceinline__ float *prefix_part(const KvView &c, const AttnArgs &a, int h, int block, int k) {

@@ -50,3 +50,12 @@ def test_room_is_of_the_rows():
     assert room(c, 28, 64 * 2048, 2048, 12000) >= 2 * 64 * 2048 * 28 * 130 * 4
     c = cache_of(256, 8, 128, 64, 0, 400)
     assert room(c, 64, 8447, 8192, 12032) < 1e9
+
+
+def test_one_state_a_part():
+    """64 prompts of 2048 tokens: a state of each row block for the prefix, one for the own
+    tiles, 1.9 GB each."""
+    c = cache_of(64, 4, 128, 64, 0, 400)
+    states = 64 * 2048 * 28 * 130 * 4
+    assert ask(c, 28, 64 * 2048, 2048, 12000).way == _lib.SHARED_PARTS
+    assert 2 * states <= room(c, 28, 64 * 2048, 2048, 12000) < 2.02 * states

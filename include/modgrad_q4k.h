@@ -524,8 +524,13 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *
  * shared_tokens reaches past them; of a prefix that is not as described, what one of the
  * sequences' pages holds is used for others. Where row starts fall, so that ranges
  * overlap, rows of ranges past the first n_tokens rows' worth may be left as they are.
- * shared_tokens is not negative; past max_pages*page_tokens it counts as that. The workspace is of
- * mgq_kv_attention_shared_workspace_bytes (0: arguments that the call refuses). */
+ * shared_tokens is not negative; past max_pages*page_tokens it counts as that.
+ * The workspace is of mgq_kv_attention_shared_workspace_bytes (0: arguments that the
+ * call refuses). Prompts take two partial rows of head_dim + 2 floats for each of
+ * their query rows, where the plain call may need next to nothing. The size does not
+ * fall where n_tokens, max_new, shared_tokens or the cache's n_seqs grow, so that
+ * memory for the largest batch does for the others (up to 2^24 work-groups of the
+ * join; larger calls read plain and need less). */
 size_t mgq_kv_attention_shared_workspace_bytes(const mgq_kv_cache *cache, int n_q_heads,
                                                int n_tokens, int max_new, int shared_tokens);
 hipError_t launch_kv_attention_shared_ex(const mgq_kv_cache *cache, const float *q,

@@ -532,7 +532,8 @@ constexpr int64_t kThinRows = 448, kThinTiles = 15000;
 // (28 heads on 4 of 128, int8): 28 rows x 16 sequences of 4000 tokens 29 us here,
 // 46 there; 63 rows x 8 of 8000 56 and 51. Heads of 256: 24 rows 25 and 29, 48
 // rows 57 and 40.
-bool kv_attn_is_wide(int dim, int64_t rows) { return rows > (dim == 256 ? 32 : 48); }
+static int64_t token_rows(int dim) { return dim == 256 ? 32 : 48; }
+bool kv_attn_is_wide(int dim, int64_t rows) { return rows > token_rows(dim); }
 
 // Most tiles of a row: the table's, or the window's and those of the first tokens, or what
 // is behind a shared prefix (a sequence that does not see all of it has only its new
@@ -548,24 +549,21 @@ static int64_t most_tiles(int64_t cap, int max_new, const AttnArgs &a) {
 // `most` there are no more parts than `most` and one for every row.
 static int64_t most_states(int64_t rows) { return kAttnGroups + std::max<int64_t>(rows, kAttnGroups); }
 
-// Room for the states of the sequences' own tiles; n_tokens counts behind a shared prefix.
-static size_t own_workspace(int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity, bool shared) {
-    const int64_t rows = (int64_t)max_new * (hq / hkv), blocks = (rows + kRows - 1) / kRows;
-    if (kv_attn_is_wide(dim, rows))
-        return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, n_tokens, max_new, capacity, shared));
-    const int64_t all = (int64_t)n_seqs * blocks * hkv;
+// States of `rows` query rows of each sequence, and the lists of them.
+static size_t token_workspace(int dim, int hkv, int n_seqs, int64_t rows) {
+    const int64_t all = (int64_t)n_seqs * ((rows + kRows - 1) / kRows) * hkv;
     return (size_t)most_states(all) * kRows * (dim + 2) * sizeof(float) + (size_t)all * sizeof(int2);
 }
 
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity) {
-    return own_workspace(dim, hq, hkv, n_seqs, 0, max_new, capacity, false);
+    const int64_t rows = (int64_t)max_new * (hq / hkv);
+    if (!kv_attn_is_wide(dim, rows)) return token_workspace(dim, hkv, n_seqs, rows);
+    return std::max<size_t>(16, kv_attn_wide_workspace(dim, hq / hkv, hkv, n_seqs, max_new, capacity));
 }
 
 // The prefix's part of a call.
 struct PrefixPlan {
     int tiles, blocks, span, run, cuts;
-    int64_t states;  // of a kv head
-    int rows;        // of a state
     bool whole;      // many rows: equal parts of each block, not runs over all
 };
 // ... as the kernels and the grids see it, but for where its states lie.
@@ -606,6 +604,10 @@ static int thin_run(int dim, int tiles, int64_t rows, int64_t own) {
     }
     return best;
 }
+// Work-groups of a kv head that are resident at once.
+static int64_t prefix_groups(int dim, int fmt, int out_f16, int hkv) {
+    return std::max(1, kv_attn_prefix_slots(dim, fmt, out_f16) / hkv);
+}
 static PrefixPlan prefix_cut(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
                              int64_t capacity, int shared_tokens) {
     PrefixPlan p = {};
@@ -624,26 +626,22 @@ static PrefixPlan prefix_cut(int dim, int fmt, int out_f16, int hq, int hkv, int
         p.run = thin_run(dim, p.tiles, (int64_t)p.blocks * hkv,
                          (int64_t)n_seqs * hkv * (((int64_t)max_new * (hq / hkv) + kRows - 1) / kRows));
         p.cuts = (p.tiles + p.run - 1) / p.run;
-        p.states = (int64_t)p.blocks * p.cuts;
-        p.rows = kRows;
         return p;
     }
     p.blocks = (int)((rows + kWideRows - 1) / kWideRows);
-    p.rows = kWideRows;
     // Runs of equal length over all blocks fill the chip best, but a run with tiles of two
     // blocks begins twice (rows, page ids, first loads: some 6 us, as long as kTwice
     // tiles); equal parts of each block are longer where the work-groups are no multiple
     // of the blocks. 4 blocks of 187 tiles on 63 groups: runs 45 us, parts 37; 33 blocks of
     // 156 on 128: parts 147, runs 137.
     constexpr int kTwice = 3;
-    const int64_t groups = std::max(1, kv_attn_prefix_slots(dim, fmt, out_f16) / hkv);
+    const int64_t groups = prefix_groups(dim, fmt, out_f16, hkv);
     const int64_t run = std::min<int64_t>(p.tiles, ((int64_t)p.blocks * p.tiles + groups - 1) / groups);
     const int64_t parts = std::min<int64_t>(p.tiles, std::max<int64_t>(1, groups / p.blocks));
     const int64_t part = (p.tiles + parts - 1) / parts;
     p.whole = part <= run + kTwice;
     p.run = (int)(p.whole ? part : run);
     p.span = p.whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
-    p.states = (p.whole ? 1 : 2) * (((int64_t)p.blocks * p.span + p.run - 1) / p.run);
     return p;
 }
 // The launches of a call of few query rows of a sequence.
@@ -698,15 +696,40 @@ SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, i
 
 static size_t whole16(size_t n) { return (n + 15) / 16 * 16; }
 
+// The workspace behind a shared prefix: room for the states of the sequences' own tiles, then
+// for the prefix's. Each is a bound that does not fall where a call grows, so that memory for
+// the largest batch does for any other; plans themselves have more states here, fewer there.
+static size_t own_room(int dim, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity, bool shared) {
+    const int64_t rows = (int64_t)max_new * (hq / hkv);
+    size_t n = token_workspace(dim, hkv, n_seqs, std::min(rows, token_rows(dim)));
+    if (kv_attn_is_wide(dim, rows))
+        n = std::max(n, kv_attn_wide_room(dim, hq / hkv, hkv, n_seqs, n_tokens, max_new, capacity, shared));
+    return whole16(n);
+}
+// Few rows: a part has a state, and there is one of each block or no more than twice the
+// slots. Many: a part of a block has one, and there is one or no more than the groups; a run
+// two, and there are no more than the groups.
+static size_t prefix_room(const PrefixPlan &p, int dim, int fmt, int group, int hkv, int n_tokens) {
+    const int64_t rows = (int64_t)n_tokens * group, few = (std::min(rows, kThinRows) + kRows - 1) / kRows * hkv;
+    int64_t lines = std::max(few, std::min(2 * (int64_t)attn_slots(dim), few * ((p.tiles + kPartTiles - 1) / kPartTiles))) * kRows;
+    if (p.cuts == 0) {
+        const int64_t blocks = p.blocks;
+        for (int f16 = 0; f16 < 2; ++f16) {
+            const int64_t groups = prefix_groups(dim, fmt, f16, hkv);
+            lines = std::max(lines, std::max(blocks, 2 * std::min(groups, blocks * p.tiles)) * hkv * kWideRows);
+        }
+    }
+    return (size_t)lines * (dim + 2) * sizeof(float);
+}
+
 size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
                                 int shared_tokens) {
-    size_t floats = 0;  // for either type of result
+    size_t prefix = 0;  // for either type of result
     for (int f16 = 0; f16 < 2; ++f16) {
         const PrefixPlan p = prefix_plan(dim, fmt, f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
-        floats = std::max(floats, (size_t)(p.states * hkv) * p.rows * (dim + 2));
+        if (p.tiles > 0) prefix = std::max(prefix, prefix_room(p, dim, fmt, hq / hkv, hkv, n_tokens));
     }
-    if (floats == 0) return kv_attn_workspace(dim, hq, hkv, n_seqs, max_new, capacity);
-    return whole16(own_workspace(dim, hq, hkv, n_seqs, n_tokens, max_new, capacity, true)) + floats * sizeof(float);
+    return own_room(dim, hq, hkv, n_seqs, n_tokens, max_new, capacity, prefix > 0) + prefix;
 }
 
 template <int D, int FMT>
@@ -744,7 +767,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
                                          x.shared_tokens);
         if (p.tiles > 0) {
             use_plan(a, p, c.n_seqs, c.n_tokens, c.max_new);
-            a.prefix = x.ws + whole16(own_workspace(dim, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap, true)) / sizeof(float);
+            a.prefix = x.ws + own_room(dim, x.hq, c.hkv, c.n_seqs, c.n_tokens, c.max_new, cap, true) / sizeof(float);
             const hipError_t e = p.cuts > 0 ? hipSuccess : kv_attn_prefix_launch(c, dim, fmt, a, stream);
             if (e != hipSuccess) return e;
         }

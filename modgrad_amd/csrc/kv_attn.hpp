@@ -96,7 +96,9 @@ __device__ __forceinline__ bool vanishing(float top, float ref) { return top < r
 
 // kv_attn_wide.hip: many query rows of a sequence.
 hipError_t kv_attn_wide_launch(const KvView &c, int dim, int fmt, const AttnArgs &a, hipStream_t stream);
-size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, bool shared);
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap);
+// ... and of that of any call no larger than this one, behind a shared prefix or not.
+size_t kv_attn_wide_room(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, bool shared);
 // Its launches: row blocks of all kv heads, splits of each, work-groups of the join (0: none)
 // and which of the two joins that is.
 struct WideGrid {

@@ -665,13 +665,22 @@ static void wide_plan(int dim, int group, int hkv, int n_seqs, int max_new, int6
     splits = std::min(splits, std::max(1, wide_slots(dim) / (row_blocks * hkv)));  // one sequence has all its blocks
 }
 
-size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, bool shared) {
+size_t kv_attn_wide_workspace(int dim, int group, int hkv, int n_seqs, int max_new, int64_t cap) {
     int row_blocks, splits;
     wide_plan(dim, group, hkv, n_seqs, max_new, cap, row_blocks, splits);
-    if (splits == 1 && !shared) return 0;
-    // behind a prefix every block has a state: as many as there are work-groups for
-    const int64_t blocks = shared ? most_row_blocks(group, n_seqs, n_tokens, max_new) : (int64_t)row_blocks * n_seqs;
-    return (size_t)(blocks * hkv * splits) * kWideRows * (dim + 2) * sizeof(float);
+    if (splits == 1) return 0;
+    return (size_t)row_blocks * hkv * n_seqs * splits * kWideRows * (dim + 2) * sizeof(float);
+}
+
+// A split block's states are no more than twice the slots, nor a whole one's (behind a prefix
+// they have one each) than the blocks: neither falls with the call.
+size_t kv_attn_wide_room(int dim, int group, int hkv, int n_seqs, int n_tokens, int max_new, int64_t cap, bool shared) {
+    int row_blocks, splits;
+    wide_plan(dim, group, hkv, n_seqs, max_new, cap, row_blocks, splits);
+    const int64_t tiles = (cap + kTile - 1) / kTile, most = (tiles + kWideChunk - 1) / kWideChunk;
+    int64_t states = most > 1 ? std::min<int64_t>(2 * wide_slots(dim), (int64_t)row_blocks * hkv * n_seqs * most) : 0;
+    if (shared) states = std::max(states, most_row_blocks(group, n_seqs, n_tokens, max_new) * hkv);
+    return (size_t)states * kWideRows * (dim + 2) * sizeof(float);
 }
 
 // LDS past 64 KiB has to be allowed, per device.

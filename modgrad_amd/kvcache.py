@@ -429,7 +429,8 @@ class KvCache:
                        n_q_heads, n_tokens, max_new, stream)
 
     def attention_workspace(self, n_q_heads: int, n_tokens: int, max_new: int, shared: int = 0):
-        """A device tensor for attend's workspace (any call with these sizes)."""
+        """A device tensor for attend's workspace (any call with these sizes; with
+        `shared`, any with no more sequences, tokens, new and shared tokens)."""
         if shared:
             n = kern.kv_attention_shared_workspace_bytes(self._ref, n_q_heads, n_tokens, max_new, shared)
         else:

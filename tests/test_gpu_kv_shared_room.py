@@ -58,3 +58,25 @@ def test_ranges_that_overlap(new):
     got = host(out)
     assert np.all(got[new] == 7) and np.all(host(guard[ws.nbytes:]) == 90)
     check(got[:new].reshape(want.shape), want, tol, False)
+
+
+def test_one_workspace_for_every_batch():
+    """Memory for the largest batch, at its exact size, does for smaller ones on each way; what
+    lies behind it stays."""
+    import torch
+    note("shared: one workspace for every batch")
+    rng = np.random.default_rng(53)
+    seqs, prefix, heads, group, dim = 40, 1344, 4, 4, 64
+    hq, own = heads * group, [60] * seqs
+    both = build(rng, prefix, own, heads, dim, 64, "i8")
+    n = both.gpu.attention_workspace(hq, seqs * 60, 60, shared=prefix).nbytes
+    guard = torch.empty(n + 4096, dtype=torch.uint8, device="cuda")
+    for new, shared in (([60] * seqs, prefix), ([1] * seqs, prefix), ([3] * seqs, 1300), ([1, 0, 60] + [0] * 37, 700),
+                        ([7] * seqs, 64), ([1] * 20 + [0] * 20, prefix)):
+        guard.fill_(90)
+        lens = [prefix + 60 if m else 0 for m in new]
+        q = (2 * rng.standard_normal((sum(new), hq, dim))).astype(np.float32)
+        want, tol = ref.attend(both.ref, q, lens, new, dim ** -0.5)
+        both.call(lens, new)
+        check(run(both, q, new, hq, dim, False, shared, workspace=guard[:n]), want, tol, False)
+        assert bool((guard[n:] == 90).all())

@@ -59,3 +59,39 @@ def test_one_state_a_part():
     states = 64 * 2048 * 28 * 130 * 4
     assert ask(c, 28, 64 * 2048, 2048, 12000).way == _lib.SHARED_PARTS
     assert 2 * states <= room(c, 28, 64 * 2048, 2048, 12000) < 2.02 * states
+
+
+def needed(p, heads, dim, wide):
+    """States that a call with this plan has, at least."""
+    cuts = -(-p.tiles // p.run) if p.run else 0
+    prefix = {_lib.SHARED_PLAIN: 0, _lib.SHARED_FEW: 16 * p.blocks * cuts, _lib.SHARED_PARTS: 128 * p.blocks * cuts,
+              _lib.SHARED_RUNS: 256 * -(-p.blocks * p.tiles // max(1, p.run))}[p.way]
+    own = 128 * p.own_groups if wide and p.join_groups else 0
+    return (prefix * heads + own) * (dim + 2) * 4
+
+
+def test_room_does_not_fall():
+    """Memory for a batch does for every smaller one: fewer tokens, new tokens, sequences or
+    shared tokens; and is enough for the states of the plan."""
+    import random
+    rng = random.Random(5)
+    ways = set()
+    for _ in range(6000):
+        dim, fmt = rng.choice((64, 96, 128, 256)), rng.randrange(2)
+        heads, group = rng.choice((1, 2, 4, 8, 16)), rng.choice((1, 2, 3, 7, 8, 16))
+        size = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))  # noqa: E731
+        seqs, new, shared = size(1, 300), size(1, 3000), size(1, 40000)
+        n = max(new, rng.randrange(seqs, seqs * new + 1))
+        low = lambda v: rng.choice((v, v, rng.randrange(1, v + 1), max(1, v - 1)))  # noqa: E731
+        seqs2, new2, shared2 = low(seqs), low(new), low(shared)
+        n2 = max(new2, low(n))
+        large, small = (cache_of(b, heads, dim, 64, fmt, 40000 // 64 + 40) for b in (seqs, seqs2))
+        hq = heads * group
+        a, b = room(large, hq, n, new, shared), room(small, hq, n2, new2, shared2)
+        assert 0 < b <= a, ((seqs, n, new, shared), (seqs2, n2, new2, shared2), heads, group, dim, fmt)
+        plain = _lib.load().mgq_kv_attention_workspace_bytes(ctypes.byref(large), hq, new)
+        for kind in (0, 1):
+            p = ask(large, hq, n, new, shared, kind)
+            ways.add(p.way)
+            assert a >= plain and a >= needed(p, heads, dim, new * group > (32 if dim == 256 else 48))
+    assert ways == {0, 1, 2, 3}

@@ -55,6 +55,12 @@ def _on_device(device) -> None:
                                       f"cuda:{cuda.current_device()}")
 
 
+def _on_gpu(device) -> None:
+    """A recorded launch goes to the device that is current then; host memory is never there."""
+    if device is not None and device.type != "cuda":
+        raise BackendError("Runtime", f"tensors on {device}")
+
+
 FORMATS = {"i8": _lib.KV_I8, "e4m3": _lib.KV_E4M3}
 
 
@@ -231,6 +237,7 @@ class RopeTable:
            x_stride: int | None = None, y_stride: int | None = None, axes: RopeAxes | None = None,
            pos_stride: int | None = None) -> "_lib.OpDesc":
         """apply as a descriptor of an op chain (q4k.Chain.from_ops)."""
+        _on_gpu(self.device)
         row = n_heads * head_dim
         if axes is not None:
             return _op(_lib.OP_ROPE_AXES, _lib.RopeAxesArgs(
@@ -481,6 +488,9 @@ class KvCache:
                   q: int = 0, q_stride: int = 0, q_out: int | None = None,
                   q_out_stride: int | None = None, n_q_heads: int = 0, axes: RopeAxes | None = None, pos: int = 0,
                   pos_stride: int | None = None) -> "_lib.OpDesc":
+        _on_gpu(self.device)
+        if rope is not None and rope.device != self.device:
+            raise BackendError("Runtime", f"rope table on {rope.device}, cache on {self.device}")
         args = _lib.KvAppendArgs(
             self.desc, _lib.Rope() if rope is None else rope.desc, k, v, q or None,
             (q if q_out is None else q_out) or None, kv_stride, q_stride,
@@ -497,6 +507,7 @@ class KvCache:
                   softcap: float = 0.0, window: int = 0, out_f16: bool = False, sinks: int = 0,
                   shared: int = 0) -> "_lib.OpDesc":
         """The workspace has to outlive the chain."""
+        _on_gpu(self.device)
         _workspace(workspace, self.device)
         args = _lib.KvAttentionArgs(
             self.desc, q, out, workspace.data_ptr(), workspace.numel() * workspace.element_size(),

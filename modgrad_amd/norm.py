@@ -16,7 +16,7 @@ import ctypes
 
 from . import _lib
 from .q4k import BackendError, _torch, kern
-from .kvcache import _elsewhere, _on_device, _op
+from .kvcache import _elsewhere, _on_device, _on_gpu, _op
 
 
 class BlockNorm:
@@ -71,6 +71,7 @@ class BlockNorm:
            gate: int = 0, gate_stride: int | None = None, h_stride: int | None = None, x_stride: int | None = None,
            h_out_stride: int | None = None, y_stride: int | None = None) -> "_lib.OpDesc":
         """apply as a descriptor of an op chain (q4k.Chain.from_ops)."""
+        _on_gpu(self.device)
         h, hs, x, xs, gate, gs, ho, hos, y, ys = self._rows(h, x, h_out, y, gate, gate_stride,
                                                             (h_stride, x_stride, h_out_stride, y_stride))
         return _op(_lib.OP_BLOCK_NORM, _lib.BlockNormArgs(

@@ -15,6 +15,7 @@ C ABI.
     cache.set_lengths([n0 + 1, n1 + 1, ...])           # the new tokens included
     cache.append(k, v, kv_stride, 8, 1, rope=rope, q=q, q_stride=qs, n_q_heads=28)
     cache.attend(q, qs, 28, out, 28 * 128, 8, 1)
+    cache.share(1, 0, 4096)                            # slot 1 behind slot 0's first 4096 tokens
 
 Addresses are device pointers as in modgrad_amd.q4k.kern; torch only allocates.
 `stream` is a torch stream, None the null stream; page tables and lengths are
@@ -305,7 +306,8 @@ class KvCache:
         self._own_cu = None
         self._ref = ctypes.byref(self.desc)
         self._free = None
-        self._held = [[] for _ in range(self.n_seqs)]
+        self._held = [[] for _ in range(self.n_seqs)]  # pages of each slot, None where given back
+        self._users = [0] * self.n_pages               # slots that have a page
 
     @classmethod
     def wrap(cls, k, v, k_scale, v_scale, page_table, seq_len, cu_tokens=None,
@@ -319,7 +321,8 @@ class KvCache:
     @classmethod
     def new(cls, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, n_seqs: int,
             max_pages: int, fmt: str = "i8", stream=None) -> "KvCache":
-        """An empty cache whose pages reserve() and release() hand out."""
+        """An empty cache whose pages reserve(), share(), give_back() and release() hand
+        out and take back."""
         torch = _torch()
         with _stream(stream):
             try:
@@ -347,27 +350,73 @@ class KvCache:
         if short > len(self._free):
             raise BackendError("OutOfMemory", f"reserve: {short} pages, {len(self._free)} free")
 
+    def _own_pages(self, what: str, *seqs) -> None:
+        if self._free is None:
+            raise BackendError("Unsupported", f"{what}: the cache wraps tables of the caller's")
+        for seq in seqs:
+            if not 0 <= seq < self.n_seqs:
+                raise BackendError("Runtime", f"{what}: sequence {seq}")
+
+    def _write(self, seq: int, first: int, pages, stream) -> None:
+        with _stream(stream):
+            self.page_table[seq, first: first + len(pages)] = _torch().tensor(pages, dtype=_torch().int32)
+
+    def _leave(self, pages) -> None:
+        """Pages that one slot less has; those that none has are free."""
+        for p in pages:
+            self._users[p] -= 1
+        self._free += [p for p in pages if self._users[p] == 0]
+
     def reserve(self, seq: int, n_tokens: int, stream=None) -> None:
         """Pages for the first n_tokens positions of slot `seq`."""
-        if self._free is None:
-            raise BackendError("Unsupported", "reserve: the cache wraps tables of the caller's")
-        if not 0 <= seq < self.n_seqs or n_tokens < 0:
+        self._own_pages("reserve", seq)
+        if n_tokens < 0:
             raise BackendError("Runtime", f"reserve: {n_tokens} tokens of sequence {seq}")
         short, held = self._short(seq, n_tokens), self._held[seq]
         self._afford(short)
         if short:
             new = [self._free.pop() for _ in range(short)]
-            with _stream(stream):
-                self.page_table[seq, len(held): len(held) + short] = _torch().tensor(new, dtype=_torch().int32)
+            for p in new:
+                self._users[p] = 1
+            self._write(seq, len(held), new, stream)
             held += new
 
+    def share(self, seq: int, other: int, n_tokens: int, stream=None) -> None:
+        """Slot `seq`, which has no pages yet, begins with those of the first n_tokens
+        positions (whole pages) of slot `other`: what attend(shared=n_tokens) reads once for
+        both. A page is free again when no slot has it; new tokens go behind it."""
+        self._own_pages("share", seq, other)
+        n = n_tokens // self.page_tokens
+        pages = self._held[other][:max(n, 0)]
+        if seq == other or self._held[seq] or n_tokens < 0 or n_tokens % self.page_tokens or len(pages) < n \
+                or None in pages:
+            raise BackendError("Runtime", f"share: {n_tokens} tokens of sequence {other} with {seq}: whole pages that "
+                                          "the one has and the other has none of")
+        for p in pages:
+            self._users[p] += 1
+        self._held[seq] = pages
+        if pages:
+            self._write(seq, 0, pages, stream)
+
+    def give_back(self, seq: int, first: int, end: int, stream=None) -> None:
+        """Pages of slot `seq` that lie in positions first .. end-1, which no call looks at
+        any more (behind the first tokens and ahead of a window)."""
+        self._own_pages("give_back", seq)
+        if not 0 <= first <= end:
+            raise BackendError("Runtime", f"give_back: positions {first} to {end}")
+        held = self._held[seq]
+        slots = range(-(-first // self.page_tokens), min(end // self.page_tokens, len(held)))
+        self._leave([held[i] for i in slots if held[i] is not None])
+        for i in slots:
+            held[i] = None
+        if slots:
+            self._write(seq, slots[0], [-1] * len(slots), stream)
+
     def release(self, seq: int, stream=None) -> None:
-        """Gives the pages of slot `seq` back and leaves it idle."""
-        if self._free is None:
-            raise BackendError("Unsupported", "release: the cache wraps tables of the caller's")
-        if not 0 <= seq < self.n_seqs:
-            raise BackendError("Runtime", f"release: sequence {seq}")
-        self._free += self._held[seq]
+        """Gives the pages of slot `seq` back, those that other slots have to them, and
+        leaves it idle."""
+        self._own_pages("release", seq)
+        self._leave([p for p in self._held[seq] if p is not None])
         self._held[seq] = []
         with _stream(stream):
             self.page_table[seq] = -1
@@ -375,7 +424,8 @@ class KvCache:
 
     def set_lengths(self, lengths, new=None, stream=None) -> None:
         """Tokens of every slot with the next call's new ones, and how many of
-        them are new (None: one each); pages are reserved for them. The tensors
+        them are new (None: one each); pages are reserved for them. New tokens do
+        not lie in pages that are shared or were given back. The tensors
         stay in place, so that recorded calls replay on the new values: one that
         was recorded with counts takes any that fit its n_tokens and max_new, one
         that was recorded with one each stays at that."""
@@ -388,6 +438,11 @@ class KvCache:
             if not 0 <= m <= n < 2 ** 30:
                 raise BackendError("Runtime", f"set_lengths: {n} tokens, {m} of them new")
         if self._free is not None:
+            for b, (n, m) in enumerate(zip(lengths, counts or [min(n, 1) for n in lengths])):
+                for p in self._held[b][(n - m) // self.page_tokens: -(-n // self.page_tokens)] if m else ():
+                    if p is None or self._users[p] > 1:
+                        raise BackendError("Runtime", f"set_lengths: new tokens {n - m} to {n} of sequence {b} in a page "
+                                                      f"that {'was given back' if p is None else 'others read'}")
             self._afford(sum(self._short(b, n) for b, n in enumerate(lengths)))  # all of them or none
             for b, n in enumerate(lengths):
                 self.reserve(b, n, stream)

@@ -518,11 +518,16 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *
 
 /* launch_kv_attention_ex, without a window, for sequences that begin with the same
  * pages: the first shared_tokens positions of every sequence with rows in the call lie
- * in the same pages, in the same order. Their whole tiles of 64 tokens are read once
- * for all rows, the rest sequence by sequence, and the two joined in f32 as the parts
- * of a long sequence are. A row sees only its own and earlier positions also where
- * shared_tokens reaches past them; of a prefix that is not as described, what one of the
- * sequences' pages holds is used for others. Where row starts fall, so that ranges
+ * in the same pages, in the same order. Their whole tiles of 64 tokens are gone through
+ * once for each 16 or 128 query rows of a kv head, whichever sequences they are of, the
+ * rest sequence by sequence, and the two joined in f32 as the parts of a long sequence
+ * are; short prefixes, by every sequence (mgq_kv_attention_shared_plan tells). That is
+ * worth it for sequences of few query rows each: those that fill blocks of 128 by
+ * themselves, or a single sequence, are faster in the plain call. A row sees only its own
+ * and earlier positions also where shared_tokens reaches past them. Nothing else limits a
+ * row: a page that the table does not name has to be missing in every sequence's list; of
+ * a prefix that is not as described, what one of the sequences' pages holds is used for
+ * others. Where row starts fall, so that ranges
  * overlap, rows of ranges past the first n_tokens rows' worth may be left as they are.
  * shared_tokens is not negative; past max_pages*page_tokens it counts as that.
  * The workspace is of mgq_kv_attention_shared_workspace_bytes (0: arguments that the

@@ -13,7 +13,9 @@
 // Many rows are bound by their bytes: 256 threads of 4 quads a row of 3584 (206 MB, 46 us,
 // 4.5 TB/s; a copy reaches 5.1), a wavefront a row up to 1024 values (16384 rows of 896:
 // 4.8 TB/s). 512 threads of 2 quads: 50 us; registers for 5 or 6 wavefronts a SIMD
-// instead of 4: 65 and 104 (spills). Few rows are bound by latency: a quad a thread.
+// instead of 4: 65 and 104 (spills). Rows that end inside a quad cost more: 4096 of 3585
+// values 63 us (2 wavefronts a SIMD), of 12001 256 (36 registers spilled; 12000: 163). Few
+// rows are bound by latency: a quad a thread.
 #include "q4k_device.hpp"
 #include "q4k_launch.hpp"
 

@@ -13,8 +13,10 @@
 // rotated by further work-groups of the same launch. A single token per sequence
 // is bound by latency (length -> page -> old scale -> store: 64 sequences, 28 + 2*4
 // heads of 128, 4.8 us); a prompt by its floats, mostly the queries' (4096 tokens, 162 MB:
-// 31-35 us, 4.9 TB/s). At positions of several axes the same: 33 single tokens 4.7 us, 3
-// prompts of 4200 tokens together on e4m3 34.
+// 31-35 us, 4.9 TB/s). At positions of several axes: 33 single tokens 4.7 us; 3 ragged
+// prompts of 3593 tokens together on e4m3 34, 3.6 TB/s (their query work-groups are as many as
+// for three prompts of the longest one's 2500, so half of 3282 have nothing to do, and
+// positions and table entries are read again for each head).
 #include "kv_device.hpp"
 #include "kv_launch.hpp"
 

@@ -524,7 +524,8 @@ static int attn_slots(int dim) { return dim == 256 ? kAttnGroups / 2 : kAttnGrou
 // over all kv heads. Above, kv_attn_prefix_kernel has fewer, dearer tiles and a launch of
 // its own. Measured (28 heads on 4 of 128, here and there; us a call): 16 tokens behind
 // 12000 28 and 38, 32 behind 12000 37 and 45, 48 behind 12000 (15700 tiles) 52 and 48, 64
-// behind 12000 63 and 59.
+// behind 12000 63 and 59. That is int8 with f32 results; e4m3 and other heads, whose tiles
+// cost other amounts, go by the same two numbers and were not measured around them.
 constexpr int64_t kThinRows = 448, kThinTiles = 15000;
 
 // Query rows of a kv head up to which this kernel takes the call, in blocks of

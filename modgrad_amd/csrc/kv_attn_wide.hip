@@ -537,8 +537,10 @@ __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FM
 //
 // Bound like the prompt's by the softmax's vector work and, where runs are short, by their
 // start (limits, query rows, page ids, first loads: 5 us) and the states: 64 tokens of 28 heads behind
-// 12000, int8 with f32 results, 12 tiles a work-group: 36-38 us, 2.1 us a tile; 530
+// 12000, int8 with f32 results, 12 tiles a work-group: 36-38 us, 2.1 us a tile; 598
 // tokens behind 10000 with f16 results, 41 tiles: 137-140 us (87 GFLOP, 630 TFLOP/s).
+// Heads of 128 on e4m3 spill 18 registers (the plain kernel 6 to 9), on int8 with f16 results 3:
+// those two calls on e4m3 take 66 and 190 us in all, on int8 61-65 and 156.
 template <int D, int FMT, bool LO>
 __global__ __launch_bounds__((WideShape<D, FMT, LO>::kThreads), (WideShape<D, FMT, LO>::kPerSimd)) void kv_attn_prefix_kernel(KvView c, AttnArgs a) {
     typedef WideShape<D, FMT, LO> W;

@@ -484,7 +484,9 @@ hipError_t launch_kv_dequant_ex(const mgq_kv_cache *cache, const int *pages, int
  * passes f32, and for sizes that the kernels cannot count: 2^28 and more rows
  * max_new*n_q_heads/n_kv_heads of a kv head; 2^27 and more groups of 16 of them,
  * over all kv heads and sequences; and, for up to 48 of them, more than 2^31 - 512
- * pairs of such a group and 64 tokens with every table full. A query row with a NaN
+ * pairs of such a group and 64 tokens with every table full, or 2^24 and more rows of
+ * all kv heads and sequences (past 16 of each, in whole groups) that can see more than 512
+ * tokens. A query row with a NaN
  * or infinity gives a row of NaN if it sees anything. Scales, and values of tokens
  * that a sequence holds, are taken as finite, as an append leaves them; what lies
  * behind its last token may be anything. Statistics and sums are f32. The queries
@@ -527,8 +529,8 @@ hipError_t launch_kv_attention_sinks_ex(const mgq_kv_cache *cache, const float *
  * and earlier positions also where shared_tokens reaches past them. Nothing else limits a
  * row: a page that the table does not name has to be missing in every sequence's list; of
  * a prefix that is not as described, what one of the sequences' pages holds is used for
- * others. Where row starts fall, so that ranges
- * overlap, rows of ranges past the first n_tokens rows' worth may be left as they are.
+ * others. Row starts must not fall: rows that two ranges hold may be of neither
+ * sequence, or be left as they are.
  * shared_tokens is not negative; past max_pages*page_tokens it counts as that.
  * The workspace is of mgq_kv_attention_shared_workspace_bytes (0: arguments that the
  * call refuses). Prompts take two partial rows of head_dim + 2 floats for each of

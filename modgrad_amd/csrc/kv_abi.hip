@@ -157,6 +157,9 @@ hipError_t attn_check(const mgq_kv_cache *c, const float *q, int64_t qs, int hq,
     if (!std::isfinite(scale * 1.4426950408889634f) || !std::isfinite(softcap * 1.4426950408889634f) ||
         (softcap > 0.0f && !std::isfinite(scale / softcap)))
         return hipErrorInvalidValue;
+    if (!kv_attn_join_fits(c->head_dim, hq / c->n_kv_heads, c->n_kv_heads, c->n_seqs, max_new,
+                           (int64_t)c->max_pages * c->page_tokens, window, sinks))
+        return hipErrorInvalidValue;
     const size_t need = shared > 0 ? mgq_kv_attention_shared_workspace_bytes(c, hq, n_tokens, max_new, shared)
                                    : mgq_kv_attention_workspace_bytes(c, hq, max_new);
     if (need == 0 || bad16(ws) || bytes < need) return hipErrorInvalidValue;

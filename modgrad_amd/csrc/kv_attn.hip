@@ -645,6 +645,11 @@ static PrefixPlan prefix_cut(int dim, int fmt, int out_f16, int hq, int hkv, int
     p.span = p.whole ? (p.tiles + p.run - 1) / p.run * p.run : p.tiles;
     return p;
 }
+static void use_window(AttnArgs &a, int window, int sinks) {
+    a.window = std::min(window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
+    a.sinks = a.window > 0 ? std::min(sinks, 1 << 30) : 0;
+}
+
 // The launches of a call of few query rows of a sequence.
 struct TokenGrid {
     int max_blocks, block_rows, states;  // row blocks of a sequence, rows of a block, states in the workspace
@@ -663,6 +668,8 @@ static TokenGrid token_grid(int dim, int hkv, int n_seqs, int max_new, int64_t c
     return g;
 }
 
+// Work-groups of 256 threads that pass what one launch counts.
+constexpr int64_t kLaunchGroups = (INT64_C(1) << 32) / 256;
 // Work-groups on the sequences' own tiles, and of the join, of a call with such a plan.
 struct OwnGrid {
     int64_t groups, join;
@@ -683,8 +690,17 @@ static OwnGrid own_grid(const PrefixPlan &p, int dim, int hq, int hkv, int n_seq
 static PrefixPlan prefix_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
                               int64_t capacity, int shared_tokens) {
     const PrefixPlan p = prefix_cut(dim, fmt, out_f16, hq, hkv, n_seqs, n_tokens, max_new, capacity, shared_tokens);
-    const bool fits = own_grid(p, dim, hq, hkv, n_seqs, n_tokens, max_new, capacity).join < (INT64_C(1) << 32) / 256;
+    const bool fits = own_grid(p, dim, hq, hkv, n_seqs, n_tokens, max_new, capacity).join < kLaunchGroups;
     return fits ? p : PrefixPlan{};
+}
+
+bool kv_attn_join_fits(int dim, int group, int hkv, int n_seqs, int max_new, int64_t capacity, int window, int sinks) {
+    const int64_t rows = (int64_t)max_new * group;
+    if (kv_attn_is_wide(dim, rows) || (int64_t)n_seqs * hkv * (rows + kRows) < kLaunchGroups) return true;
+    AttnArgs a = {};
+    a.group = group;
+    use_window(a, window, sinks);
+    return token_grid(dim, hkv, n_seqs, max_new, capacity, a).join < kLaunchGroups;
 }
 
 SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,
@@ -758,8 +774,7 @@ hipError_t kv_attn_launch(const KvView &c, int dim, int fmt, const KvAttn &x, hi
     a.out_f16 = x.out_f16;
     a.scale = x.softcap > 0.0f ? x.scale / x.softcap : x.scale * 1.4426950408889634f;
     a.softcap = x.softcap * 1.4426950408889634f;
-    a.window = std::min(x.window, 1 << 30);  // all of any sequence; pos0 - window stays in 32 bits
-    a.sinks = a.window > 0 ? std::min(x.sinks, 1 << 30) : 0;
+    use_window(a, x.window, x.sinks);
     a.ws = x.ws;
     use_plan(a, PrefixPlan{}, c.n_seqs, c.n_tokens, c.max_new);
     if (x.shared_tokens > 0) {

@@ -50,6 +50,8 @@ bool kv_attn_is_wide(int dim, int64_t rows);
 size_t kv_attn_workspace(int dim, int hq, int hkv, int n_seqs, int max_new, int64_t capacity);
 size_t kv_attn_shared_workspace(int dim, int fmt, int hq, int hkv, int n_seqs, int n_tokens, int max_new, int64_t capacity,
                                 int shared_tokens);
+// Whether one launch counts the join of a call that reads every sequence by itself.
+bool kv_attn_join_fits(int dim, int group, int hkv, int n_seqs, int max_new, int64_t capacity, int window, int sinks);
 // How a call behind a shared prefix is gone about: mgq_kv_shared_plan.
 typedef mgq_kv_shared_plan SharedPlan;
 SharedPlan kv_attn_shared_plan(int dim, int fmt, int out_f16, int hq, int hkv, int n_seqs, int n_tokens, int max_new,

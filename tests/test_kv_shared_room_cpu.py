@@ -6,6 +6,7 @@ import pytest
 
 from modgrad_amd import _lib
 from tests.test_kv_shared_plan_cpu import ask, cache_of
+from tests.test_kvcache_cpu import INVALID
 
 LAUNCH = (2 ** 32 - 1) // 256  # work-groups of 256 threads that one launch counts
 
@@ -95,3 +96,31 @@ def test_room_does_not_fall():
             ways.add(p.way)
             assert a >= plain and a >= needed(p, heads, dim, new * group > (32 if dim == 256 else 48))
     assert ways == {0, 1, 2, 3}
+
+
+@pytest.mark.parametrize("way", ["plain", "sinks", "shared"])
+def test_joins_that_no_launch_counts(way):
+    """2^20 sequences of 16 rows: refused before the first of two launches, but where every
+    row sees at most 8 tiles and none is joined."""
+    from tests.test_kv_shared_cpu import FAKE
+    L = _lib.load()
+
+    def made(seqs, max_pages, window=0):
+        c = cache_of(seqs, 1, 64, 64, 0, max_pages)
+        c.cu_tokens = None
+        args = _lib.KvAttentionArgs(c, FAKE, FAKE, FAKE, 1 << 45, 1024, 1024, 16, 0, seqs, 1, window, 0.1, 0.0)
+        op = {"plain": lambda: args, "sinks": lambda: _lib.KvAttentionSinksArgs(args, 4),
+              "shared": lambda: _lib.KvAttentionSharedArgs(args, 640)}[way]()
+        kind = {"plain": _lib.OP_KV_ATTENTION, "sinks": _lib.OP_KV_ATTENTION_SINKS,
+                "shared": _lib.OP_KV_ATTENTION_SHARED}[way]
+        d, chain = _lib.OpDesc(op=kind, w=ctypes.addressof(op)), ctypes.c_void_p()
+        code = L.mgq_chain_create_ops(ctypes.byref(d), 1, ctypes.byref(chain))
+        if chain.value:  # recorded, never launched; without a device it is not even that
+            L.mgq_chain_destroy(chain)
+        return code
+    assert made(1 << 20, 100) == INVALID
+    fits = [made((1 << 20) - 1, 100), made(1 << 20, 8)]
+    if way == "sinks":
+        assert made(1 << 20, 100, 2000) == INVALID
+        fits.append(made(1 << 20, 100, 300))  # 300 and 4: never more than 8 tiles
+    assert INVALID not in fits

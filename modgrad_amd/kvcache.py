@@ -322,7 +322,8 @@ class KvCache:
     def new(cls, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, n_seqs: int,
             max_pages: int, fmt: str = "i8", stream=None) -> "KvCache":
         """An empty cache whose pages reserve(), share(), give_back() and release() hand
-        out and take back."""
+        out and take back. Its table is theirs to write: pages entered by hand would be
+        given out or taken back beside them (wrap() is for tables of one's own)."""
         torch = _torch()
         with _stream(stream):
             try:
